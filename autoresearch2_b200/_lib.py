@@ -19,6 +19,7 @@ STATUS_BITS = {
     2: "bounded device wait timed out",
     4: "int32 arena cursor overflow",
     8: "mask has more set bits than vals holds",
+    16: "token index outside the vocabulary",
 }
 
 
@@ -27,6 +28,7 @@ class SparseFFNError(RuntimeError):
 
 
 _vp, _i64, _i32, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int, ctypes.c_size_t
+_f32 = ctypes.c_float
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -92,6 +94,20 @@ SIGNATURES = {
     "sffn_ffn_dgrad": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp,
                               _vp, _vp, _vp, _i64, _vp, _vp, _vp]),
     "sffn_wait_probe": (_int, [_int, _i64, _vp, _vp, _vp, _vp]),
+    "sffn_token_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _int, _i64, _int, _f32, _vp, _vp,
+                                   _vp, _vp, _vp, _vp, _vp]),
+    "sffn_token_logprobs_bwd": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _int, _i64, _vp, _int, _f32,
+                                       _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "sffn_distill_topk": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _int, _vp, _int, _int, _int, _f32,
+                                 _vp, _vp, _vp, _vp]),
+    "sffn_distill_topk_bwd": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _int, _vp, _int, _int, _int,
+                                     _f32, _vp, _vp, _vp, _i64, _vp]),
+    "sffn_residual_norm": (_int, [_vp, _int, _i64, _vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _int, _vp, _int,
+                                  _i64, _int, _f32, _f32, _vp, _vp, _vp, _vp]),
+    "sffn_residual_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "sffn_residual_norm_bwd": (_int, [_vp, _int, _i64, _vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _int, _vp,
+                                      _int, _i64, _int, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                      _vp]),
 }
 
 _lib = None
@@ -127,7 +143,8 @@ LAUNCHING = {"sffn_sp24_compress": 1, "sffn_gemm_sp24": 1, "sffn_sp24_overflow_a
              "sffn_ck_compact_rows": 1, "sffn_gemm_ck": 1, "sffn_live_kblocks_t": 1, "sffn_gemm_bf16_ct": 1,
              "sffn_split_bf16x3": 1, "sffn_gemm_bf16_f32out": 1, "sffn_tile_copy_slots": 1,
              "sffn_gemm_bf16_f32acc": 1, "sffn_gemm_tf32": 1, "sffn_gemm_relu": 1,
-             "sffn_round_tf32": 1}
+             "sffn_round_tf32": 1, "sffn_token_logprobs": 1, "sffn_token_logprobs_bwd": 1, "sffn_distill_topk": 1,
+             "sffn_distill_topk_bwd": 1, "sffn_residual_norm": 1, "sffn_residual_norm_bwd": 1}
 launch_count = 0
 
 # Per-entry-point CUDA event pairs, recorded while a KernelTimer is active.
@@ -164,12 +181,15 @@ class KernelTimer:
 def _launches(name, args):
     """Kernels one successful call launched: LAUNCHING's count, except where
     it depends on the arguments (the float32-output GEMM runs one launch per
-    K chunk of 1024; the tile pack without vals stops after count and scan)."""
+    K chunk of 1024; the tile pack without vals stops after count and scan;
+    the block norm's backward joins the weight gradients, if any, in a second)."""
     if name == "sffn_gemm_bf16_f32out":
         return -(-int(args[10]) // 1024)
     if name == "sffn_tile_pack":
         v = args[9]
         return 2 if v is None or getattr(v, "value", v) in (None, 0) else 3
+    if name == "sffn_residual_norm_bwd":
+        return 2 if any(getattr(v, "value", v) for v in args[22:25]) else 1
     return LAUNCHING.get(name, 0)
 
 

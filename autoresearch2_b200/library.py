@@ -27,6 +27,15 @@ outputs' shapes and dtypes, so tracing needs no device.
     sparseffn::codec15_compress(data) -> stream
     sparseffn::codec15_uncompress(stream, shape, dtype) -> data
         the 15-bit sign-strip codec, bitshifting/code.py:129-177
+    sparseffn::token_logprobs(logits, targets?, top_k, temperature, ignore_index)
+        -> (logp, entropy, top_ids, top_logp, stats)
+    sparseffn::distill_topk(logits, ids, scores, temperature, tail) -> (loss, stats)
+    sparseffn::residual_norm(x, y?, pre?, post?, gate?, groups, post_norm, scale, eps, out_dtype)
+        -> (x_new, h, stats)
+        the operators of logits.py and norms.py (without counterpart in the
+        reference), with their autograd formulas over the ops named *_bwd;
+        their functions call these ops while torch.compile traces.  Outputs
+        that a call leaves out are empty tensors here.
 
 The fused bf16 path (ffn._fused_ok, decided from dtypes, contiguity and
 shapes alone) keeps z in 128x128 tiles and returns per-row value offsets and
@@ -40,12 +49,13 @@ from torch import Tensor
 
 from . import bitshift
 from . import bitsparse as bs
-from . import ffn
+from . import ffn, logits, norms
 
 __all__ = ["OPS"]
 
 OPS = ("bitsparse_pack", "bitsparse_unpack", "tile_pack", "tile_unpack", "ffn_fwd", "ffn_bwd",
-       "codec15_compress", "codec15_uncompress")
+       "codec15_compress", "codec15_uncompress", "token_logprobs", "token_logprobs_bwd", "distill_topk",
+       "distill_topk_bwd", "residual_norm", "residual_norm_bwd")
 
 
 def _cdiv(a, b):
@@ -186,3 +196,141 @@ def codec15_uncompress(compressed: Tensor, shape: list[int], dtype: torch.dtype)
 @codec15_uncompress.register_fake
 def _(compressed, shape, dtype):
     return compressed.new_empty(shape, dtype=dtype)
+
+
+# ---------------------------------------------------------------------------
+# Output distribution (parameters are named x: the module `logits` stays reachable)
+# ---------------------------------------------------------------------------
+@torch.library.custom_op("sparseffn::token_logprobs", mutates_args=())
+def token_logprobs(x: Tensor, targets: Optional[Tensor], top_k: int, temperature: float,
+                   ignore_index: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    return logits._score_forward(x, targets, top_k, temperature, ignore_index)
+
+
+@token_logprobs.register_fake
+def _(x, targets, top_k, temperature, ignore_index):
+    lead = x.shape[:-1]
+    f32 = dict(dtype=torch.float32)
+    return (x.new_empty(lead if targets is not None else (0,), **f32), x.new_empty(lead, **f32),
+            x.new_empty((*lead, top_k), dtype=torch.int64), x.new_empty((*lead, top_k), **f32),
+            x.new_empty((*lead, 2), **f32))
+
+
+@torch.library.custom_op("sparseffn::token_logprobs_bwd", mutates_args=())
+def token_logprobs_bwd(x: Tensor, targets: Optional[Tensor], top_ids: Tensor, entropy: Tensor, stats: Tensor,
+                       g_logp: Optional[Tensor], g_entropy: Optional[Tensor], g_top: Optional[Tensor],
+                       temperature: float, ignore_index: int) -> Tensor:
+    return logits._score_backward(x, targets, top_ids, entropy, stats, g_logp, g_entropy, g_top, temperature,
+                                  ignore_index).contiguous()
+
+
+@token_logprobs_bwd.register_fake
+def _(x, targets, top_ids, entropy, stats, g_logp, g_entropy, g_top, temperature, ignore_index):
+    return x.new_empty(x.shape)
+
+
+def _score_setup(ctx, inputs, output):
+    x, targets, _, temperature, ignore_index = inputs
+    _, entropy, top_ids, _, stats = output
+    ctx.save_for_backward(x, targets, top_ids, entropy, stats)
+    ctx.args = temperature, ignore_index
+    ctx.mark_non_differentiable(top_ids, stats)
+    ctx.set_materialize_grads(False)
+
+
+def _score_bwd(ctx, g_logp, g_entropy, _ids, g_top, _stats):
+    x, targets, top_ids, entropy, stats = ctx.saved_tensors
+    grad = token_logprobs_bwd(x, targets, top_ids, entropy, stats, g_logp if targets is not None else None,
+                              g_entropy, g_top, *ctx.args)
+    return grad, None, None, None, None
+
+
+token_logprobs.register_autograd(_score_bwd, setup_context=_score_setup)
+
+
+@torch.library.custom_op("sparseffn::distill_topk", mutates_args=())
+def distill_topk(x: Tensor, ids: Tensor, scores: Tensor, temperature: float, tail: str) -> tuple[Tensor, Tensor]:
+    return logits._distill_forward(x, ids, scores, temperature, tail)
+
+
+@distill_topk.register_fake
+def _(x, ids, scores, temperature, tail):
+    return x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty((*x.shape[:-1], 4), dtype=torch.float32)
+
+
+@torch.library.custom_op("sparseffn::distill_topk_bwd", mutates_args=())
+def distill_topk_bwd(x: Tensor, ids: Tensor, scores: Tensor, stats: Tensor, g_loss: Tensor, temperature: float,
+                     tail: str) -> Tensor:
+    return logits._distill_backward(x, ids, scores, stats, g_loss, temperature, tail).contiguous()
+
+
+@distill_topk_bwd.register_fake
+def _(x, ids, scores, stats, g_loss, temperature, tail):
+    return x.new_empty(x.shape)
+
+
+def _distill_setup(ctx, inputs, output):
+    x, ids, scores, temperature, tail = inputs
+    ctx.save_for_backward(x, ids, scores, output[1])
+    ctx.args = temperature, tail
+    ctx.mark_non_differentiable(output[1])
+
+
+def _distill_bwd(ctx, g_loss, _stats):
+    return distill_topk_bwd(*ctx.saved_tensors, g_loss, *ctx.args), None, None, None, None
+
+
+distill_topk.register_autograd(_distill_bwd, setup_context=_distill_setup)
+
+
+# ---------------------------------------------------------------------------
+# Norms around a block
+# ---------------------------------------------------------------------------
+def _or_empty(like, ts):
+    return tuple(t if t is not None else like.new_empty(0) for t in ts)
+
+
+@torch.library.custom_op("sparseffn::residual_norm", mutates_args=())
+def residual_norm(x: Tensor, y: Optional[Tensor], pre: Optional[Tensor], post: Optional[Tensor],
+                  gate: Optional[Tensor], groups: int, post_norm: bool, scale: float, eps: float,
+                  out_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
+    return _or_empty(x, norms._forward(x, y, pre, post, gate, groups, post_norm, scale, eps, out_dtype, True))
+
+
+@residual_norm.register_fake
+def _(x, y, pre, post, gate, groups, post_norm, scale, eps, out_dtype):
+    return (x.new_empty(x.shape if y is not None else (0,)), x.new_empty(x.shape, dtype=out_dtype),
+            x.new_empty((x.numel() // x.shape[-1], 2), dtype=torch.float32))
+
+
+@torch.library.custom_op("sparseffn::residual_norm_bwd", mutates_args=())
+def residual_norm_bwd(x: Tensor, y: Optional[Tensor], pre: Optional[Tensor], post: Optional[Tensor],
+                      gate: Optional[Tensor], groups: int, post_norm: bool, scale: float, out_dtype: torch.dtype,
+                      stats: Tensor, dx_new: Optional[Tensor], dh: Optional[Tensor],
+                      want: list[bool]) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    return _or_empty(x, norms._backward(x, y, pre, post, gate, groups, post_norm, scale, out_dtype, stats, dx_new,
+                                        dh, want))
+
+
+@residual_norm_bwd.register_fake
+def _(x, y, pre, post, gate, groups, post_norm, scale, out_dtype, stats, dx_new, dh, want):
+    return tuple(t.new_empty(t.shape) if t is not None and w else x.new_empty(0)
+                 for t, w in zip((x, y, pre, post, gate), want))
+
+
+def _norm_setup(ctx, inputs, output):
+    x, y, pre, post, gate, groups, post_norm, scale, eps, out_dtype = inputs
+    ctx.save_for_backward(x, y, pre, post, gate, output[2])
+    ctx.args = groups, post_norm, scale, out_dtype
+    ctx.mark_non_differentiable(output[2])
+    ctx.set_materialize_grads(False)
+
+
+def _norm_bwd(ctx, dx_new, dh, _stats):
+    x, y, pre, post, gate, stats = ctx.saved_tensors
+    want = [t is not None and w for t, w in zip((x, y, pre, post, gate), ctx.needs_input_grad)]
+    grads = residual_norm_bwd(x, y, pre, post, gate, *ctx.args, stats, dx_new if y is not None else None, dh, want)
+    return *(g if w else None for g, w in zip(grads, want)), None, None, None, None, None
+
+
+residual_norm.register_autograd(_norm_bwd, setup_context=_norm_setup)

@@ -52,7 +52,8 @@ enum {
     SFFN_STATUS_VALS_OVERFLOW = 1u,  /* output would pass vals capacity; clipped  */
     SFFN_STATUS_WAIT_TIMEOUT = 2u,   /* a bounded spin-wait gave up               */
     SFFN_STATUS_CURSOR_OVERFLOW = 4u,/* int32 arena cursor would pass 2^31-1      */
-    SFFN_STATUS_VALS_SHORT = 8u      /* mask has more set bits than vals holds    */
+    SFFN_STATUS_VALS_SHORT = 8u,     /* mask has more set bits than vals holds    */
+    SFFN_STATUS_BAD_INDEX = 16u      /* a token index outside the vocabulary      */
 };
 
 /* ---- library ----------------------------------------------------------- */
@@ -537,6 +538,88 @@ int sffn_codec15_compress(const void* src, int64_t n, uint8_t* dst, int64_t dst_
  * dst[i] = field i (sign bit 0).  Reads only the first sffn_codec15_bytes(n)
  * of src's src_bytes. */
 int sffn_codec15_uncompress(const uint8_t* src, int64_t src_bytes, int64_t n, void* dst, void* stream);
+
+/* ---- output distribution -------------------------------------------------
+ * logits [rows, vocab] of dtype; row r starts s_outer * (r / inner) +
+ * s_inner * (r % inner) elements after `logits` (any alignment of the
+ * element's size; inner = rows for one row stride).  inv_t = 1 / temperature.
+ * Index tensors hold 4- or 8-byte integers (target_bytes, id_bytes).  No
+ * counterpart in the reference.
+ */
+
+/* Per row: logp of its target, entropy, the top_k largest logits' indices
+ * (larger first, equal ones by lower index, NaN above all) and log
+ * probabilities.  targets may be NULL (logp is then not written).  A row whose
+ * target equals ignore_index is not read: logp 0, entropy 0, ids -1, top_logp
+ * -inf.  A row of -inf has logp -inf, entropy 0, top_logp -inf; a row with NaN
+ * or +inf has NaN.  Another target outside the vocabulary gives NaN and sets
+ * SFFN_STATUS_BAD_INDEX.  stats [rows, 2] receives max and sum (for the
+ * backward); top_k <= 128 (SFFN_ERR_TOO_LARGE beyond), top_ids and top_logp are
+ * [rows, top_k]. */
+int sffn_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t inner, int64_t s_outer,
+                        int64_t s_inner, const void* targets, int target_bytes, int64_t ignore_index, int top_k,
+                        float inv_t, float* logp, float* entropy, float* stats, int64_t* top_ids, float* top_logp,
+                        uint32_t* status_dev, void* stream);
+
+/* Gradient with respect to the logits: grad [rows, vocab] (row stride
+ * grad_ld), of the logits' dtype, from the gradients of logp, entropy and
+ * top_logp (each NULL for zero), with what the forward wrote.  Rows left out
+ * and rows of -inf get zeros. */
+int sffn_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t inner,
+                            int64_t s_outer, int64_t s_inner, const void* targets, int target_bytes,
+                            int64_t ignore_index, const int64_t* top_ids, int top_k, float inv_t, const float* stats,
+                            const float* entropy, const float* g_logp, const float* g_entropy, const float* g_top,
+                            void* grad, int64_t grad_ld, void* stream);
+
+/* What a teacher's list leaves of its probability: */
+enum {
+    SFFN_TAIL_RENORM = 0, /* nothing: the listed mass is scaled to one          */
+    SFFN_TAIL_BUCKET = 1  /* one more class, against the student's mass off the list */
+};
+
+/* Per row: the divergence sum q (ln q - ln p) of the student's distribution p
+ * from a teacher's list of k <= 128 entries: ids [rows, k] (-1: absent; others
+ * outside the vocabulary are absent too and set SFFN_STATUS_BAD_INDEX) and
+ * scores [rows, k] (log probabilities, of score_dtype).  A row without an entry
+ * of positive weight has loss 0.  An id that stands twice counts with both
+ * weights.  stats [rows, 4] is for the backward.  With SFFN_TAIL_BUCKET the
+ * vocabulary is at most 1,600,000 (SFFN_ERR_TOO_LARGE beyond). */
+int sffn_distill_topk(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t inner, int64_t s_outer,
+                      int64_t s_inner, const void* ids, int id_bytes, const void* scores, int score_dtype, int k,
+                      int tail, float inv_t, float* loss, float* stats, uint32_t* status_dev, void* stream);
+
+/* Its gradient with respect to the logits, times g_loss [rows]. */
+int sffn_distill_topk_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t inner, int64_t s_outer,
+                          int64_t s_inner, const void* ids, int id_bytes, const void* scores, int score_dtype, int k,
+                          int tail, float inv_t, const float* stats, const float* g_loss, void* grad, int64_t grad_ld,
+                          void* stream);
+
+/* ---- norms around a block ------------------------------------------------
+ * x_new = scale * x + gate * (post_norm ? rms(y) * post : y),
+ * h = rms(x_new) * pre, rms(v) = v / sqrt(mean v^2 + eps), over rows of `width`
+ * elements (<= 16384).  x has dtype x_dtype and row stride x_ld, y and h have
+ * y_dtype (x_dtype equals it or is SFFN_F32); x_new [rows, width] has x_dtype.
+ * y NULL: h = rms(x) * pre alone.  pre, post, gate NULL: ones.  gate holds one
+ * row of `width` for every gate_rows consecutive rows.  stats [rows, 2] (NULL:
+ * not wanted) is for the backward.  No counterpart in the reference.
+ */
+int sffn_residual_norm(const void* x, int x_dtype, int64_t x_ld, const void* y, int y_dtype, int64_t y_ld,
+                       int64_t rows, int64_t width, const void* pre, int pre_dtype, const void* post, int post_dtype,
+                       const void* gate, int gate_dtype, int64_t gate_rows, int post_norm, float scale, float eps,
+                       void* x_new, void* h, float* stats, void* stream);
+
+/* Scratch of the backward when a weight's or gate's gradient is wanted
+ * (gate_rows 0: not the gate's). */
+size_t sffn_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t width, int64_t gate_rows);
+
+/* Every gradient, from dx_new and dh (contiguous; NULL for zero): dx, dy of x's
+ * and y's dtype, dpre, dpost, dgate of their weights' (each NULL: not wanted). */
+int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, const void* y, int y_dtype, int64_t y_ld,
+                           int64_t rows, int64_t width, const void* pre, int pre_dtype, const void* post,
+                           int post_dtype, const void* gate, int gate_dtype, int64_t gate_rows, int post_norm,
+                           float scale, const float* stats, const void* dx_new, const void* dh, void* dx, void* dy,
+                           void* dpre, void* dpost, void* dgate, void* workspace, size_t workspace_bytes,
+                           void* stream);
 
 /* ---- bounded waits ------------------------------------------------------ */
 
