@@ -10,6 +10,8 @@
 // All sums, maxima and statistics are float32 whatever the logits' type.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace sffn {
@@ -99,29 +101,100 @@ struct Cut {
     }
 };
 
+// Two float32 in one 64-bit register: sm_100a adds, multiplies and fuses both
+// in one instruction, and the streaming loop is as near to the issue rate as
+// to memory.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 // The running (m, s, w) of one thread, exponents in units of log 2: c = log2(e) / T.
+// s and w are kept as pairs (even and odd elements).
 struct Soft {
-    float m = LOWEST, s = 0.f, w = 0.f;
+    float m = LOWEST;
+    uint64_t s = 0, w = 0;
     __device__ __forceinline__ void raise(float to, float c) {
         const float by = fmaxf((m - to) * c, D_MIN);
         const float f = ex2(by);
-        w = fmaf(s, by, w) * f;
-        s *= f;
+        w = mul2(fma2(s, pair(by, by), w), pair(f, f));
+        s = mul2(s, pair(f, f));
         m = to;
     }
-    __device__ __forceinline__ void add(float x, float c) {
-        const float d = max_nan((x - m) * c, D_MIN);
-        const float e = ex2(d);
-        s += e;
-        w = fmaf(e, d, w);
+    __device__ __forceinline__ void add(float x0, float x1, float c) {
+        float d0, d1;
+        unpair(mul2(add2(pair(x0, x1), pair(-m, -m)), pair(c, c)), d0, d1);
+        d0 = max_nan(d0, D_MIN);
+        d1 = max_nan(d1, D_MIN);
+        const uint64_t e = pair(ex2(d0), ex2(d1));
+        s = add2(s, e);
+        w = fma2(e, pair(d0, d1), w);
     }
     __device__ __forceinline__ void one(float x, float c) {
         if (x > m) raise(x, c);
-        add(x, c);
+        add(x, -INFINITY, c);
     }
 };
 
-// Sum over the block; every thread gets it.  `slots` holds a float per warp.
+// Joins the threads' running sums: afterwards (m, s, w) is the block's, in every
+// thread.  Two barriers; the slots are for this call alone.
+template <int NT>
+struct JoinSlots {
+    float m[NT / 32];
+    float2 sw[NT / 32];
+};
+template <int NT>
+__device__ __forceinline__ void join(Soft& a, float c, JoinSlots<NT>& slots, float& m, float& s, float& w) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    m = a.m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
+    if (lane == 0) slots.m[warp] = m;
+    __syncthreads();
+    m = slots.m[0];
+#pragma unroll
+    for (int i = 1; i < NT / 32; ++i) m = fmaxf(m, slots.m[i]);
+    a.raise(m, c);
+    float s1, w1;
+    unpair(a.s, s, s1);
+    unpair(a.w, w, w1);
+    s += s1;
+    w += w1;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        s += __shfl_xor_sync(FULL, s, o);
+        w += __shfl_xor_sync(FULL, w, o);
+    }
+    if (lane == 0) slots.sw[warp] = make_float2(s, w);
+    __syncthreads();
+    s = w = 0.f;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) {
+        s += slots.sw[i].x;
+        w += slots.sw[i].y;
+    }
+}
+
+// Sum / maximum over the block for the short lists; every thread gets it.
 template <int NT>
 __device__ __forceinline__ float block_sum(float v, float* slots) {
 #pragma unroll
@@ -145,15 +218,6 @@ __device__ __forceinline__ float block_max(float v, float* slots) {
 #pragma unroll
     for (int i = 1; i < NT / 32; ++i) r = fmaxf(r, slots[i]);
     return r;
-}
-
-// Joins the threads' running sums: afterwards every thread holds the row's.
-template <int NT>
-__device__ __forceinline__ void join(Soft& a, float c, float* slots) {
-    const float m = block_max<NT>(a.m, slots);
-    a.raise(m, c);
-    a.s = block_sum<NT>(a.s, slots);
-    a.w = block_sum<NT>(a.w, slots);
 }
 
 // Order of the alternatives: larger logits first, equal ones by lower index,
@@ -187,6 +251,45 @@ __device__ __forceinline__ void each(const void* row, const Cut<DT>& cut, F&& f)
     if (t < cut.tail) f(load1<DT>(row, at), at);
 }
 
+// One pass over a row: AHEAD vectors of a thread are loaded before the first
+// is used.  edit(x, index) may replace a vector's elements; seen(max, last
+// index) is told each vector's (or single element's) largest.
+template <int DT, int NT, class Edit, class Seen>
+__device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, float c, Soft& soft, Edit&& edit, Seen&& seen) {
+    constexpr int N = Row<DT>::N, AHEAD = 4;
+    const int t = threadIdx.x;
+    auto single = [&](int i) {
+        float x[1] = {load1<DT>(row, i)};
+        edit(x, i, std::integral_constant<int, 1>());
+        soft.one(x[0], c);
+        seen(x[0], i);
+    };
+    if (t < cut.head) single(t);
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const typename Elt<DT>::bits*>(row) + cut.head);
+    for (int v0 = t; v0 < cut.nvec; v0 += NT * AHEAD) {
+        uint4 raw[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (v0 + u * NT < cut.nvec) raw[u] = __ldg(q + v0 + u * NT);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int v = v0 + u * NT;
+            if (v >= cut.nvec) break;
+            float x[N];
+            unpack<DT>(raw[u], x);
+            edit(x, cut.head + v * N, std::integral_constant<int, N>());
+            float top = x[0];
+#pragma unroll
+            for (int j = 1; j < N; ++j) top = fmaxf(top, x[j]);
+            if (top > soft.m) soft.raise(top, c);
+#pragma unroll
+            for (int j = 0; j < N; j += 2) soft.add(x[j], x[j + 1], c);
+            seen(top, cut.head + v * N + N - 1);
+        }
+    }
+    if (t < cut.tail) single(cut.head + cut.nvec * N + t);
+}
+
 // ---------------------------------------------------------------------------
 // Log probabilities, entropy and top alternatives
 // ---------------------------------------------------------------------------
@@ -206,13 +309,124 @@ struct ScoreArgs {
     uint32_t* status;
 };
 
+// The alternatives of a row (or of a block's share of one) as order keys,
+// sorted, in `best`; returns how many there are, min(k, n).
+//
+// Each thread brings the key of its own largest element (`mine`, its index
+// rounded up to its vector's last).  The k-th largest of the maxima of NT / 2 or
+// NT / 4 disjoint groups of threads is a lower bound of the k-th largest
+// element that little lies above: about k elements of a shuffled row.  Only
+// threads whose maximum reaches it look at their share again, from L2.  Where
+// more than CAP elements reach it (the largest elements lie in few threads'
+// shares) the k-th largest key is found exactly, eight bits a pass.
+constexpr int CAP = 1280;
+template <int NT>
+struct TopSlots {
+    unsigned long long keys[CAP];  // the threads' keys, then the candidates
+    unsigned long long group[NT / 2];
+    unsigned long long best[TOP_MAX];
+    unsigned long long least;
+    int hist[256];
+    int count, need;
+};
+
 template <int DT, int NT>
-__global__ void __launch_bounds__(NT) score_kernel(const ScoreArgs a) {
-    __shared__ float slots[NT / 32];
-    __shared__ unsigned long long keys[TOP_MAX];
-    __shared__ int hist[256];
-    __shared__ unsigned long long prefix_s;
-    __shared__ int need_s, count_s;
+__device__ int top_of(const void* row, const Cut<DT>& cut, int n, int k, unsigned long long mine, bool exact,
+                      TopSlots<NT>& z) {
+    const int t = threadIdx.x;
+    const int parts = k <= NT / 8 ? 4 : 2, groups = NT / parts;
+    // groups take threads t, t + groups, ...: the first groups then hold the row's
+    // first vectors, which bounds the candidates of a row of equal elements.
+    z.keys[t] = mine;
+    if (t == 0) {
+        z.least = 0;
+        z.count = 0;
+    }
+    __syncthreads();
+    if (t < groups) {
+        unsigned long long best = z.keys[t];
+        for (int i = 1; i < parts; ++i) best = max(best, z.keys[t + i * groups]);
+        z.group[t] = best;
+    }
+    __syncthreads();
+    {
+        const int g = t / parts, part = t % parts;
+        const unsigned long long key = z.group[g];
+        int above = 0;
+        for (int i = part; i < groups; i += parts) {
+            const unsigned long long other = z.group[i];
+            above += other > key || (other == key && i < g);
+        }
+        for (int o = 1; o < parts; o <<= 1) above += __shfl_xor_sync(FULL, above, o);
+        if (part == 0 && above == k - 1) z.least = key;
+    }
+    __syncthreads();
+    unsigned long long least = z.least;
+    if (!exact && mine >= least)
+        each<DT, NT>(row, cut, [&](float x, int i) {
+            const unsigned long long key = order_key(x, i);
+            if (key >= least) {
+                const int at = atomicAdd(&z.count, 1);
+                if (at < CAP) z.keys[at] = key;
+            }
+        });
+    __syncthreads();
+    int count = z.count;
+    if (exact || count > CAP) {
+        __syncthreads();
+        if (t == 0) {
+            z.least = 0;
+            z.need = min(k, n);
+            z.count = 0;
+        }
+        for (int shift = 56; shift >= 0; shift -= 8) {
+            for (int i = t; i < 256; i += NT) z.hist[i] = 0;
+            __syncthreads();
+            const unsigned long long prefix = z.least;
+            each<DT, NT>(row, cut, [&](float x, int i) {
+                const unsigned long long key = order_key(x, i);
+                if (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
+                    atomicAdd(&z.hist[(key >> shift) & 255], 1);
+            });
+            __syncthreads();
+            if (t == 0) {
+                int need = z.need, b = 255;
+                for (; b > 0 && z.hist[b] < need; --b) need -= z.hist[b];
+                z.need = need;
+                z.least = prefix | ((unsigned long long)b << shift);
+            }
+            __syncthreads();
+        }
+        least = z.least;
+        each<DT, NT>(row, cut, [&](float x, int i) {
+            const unsigned long long key = order_key(x, i);
+            if (key >= least) {
+                const int at = atomicAdd(&z.count, 1);
+                if (at < CAP) z.keys[at] = key;
+            }
+        });
+        __syncthreads();
+        count = min(z.count, CAP);
+    }
+    // Sorted by counting: `lanes` threads share a candidate.  (Keys are distinct.)
+    int lanes = 1;
+    while (lanes < 32 && count * lanes * 2 <= NT) lanes *= 2;
+    for (int i0 = 0; i0 < count; i0 += NT / lanes) {
+        const int i = i0 + t / lanes;
+        const unsigned long long key = i < count ? z.keys[i] : 0;
+        int above = 0;
+        for (int j = t % lanes; j < count; j += lanes) above += z.keys[j] > key;
+        for (int o = 1; o < lanes; o <<= 1) above += __shfl_xor_sync(FULL, above, o);
+        if (i < count && t % lanes == 0 && above < k) z.best[above] = key;
+    }
+    __syncthreads();
+    return min(count, k);
+}
+
+template <int DT, int NT, bool TOP>
+__global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a) {
+    __shared__ JoinSlots<NT> slots;
+    __shared__ typename std::conditional<TOP, TopSlots<NT>, int>::type top_slots;
     const int t = threadIdx.x;
     const int64_t r = blockIdx.x;
     int64_t target = -1;
@@ -236,62 +450,44 @@ __global__ void __launch_bounds__(NT) score_kernel(const ScoreArgs a) {
     const Cut<DT> cut(row, a.vocab);
     const float c = a.inv_t * LOG2E;
     Soft soft;
-    each<DT, NT>(row, cut, [&](float x, int) { soft.one(x, c); });
-    join<NT>(soft, c, slots);
-    const float ln_s = soft.s > 0.f || soft.s != soft.s ? logf(soft.s) : -INFINITY;
+    float top = -INFINITY;
+    int top_at = 0x7fffffff;
+    stream<DT, NT>(row, cut, c, soft, [](float*, int, auto) {}, [&](float x, int last) {
+        if (TOP && x > top) {
+            top = x;
+            top_at = last;
+        }
+    });
+    float m, s, w;
+    join<NT>(soft, c, slots, m, s, w);
+    const float ln_s = s == 0.f ? -INFINITY : logf(s);
     if (t == 0) {
         if (a.targets) {
             float lp = NAN;
             if (target >= 0 && target < a.vocab)
-                lp = soft.s == 0.f ? -INFINITY : (load1<DT>(row, target) - soft.m) * a.inv_t - ln_s;
+                lp = s == 0.f ? -INFINITY : (load1<DT>(row, target) - m) * a.inv_t - ln_s;
             else
                 atomicOr(a.status, SFFN_STATUS_BAD_INDEX);
             a.logp[r] = lp;
         }
-        a.entropy[r] = soft.s == 0.f ? 0.f : ln_s - soft.w / soft.s * LN2;
-        a.stats[2 * r] = soft.m;
-        a.stats[2 * r + 1] = soft.s;
+        a.entropy[r] = s == 0.f ? 0.f : ln_s - w / s * LN2;
+        a.stats[2 * r] = m;
+        a.stats[2 * r + 1] = s;
     }
-    if (a.top_k == 0) return;
-    // The top_k-th largest key, eight bits at a time.
-    if (t == 0) {
-        prefix_s = 0;
-        need_s = a.top_k;
-        count_s = 0;
-    }
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        for (int i = t; i < 256; i += NT) hist[i] = 0;
-        __syncthreads();
-        const unsigned long long prefix = prefix_s;
-        each<DT, NT>(row, cut, [&](float x, int i) {
-            const unsigned long long k = order_key(x, i);
-            if (shift == 56 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
-        });
-        __syncthreads();
-        if (t == 0) {
-            int need = need_s, b = 255;
-            for (; b > 0 && hist[b] < need; --b) need -= hist[b];
-            need_s = need;
-            prefix_s = prefix | ((unsigned long long)b << shift);
+    if constexpr (TOP) {
+        // A thread that saw nothing above -inf brings its first element's place;
+        // one without elements the lowest key.
+        const int first = t < cut.head ? t : t < cut.nvec ? cut.head + t * Row<DT>::N + Row<DT>::N - 1
+                        : t < cut.tail ? cut.head + cut.nvec * Row<DT>::N + t : 0x7fffffff;
+        const unsigned long long mine =
+            top > -INFINITY ? order_key(top, top_at) : first != 0x7fffffff ? order_key(-INFINITY, first) : 0ull;
+        const int k = top_of<DT, NT>(row, cut, a.vocab, a.top_k, mine, s != s, top_slots);
+        for (int i = t; i < k; i += NT) {
+            const unsigned long long key = top_slots.best[i];
+            const float x = order_value((uint32_t)(key >> 32));
+            a.top_ids[r * a.top_k + i] = 0xFFFFFFFFu - (uint32_t)key;
+            a.top_logp[r * a.top_k + i] = s == 0.f ? -INFINITY : (x - m) * a.inv_t - ln_s;
         }
-        __syncthreads();
-    }
-    const unsigned long long least = prefix_s;
-    each<DT, NT>(row, cut, [&](float x, int i) {
-        const unsigned long long k = order_key(x, i);
-        if (k >= least) {
-            const int at = atomicAdd(&count_s, 1);
-            if (at < TOP_MAX) keys[at] = k;
-        }
-    });
-    __syncthreads();
-    for (int i = t; i < a.top_k; i += NT) {
-        const unsigned long long k = keys[i];
-        int rank = 0;
-        for (int j = 0; j < a.top_k; ++j) rank += keys[j] > k;
-        const float x = order_value((uint32_t)(k >> 32));
-        a.top_ids[r * a.top_k + rank] = 0xFFFFFFFFu - (uint32_t)k;
-        a.top_logp[r * a.top_k + rank] = soft.s == 0.f ? -INFINITY : (x - soft.m) * a.inv_t - ln_s;
     }
 }
 
@@ -313,32 +509,43 @@ struct ScoreBwdArgs {
     int per;  // elements of a row that one block writes
 };
 
-// Writes f(x_j, j) to grad for the block's share of the row; 16-byte stores
-// where the gradient's row is aligned as the logits' is.
+// Writes f of the block's share of a row: f(x, n) replaces n elements in place.
+// 16-byte accesses where the gradient's row is aligned as the logits' is.
 template <int DT, int NT, class F>
 __device__ __forceinline__ void map_row(const void* row, void* out, int n, F&& f) {
     using bits = typename Elt<DT>::bits;
-    constexpr int N = Row<DT>::N;
+    constexpr int N = Row<DT>::N, AHEAD = 4;
     const int t = threadIdx.x;
     const bits* src = reinterpret_cast<const bits*>(row);
     bits* dst = reinterpret_cast<bits*>(out);
+    auto single = [&](int i) {
+        float x[2] = {Elt<DT>::to_f(src[i]), 0.f};
+        f(x, std::integral_constant<int, 2>());
+        dst[i] = Elt<DT>::from_f(x[0]);
+    };
     if (((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) != 0) {
-        for (int i = t; i < n; i += NT) dst[i] = Elt<DT>::from_f(f(Elt<DT>::to_f(src[i])));
+        for (int i = t; i < n; i += NT) single(i);
         return;
     }
     const Cut<DT> cut(row, n);
-    if (t < cut.head) dst[t] = Elt<DT>::from_f(f(Elt<DT>::to_f(src[t])));
+    if (t < cut.head) single(t);
     const uint4* q = reinterpret_cast<const uint4*>(src + cut.head);
     uint4* o = reinterpret_cast<uint4*>(dst + cut.head);
-    for (int v = t; v < cut.nvec; v += NT) {
-        float x[N];
-        unpack<DT>(__ldg(q + v), x);
+    for (int v0 = t; v0 < cut.nvec; v0 += NT * AHEAD) {
+        uint4 raw[AHEAD];
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = f(x[j]);
-        o[v] = pack<DT>(x);
+        for (int u = 0; u < AHEAD; ++u)
+            if (v0 + u * NT < cut.nvec) raw[u] = __ldg(q + v0 + u * NT);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (v0 + u * NT >= cut.nvec) break;
+            float x[N];
+            unpack<DT>(raw[u], x);
+            f(x, std::integral_constant<int, N>());
+            o[v0 + u * NT] = pack<DT>(x);
+        }
     }
-    const int at = cut.head + cut.nvec * N + t;
-    if (t < cut.tail) dst[at] = Elt<DT>::from_f(f(Elt<DT>::to_f(src[at])));
+    if (t < cut.tail) single(cut.head + cut.nvec * N + t);
 }
 
 template <int NT>
@@ -351,18 +558,58 @@ __device__ __forceinline__ void zero_row(void* out, int64_t bytes) {
     for (int64_t i = head + nv * 16 + threadIdx.x; i < bytes; i += NT) p[i] = 0;
 }
 
-// e^d / s of one logit, and ln of it (clamped, so that 0 * ln 0 is 0).
-struct Prob {
-    float m, inv_t, inv_s, ln_s;
-    __device__ __forceinline__ float p(float x) const { return expf((x - m) * inv_t) * inv_s; }
-    __device__ __forceinline__ float ln(float x) const { return max_nan((x - m) * inv_t - ln_s, D_MIN); }
+// x -> a p + b p ln p for pairs of logits.  For 16-bit gradients one exponential
+// of (x - m) log2(e) / T - log2 s, within 2^-19 of p where p is above 2^-60; for
+// float32 ones e^d by expf and 1 / s apart, which keeps p to the last bits.
+template <int DT>
+struct Weigh {
+    float m, inv_t, inv_s, ln_s, c, l2s;
+    __device__ __forceinline__ Weigh(float m_, float s, float inv_t_)
+        : m(m_), inv_t(inv_t_), inv_s(1.0f / s), ln_s(logf(s)), c(inv_t_ * LOG2E), l2s(log2f(s)) {}
+    template <int N, bool LN>
+    __device__ __forceinline__ void apply(float* x, float a, float b) const {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            if constexpr (DT == SFFN_F32) {
+#pragma unroll
+                for (int i = j; i < j + 2; ++i) {
+                    const float d = (x[i] - m) * inv_t, p = expf(d) * inv_s;
+                    x[i] = p * (LN ? fmaf(b, max_nan(d - ln_s, D_MIN), a) : a);
+                }
+            } else {
+                float d0, d1;
+                unpair(fma2(add2(pair(x[j], x[j + 1]), pair(-m, -m)), pair(c, c), pair(-l2s, -l2s)), d0, d1);
+                if (LN) {
+                    d0 = max_nan(d0, D_MIN);
+                    d1 = max_nan(d1, D_MIN);
+                }
+                uint64_t f = pair(a, a);
+                if (LN) f = fma2(pair(d0, d1), pair(b * LN2, b * LN2), f);
+                unpair(mul2(pair(ex2(d0), ex2(d1)), f), x[j], x[j + 1]);
+            }
+        }
+    }
+    // One logit's value, the same bits as in a vector.
+    __device__ __forceinline__ float one(float x, float a, float b) const {
+        float v[2] = {x, x};
+        if (b == 0.f) apply<2, false>(v, a, b);
+        else apply<2, true>(v, a, b);
+        return v[0];
+    }
+    template <int NT>
+    __device__ __forceinline__ void row(const void* row, void* out, int n, float a, float b) const {
+        if (b == 0.f)
+            map_row<DT, NT>(row, out, n, [&](float* x, auto k) { apply<decltype(k)::value, false>(x, a, b); });
+        else
+            map_row<DT, NT>(row, out, n, [&](float* x, auto k) { apply<decltype(k)::value, true>(x, a, b); });
+    }
 };
 
 template <int DT, int NT>
 __global__ void __launch_bounds__(NT) score_bwd_kernel(const ScoreBwdArgs a) {
     using bits = typename Elt<DT>::bits;
     const int t = threadIdx.x;
-    const int64_t r = blockIdx.x;
+    const int64_t r = a.rows - 1 - blockIdx.x;  // the rows that the forward read last may still be in L2
     const int begin = blockIdx.y * a.per, n = min(a.per, a.vocab - begin);
     const bits* row = reinterpret_cast<const bits*>(a.logits) + a.map.at(r);
     bits* out = reinterpret_cast<bits*>(a.grad) + r * a.grad_ld;
@@ -382,10 +629,9 @@ __global__ void __launch_bounds__(NT) score_bwd_kernel(const ScoreBwdArgs a) {
 #pragma unroll
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
     }
-    const Prob pr{a.stats[2 * r], a.inv_t, 1.0f / s, logf(s)};
-    const float base = -(total + g) - gh * a.entropy[r];
-    auto f = [&](float x) { return a.inv_t * (pr.p(x) * (base - gh * pr.ln(x))); };
-    map_row<DT, NT>(row + begin, out + begin, n, f);
+    const Weigh<DT> weigh(a.stats[2 * r], s, a.inv_t);
+    const float wa = -a.inv_t * (total + g + (gh != 0.f ? gh * a.entropy[r] : 0.f)), wb = -a.inv_t * gh;
+    weigh.template row<NT>(row + begin, out + begin, n, wa, wb);
     // The places with a gradient of their own, rewritten whole: the target and the alternatives.
     bool hit = false;
     __syncthreads();
@@ -393,10 +639,10 @@ __global__ void __launch_bounds__(NT) score_bwd_kernel(const ScoreBwdArgs a) {
         const int64_t id = a.top_ids[r * a.top_k + t];
         hit = id == target;
         if (id >= begin && id < begin + n)
-            out[id] = Elt<DT>::from_f(f(Elt<DT>::to_f(row[id])) + a.inv_t * (gt[t] + (hit ? g : 0.f)));
+            out[id] = Elt<DT>::from_f(weigh.one(Elt<DT>::to_f(row[id]), wa, wb) + a.inv_t * (gt[t] + (hit ? g : 0.f)));
     }
     if (!__syncthreads_or(hit) && t == 0 && has_target && target >= begin && target < begin + n)
-        out[target] = Elt<DT>::from_f(f(Elt<DT>::to_f(row[target])) + a.inv_t * g);
+        out[target] = Elt<DT>::from_f(weigh.one(Elt<DT>::to_f(row[target]), wa, wb) + a.inv_t * g);
 }
 
 // ---------------------------------------------------------------------------
@@ -430,11 +676,12 @@ struct DistillArgs {
 constexpr float REST_FLOOR = 1.0f / (1 << 20);
 
 template <int DT, int NT>
-__global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArgs a) {
     using bits = typename Elt<DT>::bits;
     constexpr int N = Row<DT>::N;
     extern __shared__ uint32_t on_list[];  // bucket: a bit per class, shifted so that vectors start whole
     __shared__ float slots[NT / 32];
+    __shared__ JoinSlots<NT> join_slots;
     __shared__ int ids[TOP_MAX];
     const int t = threadIdx.x;
     const int64_t r = blockIdx.x;
@@ -479,16 +726,23 @@ __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
         all_listed = __syncthreads_count(first) == a.vocab;
     }
     Soft soft;
-    each<DT, NT>(row, cut, [&](float x, int i) {
-        if (a.bucket && ((on_list[(i + pad) >> 5] >> ((i + pad) & 31)) & 1)) return;
-        soft.one(x, c);
-    });
-    join<NT>(soft, c, slots);
+    stream<DT, NT>(row, cut, c, soft, [&](float* x, int i, auto count) {
+        if (!a.bucket) return;
+        constexpr int n = decltype(count)::value;
+        const uint32_t on = on_list[(i + pad) >> 5] >> ((i + pad) & 31);
+        if (on & ((1u << n) - 1)) {
+#pragma unroll
+            for (int j = 0; j < n; ++j)
+                if ((on >> j) & 1) x[j] = -INFINITY;
+        }
+    }, [](float, int) {});
+    float m, s, w, off = 0.f;
+    join<NT>(soft, c, join_slots, m, s, w);
     const float x = id >= 0 ? Elt<DT>::to_f(row[id]) : 0.f;
-    float m = soft.m, s = soft.s, off = 0.f;
     if (a.bucket) {
-        m = block_max<NT>(id >= 0 ? fmaxf(x, soft.m) : soft.m, slots);
-        off = soft.s * ex2(fmaxf((soft.m - m) * c, D_MIN));
+        const float m_off = m, s_off = s;
+        m = block_max<NT>(id >= 0 ? fmaxf(x, m_off) : m_off, slots);
+        off = s_off * ex2(fmaxf((m_off - m) * c, D_MIN));
         s = off + block_sum<NT>(first ? ex2(max_nan((x - m) * c, D_MIN)) : 0.f, slots);
     }
     const float ln_s = s == 0.f ? -INFINITY : logf(s);
@@ -537,7 +791,7 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const DistillBwdArgs a)
     __shared__ int ids[TOP_MAX];
     __shared__ float qs[TOP_MAX];
     const int t = threadIdx.x;
-    const int64_t r = blockIdx.x;
+    const int64_t r = a.rows - 1 - blockIdx.x;  // the rows that the forward read last may still be in L2
     const int begin = blockIdx.y * a.per, n = min(a.per, a.vocab - begin);
     const bits* row = reinterpret_cast<const bits*>(a.logits) + a.map.at(r);
     bits* out = reinterpret_cast<bits*>(a.grad) + r * a.grad_ld;
@@ -554,16 +808,15 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const DistillBwdArgs a)
         ids[t] = ok ? (int)j : -1;
         qs[t] = ok ? expf(load_code(a.scores, r * a.k + t, a.score_code) - ln_z) : 0.f;
     }
-    const Prob pr{a.stats[4 * r], a.inv_t, 1.0f / s, 0.f};
-    const float gf = g * factor;
-    map_row<DT, NT>(row + begin, out + begin, n, [&](float x) { return pr.p(x) * gf; });
+    const Weigh<DT> weigh(a.stats[4 * r], s, a.inv_t);
+    weigh.template row<NT>(row + begin, out + begin, n, g * factor, 0.f);
     __syncthreads();
     if (t < a.k) {
         const int id = ids[t];
         if (id >= begin && id < begin + n) {
             float q = 0.f;  // an id that stands twice has the sum of its weights, from either entry
             for (int i = 0; i < a.k; ++i) q += ids[i] == id ? qs[i] : 0.f;
-            out[id] = Elt<DT>::from_f(g * (pr.p(Elt<DT>::to_f(row[id])) * Q - q));
+            out[id] = Elt<DT>::from_f(weigh.one(Elt<DT>::to_f(row[id]), g * Q, 0.f) - g * q);
         }
     }
 }
@@ -619,7 +872,9 @@ extern "C" int sffn_token_logprobs(const void* logits, int dtype, int64_t rows, 
     const ScoreArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, targets, target_bytes, ignore_index,
                       top_k, inv_t, logp, entropy, stats, top_ids, top_logp, status_dev};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define SFFN_CALL(DT) score_kernel<DT, 512><<<(unsigned)rows, 512, 0, st>>>(a)
+#define SFFN_CALL(DT)                                                    \
+    if (top_k) score_kernel<DT, 512, true><<<(unsigned)rows, 512, 0, st>>>(a); \
+    else score_kernel<DT, 512, false><<<(unsigned)rows, 512, 0, st>>>(a)
     SFFN_BY_DTYPE(dtype, SFFN_CALL);
 #undef SFFN_CALL
     SFFN_CHECK_LAUNCH();
