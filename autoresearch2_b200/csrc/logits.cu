@@ -8,6 +8,7 @@
 // One pass keeps the running (m, s, w = sum e^d d); a new maximum m' rescales
 //   s <- s f,  w <- (w + s (m - m')/T) f,  f = e^{(m - m')/T}.
 // All sums, maxima and statistics are float32 whatever the logits' type.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include <type_traits>
@@ -17,6 +18,7 @@
 namespace sffn {
 namespace {
 
+constexpr int SMS = 148;
 constexpr int TOP_MAX = 128;          // alternatives a row (and entries of a teacher's list)
 constexpr float LOWEST = -3.402823466e38f;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -87,18 +89,33 @@ __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int byte
     return bytes == 8 ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t) reinterpret_cast<const int32_t*>(p)[i];
 }
 
-// Where a row's 16-byte vectors begin: `head` single elements, `nvec` vectors, `tail` singles.
+// The part of a row that one block reads: `head` single elements, `nvec` 16-byte
+// vectors from the row's vector `first` on, `tail` singles from `tail_at` on.
+// With `of` blocks to the row its vectors are split evenly, the head goes to
+// the first block and the tail to the last.
 template <int DT>
 struct Cut {
-    int head, nvec, tail;
-    __device__ __forceinline__ Cut(const void* row, int n) {
+    int lead;  // elements of the row before its first vector
+    int head, first, nvec, tail, tail_at;
+    __device__ __forceinline__ Cut(const void* row, int n, int which = 0, int of = 1) {
         constexpr int N = Row<DT>::N;
         const int es = 16 / N;
         const int mis = (int)(reinterpret_cast<uintptr_t>(row) & 15u) / es;
-        head = min(n, mis ? N - mis : 0);
-        nvec = (n - head) / N;
-        tail = n - head - nvec * N;
+        lead = min(n, mis ? N - mis : 0);
+        const int all = (n - lead) / N;
+        tail_at = lead + all * N;
+        first = (int)((int64_t)all * which / of);
+        nvec = (int)((int64_t)all * (which + 1) / of) - first;
+        head = which == 0 ? lead : 0;
+        tail = which == of - 1 ? n - tail_at : 0;
     }
+    // Index of element 0 of this part's vector v.
+    __device__ __forceinline__ int at(int v) const { return lead + (first + v) * Row<DT>::N; }
+    __device__ __forceinline__ const uint4* vectors(const void* row) const {
+        return reinterpret_cast<const uint4*>(reinterpret_cast<const typename Elt<DT>::bits*>(row) + lead) + first;
+    }
+    __device__ __forceinline__ int begin() const { return head ? 0 : at(0); }
+    __device__ __forceinline__ int end() const { return tail ? tail_at + tail : at(nvec); }
 };
 
 // Two float32 in one 64-bit register: sm_100a adds, multiplies and fuses both
@@ -234,60 +251,65 @@ __device__ __forceinline__ unsigned long long order_key(float x, int i) {
     return ((unsigned long long)order_bits(x) << 32) | (0xFFFFFFFFu - (uint32_t)i);
 }
 
-// f(x, index) for every element of the row that this thread owns.
+// f(x, index) for every element of the part that this thread owns.
 template <int DT, int NT, class F>
 __device__ __forceinline__ void each(const void* row, const Cut<DT>& cut, F&& f) {
     constexpr int N = Row<DT>::N;
     const int t = threadIdx.x;
     if (t < cut.head) f(load1<DT>(row, t), t);
-    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const typename Elt<DT>::bits*>(row) + cut.head);
+    const uint4* q = cut.vectors(row);
     for (int v = t; v < cut.nvec; v += NT) {
         float x[N];
         unpack<DT>(__ldg(q + v), x);
 #pragma unroll
-        for (int j = 0; j < N; ++j) f(x[j], cut.head + v * N + j);
+        for (int j = 0; j < N; ++j) f(x[j], cut.at(v) + j);
     }
-    const int at = cut.head + cut.nvec * N + t;
-    if (t < cut.tail) f(load1<DT>(row, at), at);
+    if (t < cut.tail) f(load1<DT>(row, cut.tail_at + t), cut.tail_at + t);
 }
 
-// One pass over a row: AHEAD vectors of a thread are loaded before the first
-// is used.  edit(x, index) may replace a vector's elements; seen(max, last
-// index) is told each vector's (or single element's) largest.
+// One pass over the part: AHEAD vectors of a thread are loaded before the first
+// is used.  edit(x, index) may replace a vector's elements; seen(u, max, last
+// index) is told each vector's largest (u: its place among the AHEAD; single
+// elements come with u = 0).
+constexpr int AHEAD = 4;
 template <int DT, int NT, class Edit, class Seen>
 __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, float c, Soft& soft, Edit&& edit, Seen&& seen) {
-    constexpr int N = Row<DT>::N, AHEAD = 4;
+    constexpr int N = Row<DT>::N;
     const int t = threadIdx.x;
     auto single = [&](int i) {
         float x[1] = {load1<DT>(row, i)};
         edit(x, i, std::integral_constant<int, 1>());
         soft.one(x[0], c);
-        seen(x[0], i);
+        seen(std::integral_constant<int, 0>(), x[0], i);
     };
     if (t < cut.head) single(t);
-    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const typename Elt<DT>::bits*>(row) + cut.head);
+    const uint4* q = cut.vectors(row);
     for (int v0 = t; v0 < cut.nvec; v0 += NT * AHEAD) {
         uint4 raw[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
             if (v0 + u * NT < cut.nvec) raw[u] = __ldg(q + v0 + u * NT);
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
+        auto use = [&](auto place) {
+            constexpr int u = decltype(place)::value;
             const int v = v0 + u * NT;
-            if (v >= cut.nvec) break;
+            if (v >= cut.nvec) return;
             float x[N];
             unpack<DT>(raw[u], x);
-            edit(x, cut.head + v * N, std::integral_constant<int, N>());
+            edit(x, cut.at(v), std::integral_constant<int, N>());
             float top = x[0];
 #pragma unroll
             for (int j = 1; j < N; ++j) top = fmaxf(top, x[j]);
             if (top > soft.m) soft.raise(top, c);
 #pragma unroll
             for (int j = 0; j < N; j += 2) soft.add(x[j], x[j + 1], c);
-            seen(top, cut.head + v * N + N - 1);
-        }
+            seen(place, top, cut.at(v) + N - 1);
+        };
+        use(std::integral_constant<int, 0>());
+        use(std::integral_constant<int, 1>());
+        use(std::integral_constant<int, 2>());
+        use(std::integral_constant<int, 3>());
     }
-    if (t < cut.tail) single(cut.head + cut.nvec * N + t);
+    if (t < cut.tail) single(cut.tail_at + t);
 }
 
 // ---------------------------------------------------------------------------
@@ -307,76 +329,202 @@ struct ScoreArgs {
     int64_t* top_ids;
     float* top_logp;
     uint32_t* status;
+    int parts;  // blocks to a row (a cluster)
+};
+constexpr int MAX_PARTS = 8;
+
+// The alternatives of a block's part of a row as order keys, sorted, in `best`.
+//
+// The part falls into RUNS = 512 strided runs of vectors, and the threads bring
+// the largest element of each: its order bits and its index, rounded up to its
+// vector's last.  The k-th largest of these maxima is a lower bound of the k-th
+// largest element above which little lies: 1.15 k elements of a shuffled row for
+// k = 128.  One warp finds it, a bit of the order at a time; with many ties at
+// the bound the index decides, also a bit at a time, so that a row of equal
+// elements leaves about 8 k candidates.  Only the runs whose maximum reaches the bound are
+// read again, from L2, by all threads together.  Where more than CAP elements
+// reach it (the largest lie in few runs) or a NaN hides from the maxima, the
+// k-th largest key is found exactly, eight bits a pass over the part.
+constexpr int CAP = 1280;
+constexpr int RUNS = 512;
+struct TopSlots {
+    unsigned long long keys[CAP];  // candidates
+    unsigned long long best[TOP_MAX];
+    uint32_t run_order[RUNS];
+    int run_last[RUNS];
+    int look[RUNS];  // runs read again
+    int hist[256];
+    unsigned long long least;
+    int looks, count, need, found;
 };
 
-// The alternatives of a row (or of a block's share of one) as order keys,
-// sorted, in `best`; returns how many there are, min(k, n).
-//
-// Each thread brings the key of its own largest element (`mine`, its index
-// rounded up to its vector's last).  The k-th largest of the maxima of NT / 2 or
-// NT / 4 disjoint groups of threads is a lower bound of the k-th largest
-// element that little lies above: about k elements of a shuffled row.  Only
-// threads whose maximum reaches it look at their share again, from L2.  Where
-// more than CAP elements reach it (the largest elements lie in few threads'
-// shares) the k-th largest key is found exactly, eight bits a pass.
-constexpr int CAP = 1280;
+// A value v with at least `need` of the warp's keys (PER a lane) >= v: the
+// need-th largest key, from the highest bit in which the keys differ down, or a
+// prefix of it that already parts `need` keys from the rest; 0 with fewer keys
+// above 0.  Keys have LOW low bits that repeat the highest one, inverted.
+template <int LOW, int PER>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[PER], int need) {
+    uint32_t hi = 0, lo = 0xFFFFFFFFu;
+    int some = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        hi = max(hi, key[i]);
+        if (key[i]) {
+            lo = min(lo, key[i]);
+            ++some;
+        }
+    }
+    if (__reduce_add_sync(FULL, some) < need) return 0;
+    hi = __reduce_max_sync(FULL, hi);
+    lo = __reduce_min_sync(FULL, lo);
+    if (hi == lo) return hi;
+    const int top = 31 - __clz(hi ^ lo);
+    uint32_t v = top == 31 ? 0u : hi >> (top + 1) << (top + 1);
+    for (int bit = top; bit >= LOW; --bit) {
+        const uint32_t cand = v | (1u << bit);
+        int n[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < PER; ++i) n[i & 3] += key[i] >= cand;
+        const int all = __reduce_add_sync(FULL, (n[0] + n[1]) + (n[2] + n[3]));
+        if (all >= need) v = cand;
+        if (all == need) return v;
+    }
+    return v && !(v >> 31) ? v | ((1u << LOW) - 1) : v;
+}
+// Those bits of order_bits() of a type's values (finite or infinite).
+template <int DT> constexpr int ORDER_LOW = DT == SFFN_F32 ? 0 : DT == SFFN_BF16 ? 16 : 13;
+constexpr uint32_t ORDER_NEG_INF = 0x007FFFFFu;  // order_bits(-inf), the lowest
+
+// The k largest of z.keys[0 .. z.count) (0: no key; the others distinct), sorted
+// into z.best by counting the larger ones of each; z.found of them.
 template <int NT>
-struct TopSlots {
-    unsigned long long keys[CAP];  // the threads' keys, then the candidates
-    unsigned long long group[NT / 2];
-    unsigned long long best[TOP_MAX];
-    unsigned long long least;
-    int hist[256];
-    int count, need;
-};
+__device__ __forceinline__ void sort_keys(int k, TopSlots& z) {
+    const int t = threadIdx.x, count = z.count;
+    int lanes = 1;  // threads that share a key
+    while (lanes < 32 && count * lanes * 2 <= NT) lanes *= 2;
+    int most = 0;
+    for (int i0 = 0; i0 < count; i0 += NT / lanes) {
+        const int i = i0 + t / lanes;
+        const unsigned long long key = i < count ? z.keys[i] : 0;
+        int above = 0;
+#pragma unroll 4
+        for (int j = t % lanes; j < count; j += lanes) above += z.keys[j] > key;
+        for (int o = 1; o < lanes; o <<= 1) above += __shfl_xor_sync(FULL, above, o);
+        if (key && t % lanes == 0 && above < k) {
+            z.best[above] = key;
+            most = max(most, above + 1);
+        }
+    }
+    most = __reduce_max_sync(FULL, most);
+    if ((t & 31) == 0 && most) atomicMax(&z.found, most);
+    __syncthreads();
+}
 
 template <int DT, int NT>
-__device__ int top_of(const void* row, const Cut<DT>& cut, int n, int k, unsigned long long mine, bool exact,
-                      TopSlots<NT>& z) {
+__device__ __forceinline__ void top_of(const void* row, const Cut<DT>& cut, int k, const float (&top)[RUNS / NT],
+                                       const int (&last)[RUNS / NT], bool exact, TopSlots& z) {
+    constexpr int N = Row<DT>::N, SUB = RUNS / NT;
     const int t = threadIdx.x;
-    const int parts = k <= NT / 8 ? 4 : 2, groups = NT / parts;
-    // groups take threads t, t + groups, ...: the first groups then hold the row's
-    // first vectors, which bounds the candidates of a row of equal elements.
-    z.keys[t] = mine;
-    if (t == 0) {
-        z.least = 0;
-        z.count = 0;
+    // Runs: NT > 128 has one a thread; NT = 128 one for each place u of AHEAD.
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+        const bool any = last[u] >= 0;
+        z.run_order[u * NT + t] = any ? order_bits(top[u]) : 0u;
+        z.run_last[u * NT + t] = last[u];
     }
+    if (t == 0) z.count = z.looks = z.found = 0;
     __syncthreads();
-    if (t < groups) {
-        unsigned long long best = z.keys[t];
-        for (int i = 1; i < parts; ++i) best = max(best, z.keys[t + i * groups]);
-        z.group[t] = best;
-    }
-    __syncthreads();
-    {
-        const int g = t / parts, part = t % parts;
-        const unsigned long long key = z.group[g];
-        int above = 0;
-        for (int i = part; i < groups; i += parts) {
-            const unsigned long long other = z.group[i];
-            above += other > key || (other == key && i < g);
+    if (t < 32 && !exact) {
+        uint32_t order[RUNS / 32];
+#pragma unroll
+        for (int i = 0; i < RUNS / 32; ++i) order[i] = z.run_order[i * 32 + t];
+        const uint32_t bound = kth_largest<ORDER_LOW<DT>>(order, k);
+        int above = 0, equal = 0;
+#pragma unroll
+        for (int i = 0; i < RUNS / 32; ++i) {
+            above += order[i] > bound;
+            equal += order[i] == bound;
         }
-        for (int o = 1; o < parts; o <<= 1) above += __shfl_xor_sync(FULL, above, o);
-        if (part == 0 && above == k - 1) z.least = key;
+        above = __reduce_add_sync(FULL, above);
+        equal = __reduce_add_sync(FULL, equal);
+        uint32_t place = 0;  // 2^32 - 1 - index from which an element at the bound counts
+        if (bound && above < k && above + equal > 2 * k + 32) {
+            uint32_t at[RUNS / 32];
+#pragma unroll
+            for (int i = 0; i < RUNS / 32; ++i) at[i] = order[i] == bound ? 0xFFFFFFFFu - (uint32_t)z.run_last[i * 32 + t] : 0u;
+            place = kth_largest<0>(at, k - above);
+        }
+        if (t == 0) z.least = ((unsigned long long)bound << 32) | place;
     }
     __syncthreads();
     unsigned long long least = z.least;
-    if (!exact && mine >= least)
-        each<DT, NT>(row, cut, [&](float x, int i) {
+    if (!exact) {
+        auto candidate = [&](float x, int i) {
             const unsigned long long key = order_key(x, i);
             if (key >= least) {
                 const int at = atomicAdd(&z.count, 1);
                 if (at < CAP) z.keys[at] = key;
             }
-        });
+        };
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            const unsigned long long mine = ((unsigned long long)z.run_order[u * NT + t] << 32) | (0xFFFFFFFFu - (uint32_t)last[u]);
+            if (last[u] >= 0 && mine >= least) z.look[atomicAdd(&z.looks, 1)] = u * NT + t;
+        }
+        if (t < cut.head) candidate(load1<DT>(row, t), t);
+        if (t < cut.tail) candidate(load1<DT>(row, cut.tail_at + t), cut.tail_at + t);
+        __syncthreads();
+        const uint4* q = cut.vectors(row);
+        constexpr int STRIDE = SUB == 1 ? NT : NT * AHEAD;
+        const int looks = z.looks, per = (cut.nvec + STRIDE - 1) / STRIDE, items = looks * per;
+        const uint32_t bound = (uint32_t)(least >> 32);
+        const float floor = bound > ORDER_NEG_INF ? order_value(bound) : -INFINITY;
+        for (int i0 = t; i0 < items; i0 += NT * AHEAD) {
+            uint4 raw[AHEAD];
+            int at[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int i = i0 + u * NT;
+                at[u] = cut.nvec;
+                if (i < items) {
+                    const int round = i / looks;
+                    at[u] = z.look[i - round * looks] + round * STRIDE;
+                }
+                if (at[u] < cut.nvec) raw[u] = __ldg(q + at[u]);
+            }
+            uint32_t hits = 0;  // bit u N + j: element j of vector u reaches the bound's value
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                if (at[u] >= cut.nvec) continue;
+                float x[N];
+                unpack<DT>(raw[u], x);
+#pragma unroll
+                for (int j = 0; j < N; ++j) hits |= (uint32_t)(x[j] >= floor) << (u * N + j);
+            }
+            if (!hits) continue;
+            int to = atomicAdd(&z.count, __popc(hits));
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                if (!((hits >> (u * N)) & ((1u << N) - 1))) continue;
+                float x[N];
+                unpack<DT>(raw[u], x);
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    if (!((hits >> (u * N + j)) & 1)) continue;
+                    // those beyond the bound by their index stay out of the order (key 0)
+                    const unsigned long long key = order_key(x[j], cut.at(at[u]) + j);
+                    if (to < CAP) z.keys[to] = key >= least ? key : 0;
+                    ++to;
+                }
+            }
+        }
+    }
     __syncthreads();
-    int count = z.count;
-    if (exact || count > CAP) {
+    if (exact || z.count > CAP) {
         __syncthreads();
         if (t == 0) {
             z.least = 0;
-            z.need = min(k, n);
+            z.need = k;
             z.count = 0;
         }
         for (int shift = 56; shift >= 0; shift -= 8) {
@@ -406,33 +554,46 @@ __device__ int top_of(const void* row, const Cut<DT>& cut, int n, int k, unsigne
             }
         });
         __syncthreads();
-        count = min(z.count, CAP);
     }
-    // Sorted by counting: `lanes` threads share a candidate.  (Keys are distinct.)
-    int lanes = 1;
-    while (lanes < 32 && count * lanes * 2 <= NT) lanes *= 2;
-    for (int i0 = 0; i0 < count; i0 += NT / lanes) {
-        const int i = i0 + t / lanes;
-        const unsigned long long key = i < count ? z.keys[i] : 0;
-        int above = 0;
-        for (int j = t % lanes; j < count; j += lanes) above += z.keys[j] > key;
-        for (int o = 1; o < lanes; o <<= 1) above += __shfl_xor_sync(FULL, above, o);
-        if (i < count && t % lanes == 0 && above < k) z.best[above] = key;
+    sort_keys<NT>(k, z);
+}
+
+// What a block knows of its part of a row; the first block of a row's cluster
+// joins its fellows' through distributed shared memory.
+struct PartOut {
+    float m, s, w;
+};
+__device__ __forceinline__ void join_parts(cooperative_groups::cluster_group& cluster, int of, PartOut& mine, float c,
+                                           float& m, float& s, float& w) {
+    PartOut all[MAX_PARTS];
+#pragma unroll
+    for (int i = 0; i < MAX_PARTS; ++i) {
+        all[i] = {LOWEST, 0.f, 0.f};
+        if (i < of) all[i] = *cluster.map_shared_rank(&mine, i);
+        m = fmaxf(m, all[i].m);
     }
-    __syncthreads();
-    return min(count, k);
+    s = w = 0.f;
+#pragma unroll
+    for (int i = 0; i < MAX_PARTS; ++i) {
+        const float by = fmaxf((all[i].m - m) * c, D_MIN), f = ex2(by);
+        s += all[i].s * f;
+        w += fmaf(all[i].s, by, all[i].w) * f;
+    }
 }
 
 template <int DT, int NT, bool TOP>
 __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a) {
     __shared__ JoinSlots<NT> slots;
-    __shared__ typename std::conditional<TOP, TopSlots<NT>, int>::type top_slots;
+    __shared__ PartOut mine;
+    __shared__ typename std::conditional<TOP, TopSlots, int>::type top_slots;
     const int t = threadIdx.x;
-    const int64_t r = blockIdx.x;
+    const int of = a.parts, which = of > 1 ? blockIdx.x % of : 0;
+    const int64_t r = of > 1 ? blockIdx.x / of : blockIdx.x;
     int64_t target = -1;
     if (a.targets) {
         target = load_index(a.targets, r, a.target_bytes);
         if (target == a.ignore) {  // the row is left out: nothing of it is read
+            if (which) return;
             if (t == 0) {
                 a.logp[r] = 0.f;
                 a.entropy[r] = 0.f;
@@ -447,21 +608,37 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a)
         }
     }
     const void* row = reinterpret_cast<const typename Elt<DT>::bits*>(a.logits) + a.map.at(r);
-    const Cut<DT> cut(row, a.vocab);
+    const Cut<DT> cut(row, a.vocab, which, of);
     const float c = a.inv_t * LOG2E;
     Soft soft;
-    float top = -INFINITY;
-    int top_at = 0x7fffffff;
-    stream<DT, NT>(row, cut, c, soft, [](float*, int, auto) {}, [&](float x, int last) {
-        if (TOP && x > top) {
-            top = x;
-            top_at = last;
+    constexpr int SUB = TOP ? RUNS / NT : 1;
+    float top[SUB];
+    int last[SUB];  // -1: an empty run
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+        top[u] = -INFINITY;
+        last[u] = -1;
+    }
+    stream<DT, NT>(row, cut, c, soft, [](float*, int, auto) {}, [&](auto place, float x, int end) {
+        if constexpr (TOP) {
+            constexpr int u = SUB == 1 ? 0 : decltype(place)::value;
+            if (x > top[u] || last[u] < 0) {
+                top[u] = x;
+                last[u] = end;
+            }
         }
     });
     float m, s, w;
     join<NT>(soft, c, slots, m, s, w);
+    if constexpr (TOP) top_of<DT, NT>(row, cut, a.top_k, top, last, s != s, top_slots);
+    if (of > 1) {
+        cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        if (t == 0) mine = {m, s, w};
+        cluster.sync();
+        if (which == 0) join_parts(cluster, of, mine, c, m, s, w);
+    }
     const float ln_s = s == 0.f ? -INFINITY : logf(s);
-    if (t == 0) {
+    if (which == 0 && t == 0) {
         if (a.targets) {
             float lp = NAN;
             if (target >= 0 && target < a.vocab)
@@ -475,20 +652,42 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a)
         a.stats[2 * r + 1] = s;
     }
     if constexpr (TOP) {
-        // A thread that saw nothing above -inf brings its first element's place;
-        // one without elements the lowest key.
-        const int first = t < cut.head ? t : t < cut.nvec ? cut.head + t * Row<DT>::N + Row<DT>::N - 1
-                        : t < cut.tail ? cut.head + cut.nvec * Row<DT>::N + t : 0x7fffffff;
-        const unsigned long long mine =
-            top > -INFINITY ? order_key(top, top_at) : first != 0x7fffffff ? order_key(-INFINITY, first) : 0ull;
-        const int k = top_of<DT, NT>(row, cut, a.vocab, a.top_k, mine, s != s, top_slots);
-        for (int i = t; i < k; i += NT) {
-            const unsigned long long key = top_slots.best[i];
+        auto put = [&](int i, unsigned long long key) {
             const float x = order_value((uint32_t)(key >> 32));
             a.top_ids[r * a.top_k + i] = 0xFFFFFFFFu - (uint32_t)key;
             a.top_logp[r * a.top_k + i] = s == 0.f ? -INFINITY : (x - m) * a.inv_t - ln_s;
+        };
+        if (of == 1) {
+            for (int i = t; i < a.top_k; i += NT) put(i, top_slots.best[i]);
+        } else if (which == 0) {
+            // The parts' sorted lists: with the ceil(k / of)-th key of each at or above
+            // the least of those, k keys are; only such keys are sorted again.
+            cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+            const int k = a.top_k, deep = (k + of - 1) / of - 1;
+            unsigned long long least = ~0ull;
+            if ((t & 31) < of) {
+                const TopSlots* from = cluster.map_shared_rank(&top_slots, t & 31);
+                least = from->found > deep ? from->best[deep] : 0;
+            }
+#pragma unroll
+            for (int o = MAX_PARTS / 2; o; o >>= 1) least = min(least, __shfl_xor_sync(FULL, least, o));
+            least = __shfl_sync(FULL, least, 0);
+            if (t == 0) top_slots.count = 0;
+            __syncthreads();
+            for (int i = t; i < MAX_PARTS * TOP_MAX; i += NT) {
+                const int l = i / TOP_MAX, j = i % TOP_MAX;
+                if (l >= of || j >= k) continue;
+                const TopSlots* from = cluster.map_shared_rank(&top_slots, l);
+                if (j >= from->found) continue;
+                const unsigned long long key = from->best[j];
+                if (key >= least) top_slots.keys[atomicAdd(&top_slots.count, 1)] = key;
+            }
+            __syncthreads();
+            sort_keys<NT>(k, top_slots);
+            for (int i = t; i < k; i += NT) put(i, top_slots.best[i]);
         }
     }
+    if (of > 1) cooperative_groups::this_cluster().sync();  // nobody leaves while the first block reads
 }
 
 struct ScoreBwdArgs {
@@ -670,6 +869,7 @@ struct DistillArgs {
     float* loss;
     float* stats;  // [rows, 4]: m, s, the factor off the list, ln of renorm's sum or bucket's Q
     uint32_t* status;
+    int parts;
 };
 
 // A listed mass this near to one leaves no rest: less is the scores' own rounding.
@@ -679,67 +879,83 @@ template <int DT, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArgs a) {
     using bits = typename Elt<DT>::bits;
     constexpr int N = Row<DT>::N;
-    extern __shared__ uint32_t on_list[];  // bucket: a bit per class, shifted so that vectors start whole
+    extern __shared__ uint32_t on_list[];  // bucket: a bit for each class of this block's part
     __shared__ float slots[NT / 32];
     __shared__ JoinSlots<NT> join_slots;
+    __shared__ PartOut mine;
     __shared__ int ids[TOP_MAX];
+    static_assert(NT >= TOP_MAX, "one entry a thread");
     const int t = threadIdx.x;
-    const int64_t r = blockIdx.x;
+    const int of = a.parts, which = of > 1 ? blockIdx.x % of : 0;
+    const int64_t r = of > 1 ? blockIdx.x / of : blockIdx.x;
     const bits* row = reinterpret_cast<const bits*>(a.logits) + a.map.at(r);
-    const Cut<DT> cut(row, a.vocab);
+    const Cut<DT> cut(row, a.vocab, which, of);
     const float c = a.inv_t * LOG2E;
 
     // The list: one entry a thread (threads past it hold none).
     int id = -1;
-    float score = -INFINITY;
+    float score = -INFINITY, x = 0.f;
     if (t < a.k) {
         const int64_t j = load_index(a.ids, r * a.k + t, a.id_bytes);
         if (j >= 0 && j < a.vocab) {
             id = (int)j;
             score = load_code(a.scores, r * a.k + t, a.score_code);
-        } else if (j != -1) {
+            x = Elt<DT>::to_f(row[id]);
+        } else if (j != -1 && which == 0) {
             atomicOr(a.status, SFFN_STATUS_BAD_INDEX);
         }
         ids[t] = id;
     }
+    // Bits of the part's listed classes, shifted so that a vector's lie in one word.
+    const int pad = (N - cut.lead % N) % N;
+    const int base = (cut.begin() + pad) & ~31;
+    if (a.bucket)
+        for (int i = t; i < (cut.end() + pad - base + 31) / 32; i += NT) on_list[i] = 0;
     const float top = block_max<NT>(score, slots);
     const float z = block_sum<NT>(id >= 0 && score != -INFINITY ? expf(score - (a.bucket ? 0.f : top)) : 0.f, slots);
-    if (z == 0.f) {  // no entry of positive weight
-        if (t == 0) {
+    if (z == 0.f) {  // no entry of positive weight (every block of the row sees the same)
+        if (t == 0 && which == 0) {
             a.loss[r] = 0.f;
             for (int i = 0; i < 4; ++i) a.stats[4 * r + i] = 0.f;
         }
         return;
     }
-    const float ln_z = a.bucket ? 0.f : top + logf(z);
-    const float ln_q = score - ln_z;
-    const float q = id >= 0 ? expf(ln_q) : 0.f;
-
-    // bits of the classes on the list
-    const int pad = (N - cut.head % N) % N;
-    bool first = id >= 0, all_listed = false;
     if (a.bucket) {
-        for (int i = t; i < (a.vocab + pad + 31) / 32; i += NT) on_list[i] = 0;
+        if (id >= cut.begin() && id < cut.end()) atomicOr(&on_list[(id + pad - base) >> 5], 1u << ((id + pad - base) & 31));
         __syncthreads();
-        if (id >= 0) atomicOr(&on_list[(id + pad) >> 5], 1u << ((id + pad) & 31));
-        for (int i = 0; i < t && i < a.k && first; ++i) first = ids[i] != id;
-        all_listed = __syncthreads_count(first) == a.vocab;
     }
     Soft soft;
-    stream<DT, NT>(row, cut, c, soft, [&](float* x, int i, auto count) {
+    stream<DT, NT>(row, cut, c, soft, [&](float* v, int i, auto count) {
         if (!a.bucket) return;
         constexpr int n = decltype(count)::value;
-        const uint32_t on = on_list[(i + pad) >> 5] >> ((i + pad) & 31);
+        const uint32_t on = on_list[(i + pad - base) >> 5] >> ((i + pad - base) & 31);
         if (on & ((1u << n) - 1)) {
 #pragma unroll
             for (int j = 0; j < n; ++j)
-                if ((on >> j) & 1) x[j] = -INFINITY;
+                if ((on >> j) & 1) v[j] = -INFINITY;
         }
-    }, [](float, int) {});
-    float m, s, w, off = 0.f;
+    }, [](auto, float, int) {});
+    float m, s, w;
     join<NT>(soft, c, join_slots, m, s, w);
-    const float x = id >= 0 ? Elt<DT>::to_f(row[id]) : 0.f;
+    if (of > 1) {
+        cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        if (t == 0) mine = {m, s, w};
+        cluster.sync();
+        if (which == 0) join_parts(cluster, of, mine, c, m, s, w);
+        cluster.sync();
+        if (which) return;
+    }
+
+    const float ln_z = a.bucket ? 0.f : top + logf(z);
+    const float ln_q = score - ln_z;
+    const float q = id >= 0 ? expf(ln_q) : 0.f;
+    float off = 0.f;
+    bool all_listed = false;
     if (a.bucket) {
+        bool first = id >= 0;  // an id that stands twice is one class
+#pragma unroll 8
+        for (int i = 0; i < a.k; ++i) first &= !(i < t && ids[i] == id);
+        all_listed = __syncthreads_count(first) == a.vocab;
         const float m_off = m, s_off = s;
         m = block_max<NT>(id >= 0 ? fmaxf(x, m_off) : m_off, slots);
         off = s_off * ex2(fmaxf((m_off - m) * c, D_MIN));
@@ -844,6 +1060,39 @@ int64_t bwd_per(int64_t rows, int64_t vocab) {
     return vocab < per ? vocab : per;
 }
 
+// How a forward row is shared out.  With rows enough for eight blocks of 128 an
+// SM, one block takes a row: small blocks at different points of their rows keep
+// memory busy where one large block would wait for its own end.  With fewer, a
+// cluster of up to eight blocks takes it, each a part of at least 2048 elements;
+// where even those leave SMs half idle and a thread more than four vectors to
+// read, the blocks have 512 threads.
+struct Plan {
+    int threads, parts;
+};
+Plan plan_rows(int64_t rows, int64_t vocab, int dtype) {
+    int parts = 1;
+    while (parts < MAX_PARTS && rows * parts * 2 <= (int64_t)SMS * 8 && vocab / (parts * 2) >= 2048) parts *= 2;
+    const int64_t vectors = vocab * esize_of(dtype) / 16 / parts;
+    return {rows * parts <= 2 * SMS && vectors > 4 * 128 ? 512 : 128, parts};
+}
+
+// Launches kernel over rows x parts blocks, the parts of a row as a cluster.
+template <class Args>
+cudaError_t launch_rows(void (*kernel)(Args), const Plan& p, int64_t rows, size_t smem, cudaStream_t st, const Args& a) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * p.parts));
+    cfg.blockDim = dim3((unsigned)p.threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.parts;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = p.parts > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
 #define SFFN_BY_DTYPE(dtype, CALL)                                  \
     do {                                                            \
         if (dtype == SFFN_F32) { CALL(SFFN_F32); }                  \
@@ -869,12 +1118,14 @@ extern "C" int sffn_token_logprobs(const void* logits, int dtype, int64_t rows, 
     if (!entropy || !stats || !status_dev || (targets && !logp) || (top_k && (!top_ids || !top_logp)))
         return SFFN_ERR_ARG;
     SFFN_BIND(scope, logits);
+    const Plan p = plan_rows(rows, vocab, dtype);
     const ScoreArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, targets, target_bytes, ignore_index,
-                      top_k, inv_t, logp, entropy, stats, top_ids, top_logp, status_dev};
+                      top_k, inv_t, logp, entropy, stats, top_ids, top_logp, status_dev, p.parts};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define SFFN_CALL(DT)                                                    \
-    if (top_k) score_kernel<DT, 512, true><<<(unsigned)rows, 512, 0, st>>>(a); \
-    else score_kernel<DT, 512, false><<<(unsigned)rows, 512, 0, st>>>(a)
+#define SFFN_CALL(DT)                                                                             \
+    SFFN_CUDA_TRY(launch_rows(p.threads == 512 ? (top_k ? score_kernel<DT, 512, true> : score_kernel<DT, 512, false>) \
+                                               : (top_k ? score_kernel<DT, 128, true> : score_kernel<DT, 128, false>), \
+                              p, rows, 0, st, a))
     SFFN_BY_DTYPE(dtype, SFFN_CALL);
 #undef SFFN_CALL
     SFFN_CHECK_LAUNCH();
@@ -930,17 +1181,19 @@ extern "C" int sffn_distill_topk(const void* logits, int dtype, int64_t rows, in
     if (int rc = check_list(ids, id_bytes, scores, score_dtype, k, tail)) return rc;
     if (!loss || !stats || !status_dev) return SFFN_ERR_ARG;
     const int bucket = tail == SFFN_TAIL_BUCKET;
-    const size_t smem = bucket ? ((size_t)vocab + 8 + 31) / 32 * 4 : 0;
-    if (smem > 200 * 1024) return SFFN_ERR_TOO_LARGE;
+    if (bucket && vocab > 1600000) return SFFN_ERR_TOO_LARGE;
+    const Plan p = plan_rows(rows, vocab, dtype);
+    // a bit for every class of a part: a vector more than its share, shifted by up to 31 + 7 bits
+    const size_t smem = bucket ? ((size_t)vocab / p.parts + 64 + 31) / 32 * 4 : 0;
     SFFN_BIND(scope, logits);
     const DistillArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, ids, id_bytes, scores, score_dtype,
-                        k, bucket, inv_t, loss, stats, status_dev};
+                        k, bucket, inv_t, loss, stats, status_dev, p.parts};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define SFFN_CALL(DT)                                                                                          \
-    if (smem > 32 * 1024)                                                                                      \
-        SFFN_CUDA_TRY(cudaFuncSetAttribute(distill_kernel<DT, 512>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
-                                           200 * 1024));                                                       \
-    distill_kernel<DT, 512><<<(unsigned)rows, 512, smem, st>>>(a)
+#define SFFN_CALL(DT)                                                                                    \
+    auto* kernel = p.threads == 512 ? distill_kernel<DT, 512> : distill_kernel<DT, 128>;                  \
+    if (smem > 32 * 1024)                                                                                \
+        SFFN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)); \
+    SFFN_CUDA_TRY(launch_rows(kernel, p, rows, smem, st, a))
     SFFN_BY_DTYPE(dtype, SFFN_CALL);
 #undef SFFN_CALL
     SFFN_CHECK_LAUNCH();
