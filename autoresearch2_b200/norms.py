@@ -89,7 +89,7 @@ def _backward(x, y, pre, post, gate, groups, post_norm, scale, out_dtype, stats,
     pre, post, gate, dx_new, dh = (t.contiguous() if t is not None else None for t in (pre, post, gate, dx_new, dh))
     ws = None
     if any(g is not None for g in grads):
-        per = rows // groups if grads[2] is not None else 0
+        per = rows // groups if grads[1] is not None or grads[2] is not None else 0
         ws = _lib.workspace(_lib.load().sffn_residual_norm_bwd_workspace_bytes(rows, width, per), dev)
     call("sffn_residual_norm_bwd", ptr(x2), _lib.dtype_code(x), x2.stride(0), ptr(y2),
          _lib._DTYPES[out_dtype], y2.stride(0) if y2 is not None else 0, rows, width, ptr(pre), _code(pre),

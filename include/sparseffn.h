@@ -609,7 +609,7 @@ int sffn_residual_norm(const void* x, int x_dtype, int64_t x_ld, const void* y, 
                        void* x_new, void* h, float* stats, void* stream);
 
 /* Scratch of the backward when a weight's or gate's gradient is wanted
- * (gate_rows 0: not the gate's). */
+ * (gate_rows 0: no gate, or neither its gradient nor post's is wanted). */
 size_t sffn_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t width, int64_t gate_rows);
 
 /* Every gradient, from dx_new and dh (contiguous; NULL for zero): dx, dy of x's
