@@ -230,10 +230,28 @@ def stream_ptr(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def address(t):
+    """A tensor's address as the integer that ctypes takes for a pointer (None: NULL)."""
+    return t.data_ptr() if t is not None else None
+
+
+def stream_handle(device):
+    """The handle of the device's current stream, without the Stream object
+    around it that stream_ptr makes (a tenth of its time)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def require_cuda(*tensors):
     for t in tensors:
         if not (isinstance(t, torch.Tensor) and t.is_cuda):
             raise ValueError("autoresearch2_b200 runs on CUDA tensors only (no CPU path)")
+
+
+def once_differentiable(name):
+    """Called by a backward: refuses to run under create_graph=True, where the
+    gradient would look like a constant."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"the gradient of {name} is not differentiable again")
 
 
 # Sticky per-device status word: kernels OR SFFN_STATUS_* bits into it.

@@ -341,10 +341,11 @@ constexpr int MAX_PARTS = 8;
 // largest element above which little lies: 1.15 k elements of a shuffled row for
 // k = 128.  One warp finds it, a bit of the order at a time; with many ties at
 // the bound the index decides, also a bit at a time, so that a row of equal
-// elements leaves about 8 k candidates.  Only the runs whose maximum reaches the bound are
-// read again, from L2, by all threads together.  Where more than CAP elements
-// reach it (the largest lie in few runs) or a NaN hides from the maxima, the
-// k-th largest key is found exactly, eight bits a pass over the part.
+// elements leaves about 8 k candidates.  Where a run's maximum reaches the bound
+// the vector that holds it is read again, from L2, and all of the run where the
+// largest of its other vectors (`second`) does too.  Where more than CAP elements
+// reach it (the largest lie in few runs) or a NaN hides from the maxima, the k-th
+// largest key is found exactly, eight bits a pass over the part.
 constexpr int CAP = 1280;
 constexpr int RUNS = 512;
 struct TopSlots {
@@ -352,10 +353,10 @@ struct TopSlots {
     unsigned long long best[TOP_MAX];
     uint32_t run_order[RUNS];
     int run_last[RUNS];
-    int look[RUNS];  // runs read again
+    int look[RUNS];  // read again: vectors from the front, runs from the back
     int hist[256];
     unsigned long long least;
-    int looks, count, need, found;
+    int vectors, runs, count, need, found;
 };
 
 // A value v with at least `need` of the warp's keys (PER a lane) >= v: the
@@ -395,8 +396,8 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[PER], int 
 template <int DT> constexpr int ORDER_LOW = DT == SFFN_F32 ? 0 : DT == SFFN_BF16 ? 16 : 13;
 constexpr uint32_t ORDER_NEG_INF = 0x007FFFFFu;  // order_bits(-inf), the lowest
 
-// The k largest of z.keys[0 .. z.count) (0: no key; the others distinct), sorted
-// into z.best by counting the larger ones of each; z.found of them.
+// The k largest of z.keys[0 .. z.count), which are distinct, sorted into z.best by
+// counting the larger ones of each; z.found of them.
 template <int NT>
 __device__ __forceinline__ void sort_keys(int k, TopSlots& z) {
     const int t = threadIdx.x, count = z.count;
@@ -410,7 +411,7 @@ __device__ __forceinline__ void sort_keys(int k, TopSlots& z) {
 #pragma unroll 4
         for (int j = t % lanes; j < count; j += lanes) above += z.keys[j] > key;
         for (int o = 1; o < lanes; o <<= 1) above += __shfl_xor_sync(FULL, above, o);
-        if (key && t % lanes == 0 && above < k) {
+        if (i < count && t % lanes == 0 && above < k) {
             z.best[above] = key;
             most = max(most, above + 1);
         }
@@ -422,7 +423,8 @@ __device__ __forceinline__ void sort_keys(int k, TopSlots& z) {
 
 template <int DT, int NT>
 __device__ __forceinline__ void top_of(const void* row, const Cut<DT>& cut, int k, const float (&top)[RUNS / NT],
-                                       const int (&last)[RUNS / NT], bool exact, TopSlots& z) {
+                                       const float (&second)[RUNS / NT], const int (&last)[RUNS / NT], bool exact,
+                                       TopSlots& z) {
     constexpr int N = Row<DT>::N, SUB = RUNS / NT;
     const int t = threadIdx.x;
     // Runs: NT > 128 has one a thread; NT = 128 one for each place u of AHEAD.
@@ -432,7 +434,7 @@ __device__ __forceinline__ void top_of(const void* row, const Cut<DT>& cut, int 
         z.run_order[u * NT + t] = any ? order_bits(top[u]) : 0u;
         z.run_last[u * NT + t] = last[u];
     }
-    if (t == 0) z.count = z.looks = z.found = 0;
+    if (t == 0) z.count = z.vectors = z.runs = z.found = 0;
     __syncthreads();
     if (t < 32 && !exact) {
         uint32_t order[RUNS / 32];
@@ -459,26 +461,29 @@ __device__ __forceinline__ void top_of(const void* row, const Cut<DT>& cut, int 
     __syncthreads();
     unsigned long long least = z.least;
     if (!exact) {
-        auto candidate = [&](float x, int i) {
-            const unsigned long long key = order_key(x, i);
-            if (key >= least) {
-                const int at = atomicAdd(&z.count, 1);
-                if (at < CAP) z.keys[at] = key;
-            }
+        const uint32_t bound = (uint32_t)(least >> 32), place = (uint32_t)least;
+        const float floor = bound > ORDER_NEG_INF ? order_value(bound) : -INFINITY;
+        auto reaches = [&](float x, int i) { return x > floor || (x == floor && 0xFFFFFFFFu - (uint32_t)i >= place); };
+        auto single = [&](int i) {
+            const float x = load1<DT>(row, i);
+            if (!reaches(x, i)) return;
+            const int to = atomicAdd(&z.count, 1);
+            if (to < CAP) z.keys[to] = order_key(x, i);
         };
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
             const unsigned long long mine = ((unsigned long long)z.run_order[u * NT + t] << 32) | (0xFFFFFFFFu - (uint32_t)last[u]);
-            if (last[u] >= 0 && mine >= least) z.look[atomicAdd(&z.looks, 1)] = u * NT + t;
+            if (last[u] < 0 || mine < least) continue;
+            const int v = last[u] - cut.at(0);
+            if (second[u] >= floor) z.look[RUNS - 1 - atomicAdd(&z.runs, 1)] = u * NT + t;
+            else if (v >= 0 && v < cut.nvec * N) z.look[atomicAdd(&z.vectors, 1)] = v / N;
         }
-        if (t < cut.head) candidate(load1<DT>(row, t), t);
-        if (t < cut.tail) candidate(load1<DT>(row, cut.tail_at + t), cut.tail_at + t);
+        if (t < cut.head) single(t);
+        if (t < cut.tail) single(cut.tail_at + t);
         __syncthreads();
         const uint4* q = cut.vectors(row);
         constexpr int STRIDE = SUB == 1 ? NT : NT * AHEAD;
-        const int looks = z.looks, per = (cut.nvec + STRIDE - 1) / STRIDE, items = looks * per;
-        const uint32_t bound = (uint32_t)(least >> 32);
-        const float floor = bound > ORDER_NEG_INF ? order_value(bound) : -INFINITY;
+        const int per = (cut.nvec + STRIDE - 1) / STRIDE, vectors = z.vectors, items = vectors + z.runs * per;
         for (int i0 = t; i0 < items; i0 += NT * AHEAD) {
             uint4 raw[AHEAD];
             int at[AHEAD];
@@ -486,20 +491,22 @@ __device__ __forceinline__ void top_of(const void* row, const Cut<DT>& cut, int 
             for (int u = 0; u < AHEAD; ++u) {
                 const int i = i0 + u * NT;
                 at[u] = cut.nvec;
-                if (i < items) {
-                    const int round = i / looks;
-                    at[u] = z.look[i - round * looks] + round * STRIDE;
+                if (i < vectors) {
+                    at[u] = z.look[i];
+                } else if (i < items) {
+                    const int run = (i - vectors) / per;
+                    at[u] = z.look[RUNS - 1 - run] + (i - vectors - run * per) * STRIDE;
                 }
                 if (at[u] < cut.nvec) raw[u] = __ldg(q + at[u]);
             }
-            uint32_t hits = 0;  // bit u N + j: element j of vector u reaches the bound's value
+            uint32_t hits = 0;  // bit u N + j: element j of vector u
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 if (at[u] >= cut.nvec) continue;
                 float x[N];
                 unpack<DT>(raw[u], x);
 #pragma unroll
-                for (int j = 0; j < N; ++j) hits |= (uint32_t)(x[j] >= floor) << (u * N + j);
+                for (int j = 0; j < N; ++j) hits |= (uint32_t)reaches(x[j], cut.at(at[u]) + j) << (u * N + j);
             }
             if (!hits) continue;
             int to = atomicAdd(&z.count, __popc(hits));
@@ -511,9 +518,7 @@ __device__ __forceinline__ void top_of(const void* row, const Cut<DT>& cut, int 
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
                     if (!((hits >> (u * N + j)) & 1)) continue;
-                    // those beyond the bound by their index stay out of the order (key 0)
-                    const unsigned long long key = order_key(x[j], cut.at(at[u]) + j);
-                    if (to < CAP) z.keys[to] = key >= least ? key : 0;
+                    if (to < CAP) z.keys[to] = order_key(x[j], cut.at(at[u]) + j);
                     ++to;
                 }
             }
@@ -612,17 +617,19 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a)
     const float c = a.inv_t * LOG2E;
     Soft soft;
     constexpr int SUB = TOP ? RUNS / NT : 1;
-    float top[SUB];
-    int last[SUB];  // -1: an empty run
+    float top[SUB], second[SUB];  // of each run: the largest vector maximum, the largest of the other vectors'
+    int last[SUB];                // -1: an empty run
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
-        top[u] = -INFINITY;
+        top[u] = second[u] = -INFINITY;
         last[u] = -1;
     }
     stream<DT, NT>(row, cut, c, soft, [](float*, int, auto) {}, [&](auto place, float x, int end) {
         if constexpr (TOP) {
             constexpr int u = SUB == 1 ? 0 : decltype(place)::value;
-            if (x > top[u] || last[u] < 0) {
+            const bool first = last[u] < 0;
+            if (!first) second[u] = fmaxf(second[u], fminf(top[u], x));
+            if (x > top[u] || first) {
                 top[u] = x;
                 last[u] = end;
             }
@@ -630,7 +637,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a)
     });
     float m, s, w;
     join<NT>(soft, c, slots, m, s, w);
-    if constexpr (TOP) top_of<DT, NT>(row, cut, a.top_k, top, last, s != s, top_slots);
+    if constexpr (TOP) top_of<DT, NT>(row, cut, a.top_k, top, second, last, s != s, top_slots);
     if (of > 1) {
         cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
         if (t == 0) mine = {m, s, w};

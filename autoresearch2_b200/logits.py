@@ -17,10 +17,10 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, ptr, stream_ptr
+from ._lib import address as ptr
+from ._lib import call, stream_handle
 
 __all__ = ["TokenLogprobs", "token_logprobs", "distill_topk", "TOP_MAX"]
 
@@ -41,6 +41,9 @@ def _rows(logits):
     """(logits or a copy, rows, inner, s_outer, s_inner): row r starts at
     s_outer * (r // inner) + s_inner * (r % inner)."""
     V = logits.shape[-1]
+    if logits.is_contiguous():
+        rows = logits.numel() // V
+        return logits, rows, rows, 0, V
     if V > 1 and logits.stride(-1) != 1:
         logits = logits.contiguous()
     dims = []  # merged (size, stride) of the leading dimensions
@@ -70,8 +73,8 @@ def _grad_like(logits, rows, s_inner):
     ld = V + (s_inner - V) % n if rows > 1 else V
     at = logits.data_ptr() % 16 // logits.element_size()
     if ld == V and at == 0:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), V
-    flat = torch.empty(at + rows * ld, dtype=logits.dtype, device=logits.device)
+        return logits.new_empty(logits.shape), V
+    flat = logits.new_empty(at + rows * ld)
     strides, step = [1], ld
     for k in reversed(logits.shape[:-1]):
         strides.append(step)
@@ -106,18 +109,18 @@ def _score_forward(logits, targets, top_k, temperature, ignore_index):
     """(logp or an empty tensor, entropy, top_ids, top_logp, stats [..., 2])."""
     dev, lead = logits.device, logits.shape[:-1]
     x, rows, inner, so, si = _rows(logits)
-    f32 = dict(dtype=torch.float32, device=dev)
-    logp = torch.empty(lead if targets is not None else (0,), **f32)
-    entropy = torch.empty(lead, **f32)
-    stats = torch.empty((*lead, 2), **f32)
-    top_ids = torch.empty((*lead, top_k), dtype=torch.int64, device=dev)
-    top_logp = torch.empty((*lead, top_k), **f32)
+    f32 = torch.float32
+    logp = x.new_empty(lead if targets is not None else (0,), dtype=f32)
+    entropy = x.new_empty(lead, dtype=f32)
+    stats = x.new_empty((*lead, 2), dtype=f32)
+    top_ids = x.new_empty((*lead, top_k), dtype=torch.int64)
+    top_logp = x.new_empty((*lead, top_k), dtype=f32)
     if rows:
         t = targets.contiguous() if targets is not None else None
         call("sffn_token_logprobs", ptr(x), _lib.dtype_code(x), rows, x.shape[-1], inner, so, si, ptr(t),
              t.element_size() if t is not None else 0, ignore_index, top_k, 1.0 / temperature,
              ptr(logp), ptr(entropy), ptr(stats), ptr(top_ids), ptr(top_logp), ptr(_lib.status_word(dev)),
-             stream_ptr(dev))
+             stream_handle(dev))
     return logp, entropy, top_ids, top_logp, stats
 
 
@@ -130,7 +133,7 @@ def _score_backward(logits, targets, top_ids, entropy, stats, g_logp, g_entropy,
         call("sffn_token_logprobs_bwd", ptr(x), _lib.dtype_code(x), rows, x.shape[-1], inner, so, si, ptr(t),
              t.element_size() if t is not None else 0, ignore_index, ptr(top_ids), top_ids.shape[-1],
              1.0 / temperature, ptr(stats), ptr(entropy), ptr(g_logp), ptr(g_entropy), ptr(g_top), ptr(grad), ld,
-             stream_ptr(x.device))
+             stream_handle(x.device))
     return grad
 
 
@@ -145,8 +148,8 @@ class _TokenLogprobs(torch.autograd.Function):
         return logp, entropy, top_ids, top_logp
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_logp, g_entropy, _, g_top):
+        _lib.once_differentiable("token_logprobs")
         logits, targets, top_ids, entropy, stats = ctx.saved_tensors
         if targets is None:
             g_logp = None
@@ -189,13 +192,13 @@ def _distill_forward(logits, ids, scores, temperature, tail):
     """(loss, stats [..., 4])."""
     dev, lead = logits.device, logits.shape[:-1]
     x, rows, inner, so, si = _rows(logits)
-    loss = torch.empty(lead, dtype=torch.float32, device=dev)
-    stats = torch.empty((*lead, 4), dtype=torch.float32, device=dev)
+    loss = x.new_empty(lead, dtype=torch.float32)
+    stats = x.new_empty((*lead, 4), dtype=torch.float32)
     if rows:
         ids, scores = ids.contiguous(), scores.contiguous()
         call("sffn_distill_topk", ptr(x), _lib.dtype_code(x), rows, x.shape[-1], inner, so, si, ptr(ids),
              ids.element_size(), ptr(scores), _lib.dtype_code(scores), ids.shape[-1], TAILS[tail],
-             1.0 / temperature, ptr(loss), ptr(stats), ptr(_lib.status_word(dev)), stream_ptr(dev))
+             1.0 / temperature, ptr(loss), ptr(stats), ptr(_lib.status_word(dev)), stream_handle(dev))
     return loss, stats
 
 
@@ -206,7 +209,7 @@ def _distill_backward(logits, ids, scores, stats, g_loss, temperature, tail):
         ids, scores, g_loss = ids.contiguous(), scores.contiguous(), g_loss.contiguous()
         call("sffn_distill_topk_bwd", ptr(x), _lib.dtype_code(x), rows, x.shape[-1], inner, so, si, ptr(ids),
              ids.element_size(), ptr(scores), _lib.dtype_code(scores), ids.shape[-1], TAILS[tail],
-             1.0 / temperature, ptr(stats), ptr(g_loss), ptr(grad), ld, stream_ptr(x.device))
+             1.0 / temperature, ptr(stats), ptr(g_loss), ptr(grad), ld, stream_handle(x.device))
     return grad
 
 
@@ -219,8 +222,8 @@ class _DistillTopk(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_loss):
+        _lib.once_differentiable("distill_topk")
         logits, ids, scores, stats = ctx.saved_tensors
         return _distill_backward(logits, ids, scores, stats, g_loss, *ctx.args), None, None, None, None
 

@@ -15,10 +15,10 @@ whose order of addition is fixed: equal inputs give equal bits.
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, ptr, stream_ptr
+from ._lib import address as ptr
+from ._lib import call, stream_handle
 
 __all__ = ["residual_norm", "WIDTH_MAX"]
 
@@ -62,15 +62,15 @@ def _forward(x, y, pre, post, gate, groups, post_norm, scale, eps, out_dtype, ke
     x2 = _matrix(x, width)
     y2 = _matrix(y, width) if y is not None else None
     rows, dev = x2.shape[0], x.device
-    x_new = torch.empty(x.shape, dtype=x.dtype, device=dev) if y is not None else None
-    h = torch.empty(x.shape, dtype=out_dtype, device=dev)
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=dev) if keep else None
+    x_new = x.new_empty(x.shape) if y is not None else None
+    h = x.new_empty(x.shape, dtype=out_dtype)
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if keep else None
     if rows:
         pre, post, gate = (t.contiguous() if t is not None else None for t in (pre, post, gate))
         call("sffn_residual_norm", ptr(x2), _lib.dtype_code(x), x2.stride(0), ptr(y2), _code(h),
              y2.stride(0) if y2 is not None else 0, rows, width, ptr(pre), _code(pre), ptr(post), _code(post),
              ptr(gate), _code(gate), rows // groups, int(post_norm), scale, eps, ptr(x_new), ptr(h), ptr(stats),
-             stream_ptr(dev))
+             stream_handle(dev))
     return x_new, h, stats
 
 
@@ -80,22 +80,21 @@ def _backward(x, y, pre, post, gate, groups, post_norm, scale, out_dtype, stats,
     x2 = _matrix(x, width)
     y2 = _matrix(y, width) if y is not None else None
     rows, dev = x2.shape[0], x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
-    dy = torch.empty(y.shape, dtype=y.dtype, device=dev) if y is not None and want[1] else None
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if t is not None and w else None
-             for t, w in zip((pre, post, gate), want[2:])]
+    dx = x.new_empty(x.shape) if want[0] else None
+    dy = y.new_empty(y.shape) if y is not None and want[1] else None
+    grads = [t.new_empty(t.shape) if t is not None and w else None for t, w in zip((pre, post, gate), want[2:])]
     if not rows:
         return dx, dy, *(g.zero_() if g is not None else None for g in grads)
     pre, post, gate, dx_new, dh = (t.contiguous() if t is not None else None for t in (pre, post, gate, dx_new, dh))
     ws = None
     if any(g is not None for g in grads):
         per = rows // groups if grads[1] is not None or grads[2] is not None else 0
-        ws = _lib.workspace(_lib.load().sffn_residual_norm_bwd_workspace_bytes(rows, width, per), dev)
+        ws = x.new_empty(_lib.load().sffn_residual_norm_bwd_workspace_bytes(rows, width, per), dtype=torch.uint8)
     call("sffn_residual_norm_bwd", ptr(x2), _lib.dtype_code(x), x2.stride(0), ptr(y2),
          _lib._DTYPES[out_dtype], y2.stride(0) if y2 is not None else 0, rows, width, ptr(pre), _code(pre),
          ptr(post), _code(post), ptr(gate), _code(gate), rows // groups, int(post_norm), scale, ptr(stats),
          ptr(dx_new), ptr(dh), ptr(dx), ptr(dy), *(ptr(g) for g in grads), ptr(ws),
-         ws.numel() if ws is not None else 0, stream_ptr(dev))
+         ws.numel() if ws is not None else 0, stream_handle(dev))
     return dx, dy, *grads
 
 
@@ -109,8 +108,8 @@ class _ResidualNorm(torch.autograd.Function):
         return x_new, h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dx_new, dh):
+        _lib.once_differentiable("residual_norm")
         x, y, pre, post, gate, stats = ctx.saved_tensors
         groups, post_norm, scale, out_dtype = ctx.args
         grads = _backward(x, y, pre, post, gate, groups, post_norm, scale, out_dtype, stats, dx_new, dh,

@@ -107,15 +107,16 @@ def test_row_maps():
     base = torch.empty(4, 6, 30)
     rows = lambda t: logits._rows(t)[1:]  # noqa: E731
     assert rows(base) == (24, 24, 0, 30)
+    assert rows(torch.empty(5)) == (1, 1, 0, 5)
     assert rows(base[..., :20]) == (24, 24, 0, 30)
     assert rows(base[:, 1:]) == (20, 5, 180, 30)
     assert rows(base[:, 2]) == (4, 4, 0, 180)
-    assert rows(base[0, 0]) == (1, 1, 0, 30)
+    assert rows(base[0, 0]) == (1, 1, 0, 30) and rows(base[0, 0, :7]) == (1, 1, 0, 7)
     assert rows(base.transpose(0, 1)) == (24, 4, 30, 180)
     assert rows(base[:1].expand(4, 6, 30)) == (24, 6, 0, 30)
     assert rows(base.transpose(1, 2)) == (120, 120, 0, 6)  # copied
     assert rows(torch.empty(2, 3, 4, 50)[:, :2, 1:, :7]) == (12, 12, 0, 7)  # three strides: copied
-    assert rows(torch.empty(0, 5)) == (0, 0, 0, 5)
+    assert rows(torch.empty(0, 5)) == (0, 0, 0, 5) and rows(torch.empty(3, 0, 9)[..., :5])[0] == 0
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
