@@ -146,11 +146,16 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 }
 
 // The running (m, s, w) of one thread, exponents in units of log 2: c = log2(e) / T.
-// s and w are kept as pairs (even and odd elements).
+// s and w are kept as pairs (even and odd elements).  m need not be the largest
+// element: it is raised only past `limit`, where an exponent would pass SLACK, so
+// after a row's first vector hardly ever; e^d then reaches 2^32, whose sum over
+// any row is far inside float32.
+constexpr float SLACK = 32.0f;
 struct Soft {
-    float m = LOWEST;
+    float m = LOWEST, limit = LOWEST;
     uint64_t s = 0, w = 0;
     __device__ __forceinline__ void raise(float to, float c) {
+        limit = to + SLACK / c;
         const float by = fmaxf((m - to) * c, D_MIN);
         const float f = ex2(by);
         w = mul2(fma2(s, pair(by, by), w), pair(f, f));
@@ -167,7 +172,7 @@ struct Soft {
         w = fma2(e, pair(d0, d1), w);
     }
     __device__ __forceinline__ void one(float x, float c) {
-        if (x > m) raise(x, c);
+        if (x > limit) raise(x, c);
         add(x, -INFINITY, c);
     }
 };
@@ -268,9 +273,9 @@ __device__ __forceinline__ void each(const void* row, const Cut<DT>& cut, F&& f)
 }
 
 // One pass over the part: AHEAD vectors of a thread are loaded before the first
-// is used.  edit(x, index) may replace a vector's elements; seen(u, max, last
-// index) is told each vector's largest (u: its place among the AHEAD; single
-// elements come with u = 0).
+// is used.  edit(x, index) may replace a vector's elements; seen(u, max, which) is
+// told each vector's largest (u: its place among the AHEAD; which: the vector, or
+// -2 - index for a single element, with u = 0).
 constexpr int AHEAD = 4;
 template <int DT, int NT, class Edit, class Seen>
 __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, float c, Soft& soft, Edit&& edit, Seen&& seen) {
@@ -280,7 +285,7 @@ __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, floa
         float x[1] = {load1<DT>(row, i)};
         edit(x, i, std::integral_constant<int, 1>());
         soft.one(x[0], c);
-        seen(std::integral_constant<int, 0>(), x[0], i);
+        seen(std::integral_constant<int, 0>(), x[0], -2 - i);
     };
     if (t < cut.head) single(t);
     const uint4* q = cut.vectors(row);
@@ -299,10 +304,10 @@ __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, floa
             float top = x[0];
 #pragma unroll
             for (int j = 1; j < N; ++j) top = fmaxf(top, x[j]);
-            if (top > soft.m) soft.raise(top, c);
+            if (__any_sync(__activemask(), top > soft.limit) && top > soft.limit) soft.raise(top, c);
 #pragma unroll
             for (int j = 0; j < N; j += 2) soft.add(x[j], x[j + 1], c);
-            seen(place, top, cut.at(v) + N - 1);
+            seen(place, top, v);
         };
         use(std::integral_constant<int, 0>());
         use(std::integral_constant<int, 1>());
@@ -421,42 +426,62 @@ __device__ __forceinline__ void sort_keys(int k, TopSlots& z) {
     __syncthreads();
 }
 
+// One warp's part of top_of: an order key that at least k elements reach, from the
+// maxima of groups of GROUP runs.
+template <int DT, int GROUP>
+__device__ __forceinline__ unsigned long long bound_of(int k, const TopSlots& z) {
+    constexpr int PER = RUNS / GROUP / 32;
+    const int lane = threadIdx.x & 31;
+    uint32_t order[PER], last[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        order[i] = 0;
+        last[i] = 0xFFFFFFFFu;
+#pragma unroll
+        for (int g = 0; g < GROUP; ++g) {
+            const int run = (g * PER + i) * 32 + lane;
+            const uint32_t o = z.run_order[run], l = (uint32_t)z.run_last[run];
+            last[i] = o > order[i] ? l : o == order[i] ? min(last[i], l) : last[i];
+            order[i] = max(order[i], o);
+        }
+    }
+    const uint32_t bound = kth_largest<ORDER_LOW<DT>>(order, k);
+    int above = 0, equal = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        above += order[i] > bound;
+        equal += order[i] == bound;
+    }
+    above = __reduce_add_sync(FULL, above);
+    equal = __reduce_add_sync(FULL, equal);
+    uint32_t place = 0;  // 2^32 - 1 - index from which an element at the bound counts
+    if (bound && above < k && above + equal > 2 * k + 32) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) last[i] = order[i] == bound ? 0xFFFFFFFFu - last[i] : 0u;
+        place = kth_largest<0>(last, k - above);
+    }
+    return ((unsigned long long)bound << 32) | place;
+}
+
 template <int DT, int NT>
 __device__ __forceinline__ void top_of(const void* row, const Cut<DT>& cut, int k, const float (&top)[RUNS / NT],
-                                       const float (&second)[RUNS / NT], const int (&last)[RUNS / NT], bool exact,
+                                       const float (&second)[RUNS / NT], const int (&held)[RUNS / NT], bool exact,
                                        TopSlots& z) {
     constexpr int N = Row<DT>::N, SUB = RUNS / NT;
     const int t = threadIdx.x;
     // Runs: NT > 128 has one a thread; NT = 128 one for each place u of AHEAD.
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
-        const bool any = last[u] >= 0;
-        z.run_order[u * NT + t] = any ? order_bits(top[u]) : 0u;
-        z.run_last[u * NT + t] = last[u];
+        z.run_order[u * NT + t] = held[u] != -1 ? order_bits(top[u]) : 0u;
+        z.run_last[u * NT + t] = held[u] >= 0 ? cut.at(held[u]) + N - 1 : -2 - held[u];
     }
     if (t == 0) z.count = z.vectors = z.runs = z.found = 0;
     __syncthreads();
     if (t < 32 && !exact) {
-        uint32_t order[RUNS / 32];
-#pragma unroll
-        for (int i = 0; i < RUNS / 32; ++i) order[i] = z.run_order[i * 32 + t];
-        const uint32_t bound = kth_largest<ORDER_LOW<DT>>(order, k);
-        int above = 0, equal = 0;
-#pragma unroll
-        for (int i = 0; i < RUNS / 32; ++i) {
-            above += order[i] > bound;
-            equal += order[i] == bound;
-        }
-        above = __reduce_add_sync(FULL, above);
-        equal = __reduce_add_sync(FULL, equal);
-        uint32_t place = 0;  // 2^32 - 1 - index from which an element at the bound counts
-        if (bound && above < k && above + equal > 2 * k + 32) {
-            uint32_t at[RUNS / 32];
-#pragma unroll
-            for (int i = 0; i < RUNS / 32; ++i) at[i] = order[i] == bound ? 0xFFFFFFFFu - (uint32_t)z.run_last[i * 32 + t] : 0u;
-            place = kth_largest<0>(at, k - above);
-        }
-        if (t == 0) z.least = ((unsigned long long)bound << 32) | place;
+        // few alternatives need few maxima: those of groups of four or two runs
+        if (k <= RUNS / 16) z.least = bound_of<DT, 4>(k, z);
+        else if (k <= RUNS / 8) z.least = bound_of<DT, 2>(k, z);
+        else z.least = bound_of<DT, 1>(k, z);
     }
     __syncthreads();
     unsigned long long least = z.least;
@@ -472,11 +497,11 @@ __device__ __forceinline__ void top_of(const void* row, const Cut<DT>& cut, int 
         };
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
-            const unsigned long long mine = ((unsigned long long)z.run_order[u * NT + t] << 32) | (0xFFFFFFFFu - (uint32_t)last[u]);
-            if (last[u] < 0 || mine < least) continue;
-            const int v = last[u] - cut.at(0);
+            const unsigned long long mine =
+                ((unsigned long long)z.run_order[u * NT + t] << 32) | (0xFFFFFFFFu - (uint32_t)z.run_last[u * NT + t]);
+            if (held[u] == -1 || mine < least) continue;
             if (second[u] >= floor) z.look[RUNS - 1 - atomicAdd(&z.runs, 1)] = u * NT + t;
-            else if (v >= 0 && v < cut.nvec * N) z.look[atomicAdd(&z.vectors, 1)] = v / N;
+            else if (held[u] >= 0) z.look[atomicAdd(&z.vectors, 1)] = held[u];
         }
         if (t < cut.head) single(t);
         if (t < cut.tail) single(cut.tail_at + t);
@@ -618,26 +643,25 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a)
     Soft soft;
     constexpr int SUB = TOP ? RUNS / NT : 1;
     float top[SUB], second[SUB];  // of each run: the largest vector maximum, the largest of the other vectors'
-    int last[SUB];                // -1: an empty run
+    int held[SUB];                // the vector that holds it (-2 - index: a single element), -1 in an empty run
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
         top[u] = second[u] = -INFINITY;
-        last[u] = -1;
+        held[u] = u * NT + t < cut.nvec ? u * NT + t : -1;
     }
-    stream<DT, NT>(row, cut, c, soft, [](float*, int, auto) {}, [&](auto place, float x, int end) {
+    stream<DT, NT>(row, cut, c, soft, [](float*, int, auto) {}, [&](auto place, float x, int which_vector) {
         if constexpr (TOP) {
             constexpr int u = SUB == 1 ? 0 : decltype(place)::value;
-            const bool first = last[u] < 0;
-            if (!first) second[u] = fmaxf(second[u], fminf(top[u], x));
-            if (x > top[u] || first) {
+            second[u] = fmaxf(second[u], fminf(top[u], x));
+            if (x > top[u]) {
                 top[u] = x;
-                last[u] = end;
+                held[u] = which_vector;
             }
         }
     });
     float m, s, w;
     join<NT>(soft, c, slots, m, s, w);
-    if constexpr (TOP) top_of<DT, NT>(row, cut, a.top_k, top, second, last, s != s, top_slots);
+    if constexpr (TOP) top_of<DT, NT>(row, cut, a.top_k, top, second, held, s != s, top_slots);
     if (of > 1) {
         cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
         if (t == 0) mine = {m, s, w};
@@ -936,7 +960,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
         if (!a.bucket) return;
         constexpr int n = decltype(count)::value;
         const uint32_t on = on_list[(i + pad - base) >> 5] >> ((i + pad - base) & 31);
-        if (on & ((1u << n) - 1)) {
+        // by vote, so that it stays a branch: few vectors hold a listed class
+        if (__any_sync(__activemask(), (on & ((1u << n) - 1)) != 0)) {
 #pragma unroll
             for (int j = 0; j < n; ++j)
                 if ((on >> j) & 1) v[j] = -INFINITY;
