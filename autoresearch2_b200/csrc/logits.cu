@@ -273,12 +273,14 @@ __device__ __forceinline__ void each(const void* row, const Cut<DT>& cut, F&& f)
 }
 
 // One pass over the part: AHEAD vectors of a thread are loaded before the first
-// is used.  edit(x, index) may replace a vector's elements; seen(u, max, which) is
+// is used.  edit(x, index) may replace elements: a single one, and those of a
+// vector where marks(iteration) has bit u set; seen(u, max, which) is
 // told each vector's largest (u: its place among the AHEAD; which: the vector, or
 // -2 - index for a single element, with u = 0).
 constexpr int AHEAD = 4;
-template <int DT, int NT, class Edit, class Seen>
-__device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, float c, Soft& soft, Edit&& edit, Seen&& seen) {
+template <int DT, int NT, class Marks, class Edit, class Seen>
+__device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, float c, Soft& soft, Marks&& marks, Edit&& edit,
+                                       Seen&& seen) {
     constexpr int N = Row<DT>::N;
     const int t = threadIdx.x;
     auto single = [&](int i) {
@@ -289,18 +291,20 @@ __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, floa
     };
     if (t < cut.head) single(t);
     const uint4* q = cut.vectors(row);
+    int iteration = 0;
     for (int v0 = t; v0 < cut.nvec; v0 += NT * AHEAD) {
         uint4 raw[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
             if (v0 + u * NT < cut.nvec) raw[u] = __ldg(q + v0 + u * NT);
+        const uint32_t marked = marks(iteration++);
         auto use = [&](auto place) {
             constexpr int u = decltype(place)::value;
             const int v = v0 + u * NT;
             if (v >= cut.nvec) return;
             float x[N];
             unpack<DT>(raw[u], x);
-            edit(x, cut.at(v), std::integral_constant<int, N>());
+            if ((marked >> u) & 1) edit(x, cut.at(v), std::integral_constant<int, N>());
             float top = x[0];
 #pragma unroll
             for (int j = 1; j < N; ++j) top = fmaxf(top, x[j]);
@@ -649,7 +653,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a)
         top[u] = second[u] = -INFINITY;
         held[u] = u * NT + t < cut.nvec ? u * NT + t : -1;
     }
-    stream<DT, NT>(row, cut, c, soft, [](float*, int, auto) {}, [&](auto place, float x, int which_vector) {
+    stream<DT, NT>(row, cut, c, soft, [](int) { return 0u; }, [](float*, int, auto) {}, [&](auto place, float x, int which_vector) {
         if constexpr (TOP) {
             constexpr int u = SUB == 1 ? 0 : decltype(place)::value;
             second[u] = fmaxf(second[u], fminf(top[u], x));
@@ -695,24 +699,25 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a)
             // the least of those, k keys are; only such keys are sorted again.
             cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
             const int k = a.top_k, deep = (k + of - 1) / of - 1;
-            unsigned long long least = ~0ull;
-            if ((t & 31) < of) {
-                const TopSlots* from = cluster.map_shared_rank(&top_slots, t & 31);
-                least = from->found > deep ? from->best[deep] : 0;
-            }
-#pragma unroll
-            for (int o = MAX_PARTS / 2; o; o >>= 1) least = min(least, __shfl_xor_sync(FULL, least, o));
-            least = __shfl_sync(FULL, least, 0);
+            int* found = top_slots.look;  // of each part
             if (t == 0) top_slots.count = 0;
+            if (t < of) found[t] = cluster.map_shared_rank(&top_slots, t)->found;
             __syncthreads();
-            for (int i = t; i < MAX_PARTS * TOP_MAX; i += NT) {
-                const int l = i / TOP_MAX, j = i % TOP_MAX;
-                if (l >= of || j >= k) continue;
-                const TopSlots* from = cluster.map_shared_rank(&top_slots, l);
-                if (j >= from->found) continue;
-                const unsigned long long key = from->best[j];
-                if (key >= least) top_slots.keys[atomicAdd(&top_slots.count, 1)] = key;
+            // every part's list of at most 128 keys, several keys a thread in flight
+            constexpr int PER = MAX_PARTS * TOP_MAX / NT;
+            unsigned long long key[PER], least = ~0ull;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int l = (i * NT + t) / TOP_MAX, j = (i * NT + t) % TOP_MAX;
+                key[i] = l < of && j < found[l] ? cluster.map_shared_rank(&top_slots, l)->best[j] : 0;
+                if (l < of && j == deep) top_slots.keys[l] = key[i];
             }
+            __syncthreads();
+            for (int l = 0; l < of; ++l) least = min(least, top_slots.keys[l]);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (key[i] && key[i] >= least) top_slots.keys[atomicAdd(&top_slots.count, 1)] = key[i];
             __syncthreads();
             sort_keys<NT>(k, top_slots);
             for (int i = t; i < k; i += NT) put(i, top_slots.best[i]);
@@ -910,7 +915,9 @@ template <int DT, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArgs a) {
     using bits = typename Elt<DT>::bits;
     constexpr int N = Row<DT>::N;
-    extern __shared__ uint32_t on_list[];  // bucket: a bit for each class of this block's part
+    // bucket: a bit for each class of this block's part, and before them a bit for
+    // each of its vectors, 32 of a thread's to a word
+    extern __shared__ uint32_t marked_vectors[];
     __shared__ float slots[NT / 32];
     __shared__ JoinSlots<NT> join_slots;
     __shared__ PartOut mine;
@@ -937,11 +944,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
         }
         ids[t] = id;
     }
-    // Bits of the part's listed classes, shifted so that a vector's lie in one word.
+    // Classes are shifted so that a vector's bits lie in one word.
     const int pad = (N - cut.lead % N) % N;
     const int base = (cut.begin() + pad) & ~31;
+    const int words = (cut.nvec + 32 * NT - 1) / (32 * NT) * NT;
+    uint32_t* const on_list = marked_vectors + words;
     if (a.bucket)
-        for (int i = t; i < (cut.end() + pad - base + 31) / 32; i += NT) on_list[i] = 0;
+        for (int i = t; i < words + (cut.end() + pad - base + 31) / 32; i += NT) marked_vectors[i] = 0;
     const float top = block_max<NT>(score, slots);
     const float z = block_sum<NT>(id >= 0 && score != -INFINITY ? expf(score - (a.bucket ? 0.f : top)) : 0.f, slots);
     if (z == 0.f) {  // no entry of positive weight (every block of the row sees the same)
@@ -952,21 +961,29 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
         return;
     }
     if (a.bucket) {
-        if (id >= cut.begin() && id < cut.end()) atomicOr(&on_list[(id + pad - base) >> 5], 1u << ((id + pad - base) & 31));
+        if (id >= cut.begin() && id < cut.end()) {
+            atomicOr(&on_list[(id + pad - base) >> 5], 1u << ((id + pad - base) & 31));
+            const int v = (id - cut.at(0)) / N;
+            if (id >= cut.at(0) && v < cut.nvec) atomicOr(&marked_vectors[v / (32 * NT) * NT + v % NT], 1u << (v / NT % 32));
+        }
         __syncthreads();
     }
     Soft soft;
-    stream<DT, NT>(row, cut, c, soft, [&](float* v, int i, auto count) {
-        if (!a.bucket) return;
-        constexpr int n = decltype(count)::value;
-        const uint32_t on = on_list[(i + pad - base) >> 5] >> ((i + pad - base) & 31);
-        // by vote, so that it stays a branch: few vectors hold a listed class
-        if (__any_sync(__activemask(), (on & ((1u << n) - 1)) != 0)) {
+    static_assert(32 % AHEAD == 0, "an iteration's marks lie in one word");
+    stream<DT, NT>(row, cut, c, soft,
+                   [&](int iteration) {
+                       const int i = iteration * AHEAD;
+                       return a.bucket ? marked_vectors[i / 32 * NT + t] >> (i % 32) : 0u;
+                   },
+                   [&](float* v, int i, auto count) {
+                       if (!a.bucket) return;
+                       constexpr int n = decltype(count)::value;
+                       const uint32_t on = on_list[(i + pad - base) >> 5] >> ((i + pad - base) & 31);
 #pragma unroll
-            for (int j = 0; j < n; ++j)
-                if ((on >> j) & 1) v[j] = -INFINITY;
-        }
-    }, [](auto, float, int) {});
+                       for (int j = 0; j < n; ++j)
+                           if ((on >> j) & 1) v[j] = -INFINITY;
+                   },
+                   [](auto, float, int) {});
     float m, s, w;
     join<NT>(soft, c, join_slots, m, s, w);
     if (of > 1) {
@@ -1083,14 +1100,11 @@ int check_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int
     return SFFN_OK;
 }
 
-// Elements of a row that one block of the backward writes: a whole number of
-// 16-byte vectors of any type.
-constexpr int BWD_THREADS = 256;
-int64_t bwd_per(int64_t rows, int64_t vocab) {
-    (void)rows;
-    const int64_t per = 16384;
-    return vocab < per ? vocab : per;
-}
+// The backward's blocks: up to 16384 elements of a row each (a whole number of
+// 16-byte vectors of any type), by 256 threads, or by 128 where that leaves a
+// thread at most 8 vectors: a row of 1024 16-bit logits takes 128 of them.
+constexpr int64_t BWD_PER = 16384;
+int bwd_threads(int64_t per, int dtype) { return per * esize_of(dtype) / 16 <= 8 * 128 ? 128 : 256; }
 
 // How a forward row is shared out.  With rows enough for eight blocks of 128 an
 // SM, one block takes a row: small blocks at different points of their rows keep
@@ -1178,7 +1192,7 @@ extern "C" int sffn_token_logprobs_bwd(const void* logits, int dtype, int64_t ro
     if (!stats || !entropy || !grad || (g_top && top_k && !top_ids)) return SFFN_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(grad) % esize_of(dtype)) return SFFN_ERR_ALIGN;
     SFFN_BIND(scope, logits);
-    const int64_t per = bwd_per(rows, vocab);
+    const int64_t per = vocab < BWD_PER ? vocab : BWD_PER;
     const int64_t blocks = (vocab + per - 1) / per;
     if (blocks > 65535) return SFFN_ERR_TOO_LARGE;
     const ScoreBwdArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, targets, target_bytes, ignore_index,
@@ -1186,7 +1200,9 @@ extern "C" int sffn_token_logprobs_bwd(const void* logits, int dtype, int64_t ro
                          grad_ld, (int)per};
     const dim3 grid((unsigned)rows, (unsigned)blocks);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define SFFN_CALL(DT) score_bwd_kernel<DT, BWD_THREADS><<<grid, BWD_THREADS, 0, st>>>(a)
+#define SFFN_CALL(DT)                                                                \
+    if (bwd_threads(per, dtype) == 128) score_bwd_kernel<DT, 128><<<grid, 128, 0, st>>>(a); \
+    else score_bwd_kernel<DT, 256><<<grid, 256, 0, st>>>(a)
     SFFN_BY_DTYPE(dtype, SFFN_CALL);
 #undef SFFN_CALL
     SFFN_CHECK_LAUNCH();
@@ -1213,10 +1229,13 @@ extern "C" int sffn_distill_topk(const void* logits, int dtype, int64_t rows, in
     if (int rc = check_list(ids, id_bytes, scores, score_dtype, k, tail)) return rc;
     if (!loss || !stats || !status_dev) return SFFN_ERR_ARG;
     const int bucket = tail == SFFN_TAIL_BUCKET;
-    if (bucket && vocab > 1600000) return SFFN_ERR_TOO_LARGE;
+    if (bucket && vocab > 1400000) return SFFN_ERR_TOO_LARGE;
     const Plan p = plan_rows(rows, vocab, dtype);
-    // a bit for every class of a part: a vector more than its share, shifted by up to 31 + 7 bits
-    const size_t smem = bucket ? ((size_t)vocab / p.parts + 64 + 31) / 32 * 4 : 0;
+    // a bit for every class of a part (a vector more than its share, shifted by up
+    // to 31 + 7 bits) and for every vector, in whole words of each thread
+    const int64_t share = vocab / p.parts + 64;
+    const size_t vectors = (share * esize_of(dtype) / 16 + 32 * p.threads) / (32 * p.threads) * p.threads;
+    const size_t smem = bucket ? ((share + 31) / 32 + vectors) * 4 : 0;
     SFFN_BIND(scope, logits);
     const DistillArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, ids, id_bytes, scores, score_dtype,
                         k, bucket, inv_t, loss, stats, status_dev, p.parts};
@@ -1224,7 +1243,7 @@ extern "C" int sffn_distill_topk(const void* logits, int dtype, int64_t rows, in
 #define SFFN_CALL(DT)                                                                                    \
     auto* kernel = p.threads == 512 ? distill_kernel<DT, 512> : distill_kernel<DT, 128>;                  \
     if (smem > 32 * 1024)                                                                                \
-        SFFN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)); \
+        SFFN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
     SFFN_CUDA_TRY(launch_rows(kernel, p, rows, smem, st, a))
     SFFN_BY_DTYPE(dtype, SFFN_CALL);
 #undef SFFN_CALL
@@ -1244,14 +1263,16 @@ extern "C" int sffn_distill_topk_bwd(const void* logits, int dtype, int64_t rows
     if (!stats || !g_loss || !grad) return SFFN_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(grad) % esize_of(dtype)) return SFFN_ERR_ALIGN;
     SFFN_BIND(scope, logits);
-    const int64_t per = bwd_per(rows, vocab);
+    const int64_t per = vocab < BWD_PER ? vocab : BWD_PER;
     const int64_t blocks = (vocab + per - 1) / per;
     if (blocks > 65535) return SFFN_ERR_TOO_LARGE;
     const DistillBwdArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, ids, id_bytes, scores, score_dtype,
                            k, tail == SFFN_TAIL_BUCKET, inv_t, stats, g_loss, grad, grad_ld, (int)per};
     const dim3 grid((unsigned)rows, (unsigned)blocks);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define SFFN_CALL(DT) distill_bwd_kernel<DT, BWD_THREADS><<<grid, BWD_THREADS, 0, st>>>(a)
+#define SFFN_CALL(DT)                                                                  \
+    if (bwd_threads(per, dtype) == 128) distill_bwd_kernel<DT, 128><<<grid, 128, 0, st>>>(a); \
+    else distill_bwd_kernel<DT, 256><<<grid, 256, 0, st>>>(a)
     SFFN_BY_DTYPE(dtype, SFFN_CALL);
 #undef SFFN_CALL
     SFFN_CHECK_LAUNCH();

@@ -583,7 +583,7 @@ enum {
  * scores [rows, k] (log probabilities, of score_dtype).  A row without an entry
  * of positive weight has loss 0.  An id that stands twice counts with both
  * weights.  stats [rows, 4] is for the backward.  With SFFN_TAIL_BUCKET the
- * vocabulary is at most 1,600,000 (SFFN_ERR_TOO_LARGE beyond). */
+ * vocabulary is at most 1,400,000 (SFFN_ERR_TOO_LARGE beyond). */
 int sffn_distill_topk(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t inner, int64_t s_outer,
                       int64_t s_inner, const void* ids, int id_bytes, const void* scores, int score_dtype, int k,
                       int tail, float inv_t, float* loss, float* stats, uint32_t* status_dev, void* stream);
