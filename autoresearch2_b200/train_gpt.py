@@ -1,7 +1,7 @@
 """Data-parallel training run of the GPT harness (gpt.py) on synthetic tokens.
 
     python -m torch.distributed.run --nproc-per-node N --master-addr 127.0.0.1 \
-        -m autoresearch2_b200.train_gpt [--dense] [--check] [--batch 32] ...
+        -m autoresearch2_b200.train_gpt [--dense] [--sandwich] [--distill 64] [--check] [--batch 32] ...
 """
 import argparse
 import json
@@ -12,7 +12,7 @@ import torch
 import torch.distributed as dist
 
 from . import bitsparse as bs
-from .gpt import GPT, GPTConfig, TrainStep, flops_per_token, synthetic_batch
+from .gpt import GPT, DistillStep, GPTConfig, TrainStep, flops_per_token, synthetic_batch
 
 
 def main(argv=None):
@@ -35,6 +35,9 @@ def main(argv=None):
     ap.add_argument("--vocab", type=int, default=50304)
     ap.add_argument("--seq", type=int, default=1024)
     ap.add_argument("--dense", action="store_true", help="dense torch MLPs instead of the sparse FFN")
+    ap.add_argument("--sandwich", action="store_true", help="norms and gates after the blocks as well (GPTConfig.sandwich)")
+    ap.add_argument("--distill", type=int, default=0, metavar="K",
+                    help="train on the K top logits of a frozen dense teacher of the same shape (random weights, another seed)")
     ap.add_argument("--check", action="store_true")
     args = ap.parse_args(argv)
 
@@ -46,11 +49,15 @@ def main(argv=None):
     if world > 1:
         dist.init_process_group("nccl", timeout=timedelta(seconds=120), device_id=device)
     cfg = GPTConfig(n_layer=args.layers, n_head=args.heads, n_embd=args.width, ffn_hidden=args.hidden,
-                    vocab=args.vocab, seq_len=args.seq)
+                    vocab=args.vocab, seq_len=args.seq, sandwich=args.sandwich)
     model = GPT(cfg, sparse=not args.dense, device=device)
     net = torch.nn.parallel.DistributedDataParallel(model, device_ids=[local]) if world > 1 else model
     idx, tgt = synthetic_batch(cfg, args.batch, device, seed=rank)
-    step = TrainStep(net, idx, tgt)
+    if args.distill:
+        teacher = GPT(cfg, sparse=False, device=device, seed=1).requires_grad_(False)
+        step = DistillStep(net, teacher, idx, tgt, top_k=args.distill)
+    else:
+        step = TrainStep(net, idx, tgt)
     for _ in range(args.warmup):
         step()
     torch.cuda.synchronize(device)
@@ -79,6 +86,7 @@ def main(argv=None):
     tokens = world * args.batch * cfg.seq_len
     if rank == 0:
         print(json.dumps({"harness": "gpt", "mlp": "dense" if args.dense else "sparse_relu2", "n_gpus": world,
+                          "sandwich": args.sandwich, "distill_top_k": args.distill,
                           "tokens_per_s": round(tokens / (ms / 1e3), 1), "ms_per_step": round(ms, 3),
                           "tokens_per_step": tokens, "flops_per_token": flops_per_token(cfg),
                           "loss": round(float(loss), 4), "params_identical": ok if args.check else None}),
