@@ -1139,6 +1139,9 @@ cudaError_t launch_rows(void (*kernel)(Args), const Plan& p, int64_t rows, size_
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
+// Whether pointers (or null) lie on their elements' boundaries.
+bool lies(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
 #define SFFN_BY_DTYPE(dtype, CALL)                                  \
     do {                                                            \
         if (dtype == SFFN_F32) { CALL(SFFN_F32); }                  \
@@ -1163,6 +1166,9 @@ extern "C" int sffn_token_logprobs(const void* logits, int dtype, int64_t rows, 
     if (rows == 0) return SFFN_OK;
     if (!entropy || !stats || !status_dev || (targets && !logp) || (top_k && (!top_ids || !top_logp)))
         return SFFN_ERR_ARG;
+    if ((targets && !lies(targets, target_bytes)) || !lies(logp, 4) || !lies(entropy, 4) || !lies(stats, 4) ||
+        !lies(top_ids, 8) || !lies(top_logp, 4) || !lies(status_dev, 4))
+        return SFFN_ERR_ALIGN;
     SFFN_BIND(scope, logits);
     const Plan p = plan_rows(rows, vocab, dtype);
     const ScoreArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, targets, target_bytes, ignore_index,
@@ -1190,7 +1196,9 @@ extern "C" int sffn_token_logprobs_bwd(const void* logits, int dtype, int64_t ro
     if (top_k > TOP_MAX) return SFFN_ERR_TOO_LARGE;
     if (rows == 0) return SFFN_OK;
     if (!stats || !entropy || !grad || (g_top && top_k && !top_ids)) return SFFN_ERR_ARG;
-    if (reinterpret_cast<uintptr_t>(grad) % esize_of(dtype)) return SFFN_ERR_ALIGN;
+    if (!lies(grad, esize_of(dtype)) || (targets && !lies(targets, target_bytes)) || !lies(top_ids, 8) || !lies(stats, 4) ||
+        !lies(entropy, 4) || !lies(g_logp, 4) || !lies(g_entropy, 4) || !lies(g_top, 4))
+        return SFFN_ERR_ALIGN;
     SFFN_BIND(scope, logits);
     const int64_t per = vocab < BWD_PER ? vocab : BWD_PER;
     const int64_t blocks = (vocab + per - 1) / per;
@@ -1216,6 +1224,7 @@ int check_list(const void* ids, int id_bytes, const void* scores, int score_dtyp
     if (k < 1 || (tail != SFFN_TAIL_RENORM && tail != SFFN_TAIL_BUCKET)) return SFFN_ERR_ARG;
     if (k > TOP_MAX) return SFFN_ERR_TOO_LARGE;
     if (!ids || !scores) return SFFN_ERR_ARG;
+    if (!lies(ids, id_bytes) || !lies(scores, esize_of(score_dtype))) return SFFN_ERR_ALIGN;
     return SFFN_OK;
 }
 }  // namespace
@@ -1228,6 +1237,7 @@ extern "C" int sffn_distill_topk(const void* logits, int dtype, int64_t rows, in
     if (rows == 0) return SFFN_OK;
     if (int rc = check_list(ids, id_bytes, scores, score_dtype, k, tail)) return rc;
     if (!loss || !stats || !status_dev) return SFFN_ERR_ARG;
+    if (!lies(loss, 4) || !lies(stats, 4) || !lies(status_dev, 4)) return SFFN_ERR_ALIGN;
     const int bucket = tail == SFFN_TAIL_BUCKET;
     if (bucket && vocab > 1400000) return SFFN_ERR_TOO_LARGE;
     const Plan p = plan_rows(rows, vocab, dtype);
@@ -1261,7 +1271,7 @@ extern "C" int sffn_distill_topk_bwd(const void* logits, int dtype, int64_t rows
     if (rows == 0) return SFFN_OK;
     if (int rc = check_list(ids, id_bytes, scores, score_dtype, k, tail)) return rc;
     if (!stats || !g_loss || !grad) return SFFN_ERR_ARG;
-    if (reinterpret_cast<uintptr_t>(grad) % esize_of(dtype)) return SFFN_ERR_ALIGN;
+    if (!lies(grad, esize_of(dtype)) || !lies(stats, 4) || !lies(g_loss, 4)) return SFFN_ERR_ALIGN;
     SFFN_BIND(scope, logits);
     const int64_t per = vocab < BWD_PER ? vocab : BWD_PER;
     const int64_t blocks = (vocab + per - 1) / per;

@@ -834,6 +834,9 @@ int check_norm(int x_dtype, int y_dtype, int64_t rows, int64_t width, int64_t x_
     return SFFN_OK;
 }
 
+// Whether a pointer lies on its element's boundary.
+bool lies(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % esize_of(dtype) == 0; }
+bool lies8(const void* p) { return reinterpret_cast<uintptr_t>(p) % 8 == 0; }
 bool row_aligned(const void* p, int64_t ld, int dtype) { return !p || (aligned16(p) && ld * esize_of(dtype) % 16 == 0); }
 
 
@@ -863,6 +866,9 @@ extern "C" int sffn_residual_norm(const void* x, int x_dtype, int64_t x_ld, cons
     if (!(eps > 0.f) || (post && !post_norm)) return SFFN_ERR_ARG;
     if (rows == 0) return SFFN_OK;
     if (!x || !h || (y && !x_new)) return SFFN_ERR_ARG;
+    if (!lies(x, x_dtype) || !lies(y, y_dtype) || !lies(x_new, x_dtype) || !lies(h, y_dtype) || !lies(pre, pre_dtype) ||
+        !lies(post, post_dtype) || !lies(gate, gate_dtype) || !lies8(stats))
+        return SFFN_ERR_ALIGN;
     SFFN_BIND(scope, x);
     const bool vec = width % CH == 0 && row_aligned(x, x_ld, x_dtype) && row_aligned(y, y_ld, y_dtype) &&
                      row_aligned(x_new, width, x_dtype) && row_aligned(h, width, y_dtype) &&
@@ -901,6 +907,10 @@ extern "C" int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, 
     if ((dpre && !pre) || (dpost && !post) || (dgate && !gate) || (dy && !y) || (post && !post_norm)) return SFFN_ERR_ARG;
     if (rows == 0) return SFFN_OK;
     if (!x || !stats) return SFFN_ERR_ARG;
+    if (!lies(x, x_dtype) || !lies(y, y_dtype) || !lies(dx_new, x_dtype) || !lies(dh, y_dtype) || !lies(dx, x_dtype) ||
+        !lies(dy, y_dtype) || !lies(pre, pre_dtype) || !lies(post, post_dtype) || !lies(gate, gate_dtype) ||
+        !lies(dpre, pre_dtype) || !lies(dpost, post_dtype) || !lies(dgate, gate_dtype) || !lies8(stats))
+        return SFFN_ERR_ALIGN;
     const bool shared_gate = !gate || gate_rows >= rows;
     const int want = (dpre ? WANT_PRE : 0) | (dpost ? WANT_POST : 0) | (dgate ? WANT_GATE : 0);
     const Shape s = shape_of(rows, width, 1, 1);

@@ -204,6 +204,7 @@ def _(compressed, shape, dtype):
 @torch.library.custom_op("sparseffn::token_logprobs", mutates_args=())
 def token_logprobs(x: Tensor, targets: Optional[Tensor], top_k: int, temperature: float,
                    ignore_index: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    logits._check_score(x, targets, top_k, temperature)
     return logits._score_forward(x, targets, top_k, temperature, ignore_index)
 
 
@@ -220,8 +221,14 @@ def _(x, targets, top_k, temperature, ignore_index):
 def token_logprobs_bwd(x: Tensor, targets: Optional[Tensor], top_ids: Tensor, entropy: Tensor, stats: Tensor,
                        g_logp: Optional[Tensor], g_entropy: Optional[Tensor], g_top: Optional[Tensor],
                        temperature: float, ignore_index: int) -> Tensor:
-    return logits._score_backward(x, targets, top_ids, entropy, stats, g_logp, g_entropy, g_top, temperature,
-                                  ignore_index).contiguous()
+    lead, k = x.shape[:-1], top_ids.shape[-1]
+    logits._check_score(x, targets, k, temperature)
+    for name, t, shape in (("entropy", entropy, lead), ("stats", stats, (*lead, 2)), ("g_logp", g_logp, lead),
+                           ("g_entropy", g_entropy, lead), ("g_top", g_top, (*lead, k))):
+        logits._check_kept(name, t, shape, x.device)
+    logits._check_kept("top_ids", top_ids, (*lead, k), x.device, torch.int64)
+    return logits._score_backward(x, targets, top_ids.contiguous(), entropy.contiguous(), stats.contiguous(), g_logp,
+                                  g_entropy, g_top, temperature, ignore_index).contiguous()
 
 
 @token_logprobs_bwd.register_fake
@@ -250,6 +257,7 @@ token_logprobs.register_autograd(_score_bwd, setup_context=_score_setup)
 
 @torch.library.custom_op("sparseffn::distill_topk", mutates_args=())
 def distill_topk(x: Tensor, ids: Tensor, scores: Tensor, temperature: float, tail: str) -> tuple[Tensor, Tensor]:
+    logits._check_distill(x, ids, scores, temperature, tail)
     return logits._distill_forward(x, ids, scores, temperature, tail)
 
 
@@ -261,7 +269,10 @@ def _(x, ids, scores, temperature, tail):
 @torch.library.custom_op("sparseffn::distill_topk_bwd", mutates_args=())
 def distill_topk_bwd(x: Tensor, ids: Tensor, scores: Tensor, stats: Tensor, g_loss: Tensor, temperature: float,
                      tail: str) -> Tensor:
-    return logits._distill_backward(x, ids, scores, stats, g_loss, temperature, tail).contiguous()
+    logits._check_distill(x, ids, scores, temperature, tail)
+    logits._check_kept("stats", stats, (*x.shape[:-1], 4), x.device)
+    logits._check_kept("g_loss", g_loss, x.shape[:-1], x.device)
+    return logits._distill_backward(x, ids, scores, stats.contiguous(), g_loss, temperature, tail).contiguous()
 
 
 @distill_topk_bwd.register_fake
@@ -294,6 +305,8 @@ def _or_empty(like, ts):
 def residual_norm(x: Tensor, y: Optional[Tensor], pre: Optional[Tensor], post: Optional[Tensor],
                   gate: Optional[Tensor], groups: int, post_norm: bool, scale: float, eps: float,
                   out_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
+    norms._check(x, y, pre, post, gate, post_norm, scale, eps, out_dtype)
+    norms._check_groups(x, gate, groups)
     return _or_empty(x, norms._forward(x, y, pre, post, gate, groups, post_norm, scale, eps, out_dtype, True))
 
 
@@ -308,6 +321,9 @@ def residual_norm_bwd(x: Tensor, y: Optional[Tensor], pre: Optional[Tensor], pos
                       gate: Optional[Tensor], groups: int, post_norm: bool, scale: float, out_dtype: torch.dtype,
                       stats: Tensor, dx_new: Optional[Tensor], dh: Optional[Tensor],
                       want: list[bool]) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    norms._check(x, y, pre, post, gate, post_norm, scale, 1.0, out_dtype)
+    norms._check_groups(x, gate, groups)
+    norms._check_backward(x, y, dx_new, dh, stats, out_dtype)
     return _or_empty(x, norms._backward(x, y, pre, post, gate, groups, post_norm, scale, out_dtype, stats, dx_new,
                                         dh, want))
 

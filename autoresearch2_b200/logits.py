@@ -102,6 +102,12 @@ def _check_index(name, t, shape, device):
         raise ValueError(f"{name} is on {t.device}, the logits on {device}")
 
 
+def _check_kept(name, t, shape, device, dtype=torch.float32):
+    """What a backward op is given of the forward and of upstream gradients."""
+    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device):
+        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)} on {device}")
+
+
 # ---------------------------------------------------------------------------
 # token_logprobs
 # ---------------------------------------------------------------------------
@@ -157,6 +163,15 @@ class _TokenLogprobs(torch.autograd.Function):
                 None, None, None, None)
 
 
+def _check_score(logits, targets, top_k, temperature):
+    _check_logits("token_logprobs", logits, temperature)
+    V = logits.shape[-1]
+    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= min(V, TOP_MAX):
+        raise ValueError(f"top_k must be an integer in [0, {min(V, TOP_MAX)}], got {top_k!r}")
+    if targets is not None:
+        _check_index("targets", targets, logits.shape[:-1], logits.device)
+
+
 def token_logprobs(logits, targets=None, top_k=0, temperature=1.0, ignore_index=-100) -> TokenLogprobs:
     """Log probabilities of `targets` under softmax(logits / temperature), the
     entropy of each row, and its top_k (<= 128) alternatives, largest first,
@@ -170,12 +185,7 @@ def token_logprobs(logits, targets=None, top_k=0, temperature=1.0, ignore_index=
     -inf, entropy 0, gradient 0.  A row holding NaN or +inf has NaN.  Another
     target outside [0, V) gives NaN and sets the library's status word
     (check_status() reports it)."""
-    _check_logits("token_logprobs", logits, temperature)
-    V = logits.shape[-1]
-    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= min(V, TOP_MAX):
-        raise ValueError(f"top_k must be an integer in [0, {min(V, TOP_MAX)}], got {top_k!r}")
-    if targets is not None:
-        _check_index("targets", targets, logits.shape[:-1], logits.device)
+    _check_score(logits, targets, top_k, temperature)
     if torch.compiler.is_compiling():
         r = torch.ops.sparseffn.token_logprobs(logits, targets, top_k, temperature, ignore_index)
     elif torch.is_grad_enabled() and logits.requires_grad:
@@ -228,6 +238,21 @@ class _DistillTopk(torch.autograd.Function):
         return _distill_backward(logits, ids, scores, stats, g_loss, *ctx.args), None, None, None, None
 
 
+def _check_distill(logits, teacher_ids, teacher_scores, temperature, tail):
+    _check_logits("distill_topk", logits, temperature)
+    if tail not in TAILS:
+        raise ValueError(f"tail must be one of {sorted(TAILS)}, got {tail!r}")
+    if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.dim() < 1 or not 1 <= teacher_ids.shape[-1] <= TOP_MAX:
+        raise ValueError(f"teacher_ids must be [..., K] with 1 <= K <= {TOP_MAX}")
+    shape = (*logits.shape[:-1], teacher_ids.shape[-1])
+    _check_index("teacher_ids", teacher_ids, shape, logits.device)
+    _lib.require_cuda(teacher_scores)
+    _lib.dtype_code(teacher_scores)
+    if tuple(teacher_scores.shape) != shape or teacher_scores.device != logits.device:
+        raise ValueError(f"teacher_scores must have shape {shape} on {logits.device}, got "
+                         f"{tuple(teacher_scores.shape)} on {teacher_scores.device}")
+
+
 def distill_topk(logits, teacher_ids, teacher_scores, temperature=1.0, tail="renorm"):
     """float32 [...]: for each row the divergence sum q (ln q - ln p) of the
     student's distribution p = softmax(logits / temperature) from a teacher's
@@ -250,18 +275,7 @@ def distill_topk(logits, teacher_ids, teacher_scores, temperature=1.0, tail="ren
     Where the student gives a listed class no probability the loss is +inf.
     Other ids outside [0, V) count as absent and set the library's status word
     (check_status() reports it).  The loss carries no factor T^2."""
-    _check_logits("distill_topk", logits, temperature)
-    if tail not in TAILS:
-        raise ValueError(f"tail must be one of {sorted(TAILS)}, got {tail!r}")
-    if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.dim() < 1 or not 1 <= teacher_ids.shape[-1] <= TOP_MAX:
-        raise ValueError(f"teacher_ids must be [..., K] with 1 <= K <= {TOP_MAX}")
-    shape = (*logits.shape[:-1], teacher_ids.shape[-1])
-    _check_index("teacher_ids", teacher_ids, shape, logits.device)
-    _lib.require_cuda(teacher_scores)
-    _lib.dtype_code(teacher_scores)
-    if tuple(teacher_scores.shape) != shape or teacher_scores.device != logits.device:
-        raise ValueError(f"teacher_scores must have shape {shape} on {logits.device}, got "
-                         f"{tuple(teacher_scores.shape)} on {teacher_scores.device}")
+    _check_distill(logits, teacher_ids, teacher_scores, temperature, tail)
     if teacher_scores.requires_grad and torch.is_grad_enabled():
         raise ValueError("no gradient flows to teacher_scores: detach them")
     if torch.compiler.is_compiling():

@@ -23,12 +23,28 @@ from ._lib import call, stream_handle
 __all__ = ["residual_norm", "WIDTH_MAX"]
 
 WIDTH_MAX = 16384  # elements of a row
+F32_MAX = torch.finfo(torch.float32).max
 
 
 def _matrix(t, width):
     """t as [rows, width] with dense rows (a view where the strides allow one)."""
     t = t.reshape(-1, width) if t.dim() != 2 else t
     return t if width == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _check_groups(x, gate, groups):
+    """The ops' way to say what _gate_groups found."""
+    rows = x.numel() // x.shape[-1]
+    if groups < 1 or (rows and rows % groups) or (gate is not None and rows and gate.numel() != groups * x.shape[-1]):
+        raise ValueError(f"a gate of {groups} rows does not divide {rows} rows evenly")
+
+
+def _check_backward(x, y, dx_new, dh, stats, out_dtype):
+    for name, t, like, dtype in (("dx_new", dx_new, x, x.dtype), ("dh", dh, x, out_dtype)):
+        if t is not None and (t.shape != like.shape or t.dtype != dtype or t.device != x.device):
+            raise ValueError(f"{name} must be {dtype} of shape {tuple(like.shape)} on {x.device}")
+    if stats.numel() != 2 * (x.numel() // x.shape[-1]) or stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise ValueError("stats are the forward's")
 
 
 def _code(t):
@@ -117,24 +133,8 @@ class _ResidualNorm(torch.autograd.Function):
         return *grads, None, None, None, None, None
 
 
-def residual_norm(x, y=None, pre_weight=None, post_weight=None, gate=None, post_norm=False, residual_scale=1.0,
-                  eps=1e-6, out_dtype=None):
-    """(x_new, h): the residual stream after a block, and its norm for the next.
-
-    x [..., D], D <= 16384; y of x's shape, or None (the first norm of a stack:
-    x_new is x itself).  x and y share a type, or x is float32 and y bfloat16
-    or float16; x_new has x's type and h y's (out_dtype, or x's, without y).
-    pre_weight and post_weight [D] (post_weight only with post_norm) and gate
-    may each have any of the three types, and None for ones.
-
-    gate is [D]; or [G, D], each row for one of G equal runs of x's rows; or
-    x's leading dimensions up to some one, then ones, then D (for x [B, T, D]
-    one gate a sequence is [B, 1, D]).  A [G, D] gate is not broadcast against
-    x's last two dimensions.
-
-    Rows are read in place where one stride fits them all.  Arithmetic,
-    statistics and sums are float32, each output is rounded once; h comes from
-    the unrounded x_new."""
+def _check(x, y, pre_weight, post_weight, gate, post_norm, residual_scale, eps, out_dtype):
+    """h's type, of arguments that are refused otherwise (the gate's rows: _gate_groups)."""
     _lib.require_cuda(*(t for t in (x, y, pre_weight, post_weight, gate) if t is not None))
     if x.dim() < 1 or not 1 <= x.shape[-1] <= WIDTH_MAX:
         raise ValueError(f"residual_norm takes x [..., D] with 1 <= D <= {WIDTH_MAX}, got {tuple(x.shape)}")
@@ -160,8 +160,30 @@ def residual_norm(x, y=None, pre_weight=None, post_weight=None, gate=None, post_
             raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(t.shape)}")
     if post_weight is not None and not post_norm:
         raise ValueError("post_weight goes with post_norm=True")
-    if not (math.isfinite(residual_scale) and math.isfinite(eps) and eps > 0):
+    if not (abs(residual_scale) <= F32_MAX and 2.0 ** -126 <= eps <= F32_MAX):
         raise ValueError(f"residual_scale must be finite and eps positive, got {residual_scale!r}, {eps!r}")
+    return out_dtype
+
+
+def residual_norm(x, y=None, pre_weight=None, post_weight=None, gate=None, post_norm=False, residual_scale=1.0,
+                  eps=1e-6, out_dtype=None):
+    """(x_new, h): the residual stream after a block, and its norm for the next.
+
+    x [..., D], D <= 16384; y of x's shape, or None (the first norm of a stack:
+    x_new is x itself).  x and y share a type, or x is float32 and y bfloat16
+    or float16; x_new has x's type and h y's (out_dtype, or x's, without y).
+    pre_weight and post_weight [D] (post_weight only with post_norm) and gate
+    may each have any of the three types, and None for ones.
+
+    gate is [D]; or [G, D], each row for one of G equal runs of x's rows; or
+    x's leading dimensions up to some one, then ones, then D (for x [B, T, D]
+    one gate a sequence is [B, 1, D]).  A [G, D] gate is not broadcast against
+    x's last two dimensions.
+
+    Rows are read in place where one stride fits them all.  Arithmetic,
+    statistics and sums are float32, each output is rounded once; h comes from
+    the unrounded x_new."""
+    out_dtype = _check(x, y, pre_weight, post_weight, gate, post_norm, residual_scale, eps, out_dtype)
     groups = _gate_groups(gate, x) if gate is not None and x.numel() else 1
     args = (x, y, pre_weight, post_weight, gate, groups, bool(post_norm), float(residual_scale), float(eps), out_dtype)
     if torch.compiler.is_compiling():

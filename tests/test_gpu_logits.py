@@ -561,3 +561,39 @@ def test_library_ops():
     got.backward()
     torch._dynamo.reset()
     assert torch.equal(want, got) and torch.equal(a.grad, b.grad)
+
+
+def test_gradients_are_not_differentiable_again():
+    x, t, ids, scores = inputs(5, rows=4, V=50)
+    x.requires_grad_()
+    for out in (sf.token_logprobs(x, t).logp, sf.distill_topk(x, ids, scores)):
+        with pytest.raises(RuntimeError, match="not differentiable again"):
+            torch.autograd.grad(out.sum(), x, create_graph=True)
+
+
+def test_logits_changed_before_the_backward_are_refused():
+    x, t, _, _ = inputs(5, rows=4, V=50)
+    x.requires_grad_()
+    y = x * 1
+    out = sf.token_logprobs(y, t).logp.sum()
+    with torch.no_grad():
+        y.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
+
+
+def test_ops_refuse_what_the_functions_refuse():
+    ops = torch.ops.sparseffn
+    x, t, ids, scores = inputs(5, rows=4, V=50)
+    logp, ent, top, _, stats = ops.token_logprobs(x, t, 3, 1.0, -100)
+    loss, kept = ops.distill_topk(x, ids, scores, 1.0, "bucket")
+    bad = [lambda: ops.token_logprobs(x, t[:3], 3, 1.0, -100), lambda: ops.token_logprobs(x, t, 51, 1.0, -100),
+           lambda: ops.token_logprobs_bwd(x, t, top, ent, stats[:2], logp, None, None, 1.0, -100),
+           lambda: ops.token_logprobs_bwd(x, t, top[:, :2], ent, stats, None, None, logp[:, None].expand(4, 3)[:, :3][:2], 1.0, -100),
+           lambda: ops.token_logprobs_bwd(x, t, top, ent, stats, logp.half(), None, None, 1.0, -100),
+           lambda: ops.distill_topk(x, ids[:2], scores, 1.0, "bucket"),
+           lambda: ops.distill_topk_bwd(x, ids, scores, kept[:, :2], loss, 1.0, "bucket"),
+           lambda: ops.distill_topk_bwd(x, ids, scores, kept, loss[:1], 1.0, "bucket")]
+    for f in bad:
+        with pytest.raises(ValueError):
+            f()

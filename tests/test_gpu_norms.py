@@ -296,3 +296,28 @@ def test_library_op():
     torch.compile(f, backend="aot_eager", fullgraph=True)(*two).backward()
     torch._dynamo.reset()
     assert all(torch.equal(p.grad, q.grad) for p, q in zip(one, two))
+
+
+def test_gradients_are_not_differentiable_again():
+    x = randn(3, 16, seed=1).requires_grad_()
+    _, h = sf.residual_norm(x, x)
+    with pytest.raises(RuntimeError, match="not differentiable again"):
+        torch.autograd.grad(h.sum(), x, create_graph=True)
+
+
+def test_ops_refuse_what_the_function_refuses():
+    op, bwd = torch.ops.sparseffn.residual_norm, torch.ops.sparseffn.residual_norm_bwd
+    D = 64
+    x, y, gate = randn(6, D, seed=1), randn(6, D, seed=2), randn(2, D, seed=3)
+    _, _, stats = op(x, y, None, None, gate, 2, False, 1.0, 1e-6, F32)
+    rest = (False, 1.0, F32)
+    bad = [lambda: op(x, y, None, None, gate, 4, False, 1.0, 1e-6, F32), lambda: op(x, y, None, None, gate, 3, False, 1.0, 1e-6, F32),
+           lambda: op(x, y[:5], None, None, None, 1, False, 1.0, 1e-6, F32), lambda: op(x, y, gate[0, :9], None, None, 1, False, 1.0, 1e-6, F32),
+           lambda: op(x, y, None, None, None, 0, False, 1.0, 1e-6, F32),
+           lambda: bwd(x, y, None, None, gate, 3, *rest, stats, x, y, [True] * 5),
+           lambda: bwd(x, y, None, None, gate, 2, *rest, stats[:4], x, y, [True] * 5),
+           lambda: bwd(x, y, None, None, gate, 2, *rest, stats, x[:5], y, [True] * 5),
+           lambda: bwd(x, y, None, None, gate, 2, *rest, stats, x, y.half(), [True] * 5)]
+    for f in bad:
+        with pytest.raises(ValueError):
+            f()

@@ -90,9 +90,10 @@ def test_residual_norm_refusals():
         refused(ValueError, "post_norm=True", f, x, x, w, w)
         refused(ValueError, "go with a block output", f, x, None, w, residual_scale=0.5)
         refused(ValueError, "go with a block output", f, x, gate=w)
-        for eps in (0.0, -1e-6, INF, float("nan")):
+        for eps in (0.0, -1e-6, INF, float("nan"), 1e-40):
             refused(ValueError, "eps", f, x, x, eps=eps)
-        refused(ValueError, "residual_scale", f, x, x, residual_scale=INF)
+        for scale in (INF, -1e39, float("nan")):
+            refused(ValueError, "residual_scale", f, x, x, residual_scale=scale)
         refused(ValueError, "evenly", f, x, x, gate=cuda(4, 8))
         refused(ValueError, "last dimension", f, x, x, gate=cuda(6, 1))
         y = cuda(2, 3, 8)
@@ -166,6 +167,8 @@ def test_c_scores_refusals(lib):
         assert rc(**{f"_{i}": None}) == 1
     assert rc(_3=1 << 31) == 8 and rc(_2=1 << 32) == 8
     assert rc(_2=0, _0=None) == 0  # no rows: nothing to do
+    for i, off in ((7, 4), (12, 2), (13, 2), (14, 2), (15, 4), (16, 2), (17, 1)):
+        assert rc(**{f"_{i}": vp((1 << 20) + off)}) == 3
 
     ok = [P, 0, 4, 100, 4, 0, 100, P, 8, -100, P, 5, 1.0, P, P, P, P, P, P, 100, None]
 
@@ -216,6 +219,8 @@ def test_c_norm_refusals(lib):
     assert rc(f, ok, _3=None) == 1 and rc(f, ok, _15=0) == 1 and rc(f, ok, _17=0.0) == 1
     assert rc(f, ok, _0=None) == 1 and rc(f, ok, _18=None) == 1 and rc(f, ok, _19=None) == 1
     assert rc(f, ok, _6=0) == 0
+    for i, off in ((0, 2), (3, 1), (8, 2), (10, 2), (12, 2), (18, 2), (19, 1), (20, 4)):
+        assert rc(f, ok, **{f"_{i}": vp((1 << 20) + off)}) == 3
     b = [P, 0, 64, P, 1, 64, 10, 64, P, 0, P, 0, P, 0, 5, 1, 1.0, P, P, P, P, P, P, P, P, P, 1 << 20, None]
     f = lib.sffn_residual_norm_bwd
     need = lib.sffn_residual_norm_bwd_workspace_bytes(10, 64, 5)
