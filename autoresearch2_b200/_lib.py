@@ -103,11 +103,11 @@ SIGNATURES = {
     "sffn_distill_topk_bwd": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _int, _vp, _int, _int, _int,
                                      _f32, _vp, _vp, _vp, _i64, _vp]),
     "sffn_residual_norm": (_int, [_vp, _int, _i64, _vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _int, _vp, _int,
-                                  _i64, _int, _f32, _f32, _vp, _vp, _vp, _vp]),
+                                  _i64, _int, _f32, _f32, _vp, _vp, _vp, _vp, _vp]),
     "sffn_residual_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "sffn_residual_norm_bwd": (_int, [_vp, _int, _i64, _vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _int, _vp,
                                       _int, _i64, _int, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
-                                      _vp]),
+                                      _vp, _vp]),
 }
 
 _lib = None

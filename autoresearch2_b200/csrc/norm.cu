@@ -34,6 +34,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace sffn {
 namespace {
@@ -306,22 +307,44 @@ __device__ __forceinline__ void take8(uint32_t from, int threads, Pair* x) {
     }
 }
 
+// Stores v at this block's shared address `to` in block `rank` of the cluster and
+// counts its 4 bytes at that block's `barrier`.
+__device__ __forceinline__ void send(uint32_t to, uint32_t barrier, int rank, float v) {
+    asm volatile(
+        "{\n\t.reg .b32 a, b;\n\t"
+        "mapa.shared::cluster.u32 a, %0, %2;\n\t"
+        "mapa.shared::cluster.u32 b, %1, %2;\n\t"
+        "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [a], %3, [b];\n\t}"
+        ::"r"(to), "r"(barrier), "r"(rank), "r"(__float_as_uint(v)) : "memory");
+}
+
 // Sums of N values over the threads that share rows.  In a warp the lanes halve
 // the values among them while they add: log2 N exchanges of N / 2, N / 4, ... values,
-// then of one.  The warps' sums meet in slots (of every block of a cluster), and
-// every thread adds them up in the same order.  Two slot sets alternate: a set is
-// written again only after the other set's barrier, which every reader of it has
-// passed.
-template <int N>
+// then of one.  The warps' sums meet in slots, and every thread adds them up in
+// the same order.  Two slot sets alternate: a set is written again only after the
+// other set's barrier, which every reader of it has passed.
+//
+// In a cluster each warp stores its sums to every block's slots (st.async), and
+// an mbarrier of each set counts the bytes: unlike the cluster's own barrier that
+// does not wait until the rows' stores to global memory are acknowledged (float32
+// 8192x8192 with bf16: 181 -> 138 us forward, 314 -> 239 us backward).  The wait is
+// bounded: when it runs out it sets SFFN_STATUS_WAIT_TIMEOUT and no later one waits.
+template <int N, bool WIDE>
 struct RowSums {
     static constexpr int POW = N <= 1 ? 1 : N <= 2 ? 2 : 4;
     static_assert(N <= 4, "one 16-byte slot a warp");
     float4* slots;  // [2][fold] of this group, zeroed
     int warps, warp, lane, bar, parts, part;
     int fold;  // the power of two that covers warps * parts
+    uint64_t* filled;  // [2], of a cluster
+    uint32_t* status;
     int set = 0;
-    __device__ __forceinline__ RowSums(float4* slots_, int fold_, int warps_, int warp_, int lane_, int bar_, int parts_, int part_)
-        : slots(slots_), warps(warps_), warp(warp_), lane(lane_), bar(bar_), parts(parts_), part(part_), fold(fold_) {}
+    uint32_t phase = 0;  // bit i: the parity that set i's barrier completes next
+    bool gave_up = false;
+    __device__ __forceinline__ RowSums(float4* slots_, int fold_, int warps_, int warp_, int lane_, int bar_, int parts_, int part_,
+                                       uint64_t* filled_, uint32_t* status_)
+        : slots(slots_), warps(warps_), warp(warp_), lane(lane_), bar(bar_), parts(parts_), part(part_), fold(fold_),
+          filled(filled_), status(status_) {}
     __device__ __forceinline__ void operator()(float (&v)[N]) {
         float w[POW];
 #pragma unroll
@@ -338,7 +361,7 @@ struct RowSums {
         }
 #pragma unroll
         for (; o; o >>= 1) w[0] += __shfl_xor_sync(FULL, w[0], o);
-        if (fold == 1) {  // one warp: value i is in lanes i * 32 / POW on
+        if (!WIDE && fold == 1) {  // one warp: value i is in lanes i * 32 / POW on
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] = __shfl_sync(FULL, w[0], i * (32 / POW));
             return;
@@ -346,17 +369,23 @@ struct RowSums {
         float4* s = slots + set;
         set ^= fold;
         float* mine = reinterpret_cast<float*>(s + part * warps + warp) + lane / (32 / POW);
-        if (parts == 1) {
+        if constexpr (!WIDE) {
             if (lane % (32 / POW) == 0) *mine = w[0];
             asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(warps * 32) : "memory");
         } else {
-            cg::cluster_group cluster = cg::this_cluster();
+            const int which = s != slots;
+            uint64_t* full = filled + which;
+            if (threadIdx.x == 0) mbar_arrive_expect_tx(full, parts * warps * POW * 4);
             if (lane % (32 / POW) == 0)
-                for (int i = 0; i < parts; ++i) *cluster.map_shared_rank(mine, i) = w[0];
-            cluster.sync();
+                for (int i = 0; i < parts; ++i) send(smem_u32(mine), smem_u32(full), i, w[0]);
+            if (!gave_up && !mbar_wait_bounded(full, (phase >> which) & 1)) {
+                gave_up = true;
+                atomicOr(status, SFFN_STATUS_WAIT_TIMEOUT);
+            }
+            phase ^= 1u << which;
         }
         float4 q = s[lane & (fold - 1)];
-        if (fold > 32) {
+        if (WIDE && fold > 32) {
             const float4 p = s[(lane & (fold - 1)) + 32];
             q.x += p.x;
             q.y += p.y;
@@ -399,26 +428,36 @@ struct NormArgs {
     float scale, eps;
     void *x_new, *h;
     float* stats;  // [rows, 2]: r1, r2; null: not kept
+    uint32_t* status;
 };
 
-template <int TX, int TY, bool VEC>
+template <int TX, int TY, bool VEC, bool WIDE>
 __global__ void __launch_bounds__(MAX_WARPS * 32, FWD_RING<TX, TY, VEC> ? 1 : 2) norm_kernel(const NormArgs a) {
     constexpr int R = FWD_ROWS<TX, TY, VEC>, S = STAGES<TX, TY>, ROW = BYTES<TX> + BYTES<TY>;
     constexpr bool ringed = FWD_RING<TX, TY, VEC>;
     constexpr int MODE = mode_of(TX, TY, VEC);
     extern __shared__ float4 ring[];
     __shared__ float4 slots[SLOTS];
+    __shared__ uint64_t filled[WIDE ? 2 : 1];
     using bx = typename Elt<TX>::bits;
     using by = typename Elt<TY>::bits;
     const int threads = blockDim.x, lane = threadIdx.x & 31, warps = a.shape.warps;
     const int group = (threadIdx.x >> 5) / warps, warp = (threadIdx.x >> 5) % warps;
-    const int parts = a.shape.parts, part = parts > 1 ? blockIdx.x % parts : 0;
+    const int parts = WIDE ? a.shape.parts : 1, part = WIDE ? blockIdx.x % parts : 0;
     const Place<MODE> pl(warp, lane, part * a.shape.cols, min(a.width, (part + 1) * a.shape.cols));
     for (int i = threadIdx.x; i < SLOTS; i += threads) slots[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (parts > 1) cg::this_cluster().sync();
-    else __syncthreads();
+    if constexpr (WIDE) {
+        if (threadIdx.x == 0) {
+            mbar_init(&filled[0], 1);
+            mbar_init(&filled[1], 1);
+            fence_mbar_init();
+        }
+        cg::this_cluster().sync();
+    } else {
+        __syncthreads();
+    }
     const int fold = fold_of(warps * parts);
-    RowSums<R> sum(slots + group * 2 * fold, fold, warps, warp, lane, group + 1, parts, part);
+    RowSums<R, WIDE> sum(slots + group * 2 * fold, fold, warps, warp, lane, group + 1, parts, part, filled, a.status);
     const float inv_width = 1.0f / a.width;
     const int64_t begin = ((int64_t)(blockIdx.x / parts) * a.shape.groups + group) * a.shape.per;
     const int rows = (int)max((int64_t)0, min(a.rows - begin, a.shape.per));
@@ -522,7 +561,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, FWD_RING<TX, TY, VEC> ? 1 : 2)
         } while (k0 < min(R, rows - r0));
         from = from + stage_bytes == ring_end ? base : from + stage_bytes;
     }
-    if (parts > 1) cg::this_cluster().sync();  // no block leaves while a fellow may write its slots
+    if constexpr (WIDE) cg::this_cluster().sync();  // no block leaves while a fellow may write its slots
 }
 
 struct NormBwdArgs {
@@ -542,28 +581,38 @@ struct NormBwdArgs {
     float* part;              // [blocks / parts][3][width]: dw_pre, dw_post, dgate (of one shared gate row)
     float* gate_part;         // [units + gate rows][width], where gates are not shared by all rows and a sum is wanted; else null
     int want;                 // bits 0..2: dw_pre, dw_post, dgate
+    uint32_t* status;
 };
 
 enum { WANT_PRE = 1, WANT_POST = 2, WANT_GATE = 4 };
 
-template <int TX, int TY, bool VEC>
+template <int TX, int TY, bool VEC, bool WIDE>
 __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormBwdArgs a) {
     constexpr int S = BWD_STAGES<TX, TY>, ROW = 2 * (BYTES<TX> + BYTES<TY>);
     constexpr bool ringed = BWD_RING<TX, TY, VEC>;
     constexpr int MODE = mode_of(TX, TY, VEC);
     extern __shared__ float4 ring[];  // and, at the end, [warps * 32][2]: the join of the block's groups
     __shared__ float4 slots[SLOTS];
+    __shared__ uint64_t filled[WIDE ? 2 : 1];
     using bx = typename Elt<TX>::bits;
     using by = typename Elt<TY>::bits;
     const int threads = blockDim.x, lane = threadIdx.x & 31, warps = a.shape.warps;
     const int group = (threadIdx.x >> 5) / warps, warp = (threadIdx.x >> 5) % warps;
-    const int parts = a.shape.parts, part = parts > 1 ? blockIdx.x % parts : 0;
+    const int parts = WIDE ? a.shape.parts : 1, part = WIDE ? blockIdx.x % parts : 0;
     const Place<MODE> pl(warp, lane, part * a.shape.cols, min(a.width, (part + 1) * a.shape.cols));
     for (int i = threadIdx.x; i < SLOTS; i += threads) slots[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (parts > 1) cg::this_cluster().sync();
-    else __syncthreads();
+    if constexpr (WIDE) {
+        if (threadIdx.x == 0) {
+            mbar_init(&filled[0], 1);
+            mbar_init(&filled[1], 1);
+            fence_mbar_init();
+        }
+        cg::this_cluster().sync();
+    } else {
+        __syncthreads();
+    }
     const int fold = fold_of(warps * parts);
-    RowSums<3> sum(slots + group * 2 * fold, fold, warps, warp, lane, group + 1, parts, part);
+    RowSums<3, WIDE> sum(slots + group * 2 * fold, fold, warps, warp, lane, group + 1, parts, part, filled, a.status);
     const float inv_width = 1.0f / a.width;
     const int64_t block = blockIdx.x / parts;
     const int64_t unit = block * a.shape.groups + group, begin = unit * a.shape.per;
@@ -697,7 +746,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
 #pragma unroll
         for (int i = 0; i < 4; ++i) z[i] = mul2(w[i], z[i]);  // dgate
     }
-    if (parts > 1) cg::this_cluster().sync();  // no block leaves while a fellow may write its slots
+    if constexpr (WIDE) cg::this_cluster().sync();  // no block leaves while a fellow may write its slots
     // The block's groups join their sums in order, through the ring (whose copies
     // are done: the last waits left only empty groups); one row of each is written.
     __syncthreads();
@@ -860,12 +909,12 @@ extern "C" int sffn_residual_norm(const void* x, int x_dtype, int64_t x_ld, cons
                                   int64_t rows, int64_t width, const void* pre, int pre_dtype, const void* post,
                                   int post_dtype, const void* gate, int gate_dtype, int64_t gate_rows,
                                   int post_norm, float scale, float eps, void* x_new, void* h, float* stats,
-                                  void* stream) {
+                                  uint32_t* status_dev, void* stream) {
     const Params p{pre, post, gate, pre_dtype, post_dtype, gate_dtype};
     if (int rc = check_norm(x_dtype, y_dtype, rows, width, x_ld, y != nullptr, y_ld, p, gate_rows)) return rc;
     if (!(eps > 0.f) || (post && !post_norm)) return SFFN_ERR_ARG;
     if (rows == 0) return SFFN_OK;
-    if (!x || !h || (y && !x_new)) return SFFN_ERR_ARG;
+    if (!x || !h || (y && !x_new) || !status_dev) return SFFN_ERR_ARG;
     if (!lies(x, x_dtype) || !lies(y, y_dtype) || !lies(x_new, x_dtype) || !lies(h, y_dtype) || !lies(pre, pre_dtype) ||
         !lies(post, post_dtype) || !lies(gate, gate_dtype) || !lies8(stats))
         return SFFN_ERR_ALIGN;
@@ -877,10 +926,11 @@ extern "C" int sffn_residual_norm(const void* x, int x_dtype, int64_t x_ld, cons
     const bool ringed = vec && (x_dtype != SFFN_F32 || y_dtype != SFFN_F32);
     const Shape s = ringed ? shape_of(rows, width, 4, 1) : shape_of(rows, width, 1, 2);
     const NormArgs a{x, y, x_ld, y_ld, rows, (int)width, s, pre, post, gate, pre_dtype, post_dtype, gate_dtype,
-                     gate_rows, post_norm, scale, eps, x_new, h, stats};
+                     gate_rows, post_norm, scale, eps, x_new, h, stats, status_dev};
     return by_types(x_dtype, y_dtype, [&](auto tx, auto ty) -> int {
         constexpr int TX = decltype(tx)::value, TY = decltype(ty)::value;
-        SFFN_CUDA_TRY(launch(vec ? norm_kernel<TX, TY, true> : norm_kernel<TX, TY, false>, s,
+        SFFN_CUDA_TRY(launch(s.parts > 1 ? (vec ? norm_kernel<TX, TY, true, true> : norm_kernel<TX, TY, false, true>)
+                                         : (vec ? norm_kernel<TX, TY, true, false> : norm_kernel<TX, TY, false, false>), s,
                              ringed ? STAGES<TX, TY> * FWD_ROWS<TX, TY, true> * (BYTES<TX> + BYTES<TY>) * s.threads() : 0,
                              static_cast<cudaStream_t>(stream), a));
         return SFFN_OK;
@@ -901,12 +951,12 @@ extern "C" int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, 
                                       int64_t gate_rows, int post_norm, float scale, const float* stats,
                                       const void* dx_new, const void* dh, void* dx, void* dy, void* dpre,
                                       void* dpost, void* dgate, void* workspace, size_t workspace_bytes,
-                                      void* stream) {
+                                      uint32_t* status_dev, void* stream) {
     const Params p{pre, post, gate, pre_dtype, post_dtype, gate_dtype};
     if (int rc = check_norm(x_dtype, y_dtype, rows, width, x_ld, y != nullptr, y_ld, p, gate_rows)) return rc;
     if ((dpre && !pre) || (dpost && !post) || (dgate && !gate) || (dy && !y) || (post && !post_norm)) return SFFN_ERR_ARG;
     if (rows == 0) return SFFN_OK;
-    if (!x || !stats) return SFFN_ERR_ARG;
+    if (!x || !stats || !status_dev) return SFFN_ERR_ARG;
     if (!lies(x, x_dtype) || !lies(y, y_dtype) || !lies(dx_new, x_dtype) || !lies(dh, y_dtype) || !lies(dx, x_dtype) ||
         !lies(dy, y_dtype) || !lies(pre, pre_dtype) || !lies(post, post_dtype) || !lies(gate, gate_dtype) ||
         !lies(dpre, pre_dtype) || !lies(dpost, post_dtype) || !lies(dgate, gate_dtype) || !lies8(stats))
@@ -929,11 +979,13 @@ extern "C" int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, 
     const int64_t sets = s.blocks / s.parts;
     float* gate_part = (dgate || dpost) && !shared_gate ? part + sets * 3 * width : nullptr;
     const NormBwdArgs a{x, y, x_ld, y_ld, rows, (int)width, s, pre, post, gate, pre_dtype, post_dtype, gate_dtype,
-                        gate_rows, post_norm, y ? scale : 1.0f, stats, dx_new, dh, dx, dy, part, gate_part, want};
+                        gate_rows, post_norm, y ? scale : 1.0f, stats, dx_new, dh, dx, dy, part, gate_part, want,
+                        status_dev};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int rc = by_types(x_dtype, y_dtype, [&](auto tx, auto ty) -> int {
         constexpr int TX = decltype(tx)::value, TY = decltype(ty)::value;
-        SFFN_CUDA_TRY(launch(vec ? norm_bwd_kernel<TX, TY, true> : norm_bwd_kernel<TX, TY, false>, s,
+        SFFN_CUDA_TRY(launch(s.parts > 1 ? (vec ? norm_bwd_kernel<TX, TY, true, true> : norm_bwd_kernel<TX, TY, false, true>)
+                                         : (vec ? norm_bwd_kernel<TX, TY, true, false> : norm_bwd_kernel<TX, TY, false, false>), s,
                              vec || BWD_RING<TX, TY, false> ? BWD_STAGES<TX, TY> * 2 * (BYTES<TX> + BYTES<TY>) * s.threads()
                                                         : s.warps * 32 * 32,
                              st, a));

@@ -86,7 +86,7 @@ def _forward(x, y, pre, post, gate, groups, post_norm, scale, eps, out_dtype, ke
         call("sffn_residual_norm", ptr(x2), _lib.dtype_code(x), x2.stride(0), ptr(y2), _code(h),
              y2.stride(0) if y2 is not None else 0, rows, width, ptr(pre), _code(pre), ptr(post), _code(post),
              ptr(gate), _code(gate), rows // groups, int(post_norm), scale, eps, ptr(x_new), ptr(h), ptr(stats),
-             stream_handle(dev))
+             ptr(_lib.status_word(dev)), stream_handle(dev))
     return x_new, h, stats
 
 
@@ -110,7 +110,7 @@ def _backward(x, y, pre, post, gate, groups, post_norm, scale, out_dtype, stats,
          _lib._DTYPES[out_dtype], y2.stride(0) if y2 is not None else 0, rows, width, ptr(pre), _code(pre),
          ptr(post), _code(post), ptr(gate), _code(gate), rows // groups, int(post_norm), scale, ptr(stats),
          ptr(dx_new), ptr(dh), ptr(dx), ptr(dy), *(ptr(g) for g in grads), ptr(ws),
-         ws.numel() if ws is not None else 0, stream_handle(dev))
+         ws.numel() if ws is not None else 0, ptr(_lib.status_word(dev)), stream_handle(dev))
     return dx, dy, *grads
 
 

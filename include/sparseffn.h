@@ -601,12 +601,13 @@ int sffn_distill_topk_bwd(const void* logits, int dtype, int64_t rows, int64_t v
  * y_dtype (x_dtype equals it or is SFFN_F32); x_new [rows, width] has x_dtype.
  * y NULL: h = rms(x) * pre alone.  pre, post, gate NULL: ones.  gate holds one
  * row of `width` for every gate_rows consecutive rows.  stats [rows, 2] (NULL:
- * not wanted) is for the backward.  No counterpart in the reference.
+ * not wanted) is for the backward.  Rows wider than 4096 wait, within bounds, for
+ * sums of other blocks (SFFN_STATUS_WAIT_TIMEOUT).  No counterpart in the reference.
  */
 int sffn_residual_norm(const void* x, int x_dtype, int64_t x_ld, const void* y, int y_dtype, int64_t y_ld,
                        int64_t rows, int64_t width, const void* pre, int pre_dtype, const void* post, int post_dtype,
                        const void* gate, int gate_dtype, int64_t gate_rows, int post_norm, float scale, float eps,
-                       void* x_new, void* h, float* stats, void* stream);
+                       void* x_new, void* h, float* stats, uint32_t* status_dev, void* stream);
 
 /* Scratch of the backward when a weight's or gate's gradient is wanted
  * (gate_rows 0: no gate, or neither its gradient nor post's is wanted). */
@@ -619,7 +620,7 @@ int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, const void*
                            int post_dtype, const void* gate, int gate_dtype, int64_t gate_rows, int post_norm,
                            float scale, const float* stats, const void* dx_new, const void* dh, void* dx, void* dy,
                            void* dpre, void* dpost, void* dgate, void* workspace, size_t workspace_bytes,
-                           void* stream);
+                           uint32_t* status_dev, void* stream);
 
 /* ---- bounded waits ------------------------------------------------------ */
 

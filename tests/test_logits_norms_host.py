@@ -205,7 +205,7 @@ def test_c_distill_refusals(lib):
 
 
 def test_c_norm_refusals(lib):
-    ok = [P, 0, 64, P, 1, 64, 10, 64, P, 0, P, 0, P, 0, 5, 1, 1.0, 1e-6, P, P, P, None]
+    ok = [P, 0, 64, P, 1, 64, 10, 64, P, 0, P, 0, P, 0, 5, 1, 1.0, 1e-6, P, P, P, P, None]
 
     def rc(f, base, **changes):
         a = list(base)
@@ -217,11 +217,11 @@ def test_c_norm_refusals(lib):
     assert rc(f, ok, _1=1, _4=2) == 2 and rc(f, ok, _1=1, _4=0) == 2 and rc(f, ok, _9=4) == 2
     assert rc(f, ok, _6=-1) == 1 and rc(f, ok, _7=0) == 1 and rc(f, ok, _7=16385) == 8 and rc(f, ok, _14=0) == 1
     assert rc(f, ok, _3=None) == 1 and rc(f, ok, _15=0) == 1 and rc(f, ok, _17=0.0) == 1
-    assert rc(f, ok, _0=None) == 1 and rc(f, ok, _18=None) == 1 and rc(f, ok, _19=None) == 1
+    assert rc(f, ok, _0=None) == 1 and rc(f, ok, _18=None) == 1 and rc(f, ok, _19=None) == 1 and rc(f, ok, _21=None) == 1
     assert rc(f, ok, _6=0) == 0
     for i, off in ((0, 2), (3, 1), (8, 2), (10, 2), (12, 2), (18, 2), (19, 1), (20, 4)):
         assert rc(f, ok, **{f"_{i}": vp((1 << 20) + off)}) == 3
-    b = [P, 0, 64, P, 1, 64, 10, 64, P, 0, P, 0, P, 0, 5, 1, 1.0, P, P, P, P, P, P, P, P, P, 1 << 20, None]
+    b = [P, 0, 64, P, 1, 64, 10, 64, P, 0, P, 0, P, 0, 5, 1, 1.0, P, P, P, P, P, P, P, P, P, 1 << 20, P, None]
     f = lib.sffn_residual_norm_bwd
     need = lib.sffn_residual_norm_bwd_workspace_bytes(10, 64, 5)
     assert rc(f, b, _26=need - 1) == 4 and rc(f, b, _25=None) == 3 and rc(f, b, _25=vp(8)) == 3
@@ -231,7 +231,7 @@ def test_c_norm_refusals(lib):
 
 
 def test_launches_of_the_norm_backward():
-    base = [None] * 28
+    base = [None] * 29
     assert _lib._launches("sffn_residual_norm_bwd", base) == 1
     assert _lib._launches("sffn_residual_norm_bwd", base[:23] + [vp(16)] + base[24:]) == 2
     assert _lib._launches("sffn_residual_norm_bwd", base[:23] + [vp(0)] + base[24:]) == 1
