@@ -223,32 +223,6 @@ __device__ __forceinline__ void join(Soft& a, float c, JoinSlots<NT>& slots, flo
     }
 }
 
-// Sum / maximum over the block for the short lists; every thread gets it.
-template <int NT>
-__device__ __forceinline__ float block_sum(float v, float* slots) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float r = 0.f;
-#pragma unroll
-    for (int i = 0; i < NT / 32; ++i) r += slots[i];
-    return r;
-}
-template <int NT>
-__device__ __forceinline__ float block_max(float v, float* slots) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float r = slots[0];
-#pragma unroll
-    for (int i = 1; i < NT / 32; ++i) r = fmaxf(r, slots[i]);
-    return r;
-}
-
 // Order of the alternatives: larger logits first, equal ones by lower index,
 // NaN above all (as torch.sort has it); -0 equals +0.
 __device__ __forceinline__ uint32_t order_bits(float x) {
@@ -930,10 +904,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
     // bucket: a bit for each class of this block's part, and before them a bit for
     // each of its vectors, 32 of a thread's to a word
     extern __shared__ uint32_t marked_vectors[];
-    __shared__ float slots[NT / 32];
     __shared__ JoinSlots<NT> join_slots;
     __shared__ PartOut mine;
     __shared__ int ids[TOP_MAX];
+    __shared__ float scores[TOP_MAX], logits_of[TOP_MAX];
+    __shared__ bool firsts[TOP_MAX];
     static_assert(NT >= TOP_MAX, "one entry a thread");
     const int t = threadIdx.x;
     const int of = a.parts, which = of > 1 ? blockIdx.x % of : 0;
@@ -942,11 +917,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
     const Cut<DT> cut(row, a.vocab, which, of);
     const float c = a.inv_t * LOG2E;
 
-    // The list: one entry a thread (threads past it hold none).
+    // The list: one entry a thread.
     int id = -1;
-    float score = -INFINITY, x = 0.f;
+    bool weighs = false;
     if (t < a.k) {
         const int64_t j = load_index(a.ids, r * a.k + t, a.id_bytes);
+        float score = -INFINITY, x = 0.f;
         if (j >= 0 && j < a.vocab) {
             id = (int)j;
             score = load_code(a.scores, r * a.k + t, a.score_code);
@@ -955,6 +931,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
             atomicOr(a.status, SFFN_STATUS_BAD_INDEX);
         }
         ids[t] = id;
+        scores[t] = score;
+        logits_of[t] = x;
+        weighs = score != -INFINITY;
     }
     // Classes are shifted so that a vector's bits lie in one word.
     const int pad = (N - cut.lead % N) % N;
@@ -963,9 +942,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
     uint32_t* const on_list = marked_vectors + words;
     if (a.bucket)
         for (int i = t; i < words + (cut.end() + pad - base + 31) / 32; i += NT) marked_vectors[i] = 0;
-    const float top = block_max<NT>(score, slots);
-    const float z = block_sum<NT>(id >= 0 && score != -INFINITY ? expf(score - (a.bucket ? 0.f : top)) : 0.f, slots);
-    if (z == 0.f) {  // no entry of positive weight (every block of the row sees the same)
+    if (!__syncthreads_or(weighs)) {  // no entry of positive weight (every block of the row sees the same)
         if (t == 0 && which == 0) {
             a.loss[r] = 0.f;
             for (int i = 0; i < 4; ++i) a.stats[4 * r + i] = 0.f;
@@ -973,29 +950,34 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
         return;
     }
     if (a.bucket) {
+        bool first = id >= 0, twice = of > 1;  // an id that stands twice is one class: its first entry's
         if (id >= cut.begin() && id < cut.end()) {
-            atomicOr(&on_list[(id + pad - base) >> 5], 1u << ((id + pad - base) & 31));
+            const int at = id + pad - base;
+            twice |= (atomicOr(&on_list[at >> 5], 1u << (at & 31)) >> (at & 31)) & 1;
             const int v = (id - cut.at(0)) / N;
             if (id >= cut.at(0) && v < cut.nvec) atomicOr(&marked_vectors[v / (32 * NT) * NT + v % NT], 1u << (v / NT % 32));
         }
-        __syncthreads();
+        if (__syncthreads_or(twice))
+#pragma unroll 8
+            for (int i = 0; i < a.k; ++i) first &= !(i < t && ids[i] == id);
+        if (t < a.k) firsts[t] = first;
     }
     Soft soft;
     static_assert(32 % AHEAD == 0, "an iteration's marks lie in one word");
     stream<DT, NT, false>(row, cut, c, soft,
-                   [&](int iteration) {
-                       const int i = iteration * AHEAD;
-                       return a.bucket ? marked_vectors[i / 32 * NT + t] >> (i % 32) : 0u;
-                   },
-                   [&](float* v, int i, auto count) {
-                       if (!a.bucket) return;
-                       constexpr int n = decltype(count)::value;
-                       const uint32_t on = on_list[(i + pad - base) >> 5] >> ((i + pad - base) & 31);
+                          [&](int iteration) {
+                              const int i = iteration * AHEAD;
+                              return a.bucket ? marked_vectors[i / 32 * NT + t] >> (i % 32) : 0u;
+                          },
+                          [&](float* v, int i, auto count) {
+                              if (!a.bucket) return;
+                              constexpr int n = decltype(count)::value;
+                              const uint32_t on = on_list[(i + pad - base) >> 5] >> ((i + pad - base) & 31);
 #pragma unroll
-                       for (int j = 0; j < n; ++j)
-                           if ((on >> j) & 1) v[j] = -INFINITY;
-                   },
-                   [](auto, float, int) {});
+                              for (int j = 0; j < n; ++j)
+                                  if ((on >> j) & 1) v[j] = -INFINITY;
+                          },
+                          [](auto, float, int) {});
     float m, s, w;
     join<NT>(soft, c, join_slots, m, s, w);
     if (of > 1) {
@@ -1007,24 +989,64 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
         if (which) return;
     }
 
+    // The rest is one warp's: the list's sums need no barrier so.
+    if (t >= 32) return;
+    constexpr int PER = TOP_MAX / 32;
+    auto max_of = [](float v) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+        return v;
+    };
+    auto sum_of = [](float v) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+        return v;
+    };
+    float score[PER], x[PER];
+    bool on[PER];
+    float top = -INFINITY, m_on = m;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int e = i * 32 + t;
+        on[i] = e < a.k && ids[e] >= 0;
+        score[i] = on[i] ? scores[e] : -INFINITY;
+        x[i] = on[i] ? logits_of[e] : -INFINITY;
+        top = fmaxf(top, score[i]);
+        m_on = fmaxf(m_on, x[i]);
+    }
+    top = a.bucket ? 0.f : max_of(top);
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (score[i] != -INFINITY) z += expf(score[i] - top);
+    z = sum_of(z);
     const float ln_z = a.bucket ? 0.f : top + logf(z);
-    const float ln_q = score - ln_z;
-    const float q = id >= 0 ? expf(ln_q) : 0.f;
     float off = 0.f;
     bool all_listed = false;
     if (a.bucket) {
-        bool first = id >= 0;  // an id that stands twice is one class
-#pragma unroll 8
-        for (int i = 0; i < a.k; ++i) first &= !(i < t && ids[i] == id);
-        all_listed = __syncthreads_count(first) == a.vocab;
         const float m_off = m, s_off = s;
-        m = block_max<NT>(id >= 0 ? fmaxf(x, m_off) : m_off, slots);
+        m = max_of(m_on);
         off = s_off * ex2(fmaxf((m_off - m) * c, D_MIN));
-        s = off + block_sum<NT>(first ? ex2(max_nan((x - m) * c, D_MIN)) : 0.f, slots);
+        float s_on = 0.f;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (on[i] && firsts[i * 32 + t]) {
+                s_on += ex2(max_nan((x[i] - m) * c, D_MIN));
+                ++n;
+            }
+        s = off + sum_of(s_on);
+        all_listed = __reduce_add_sync(FULL, n) == a.vocab;
     }
     const float ln_s = s == 0.f ? -INFINITY : logf(s);
-    const float ln_p = s == 0.f ? -INFINITY : (x - m) * a.inv_t - ln_s;
-    float loss = block_sum<NT>(q != 0.f ? q * (ln_q - ln_p) : 0.f, slots);
+    float loss = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const float ln_q = score[i] - ln_z, q = on[i] ? expf(ln_q) : 0.f;
+        const float ln_p = s == 0.f ? -INFINITY : (x[i] - m) * a.inv_t - ln_s;
+        if (q != 0.f) loss += q * (ln_q - ln_p);
+    }
+    loss = sum_of(loss);
     if (t == 0) {
         float factor = 1.f, more = ln_z;
         if (a.bucket) {

@@ -327,7 +327,7 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t barrier, int rank, fl
 // In a cluster each warp stores its sums to every block's slots (st.async), and
 // an mbarrier of each set counts the bytes: unlike the cluster's own barrier that
 // does not wait until the rows' stores to global memory are acknowledged (float32
-// 8192x8192 with bf16: 181 -> 138 us forward, 314 -> 239 us backward).  The wait is
+// 8192x8192 with bf16: 181 -> 155 us forward, 314 -> 273 us backward).  The wait is
 // bounded: when it runs out it sets SFFN_STATUS_WAIT_TIMEOUT and no later one waits.
 template <int N, bool WIDE>
 struct RowSums {

@@ -597,3 +597,17 @@ def test_ops_refuse_what_the_functions_refuse():
     for f in bad:
         with pytest.raises(ValueError):
             f()
+
+
+@pytest.mark.parametrize("rows", [3, 2000])
+def test_ids_listed_twice_give_equal_bits(rows):
+    """Whichever entry's thread comes first: the loss and its gradient are the same bits each time."""
+    x = randn(rows, 5000, seed=1, scale=2.0, dtype=torch.bfloat16).requires_grad_()
+    ids = torch.randint(0, 40, (rows, 100), generator=gen(2), device=DEV) * 120
+    scores = torch.log_softmax(randn(rows, 120, seed=3), -1)[:, :100].contiguous()
+    runs = []
+    for _ in range(8):
+        loss = sf.distill_topk(x, ids, scores, tail="bucket")
+        runs.append((loss.detach(), torch.autograd.grad(loss.sum(), x)[0]))
+    assert all(torch.equal(a, runs[0][0]) and torch.equal(b, runs[0][1]) for a, b in runs)
+    check_distill(x[:3], ids[:3], scores[:3], "bucket")
