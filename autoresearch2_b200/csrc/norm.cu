@@ -790,30 +790,35 @@ struct JoinArgs {
     int pre_code, post_code, gate_code;
 };
 
-__global__ void norm_join_kernel(const JoinArgs a) {
-    __shared__ float s[32][33];
+template <int JOIN_ROWS>  // threads of a column
+__global__ void __launch_bounds__(32 * JOIN_ROWS) norm_join_kernel(const JoinArgs a) {
+    __shared__ float s[JOIN_ROWS][32];
     const int x = threadIdx.x, y = threadIdx.y;
     const int col = blockIdx.x * 32 + x;
-    for (int64_t which = blockIdx.y; which < 3 + (a.gate_part && a.dgate ? (a.rows + a.gate_rows - 1) / a.gate_rows : 0);
-         which += gridDim.y) {
+    const int64_t gates = a.gate_part && a.dgate ? (a.rows + a.gate_rows - 1) / a.gate_rows : 0;
+    for (int64_t which = blockIdx.y; which < 3 + gates; which += gridDim.y) {
         if (which < 3 && (!((a.want >> which) & 1) || (which == 2 && a.gate_part))) continue;
-        float v = 0.f;
-        if (col < a.width) {
-            if (which < 3) {
-                for (int64_t b = y; b < a.blocks; b += 32) v += a.part[(b * 3 + which) * a.width + col];
-            } else {
-                const int64_t g = which - 3;
-                const int64_t first = g * a.gate_rows / a.per, last = (min(a.rows, (g + 1) * a.gate_rows) - 1) / a.per;
-                for (int64_t u = first + y; u <= last; u += 32) v += a.gate_part[(u + g) * a.width + col];
-            }
+        // rows first .. last, `step` floats apart, of the sums
+        const float* from = a.part + which * a.width;
+        int64_t first = 0, last = a.blocks - 1, step = 3 * (int64_t)a.width;
+        if (which >= 3) {  // the units that hold rows of gate row g
+            const int64_t g = which - 3;
+            from = a.gate_part + g * a.width;
+            first = g * a.gate_rows / a.per;
+            last = (min(a.rows, (g + 1) * a.gate_rows) - 1) / a.per;
+            step = a.width;
         }
+        float v = 0.f;
+        if (col < a.width)
+#pragma unroll 4
+            for (int64_t u = first + y; u <= last; u += JOIN_ROWS) v += from[u * step + col];
         __syncthreads();
         s[y][x] = v;
         __syncthreads();
         if (y == 0 && col < a.width) {
             float total = 0.f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) total += s[i][x];
+            for (int i = 0; i < JOIN_ROWS; ++i) total += s[i][x];
             if (which == 0) store_code(a.dpre, col, a.pre_code, total);
             else if (which == 1) store_code(a.dpost, col, a.post_code, total);
             else store_code(a.dgate, (which == 2 ? 0 : which - 3) * a.width + col, a.gate_code, total);
@@ -997,7 +1002,12 @@ extern "C" int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, 
                          dpre, dpost, dgate, pre_dtype, post_dtype, gate_dtype};
         const int64_t gates = gate_part ? (rows + gate_rows - 1) / gate_rows : 0;
         const int64_t ny = 3 + gates < 65535 ? 3 + gates : 65535;
-        norm_join_kernel<<<dim3((unsigned)((width + 31) / 32), (unsigned)ny), dim3(32, 32), 0, st>>>(j);
+        // Where the columns fill the SMs 8 threads add one up (the whole backward of
+        // 8192x8192 with 8 gate rows: 237 us, with 32 threads 273); fewer columns take
+        // 32, whose loads are in flight together (32768x768: 61 us, with 8 threads 63).
+        const dim3 grid((unsigned)((width + 31) / 32), (unsigned)ny);
+        if ((int64_t)grid.x * grid.y >= 4 * SMS) norm_join_kernel<8><<<grid, dim3(32, 8), 0, st>>>(j);
+        else norm_join_kernel<32><<<grid, dim3(32, 32), 0, st>>>(j);
         SFFN_CHECK_LAUNCH();
     }
     return SFFN_OK;
