@@ -315,7 +315,7 @@ struct ScoreArgs {
     int64_t ignore;
     int top_k;
     float inv_t;
-    float *logp, *entropy, *stats;
+    float *logp, *entropy, *stats;  // stats null: not kept
     int64_t* top_ids;
     float* top_logp;
     uint32_t* status;
@@ -612,8 +612,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a)
             if (t == 0) {
                 a.logp[r] = 0.f;
                 a.entropy[r] = 0.f;
-                a.stats[2 * r] = 0.f;
-                a.stats[2 * r + 1] = 0.f;
+                if (a.stats) a.stats[2 * r] = a.stats[2 * r + 1] = 0.f;
             }
             for (int i = t; i < a.top_k; i += NT) {
                 a.top_ids[r * a.top_k + i] = -1;
@@ -664,8 +663,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a)
             a.logp[r] = lp;
         }
         a.entropy[r] = s == 0.f ? 0.f : ln_s - w / s * LN2;
-        a.stats[2 * r] = m;
-        a.stats[2 * r + 1] = s;
+        if (a.stats) {
+            a.stats[2 * r] = m;
+            a.stats[2 * r + 1] = s;
+        }
     }
     if constexpr (TOP) {
         auto put = [&](int i, unsigned long long key) {
@@ -945,7 +946,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
     if (!__syncthreads_or(weighs)) {  // no entry of positive weight (every block of the row sees the same)
         if (t == 0 && which == 0) {
             a.loss[r] = 0.f;
-            for (int i = 0; i < 4; ++i) a.stats[4 * r + i] = 0.f;
+            for (int i = 0; a.stats && i < 4; ++i) a.stats[4 * r + i] = 0.f;
         }
         return;
     }
@@ -1060,6 +1061,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
             }
         }
         a.loss[r] = loss;
+        if (!a.stats) return;
         a.stats[4 * r] = m;
         a.stats[4 * r + 1] = s;
         a.stats[4 * r + 2] = factor;
@@ -1198,7 +1200,7 @@ extern "C" int sffn_token_logprobs(const void* logits, int dtype, int64_t rows, 
     if (top_k < 0 || top_k > vocab) return SFFN_ERR_ARG;
     if (top_k > TOP_MAX) return SFFN_ERR_TOO_LARGE;
     if (rows == 0) return SFFN_OK;
-    if (!entropy || !stats || !status_dev || (targets && !logp) || (top_k && (!top_ids || !top_logp)))
+    if (!entropy || !status_dev || (targets && !logp) || (top_k && (!top_ids || !top_logp)))
         return SFFN_ERR_ARG;
     if ((targets && !lies(targets, target_bytes)) || !lies(logp, 4) || !lies(entropy, 4) || !lies(stats, 4) ||
         !lies(top_ids, 8) || !lies(top_logp, 4) || !lies(status_dev, 4))
@@ -1270,7 +1272,7 @@ extern "C" int sffn_distill_topk(const void* logits, int dtype, int64_t rows, in
     if (int rc = check_logits(logits, dtype, rows, vocab, inner, s_outer, s_inner, inv_t)) return rc;
     if (rows == 0) return SFFN_OK;
     if (int rc = check_list(ids, id_bytes, scores, score_dtype, k, tail)) return rc;
-    if (!loss || !stats || !status_dev) return SFFN_ERR_ARG;
+    if (!loss || !status_dev) return SFFN_ERR_ARG;
     if (!lies(loss, 4) || !lies(stats, 4) || !lies(status_dev, 4)) return SFFN_ERR_ALIGN;
     const int bucket = tail == SFFN_TAIL_BUCKET;
     if (bucket && vocab > 1400000) return SFFN_ERR_TOO_LARGE;

@@ -111,14 +111,14 @@ def _check_kept(name, t, shape, device, dtype=torch.float32):
 # ---------------------------------------------------------------------------
 # token_logprobs
 # ---------------------------------------------------------------------------
-def _score_forward(logits, targets, top_k, temperature, ignore_index):
-    """(logp or an empty tensor, entropy, top_ids, top_logp, stats [..., 2])."""
+def _score_forward(logits, targets, top_k, temperature, ignore_index, keep=True):
+    """(logp or an empty tensor, entropy, top_ids, top_logp, stats [..., 2]; None without keep)."""
     dev, lead = logits.device, logits.shape[:-1]
     x, rows, inner, so, si = _rows(logits)
     f32 = torch.float32
     logp = x.new_empty(lead if targets is not None else (0,), dtype=f32)
     entropy = x.new_empty(lead, dtype=f32)
-    stats = x.new_empty((*lead, 2), dtype=f32)
+    stats = x.new_empty((*lead, 2), dtype=f32) if keep else None
     top_ids = x.new_empty((*lead, top_k), dtype=torch.int64)
     top_logp = x.new_empty((*lead, top_k), dtype=f32)
     if rows:
@@ -191,19 +191,19 @@ def token_logprobs(logits, targets=None, top_k=0, temperature=1.0, ignore_index=
     elif torch.is_grad_enabled() and logits.requires_grad:
         r = _TokenLogprobs.apply(logits, targets, top_k, temperature, ignore_index)
     else:
-        r = _score_forward(logits, targets, top_k, temperature, ignore_index)
+        r = _score_forward(logits, targets, top_k, temperature, ignore_index, keep=False)
     return TokenLogprobs(r[0] if targets is not None else None, r[1], r[2], r[3])
 
 
 # ---------------------------------------------------------------------------
 # distill_topk
 # ---------------------------------------------------------------------------
-def _distill_forward(logits, ids, scores, temperature, tail):
-    """(loss, stats [..., 4])."""
+def _distill_forward(logits, ids, scores, temperature, tail, keep=True):
+    """(loss, stats [..., 4]; None without keep)."""
     dev, lead = logits.device, logits.shape[:-1]
     x, rows, inner, so, si = _rows(logits)
     loss = x.new_empty(lead, dtype=torch.float32)
-    stats = x.new_empty((*lead, 4), dtype=torch.float32)
+    stats = x.new_empty((*lead, 4), dtype=torch.float32) if keep else None
     if rows:
         ids, scores = ids.contiguous(), scores.contiguous()
         call("sffn_distill_topk", ptr(x), _lib.dtype_code(x), rows, x.shape[-1], inner, so, si, ptr(ids),
@@ -282,4 +282,4 @@ def distill_topk(logits, teacher_ids, teacher_scores, temperature=1.0, tail="ren
         return torch.ops.sparseffn.distill_topk(logits, teacher_ids, teacher_scores, temperature, tail)[0]
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillTopk.apply(logits, teacher_ids, teacher_scores, temperature, tail)
-    return _distill_forward(logits, teacher_ids, teacher_scores, temperature, tail)[0]
+    return _distill_forward(logits, teacher_ids, teacher_scores, temperature, tail, keep=False)[0]

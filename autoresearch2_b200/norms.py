@@ -47,8 +47,12 @@ def _check_backward(x, y, dx_new, dh, stats, out_dtype):
         raise ValueError("stats are the forward's")
 
 
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _code(t):
-    return _lib.dtype_code(t) if t is not None else 0
+    return _lib._DTYPES[t.dtype] if t is not None else 0
 
 
 def _gate_groups(gate, x):
@@ -74,44 +78,53 @@ def _gate_groups(gate, x):
 
 def _forward(x, y, pre, post, gate, groups, post_norm, scale, eps, out_dtype, keep):
     """(x_new or None, h, stats or None)."""
-    width = x.shape[-1]
+    width, codes = x.shape[-1], _lib._DTYPES
     x2 = _matrix(x, width)
-    y2 = _matrix(y, width) if y is not None else None
     rows, dev = x2.shape[0], x.device
-    x_new = x.new_empty(x.shape) if y is not None else None
+    x_new, py, y_ld = None, None, 0
+    if y is not None:
+        y2 = _matrix(y, width)
+        x_new, py, y_ld = x.new_empty(x.shape), y2.data_ptr(), y2.stride(0)
     h = x.new_empty(x.shape, dtype=out_dtype)
     stats = x.new_empty((rows, 2), dtype=torch.float32) if keep else None
     if rows:
-        pre, post, gate = (t.contiguous() if t is not None else None for t in (pre, post, gate))
-        call("sffn_residual_norm", ptr(x2), _lib.dtype_code(x), x2.stride(0), ptr(y2), _code(h),
-             y2.stride(0) if y2 is not None else 0, rows, width, ptr(pre), _code(pre), ptr(post), _code(post),
-             ptr(gate), _code(gate), rows // groups, int(post_norm), scale, eps, ptr(x_new), ptr(h), ptr(stats),
-             ptr(_lib.status_word(dev)), stream_handle(dev))
+        pre, post, gate = _dense(pre), _dense(post), _dense(gate)
+        call("sffn_residual_norm", x2.data_ptr(), codes[x.dtype], x2.stride(0), py, codes[out_dtype], y_ld, rows, width,
+             ptr(pre), _code(pre), ptr(post), _code(post), ptr(gate), _code(gate), rows // groups, int(post_norm), scale,
+             eps, ptr(x_new), h.data_ptr(), ptr(stats), _lib.status_word(dev).data_ptr(), stream_handle(dev))
     return x_new, h, stats
 
 
 def _backward(x, y, pre, post, gate, groups, post_norm, scale, out_dtype, stats, dx_new, dh, want):
     """Gradients of (x, y, pre, post, gate); None where `want` is false."""
-    width = x.shape[-1]
+    width, codes = x.shape[-1], _lib._DTYPES
     x2 = _matrix(x, width)
-    y2 = _matrix(y, width) if y is not None else None
     rows, dev = x2.shape[0], x.device
+    py, y_ld, dy = None, 0, None
+    if y is not None:
+        y2 = _matrix(y, width)
+        py, y_ld = y2.data_ptr(), y2.stride(0)
+        dy = y.new_empty(y.shape) if want[1] else None
     dx = x.new_empty(x.shape) if want[0] else None
-    dy = y.new_empty(y.shape) if y is not None and want[1] else None
-    grads = [t.new_empty(t.shape) if t is not None and w else None for t, w in zip((pre, post, gate), want[2:])]
+    dpre = pre.new_empty(pre.shape) if pre is not None and want[2] else None
+    dpost = post.new_empty(post.shape) if post is not None and want[3] else None
+    dgate = gate.new_empty(gate.shape) if gate is not None and want[4] else None
     if not rows:
-        return dx, dy, *(g.zero_() if g is not None else None for g in grads)
-    pre, post, gate, dx_new, dh = (t.contiguous() if t is not None else None for t in (pre, post, gate, dx_new, dh))
-    ws = None
-    if any(g is not None for g in grads):
-        per = rows // groups if grads[1] is not None or grads[2] is not None else 0
-        ws = x.new_empty(_lib.load().sffn_residual_norm_bwd_workspace_bytes(rows, width, per), dtype=torch.uint8)
-    call("sffn_residual_norm_bwd", ptr(x2), _lib.dtype_code(x), x2.stride(0), ptr(y2),
-         _lib._DTYPES[out_dtype], y2.stride(0) if y2 is not None else 0, rows, width, ptr(pre), _code(pre),
-         ptr(post), _code(post), ptr(gate), _code(gate), rows // groups, int(post_norm), scale, ptr(stats),
-         ptr(dx_new), ptr(dh), ptr(dx), ptr(dy), *(ptr(g) for g in grads), ptr(ws),
-         ws.numel() if ws is not None else 0, ptr(_lib.status_word(dev)), stream_handle(dev))
-    return dx, dy, *grads
+        for g in (dpre, dpost, dgate):
+            if g is not None:
+                g.zero_()
+        return dx, dy, dpre, dpost, dgate
+    pre, post, gate, dx_new, dh = _dense(pre), _dense(post), _dense(gate), _dense(dx_new), _dense(dh)
+    ws, ws_bytes = None, 0
+    if dpre is not None or dpost is not None or dgate is not None:
+        per = rows // groups if dpost is not None or dgate is not None else 0
+        ws_bytes = _lib.load().sffn_residual_norm_bwd_workspace_bytes(rows, width, per)
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    call("sffn_residual_norm_bwd", x2.data_ptr(), codes[x.dtype], x2.stride(0), py, codes[out_dtype], y_ld, rows, width,
+         ptr(pre), _code(pre), ptr(post), _code(post), ptr(gate), _code(gate), rows // groups, int(post_norm), scale,
+         stats.data_ptr(), ptr(dx_new), ptr(dh), ptr(dx), ptr(dy), ptr(dpre), ptr(dpost), ptr(dgate), ptr(ws), ws_bytes,
+         _lib.status_word(dev).data_ptr(), stream_handle(dev))
+    return dx, dy, dpre, dpost, dgate
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -135,14 +148,14 @@ class _ResidualNorm(torch.autograd.Function):
 
 def _check(x, y, pre_weight, post_weight, gate, post_norm, residual_scale, eps, out_dtype):
     """h's type, of arguments that are refused otherwise (the gate's rows: _gate_groups)."""
-    _lib.require_cuda(*(t for t in (x, y, pre_weight, post_weight, gate) if t is not None))
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= WIDTH_MAX:
-        raise ValueError(f"residual_norm takes x [..., D] with 1 <= D <= {WIDTH_MAX}, got {tuple(x.shape)}")
-    for name, t in (("x", x), ("y", y), ("pre_weight", pre_weight), ("post_weight", post_weight), ("gate", gate)):
+    for t in (x, y, pre_weight, post_weight, gate):
         if t is not None:
+            _lib.require_cuda(t)
             _lib.dtype_code(t)
             if t.device != x.device:
-                raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+                raise ValueError(f"a tensor is on {t.device}, x on {x.device}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= WIDTH_MAX:
+        raise ValueError(f"residual_norm takes x [..., D] with 1 <= D <= {WIDTH_MAX}, got {tuple(x.shape)}")
     if y is None:
         if post_norm or post_weight is not None or gate is not None or residual_scale != 1.0:
             raise ValueError("post_norm, post_weight, gate and residual_scale go with a block output y")
@@ -153,10 +166,10 @@ def _check(x, y, pre_weight, post_weight, gate, post_norm, residual_scale, eps, 
         if out_dtype not in (None, y.dtype):
             raise TypeError(f"h has y's type {y.dtype}; out_dtype is for calls without y")
         out_dtype = y.dtype
-    if out_dtype not in _lib._DTYPES or (out_dtype != x.dtype and x.dtype != torch.float32):
+    if out_dtype != x.dtype and (out_dtype not in _lib._DTYPES or x.dtype != torch.float32):
         raise TypeError(f"x is {x.dtype}: h may be of the same type, or x float32 and h bfloat16 or float16")
     for name, t in (("pre_weight", pre_weight), ("post_weight", post_weight)):
-        if t is not None and tuple(t.shape) != (x.shape[-1],):
+        if t is not None and t.shape != x.shape[-1:]:
             raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(t.shape)}")
     if post_weight is not None and not post_norm:
         raise ValueError("post_weight goes with post_norm=True")
