@@ -1136,10 +1136,20 @@ int check_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int
     return SFFN_OK;
 }
 
-// The backward's blocks: up to 16384 elements of a row each (a whole number of
-// 16-byte vectors of any type), by 256 threads, or by 128 where that leaves a
-// thread at most 8 vectors: a row of 1024 16-bit logits takes 128 of them.
-constexpr int64_t BWD_PER = 16384;
+// Elements of a row that one block of the backward writes (whole 16-byte vectors
+// of any type): 65536, so that what a block does before its first vector counts
+// little (16384x50304 bf16: 509 us, with 16384 elements 561; with a list 535 and
+// 610); 16384 where that leaves fewer than 8192 blocks, whose last ones would
+// run alone (1000x131072 float32: 172 us instead of 182); down to 4096 for a
+// handful of rows (3x200003: 3.7 us, with 16384 elements 5.5).
+int64_t bwd_per(int64_t rows, int64_t vocab) {
+    int64_t per = 65536;
+    const auto blocks = [&] { return rows * ((vocab + per - 1) / per); };
+    while (per > 16384 && blocks() < 8192) per /= 2;
+    while (per > 4096 && blocks() < 4 * SMS) per /= 2;
+    return vocab < per ? vocab : per;
+}
+// By 256 threads, or by 128 where that leaves a thread at most 8 vectors.
 int bwd_threads(int64_t per, int dtype) { return per * esize_of(dtype) / 16 <= 8 * 128 ? 128 : 256; }
 
 // How a forward row is shared out.  With rows enough for eight blocks of 128 an
@@ -1236,7 +1246,7 @@ extern "C" int sffn_token_logprobs_bwd(const void* logits, int dtype, int64_t ro
         !lies(entropy, 4) || !lies(g_logp, 4) || !lies(g_entropy, 4) || !lies(g_top, 4))
         return SFFN_ERR_ALIGN;
     SFFN_BIND(scope, logits);
-    const int64_t per = vocab < BWD_PER ? vocab : BWD_PER;
+    const int64_t per = bwd_per(rows, vocab);
     const int64_t blocks = (vocab + per - 1) / per;
     if (blocks > 65535) return SFFN_ERR_TOO_LARGE;
     const ScoreBwdArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, targets, target_bytes, ignore_index,
@@ -1309,7 +1319,7 @@ extern "C" int sffn_distill_topk_bwd(const void* logits, int dtype, int64_t rows
     if (!stats || !g_loss || !grad) return SFFN_ERR_ARG;
     if (!lies(grad, esize_of(dtype)) || !lies(stats, 4) || !lies(g_loss, 4)) return SFFN_ERR_ALIGN;
     SFFN_BIND(scope, logits);
-    const int64_t per = vocab < BWD_PER ? vocab : BWD_PER;
+    const int64_t per = bwd_per(rows, vocab);
     const int64_t blocks = (vocab + per - 1) / per;
     if (blocks > 65535) return SFFN_ERR_TOO_LARGE;
     const DistillBwdArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, ids, id_bytes, scores, score_dtype,
