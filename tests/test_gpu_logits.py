@@ -611,3 +611,18 @@ def test_ids_listed_twice_give_equal_bits(rows):
         runs.append((loss.detach(), torch.autograd.grad(loss.sum(), x)[0]))
     assert all(torch.equal(a, runs[0][0]) and torch.equal(b, runs[0][1]) for a, b in runs)
     check_distill(x[:3], ids[:3], scores[:3], "bucket")
+
+
+@pytest.mark.parametrize("rows,V", [(3, 50000), (1300, 257)])
+def test_calls_without_gradients_give_the_bits_of_calls_with(rows, V):
+    x = randn(rows, V, seed=51, scale=2.0, dtype=torch.bfloat16)
+    t = torch.randint(0, V, (rows,), generator=gen(52), device=DEV)
+    ids, scores = teacher_list(randn(rows, V, seed=53, scale=2.0), 9)
+    leaf = x.clone().requires_grad_()
+    for call in (lambda x: sf.token_logprobs(x, t, top_k=7), lambda x: (sf.distill_topk(x, ids, scores, tail="bucket"),)):
+        kept = call(leaf)
+        with torch.no_grad():
+            inside = call(leaf)
+        for got in (call(x), inside):
+            for a, b in zip(got, kept):
+                assert not a.requires_grad and torch.equal(a, b)
