@@ -1138,7 +1138,7 @@ int check_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int
                  int64_t s_inner, float inv_t) {
     if (!dtype_ok(dtype)) return SFFN_ERR_DTYPE;
     if (rows < 0 || vocab < 1 || inner < 1 || s_outer < 0 || s_inner < 0) return SFFN_ERR_ARG;
-    if (!(inv_t > 0.f) || !isfinite(inv_t)) return SFFN_ERR_ARG;
+    if (!(inv_t > 0.f && inv_t < 2e30f)) return SFFN_ERR_ARG;  // D_MIN inv_t and c stay finite
     if (rows > 0 && !logits) return SFFN_ERR_ARG;
     if (rows > 0x7fffffffll || vocab > (1ll << 30)) return SFFN_ERR_TOO_LARGE;
     if (reinterpret_cast<uintptr_t>(logits) % esize_of(dtype)) return SFFN_ERR_ALIGN;

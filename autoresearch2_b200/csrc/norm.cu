@@ -19,7 +19,7 @@
 // backward six, and two things keep it from memory's rate: the instructions a
 // row costs beside its arithmetic, and the waits for its sums.  So a thread keeps
 // 8 columns for all its rows, with their weights and its sums of the weight
-// gradients in registers, and works on up to 4 rows at a time (backward: 2):
+// gradients in registers, and works on up to 4 rows at a time (backward: one):
 // their sums over a warp are formed together, each shuffle halving the number of
 // values a lane still carries, with one barrier for all.  Meanwhile its own part
 // of the next rows is copied to shared memory (cp.async; as each piece is copied
@@ -892,7 +892,6 @@ int check_norm(int x_dtype, int y_dtype, int64_t rows, int64_t width, int64_t x_
 bool lies(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % esize_of(dtype) == 0; }
 bool lies8(const void* p) { return reinterpret_cast<uintptr_t>(p) % 8 == 0; }
 bool row_aligned(const void* p, int64_t ld, int dtype) { return !p || (aligned16(p) && ld * esize_of(dtype) % 16 == 0); }
-
 
 template <class F>
 int by_types(int x_dtype, int y_dtype, F&& f) {

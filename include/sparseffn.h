@@ -542,7 +542,8 @@ int sffn_codec15_uncompress(const uint8_t* src, int64_t src_bytes, int64_t n, vo
 /* ---- output distribution -------------------------------------------------
  * logits [rows, vocab] of dtype; row r starts s_outer * (r / inner) +
  * s_inner * (r % inner) elements after `logits` (any alignment of the
- * element's size; inner = rows for one row stride).  inv_t = 1 / temperature.
+ * element's size; inner = rows for one row stride).  inv_t = 1 / temperature,
+ * positive and below 2e30.
  * Index tensors hold 4- or 8-byte integers (target_bytes, id_bytes).  No
  * counterpart in the reference.
  */
@@ -554,8 +555,8 @@ int sffn_codec15_uncompress(const uint8_t* src, int64_t src_bytes, int64_t n, vo
  * -inf.  A row of -inf has logp -inf, entropy 0, top_logp -inf; a row with NaN
  * or +inf has NaN.  Another target outside the vocabulary gives NaN and sets
  * SFFN_STATUS_BAD_INDEX.  stats [rows, 2] receives max and sum for the
- * backward (NULL: not wanted); top_k <= 128 (SFFN_ERR_TOO_LARGE beyond), top_ids and top_logp are
- * [rows, top_k]. */
+ * backward (NULL: not wanted); top_k <= 128 (SFFN_ERR_TOO_LARGE beyond),
+ * top_ids and top_logp are [rows, top_k]. */
 int sffn_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t inner, int64_t s_outer,
                         int64_t s_inner, const void* targets, int target_bytes, int64_t ignore_index, int top_k,
                         float inv_t, float* logp, float* entropy, float* stats, int64_t* top_ids, float* top_logp,
@@ -582,9 +583,9 @@ enum {
  * outside the vocabulary are absent too and set SFFN_STATUS_BAD_INDEX) and
  * scores [rows, k] (log probabilities, of score_dtype).  A row without an entry
  * of positive weight has loss 0.  An id that stands twice counts with both
- * weights.  stats [rows, 4] is for the backward (NULL: not
- * wanted).  With SFFN_TAIL_BUCKET the
- * vocabulary is at most 1,400,000 (SFFN_ERR_TOO_LARGE beyond). */
+ * weights.  stats [rows, 4] is for the backward (NULL: not wanted).  With
+ * SFFN_TAIL_BUCKET the vocabulary is at most 1,400,000 (SFFN_ERR_TOO_LARGE
+ * beyond). */
 int sffn_distill_topk(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t inner, int64_t s_outer,
                       int64_t s_inner, const void* ids, int id_bytes, const void* scores, int score_dtype, int k,
                       int tail, float inv_t, float* loss, float* stats, uint32_t* status_dev, void* stream);

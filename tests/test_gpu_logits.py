@@ -191,6 +191,25 @@ def test_score_extreme_float32_logits():
     check_score(x[2:], torch.tensor([3], device=DEV), 4, T=1e-3)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_score_at_the_limits_of_the_temperature(dtype):
+    """So hot that every class is alike; so cold that the largest logit has all."""
+    V = 3001
+    x = (torch.randperm(V, generator=gen(14), device=DEV) / 1024).repeat(3, 1).to(dtype)
+    x[1, 7] = 5.0
+    x[:, 90] = 8.0
+    t = torch.full((3,), 90, device=DEV)
+    x.requires_grad_()
+    r = sf.token_logprobs(x, t, top_k=1, temperature=1e30)
+    close(r.logp, torch.full((3,), -math.log(V), dtype=F64, device=DEV), torch.tensor(E(V) + 4 * U * math.log(V), device=DEV))
+    close(r.entropy, torch.full((3,), math.log(V), dtype=F64, device=DEV), torch.tensor((2 + 2 * math.log(V)) * E(V), device=DEV))
+    r = sf.token_logprobs(x, t, top_k=1, temperature=1e-30)
+    assert r.logp.tolist() == r.entropy.tolist() == r.top_logp[:, 0].tolist() == [0.0] * 3
+    assert r.top_ids[:, 0].tolist() == [90] * 3
+    if dtype == torch.float32:  # 1 / T is in the range of the gradient's type
+        assert not torch.autograd.grad(r.logp.sum() + r.entropy.sum(), x)[0].any()
+
+
 @pytest.mark.parametrize("V", [100, 20000])
 def test_score_nan_and_inf_rows(V):
     x = randn(3, V, seed=1)

@@ -51,7 +51,7 @@ def test_token_logprobs_refusals():
         for k in (-1, 11, 2.0, True):
             refused(ValueError, "top_k", f, x, t, top_k=k)
         refused(ValueError, "top_k", f, cuda(3, 1000), t, top_k=129)
-        for temperature in (0, -1.0, INF, float("nan"), 1e-320, "1"):
+        for temperature in (0, -1.0, INF, float("nan"), 1e-320, 2e-39, 1e-31, 1e31, "1"):
             refused(ValueError, "temperature", f, x, t, temperature=temperature)
 
 
@@ -161,7 +161,7 @@ def test_c_scores_refusals(lib):
     assert rc(_1=3) == 2 and rc(_2=-1) == 1 and rc(_3=0) == 1 and rc(_4=0) == 1 and rc(_5=-1) == 1
     assert rc(_0=None) == 1 and rc(_0=vp(2)) == 3 and rc(_0=vp(3), _1=1) == 3
     assert rc(_8=2) == 1 and rc(_10=-1) == 1 and rc(_10=101) == 1 and rc(_3=1000, _10=129) == 8
-    for t in (0.0, -1.0, INF, float("nan")):
+    for t in (0.0, -1.0, INF, float("nan"), 3e30):
         assert rc(_11=t) == 1
     for i in (12, 13, 15, 16, 17):
         assert rc(**{f"_{i}": None}) == 1
