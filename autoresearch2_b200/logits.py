@@ -73,7 +73,7 @@ def _grad_like(logits, rows, s_inner):
     ld = V + (s_inner - V) % n if rows > 1 else V
     at = logits.data_ptr() % 16 // logits.element_size()
     if ld == V and at == 0:
-        return logits.new_empty(logits.shape), V
+        return torch.empty_like(logits, memory_format=torch.contiguous_format), V
     flat = logits.new_empty(at + rows * ld)
     strides, step = [1], ld
     for k in reversed(logits.shape[:-1]):
@@ -115,11 +115,11 @@ def _score_forward(logits, targets, top_k, temperature, ignore_index, keep=True)
     dev, lead = logits.device, logits.shape[:-1]
     x, rows, inner, so, si = _rows(logits)
     f32 = torch.float32
-    logp = x.new_empty(lead if targets is not None else (0,), dtype=f32)
     entropy = x.new_empty(lead, dtype=f32)
+    logp = torch.empty_like(entropy) if targets is not None else x.new_empty(0, dtype=f32)
     stats = x.new_empty((*lead, 2), dtype=f32) if keep else None
     top_ids = x.new_empty((*lead, top_k), dtype=torch.int64)
-    top_logp = x.new_empty((*lead, top_k), dtype=f32)
+    top_logp = torch.empty_like(top_ids, dtype=f32)
     if rows:
         t = targets.contiguous() if targets is not None else None
         call("sffn_token_logprobs", ptr(x), _lib.dtype_code(x), rows, x.shape[-1], inner, so, si, ptr(t),
