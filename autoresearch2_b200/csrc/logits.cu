@@ -253,14 +253,25 @@ __device__ __forceinline__ void each(const void* row, const Cut<DT>& cut, F&& f)
     if (t < cut.tail) f(load1<DT>(row, cut.tail_at + t), cut.tail_at + t);
 }
 
+// f(entry) for the k <= TOP_MAX entries of a row's list, dealt out to the block's threads.
+template <int NT, class F>
+__device__ __forceinline__ void entries(int k, F&& f) {
+    if constexpr (NT >= TOP_MAX) {
+        if ((int)threadIdx.x < k) f((int)threadIdx.x);
+    } else {
+        for (int e = threadIdx.x; e < k; e += NT) f(e);
+    }
+}
+
 // One pass over the part: several vectors of a thread are loaded before the first
-// is used, DEEP of them where the pass has few other values to hold (8 instead of
-// 4: 16384x50304 bf16 scored in 282 us instead of 290, distilled with the bucket
-// in 330 instead of 354, 2047x32003 float32 in 43 instead of 48; rows of 1024 go
-// from 69 to 76 us for 32768), AHEAD beside the search of the alternatives.  edit(x, index) may replace elements: a single one, and those of a
-// vector where marks(iteration) has bit u set; seen(u, max, which) is
-// told each vector's largest (u: its place among those; which: the vector, or
-// -2 - index for a single element, with u = 0).  AGAIN: some are read again.
+// is used: DEEP of them (by blocks of 128, 8 instead of 4: 16384x50304 bf16 scored
+// in 282 us instead of 290, distilled with the bucket in 330 instead of 354), but
+// AHEAD beside the search of the alternatives, whose registers 8 would spill (8192
+// rows of it, k = 64: 257 us instead of 216).  edit(x, index) may replace elements:
+// a single one, and those of a vector where marks(iteration) has bit u set;
+// seen(u, max, which) is told each vector's largest (u: its place among those;
+// which: the vector, or -2 - index for a single element, with u = 0).  AGAIN: some
+// are read again.
 constexpr int AHEAD = 4, DEEP = 8;
 template <int DT, int NT, bool AGAIN, class Marks, class Edit, class Seen>
 __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, float c, Soft& soft, Marks&& marks, Edit&& edit,
@@ -645,8 +656,12 @@ __device__ __forceinline__ void join_parts(cooperative_groups::cluster_group& cl
     }
 }
 
+// Blocks of NT threads that an SM holds: with 64 registers a thread, or 72 in small
+// blocks, which spill nothing so.
+constexpr int blocks_per_sm(int nt) { return nt < 128 ? 896 / nt : 1024 / nt; }
+
 template <int DT, int NT, bool TOP>
-__global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const ScoreArgs a) {
+__global__ void __launch_bounds__(NT, blocks_per_sm(NT)) score_kernel(const ScoreArgs a) {
     __shared__ JoinSlots<NT> slots;
     __shared__ PartOut mine;
     __shared__ typename std::conditional<TOP, TopSlots, int>::type top_slots;
@@ -906,12 +921,13 @@ __global__ void __launch_bounds__(NT) score_bwd_kernel(const ScoreBwdArgs a) {
     // The places with a gradient of their own, rewritten whole: the target and the alternatives.
     bool hit = false;
     __syncthreads();
-    if (gt && t < a.top_k) {
-        const int64_t id = a.top_ids[r * a.top_k + t];
-        hit = id == target;
-        if (id >= begin && id < begin + n)
-            out[id] = Elt<DT>::from_f(weigh.one(Elt<DT>::to_f(row[id]), wa, wb) + a.inv_t * (gt[t] + (hit ? g : 0.f)));
-    }
+    if (gt)
+        entries<NT>(a.top_k, [&](int e) {
+            const int64_t id = a.top_ids[r * a.top_k + e];
+            hit |= id == target;
+            if (id >= begin && id < begin + n)
+                out[id] = Elt<DT>::from_f(weigh.one(Elt<DT>::to_f(row[id]), wa, wb) + a.inv_t * (gt[e] + (id == target ? g : 0.f)));
+        });
     if (!__syncthreads_or(hit) && t == 0 && has_target && target >= begin && target < begin + n)
         out[target] = Elt<DT>::from_f(weigh.one(Elt<DT>::to_f(row[target]), wa, wb) + a.inv_t * g);
 }
@@ -948,7 +964,7 @@ struct DistillArgs {
 constexpr float REST_FLOOR = 1.0f / (1 << 20);
 
 template <int DT, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(NT, blocks_per_sm(NT)) distill_kernel(const DistillArgs a) {
     using bits = typename Elt<DT>::bits;
     constexpr int N = Row<DT>::N;
     // bucket: a bit for each class of this block's part, and before them a bit for
@@ -959,7 +975,6 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
     __shared__ int ids[TOP_MAX];
     __shared__ float scores[TOP_MAX], logits_of[TOP_MAX];
     __shared__ bool firsts[TOP_MAX];
-    static_assert(NT >= TOP_MAX, "one entry a thread");
     const int t = threadIdx.x;
     const int of = a.parts, which = of > 1 ? blockIdx.x % of : 0;
     const int64_t r = of > 1 ? blockIdx.x / of : blockIdx.x;
@@ -967,24 +982,24 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
     const Cut<DT> cut(row, a.vocab, which, of);
     const float c = a.inv_t * LOG2E;
 
-    // The list: one entry a thread.
-    int id = -1;
+    // The list
     bool weighs = false;
-    if (t < a.k) {
-        const int64_t j = load_index(a.ids, r * a.k + t, a.id_bytes);
+    entries<NT>(a.k, [&](int e) {
+        const int64_t j = load_index(a.ids, r * a.k + e, a.id_bytes);
+        int id = -1;
         float score = -INFINITY, x = 0.f;
         if (j >= 0 && j < a.vocab) {
             id = (int)j;
-            score = load_code(a.scores, r * a.k + t, a.score_code);
+            score = load_code(a.scores, r * a.k + e, a.score_code);
             x = Elt<DT>::to_f(row[id]);
         } else if (j != -1 && which == 0) {
             atomicOr(a.status, SFFN_STATUS_BAD_INDEX);
         }
-        ids[t] = id;
-        scores[t] = score;
-        logits_of[t] = x;
-        weighs = score != -INFINITY;
-    }
+        ids[e] = id;
+        scores[e] = score;
+        logits_of[e] = x;
+        weighs |= score != -INFINITY;
+    });
     // Classes are shifted so that a vector's bits lie in one word.
     const int pad = (N - cut.lead % N) % N;
     const int base = (cut.begin() + pad) & ~31;
@@ -1000,17 +1015,24 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const DistillArg
         return;
     }
     if (a.bucket) {
-        bool first = id >= 0, twice = of > 1;  // an id that stands twice is one class: its first entry's
-        if (id >= cut.begin() && id < cut.end()) {
+        bool twice = of > 1;  // an id that stands twice is one class: its first entry's
+        entries<NT>(a.k, [&](int e) {
+            const int id = ids[e];
+            if (id < cut.begin() || id >= cut.end()) return;
             const int at = id + pad - base;
             twice |= (atomicOr(&on_list[at >> 5], 1u << (at & 31)) >> (at & 31)) & 1;
             const int v = (id - cut.at(0)) / N;
             if (id >= cut.at(0) && v < cut.nvec) atomicOr(&marked_vectors[v / (32 * NT) * NT + v % NT], 1u << (v / NT % 32));
-        }
-        if (__syncthreads_or(twice))
+        });
+        twice = __syncthreads_or(twice);
+        entries<NT>(a.k, [&](int e) {
+            const int id = ids[e];
+            bool first = id >= 0;
+            if (twice)
 #pragma unroll 8
-            for (int i = 0; i < a.k; ++i) first &= !(i < t && ids[i] == id);
-        if (t < a.k) firsts[t] = first;
+                for (int i = 0; i < a.k; ++i) first &= !(i < e && ids[i] == id);
+            firsts[e] = first;
+        });
     }
     Soft soft;
     static_assert(32 % DEEP == 0, "an iteration's marks lie in one word");
@@ -1152,23 +1174,22 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const DistillBwdArgs a)
     }
     const float g = a.g_loss[r] * a.inv_t, factor = a.stats[4 * r + 2], more = a.stats[4 * r + 3];
     const float Q = a.bucket ? more : 1.f, ln_z = a.bucket ? 0.f : more;
-    if (t < a.k) {
-        const int64_t j = load_index(a.ids, r * a.k + t, a.id_bytes);
+    entries<NT>(a.k, [&](int e) {
+        const int64_t j = load_index(a.ids, r * a.k + e, a.id_bytes);
         const bool ok = j >= 0 && j < a.vocab;
-        ids[t] = ok ? (int)j : -1;
-        qs[t] = ok ? expf(load_code(a.scores, r * a.k + t, a.score_code) - ln_z) : 0.f;
-    }
+        ids[e] = ok ? (int)j : -1;
+        qs[e] = ok ? expf(load_code(a.scores, r * a.k + e, a.score_code) - ln_z) : 0.f;
+    });
     const Weigh<DT> weigh(a.stats[4 * r], s, a.inv_t);
     weigh.template row<NT, false>(row + begin, out + begin, n, g * factor, 0.f);
     __syncthreads();
-    if (t < a.k) {
-        const int id = ids[t];
-        if (id >= begin && id < begin + n) {
-            float q = 0.f;  // an id that stands twice has the sum of its weights, from either entry
-            for (int i = 0; i < a.k; ++i) q += ids[i] == id ? qs[i] : 0.f;
-            out[id] = Elt<DT>::from_f(weigh.one(Elt<DT>::to_f(row[id]), g * Q, 0.f) - g * q);
-        }
-    }
+    entries<NT>(a.k, [&](int e) {
+        const int id = ids[e];
+        if (id < begin || id >= begin + n) return;
+        float q = 0.f;  // an id that stands twice has the sum of its weights, from either entry
+        for (int i = 0; i < a.k; ++i) q += ids[i] == id ? qs[i] : 0.f;
+        out[id] = Elt<DT>::from_f(weigh.one(Elt<DT>::to_f(row[id]), g * Q, 0.f) - g * q);
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -1198,23 +1219,39 @@ int64_t bwd_per(int64_t rows, int64_t vocab) {
     while (per > 4096 && blocks() < 4 * SMS) per /= 2;
     return vocab < per ? vocab : per;
 }
-// By 256 threads, or by 128 where that leaves a thread at most 8 vectors.
-int bwd_threads(int64_t per, int dtype) { return per * esize_of(dtype) / 16 <= 8 * 128 ? 128 : 256; }
+// By 256 threads, by 128 where that leaves a thread at most 8 vectors, by one warp
+// where that does (rows of 4 KB: 32768x1024 bf16 score 28 us, by 128 threads 55;
+// with a list 38 and 69): what a block does once a row counts most there.
+int bwd_threads(int64_t per, int dtype) {
+    const int64_t vectors = per * esize_of(dtype) / 16;
+    return vectors <= 8 * 32 ? 32 : vectors <= 8 * 128 ? 128 : 256;
+}
 
-// How a forward row is shared out.  With rows enough for eight blocks of 128 an
-// SM, one block takes a row: small blocks at different points of their rows keep
-// memory busy where one large block would wait for its own end.  With fewer, a
-// cluster of up to eight blocks takes it, each a part of at least 2048 elements;
-// where even those leave SMs half idle and a thread more than four vectors to
-// read, the blocks have 512 threads.
+// How a forward row is shared out.  With more than eight rows an SM, one block
+// takes a row: small blocks at different points of their rows keep memory busy
+// where one large block would wait for its own end, and the smaller the block, the
+// less a row costs beside its stream.  So it has `least` threads where the row is
+// at most 32 KB or a thread's loads are one go, else `wide`.  Scores: 32 and 64
+// (bf16, beside 128: 32768x1024 28 us and 74, 32768x8192 96 and 128; 16384x50304
+// 271 and 283; but float32 16384x16384 166 and 158).  Distillation: 32 and 128
+// (32768x1024 53 us and 109, 32768x8192 159 and 198; 64 threads would gain
+// nothing at 16384x50304, and at 131072 classes their bit lists leave room for few
+// blocks: 276 us and 175).  With alternatives: 128, for the runs.
+// With fewer rows, a cluster of up to eight blocks of 128 takes a row, each a part
+// of at least 2048 elements; where even those leave SMs half idle and a thread
+// more than four vectors to read, the blocks have 512 threads.
 struct Plan {
     int threads, parts;
 };
-Plan plan_rows(int64_t rows, int64_t vocab, int dtype) {
+Plan plan_rows(int64_t rows, int64_t vocab, int dtype, int least, int wide) {
     int parts = 1;
     while (parts < MAX_PARTS && rows * parts * 2 <= (int64_t)SMS * 8 && vocab / (parts * 2) >= 2048) parts *= 2;
     const int64_t vectors = vocab * esize_of(dtype) / 16 / parts;
-    return {rows * parts <= 2 * SMS && vectors > 4 * 128 ? 512 : 128, parts};
+    if (rows * parts <= 2 * SMS && vectors > 4 * 128) return {512, parts};
+    if (parts > 1) return {128, parts};
+    if (vectors <= DEEP * 32) return {least, 1};
+    if (rows <= (int64_t)SMS * 8) return {128, 1};
+    return {vectors <= 2048 ? least : wide, 1};
 }
 
 // Launches kernel over rows x parts blocks, the parts of a row as a cluster.
@@ -1265,13 +1302,15 @@ extern "C" int sffn_token_logprobs(const void* logits, int dtype, int64_t rows, 
         !lies(top_ids, 8) || !lies(top_logp, 4) || !lies(status_dev, 4))
         return SFFN_ERR_ALIGN;
     SFFN_BIND(scope, logits);
-    const Plan p = plan_rows(rows, vocab, dtype);
+    const Plan p = plan_rows(rows, vocab, dtype, top_k ? 128 : 32, top_k ? 128 : 64);
     const ScoreArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, targets, target_bytes, ignore_index,
                       top_k, inv_t, logp, entropy, stats, top_ids, top_logp, status_dev, p.parts};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define SFFN_CALL(DT)                                                                             \
-    SFFN_CUDA_TRY(launch_rows(p.threads == 512 ? (top_k ? score_kernel<DT, 512, true> : score_kernel<DT, 512, false>) \
-                                               : (top_k ? score_kernel<DT, 128, true> : score_kernel<DT, 128, false>), \
+#define SFFN_CALL(DT)                                                                                    \
+    SFFN_CUDA_TRY(launch_rows(top_k ? (p.threads == 512 ? score_kernel<DT, 512, true> : score_kernel<DT, 128, true>) \
+                              : p.threads == 512 ? score_kernel<DT, 512, false>                          \
+                              : p.threads == 128 ? score_kernel<DT, 128, false>                          \
+                              : p.threads == 64 ? score_kernel<DT, 64, false> : score_kernel<DT, 32, false>, \
                               p, rows, 0, st, a))
     SFFN_BY_DTYPE(dtype, SFFN_CALL);
 #undef SFFN_CALL
@@ -1302,9 +1341,11 @@ extern "C" int sffn_token_logprobs_bwd(const void* logits, int dtype, int64_t ro
                          top_k, inv_t, entropy, stats, top_ids, g_logp, g_entropy, top_k ? g_top : nullptr, grad,
                          grad_ld, (int)per};
     const dim3 grid((unsigned)rows, (unsigned)blocks);
+    const int nt = bwd_threads(per, dtype);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define SFFN_CALL(DT)                                                                \
-    if (bwd_threads(per, dtype) == 128) score_bwd_kernel<DT, 128><<<grid, 128, 0, st>>>(a); \
+    if (nt == 32) score_bwd_kernel<DT, 32><<<grid, 32, 0, st>>>(a); \
+    else if (nt == 128) score_bwd_kernel<DT, 128><<<grid, 128, 0, st>>>(a); \
     else score_bwd_kernel<DT, 256><<<grid, 256, 0, st>>>(a)
     SFFN_BY_DTYPE(dtype, SFFN_CALL);
 #undef SFFN_CALL
@@ -1335,7 +1376,7 @@ extern "C" int sffn_distill_topk(const void* logits, int dtype, int64_t rows, in
     if (!lies(loss, 4) || !lies(stats, 4) || !lies(status_dev, 4)) return SFFN_ERR_ALIGN;
     const int bucket = tail == SFFN_TAIL_BUCKET;
     if (bucket && vocab > 1400000) return SFFN_ERR_TOO_LARGE;
-    const Plan p = plan_rows(rows, vocab, dtype);
+    const Plan p = plan_rows(rows, vocab, dtype, 32, 128);
     // a bit for every class of a part (a vector more than its share, shifted by up
     // to 31 + 7 bits) and for every vector, in whole words of each thread
     const int64_t share = vocab / p.parts + 64;
@@ -1346,7 +1387,8 @@ extern "C" int sffn_distill_topk(const void* logits, int dtype, int64_t rows, in
                         k, bucket, inv_t, loss, stats, status_dev, p.parts};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define SFFN_CALL(DT)                                                                                    \
-    auto* kernel = p.threads == 512 ? distill_kernel<DT, 512> : distill_kernel<DT, 128>;                  \
+    auto* kernel = p.threads == 512 ? distill_kernel<DT, 512> : p.threads == 128 ? distill_kernel<DT, 128> \
+                                                                 : distill_kernel<DT, 32>;             \
     if (smem > 32 * 1024)                                                                                \
         SFFN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
     SFFN_CUDA_TRY(launch_rows(kernel, p, rows, smem, st, a))
@@ -1374,9 +1416,11 @@ extern "C" int sffn_distill_topk_bwd(const void* logits, int dtype, int64_t rows
     const DistillBwdArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, ids, id_bytes, scores, score_dtype,
                            k, tail == SFFN_TAIL_BUCKET, inv_t, stats, g_loss, grad, grad_ld, (int)per};
     const dim3 grid((unsigned)rows, (unsigned)blocks);
+    const int nt = bwd_threads(per, dtype);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define SFFN_CALL(DT)                                                                  \
-    if (bwd_threads(per, dtype) == 128) distill_bwd_kernel<DT, 128><<<grid, 128, 0, st>>>(a); \
+    if (nt == 32) distill_bwd_kernel<DT, 32><<<grid, 32, 0, st>>>(a); \
+    else if (nt == 128) distill_bwd_kernel<DT, 128><<<grid, 128, 0, st>>>(a); \
     else distill_bwd_kernel<DT, 256><<<grid, 256, 0, st>>>(a)
     SFFN_BY_DTYPE(dtype, SFFN_CALL);
 #undef SFFN_CALL

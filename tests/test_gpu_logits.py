@@ -4,7 +4,8 @@ out below), at the sizes, masks and strides where such kernels go wrong, and of
 their gradients against the formula and against central differences.
 
 Tolerances.  u = 2^-24 is half a float32 step.  One thread adds at most
-V / 128 + 64 terms in a row before the tree of a block, the exponential is
+V / 128 + 64 terms to each of its two sums before the tree of a block (by 32
+threads V / 64, at the sizes below no more), the exponential is
 within 2^-22 = 4 u, and an exponent d carries 3 roundings, 3 u |d|, whose mean
 under p is at most 3 u ln V.  So ln s is within
 
@@ -135,6 +136,22 @@ def test_score(dtype, rows, V, k, T):
     logits = randn(rows, V, seed=V + k, scale=3.0, dtype=dtype)
     targets = torch.randint(0, V, (rows,), generator=gen(1), device=DEV)
     check_score(logits, targets, k, T)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", [(1301, 771), (1301, 5003), (1190, 16411)])
+def test_many_rows(dtype, rows, V):
+    """Rows enough for a small block each."""
+    x = randn(rows, V, seed=V, scale=2.5, dtype=dtype)
+    x[::7, ::2] = -INF
+    x[5] = -INF
+    t = torch.randint(0, V, (rows,), generator=gen(2), device=DEV)
+    t[::5] = -100
+    check_score(x, t, 0)
+    ids, scores = teacher_list(x, 70)
+    ids[3::4, 1::3] = -1
+    for tail in ("renorm", "bucket"):
+        check_distill(x, ids, scores, tail)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
