@@ -5,6 +5,7 @@ raises instead of falling back to another implementation.
 """
 import ctypes
 import os
+import threading
 
 import torch
 
@@ -239,6 +240,20 @@ def stream_handle(device):
     """The handle of the device's current stream, without the Stream object
     around it that stream_ptr makes (a tenth of its time)."""
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_thread = threading.local()
+
+
+def bind_thread(device):
+    """Makes the thread's current device, where it is `device`, current in the
+    CUDA runtime too.  Autograd's worker threads put that off until their first
+    torch kernel, and each allocation before it asks the driver whether the
+    device is in use (6 us instead of 1.3)."""
+    if not getattr(_thread, "bound", False):
+        _thread.bound = True
+        if torch.cuda.current_device() == device.index:
+            torch.cuda.set_device(device)
 
 
 def require_cuda(*tensors):

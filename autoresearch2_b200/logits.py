@@ -130,6 +130,7 @@ def _score_forward(logits, targets, top_k, temperature, ignore_index, keep=True)
 
 
 def _score_backward(logits, targets, top_ids, entropy, stats, g_logp, g_entropy, g_top, temperature, ignore_index):
+    _lib.bind_thread(logits.device)
     x, rows, inner, so, si = _rows(logits)
     grad, ld = _grad_like(x, rows, si)
     if rows:
@@ -212,6 +213,7 @@ def _distill_forward(logits, ids, scores, temperature, tail, keep=True):
 
 
 def _distill_backward(logits, ids, scores, stats, g_loss, temperature, tail):
+    _lib.bind_thread(logits.device)
     x, rows, inner, so, si = _rows(logits)
     grad, ld = _grad_like(x, rows, si)
     if rows:

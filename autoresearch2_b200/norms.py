@@ -102,6 +102,7 @@ def _forward(x, y, pre, post, gate, groups, post_norm, scale, eps, out_dtype, ke
 
 def _backward(x, y, pre, post, gate, groups, post_norm, scale, out_dtype, stats, dx_new, dh, want):
     """Gradients of (x, y, pre, post, gate); None where `want` is false."""
+    _lib.bind_thread(x.device)
     width, codes = x.shape[-1], _lib._DTYPES
     x2 = _matrix(x, width)
     rows, dev = x2.shape[0], x.device
