@@ -890,8 +890,9 @@ struct Weigh {
     }
 };
 
+// (with the 54 registers it would take unbounded: 539 us where it takes 509)
 template <int DT, int NT>
-__global__ void __launch_bounds__(NT) score_bwd_kernel(const ScoreBwdArgs a) {
+__global__ void __launch_bounds__(NT, NT < 128 ? 32 : 1280 / NT) score_bwd_kernel(const ScoreBwdArgs a) {
     using bits = typename Elt<DT>::bits;
     const int t = threadIdx.x;
     const int64_t r = a.rows - 1 - blockIdx.x;  // the rows that the forward read last may still be in L2
