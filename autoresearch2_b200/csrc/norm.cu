@@ -833,7 +833,9 @@ constexpr int64_t MAX_WIDTH = (int64_t)MAX_PARTS * MAX_WARPS * 32 * CH;
 
 // A block holds as many groups as make about 512 threads, but no more than there
 // are rows (`at_a_time` of them to a group) for all SMs; one such block runs on
-// an SM (128 registers a thread).
+// an SM (128 registers a thread).  Of clusters of 4 blocks the SMs of one GPC
+// hold 33 together, not 37: with 37 the last ones ran alone, in twice the time
+// (bf16 4096x16384: 234 us forward, 397 backward; with 32 137 and 232).
 Shape shape_of(int64_t rows, int64_t width, int at_a_time, int blocks_per_sm) {
     Shape s;
     const int64_t block_cols = MAX_WARPS * 32 * CH;
@@ -843,7 +845,8 @@ Shape shape_of(int64_t rows, int64_t width, int at_a_time, int blocks_per_sm) {
     s.groups = s.parts > 1 ? 1 : MAX_WARPS / s.warps;
     const int64_t share = rows / (SMS * at_a_time);
     if (share < s.groups) s.groups = (int)std::max<int64_t>(share, 1);
-    const int64_t most = (int64_t)SMS * blocks_per_sm / s.parts * (MAX_WARPS / (s.warps * s.groups));
+    const int64_t fit = s.parts == 4 ? 32 : SMS / s.parts;
+    const int64_t most = fit * blocks_per_sm * (MAX_WARPS / (s.warps * s.groups));
     const int64_t want = (rows + s.groups - 1) / s.groups;
     const int64_t sets = want < most ? want : most;
     s.per = (rows + sets * s.groups - 1) / (sets * s.groups);
