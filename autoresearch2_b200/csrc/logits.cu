@@ -158,6 +158,9 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // after a row's first vector hardly ever; e^d then reaches 2^32, whose sum over
 // any row is far inside float32.
 constexpr float SLACK = 32.0f;
+// Without W (distillation, which wants no entropy) no w is kept, nor are exponents
+// held above -inf for it: 16384x50304 bf16 with the bucket 307 us instead of 332.
+template <bool W>
 struct Soft {
     float m = LOWEST, limit = LOWEST;
     uint64_t s = 0, w = 0;
@@ -165,18 +168,20 @@ struct Soft {
         limit = to + SLACK / c;
         const float by = fmaxf((m - to) * c, D_MIN);
         const float f = ex2(by);
-        w = mul2(fma2(s, pair(by, by), w), pair(f, f));
+        if (W) w = mul2(fma2(s, pair(by, by), w), pair(f, f));
         s = mul2(s, pair(f, f));
         m = to;
     }
     __device__ __forceinline__ void add(float x0, float x1, float c) {
         float d0, d1;
         unpair(mul2(add2(pair(x0, x1), pair(-m, -m)), pair(c, c)), d0, d1);
-        d0 = max_nan(d0, D_MIN);
-        d1 = max_nan(d1, D_MIN);
+        if (W) {
+            d0 = max_nan(d0, D_MIN);
+            d1 = max_nan(d1, D_MIN);
+        }
         const uint64_t e = pair(ex2(d0), ex2(d1));
         s = add2(s, e);
-        w = fma2(e, pair(d0, d1), w);
+        if (W) w = fma2(e, pair(d0, d1), w);
     }
     __device__ __forceinline__ void one(float x, float c) {
         if (x > limit) raise(x, c);
@@ -191,8 +196,8 @@ struct JoinSlots {
     float m[NT / 32];
     float2 sw[NT / 32];
 };
-template <int NT>
-__device__ __forceinline__ void join(Soft& a, float c, JoinSlots<NT>& slots, float& m, float& s, float& w) {
+template <int NT, bool W>
+__device__ __forceinline__ void join(Soft<W>& a, float c, JoinSlots<NT>& slots, float& m, float& s, float& w) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     m = a.m;
 #pragma unroll
@@ -265,7 +270,7 @@ __device__ __forceinline__ void entries(int k, F&& f) {
 
 // One pass over the part: several vectors of a thread are loaded before the first
 // is used: DEEP of them (by blocks of 128, 8 instead of 4: 16384x50304 bf16 scored
-// in 282 us instead of 290, distilled with the bucket in 330 instead of 354), but
+// in 282 us instead of 290, distilled, w kept, in 330 instead of 354), but
 // AHEAD beside the search of the alternatives, whose registers 8 would spill (8192
 // rows of it, k = 64: 257 us instead of 216).  edit(x, index) may replace elements:
 // a single one, and those of a vector where marks(iteration) has bit u set;
@@ -273,8 +278,8 @@ __device__ __forceinline__ void entries(int k, F&& f) {
 // which: the vector, or -2 - index for a single element, with u = 0).  AGAIN: some
 // are read again.
 constexpr int AHEAD = 4, DEEP = 8;
-template <int DT, int NT, bool AGAIN, class Marks, class Edit, class Seen>
-__device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, float c, Soft& soft, Marks&& marks, Edit&& edit,
+template <int DT, int NT, bool AGAIN, bool W, class Marks, class Edit, class Seen>
+__device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, float c, Soft<W>& soft, Marks&& marks, Edit&& edit,
                                        Seen&& seen) {
     constexpr int N = Row<DT>::N, LOADS = AGAIN ? AHEAD : DEEP;
     const int t = threadIdx.x;
@@ -688,7 +693,7 @@ __global__ void __launch_bounds__(NT, blocks_per_sm(NT)) score_kernel(const Scor
     const void* row = reinterpret_cast<const typename Elt<DT>::bits*>(a.logits) + a.map.at(r);
     const Cut<DT> cut(row, a.vocab, which, of);
     const float c = a.inv_t * LOG2E;
-    Soft soft;
+    Soft<true> soft;
     constexpr int SUB = TOP ? RUNS / NT : 1;
     float top[SUB], second[SUB];  // of each run: the largest vector maximum, the largest of the other vectors'
     int held[SUB];                // the vector that holds it (-2 - index: a single element), -1 in an empty run
@@ -1035,7 +1040,7 @@ __global__ void __launch_bounds__(NT, blocks_per_sm(NT)) distill_kernel(const Di
             firsts[e] = first;
         });
     }
-    Soft soft;
+    Soft<false> soft;
     static_assert(32 % DEEP == 0, "an iteration's marks lie in one word");
     stream<DT, NT, false>(row, cut, c, soft,
                           [&](int iteration) {
@@ -1235,9 +1240,9 @@ int bwd_threads(int64_t per, int dtype) {
 // at most 32 KB or a thread's loads are one go, else `wide`.  Scores: 32 and 64
 // (bf16, beside 128: 32768x1024 28 us and 74, 32768x8192 96 and 128; 16384x50304
 // 271 and 283; but float32 16384x16384 166 and 158).  Distillation: 32 and 128
-// (32768x1024 53 us and 109, 32768x8192 159 and 198; 64 threads would gain
-// nothing at 16384x50304, and at 131072 classes their bit lists leave room for few
-// blocks: 276 us and 175).  With alternatives: 128, for the runs.
+// (both with w still kept: 32768x1024 53 us and 109, 32768x8192 159 and 198; 64
+// threads would gain nothing at 16384x50304, and at 131072 classes their bit lists
+// leave room for few blocks: 276 us and 175).  With alternatives: 128, for the runs.
 // With fewer rows, a cluster of up to eight blocks of 128 takes a row, each a part
 // of at least 2048 elements; where even those leave SMs half idle and a thread
 // more than four vectors to read, the blocks have 512 threads.
