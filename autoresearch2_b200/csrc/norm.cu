@@ -83,6 +83,11 @@ __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
     Pair r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
@@ -329,8 +334,9 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t barrier, int rank, fl
 // does not wait until the rows' stores to global memory are acknowledged (float32
 // 8192x8192 with bf16: 181 -> 155 us forward, 314 -> 273 us backward).  The wait is
 // bounded: when it runs out it sets SFFN_STATUS_WAIT_TIMEOUT and no later one waits.
-template <int N, bool WIDE>
+template <int N, bool WIDE, int SUBS>
 struct RowSums {
+    static constexpr int LANES = 32 / SUBS;
     static constexpr int POW = N <= 1 ? 1 : N <= 2 ? 2 : 4;
     static_assert(N <= 4, "one 16-byte slot a warp");
     float4* slots;  // [2][fold] of this group, zeroed
@@ -349,7 +355,7 @@ struct RowSums {
         float w[POW];
 #pragma unroll
         for (int i = 0; i < POW; ++i) w[i] = i < N ? v[i < N ? i : 0] : 0.f;
-        int o = 16;
+        int o = LANES / 2;
 #pragma unroll
         for (int n = POW; n > 1; n >>= 1, o >>= 1) {
             const bool up = lane & o;
@@ -361,9 +367,9 @@ struct RowSums {
         }
 #pragma unroll
         for (; o; o >>= 1) w[0] += __shfl_xor_sync(FULL, w[0], o);
-        if (!WIDE && fold == 1) {  // one warp: value i is in lanes i * 32 / POW on
+        if (SUBS > 1 || (!WIDE && fold == 1)) {  // one warp: value i is in lanes i * LANES / POW on
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = __shfl_sync(FULL, w[0], i * (32 / POW));
+            for (int i = 0; i < N; ++i) v[i] = __shfl_sync(FULL, w[0], (SUBS > 1 ? lane & ~(LANES - 1) : 0) + i * (LANES / POW));
             return;
         }
         float4* s = slots + set;
@@ -431,7 +437,7 @@ struct NormArgs {
     uint32_t* status;
 };
 
-template <int TX, int TY, bool VEC, bool WIDE>
+template <int TX, int TY, bool VEC, bool WIDE, int SUBS>
 __global__ void __launch_bounds__(MAX_WARPS * 32, FWD_RING<TX, TY, VEC> ? 1 : 2) norm_kernel(const NormArgs a) {
     constexpr int R = FWD_ROWS<TX, TY, VEC>, S = STAGES<TX, TY>, ROW = BYTES<TX> + BYTES<TY>;
     constexpr bool ringed = FWD_RING<TX, TY, VEC>;
@@ -444,7 +450,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, FWD_RING<TX, TY, VEC> ? 1 : 2)
     const int threads = blockDim.x, lane = threadIdx.x & 31, warps = a.shape.warps;
     const int group = (threadIdx.x >> 5) / warps, warp = (threadIdx.x >> 5) % warps;
     const int parts = WIDE ? a.shape.parts : 1, part = WIDE ? blockIdx.x % parts : 0;
-    const Place<MODE> pl(warp, lane, part * a.shape.cols, min(a.width, (part + 1) * a.shape.cols));
+    const int sub = SUBS > 1 ? lane / (32 / SUBS) : 0;  // which of the SUBS rows that the warp has side by side
+    const Place<MODE> pl(warp, lane % (32 / SUBS), part * a.shape.cols, min(a.width, (part + 1) * a.shape.cols));
     for (int i = threadIdx.x; i < SLOTS; i += threads) slots[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (WIDE) {
         if (threadIdx.x == 0) {
@@ -457,10 +464,13 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, FWD_RING<TX, TY, VEC> ? 1 : 2)
         __syncthreads();
     }
     const int fold = fold_of(warps * parts);
-    RowSums<R, WIDE> sum(slots + group * 2 * fold, fold, warps, warp, lane, group + 1, parts, part, filled, a.status);
+    RowSums<R, WIDE, SUBS> sum(slots + group * 2 * fold, fold, warps, warp, lane, group + 1, parts, part, filled, a.status);
     const float inv_width = 1.0f / a.width;
     const int64_t begin = ((int64_t)(blockIdx.x / parts) * a.shape.groups + group) * a.shape.per;
-    const int rows = (int)max((int64_t)0, min(a.rows - begin, a.shape.per));
+    const int count = (int)max((int64_t)0, min(a.rows - begin, a.shape.per));
+    const int rows = (count + SUBS - 1) / SUBS;  // of this lane, the last one perhaps behind the end
+    auto row_of = [&](int r) { return (int64_t)r * SUBS + sub; };
+    auto there = [&](int r) { return SUBS == 1 || r * SUBS + sub < count; };
     const bx* const px = reinterpret_cast<const bx*>(a.x) + begin * a.x_ld;
     const by* const py = reinterpret_cast<const by*>(a.y) + (a.y ? begin * a.y_ld : 0);
     bx* const po = reinterpret_cast<bx*>(a.x_new) + (a.x_new ? begin * a.width : 0);
@@ -472,8 +482,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, FWD_RING<TX, TY, VEC> ? 1 : 2)
     auto ahead = [&]() {
 #pragma unroll
         for (int k = 0; k < R; ++k)
-            if (next + k < rows) {
-                const int64_t r = next + k;
+            if (next + k < rows && there(next + k)) {
+                const int64_t r = row_of(next + k);
                 copy8<TX, MODE>(to + ROW * k * threads, threads, px + r * a.x_ld + pl.from, pl);
                 if (a.y) copy8<TY, MODE>(to + (ROW * k + BYTES<TX>) * threads, threads, py + r * a.y_ld + pl.from, pl);
             }
@@ -514,9 +524,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, FWD_RING<TX, TY, VEC> ? 1 : 2)
                 Pair ss = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) y[k][i] = 0;
-                if (a.y && k >= k0 && k < k1) {
+                if (a.y && k >= k0 && k < k1 && there(r0 + k)) {
                     if constexpr (ringed) take8<TY, MODE>(from + (ROW * k + BYTES<TX>) * threads, threads, y[k]);
-                    else load8<TY, MODE>(py + (r0 + k) * a.y_ld, pl, y[k]);
+                    else load8<TY, MODE>(py + row_of(r0 + k) * a.y_ld, pl, y[k]);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) ss = fma2(y[k][i], y[k][i], ss);
@@ -531,9 +541,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, FWD_RING<TX, TY, VEC> ? 1 : 2)
             for (int k = 0; k < R; ++k) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[k][i] = 0;
-                if (k >= k0 && k < k1) {
+                if (k >= k0 && k < k1 && there(r0 + k)) {
                     if constexpr (ringed) take8<TX, MODE>(from + ROW * k * threads, threads, x[k]);
-                    else load8<TX, MODE>(px + (r0 + k) * a.x_ld, pl, x[k]);
+                    else load8<TX, MODE>(px + row_of(r0 + k) * a.x_ld, pl, x[k]);
                     if (a.y) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
@@ -548,14 +558,14 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, FWD_RING<TX, TY, VEC> ? 1 : 2)
             sum(t);
 #pragma unroll
             for (int k = 0; k < R; ++k) {
-                if (k < k0 || k >= k1) continue;
-                if (a.y) store8<TX, MODE>(po + (int64_t)(r0 + k) * a.width, pl, x[k]);
+                if (k < k0 || k >= k1 || !there(r0 + k)) continue;
+                if (a.y) store8<TX, MODE>(po + row_of(r0 + k) * a.width, pl, x[k]);
                 t[k] = rsqrtf(fmaf(t[k], inv_width, a.eps));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[k][i] = mul2(mul2(x[k][i], both(t[k])), pre[i]);
-                store8<TY, MODE>(ph + (int64_t)(r0 + k) * a.width, pl, x[k]);
-                if (a.stats && part == 0 && warp == 0 && lane == 0)
-                    reinterpret_cast<float2*>(a.stats)[begin + r0 + k] = make_float2(r1[k], t[k]);
+                store8<TY, MODE>(ph + row_of(r0 + k) * a.width, pl, x[k]);
+                if (a.stats && part == 0 && warp == 0 && lane % (32 / SUBS) == 0)
+                    reinterpret_cast<float2*>(a.stats)[begin + row_of(r0 + k)] = make_float2(r1[k], t[k]);
             }
             k0 = k1;
         } while (k0 < min(R, rows - r0));
@@ -586,7 +596,7 @@ struct NormBwdArgs {
 
 enum { WANT_PRE = 1, WANT_POST = 2, WANT_GATE = 4 };
 
-template <int TX, int TY, bool VEC, bool WIDE>
+template <int TX, int TY, bool VEC, bool WIDE, int SUBS>
 __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormBwdArgs a) {
     constexpr int S = BWD_STAGES<TX, TY>, ROW = 2 * (BYTES<TX> + BYTES<TY>);
     constexpr bool ringed = BWD_RING<TX, TY, VEC>;
@@ -599,7 +609,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
     const int threads = blockDim.x, lane = threadIdx.x & 31, warps = a.shape.warps;
     const int group = (threadIdx.x >> 5) / warps, warp = (threadIdx.x >> 5) % warps;
     const int parts = WIDE ? a.shape.parts : 1, part = WIDE ? blockIdx.x % parts : 0;
-    const Place<MODE> pl(warp, lane, part * a.shape.cols, min(a.width, (part + 1) * a.shape.cols));
+    const int sub = SUBS > 1 ? lane / (32 / SUBS) : 0;  // which of the SUBS rows that the warp has side by side
+    const Place<MODE> pl(warp, lane % (32 / SUBS), part * a.shape.cols, min(a.width, (part + 1) * a.shape.cols));
     for (int i = threadIdx.x; i < SLOTS; i += threads) slots[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (WIDE) {
         if (threadIdx.x == 0) {
@@ -612,25 +623,27 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
         __syncthreads();
     }
     const int fold = fold_of(warps * parts);
-    RowSums<3, WIDE> sum(slots + group * 2 * fold, fold, warps, warp, lane, group + 1, parts, part, filled, a.status);
+    RowSums<3, WIDE, SUBS> sum(slots + group * 2 * fold, fold, warps, warp, lane, group + 1, parts, part, filled, a.status);
     const float inv_width = 1.0f / a.width;
     const int64_t block = blockIdx.x / parts;
     const int64_t unit = block * a.shape.groups + group, begin = unit * a.shape.per;
-    const int rows = (int)max((int64_t)0, min(a.rows - begin, a.shape.per));
-    const int64_t flat = begin * a.width;  // of the contiguous arrays
+    const int count = (int)max((int64_t)0, min(a.rows - begin, a.shape.per));
+    const int rows = (count + SUBS - 1) / SUBS;  // of this lane, the last one perhaps behind the end
+    auto there = [&](int r) { return SUBS == 1 || r * SUBS + sub < count; };
+    const int64_t flat = (begin + sub) * a.width;  // of the contiguous arrays
     const bool has_x = a.dx_new != nullptr, has_y = a.y != nullptr, has_h = a.dh != nullptr;
-    const bx* px = reinterpret_cast<const bx*>(a.x) + begin * a.x_ld;
-    const by* py = has_y ? reinterpret_cast<const by*>(a.y) + begin * a.y_ld : nullptr;
+    const bx* px = reinterpret_cast<const bx*>(a.x) + (begin + sub) * a.x_ld;
+    const by* py = has_y ? reinterpret_cast<const by*>(a.y) + (begin + sub) * a.y_ld : nullptr;
     const bx* pe = has_x ? reinterpret_cast<const bx*>(a.dx_new) + flat : nullptr;
     const by* pt = has_h ? reinterpret_cast<const by*>(a.dh) + flat : nullptr;
     bx* po = a.dx ? reinterpret_cast<bx*>(a.dx) + flat : nullptr;
     by* pq = a.dy ? reinterpret_cast<by*>(a.dy) + flat : nullptr;
-    const float2* stats = reinterpret_cast<const float2*>(a.stats) + begin;
+    const float2* stats = reinterpret_cast<const float2*>(a.stats) + begin + sub;
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(ring);
     const uint32_t stage_bytes = ROW * threads, ring_end = base + S * stage_bytes;
     const uint32_t at_e = BYTES<TX> * threads, at_y = 2 * at_e, at_t = at_y + BYTES<TY> * threads;
     uint32_t to = base, from = base;
-    int left = rows;  // to copy
+    int left = count - sub;  // to copy, at most
     const bx *cx = px + pl.from, *ce = pe + pl.from;  // of the next row to copy
     const by *cy = py + pl.from, *ct = pt + pl.from;
     auto ahead = [&]() {
@@ -641,11 +654,11 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
             if (has_h) copy8<TY, MODE>(to + at_t, threads, ct, pl);
         }
         copy_commit();
-        --left;
-        cx += a.x_ld;
-        cy += a.y_ld;
-        ce += a.width;
-        ct += a.width;
+        left -= SUBS;
+        cx += SUBS * a.x_ld;
+        cy += SUBS * a.y_ld;
+        ce += SUBS * a.width;
+        ct += SUBS * a.width;
         to = to + stage_bytes == ring_end ? base : to + stage_bytes;
     };
     if constexpr (ringed) {
@@ -665,10 +678,10 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
     for (int i = 0; i < 4; ++i) dpre[i] = z[i] = dpost[i] = 0;
     int gate_end = a.gate ? 0 : rows;  // the first row with another gate row than gain's, the gate_at-th
     int64_t gate_at = 0;
-    float2 next = rows ? stats[0] : make_float2(0.f, 0.f);
+    float2 next = rows && there(0) ? stats[0] : make_float2(0.f, 0.f);
     for (int r = 0; r < rows; ++r) {
         const float r1 = next.x, r2 = next.y;
-        if (r + 1 < rows) next = stats[r + 1];
+        if (r + 1 < rows && there(r + 1)) next = stats[(r + 1) * SUBS];
         if constexpr (ringed) ahead();
         if (r >= gate_end) {
             gate_at = (begin + r) / a.gate_rows;
@@ -683,6 +696,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
             take8<TY, MODE>(from + at_y, threads, y);
             take8<TY, MODE>(from + at_t, threads, t);
             from = from + stage_bytes == ring_end ? base : from + stage_bytes;
+            if (!there(r))
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = e[i] = y[i] = t[i] = 0;
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) e[i] = y[i] = t[i] = 0;
@@ -719,10 +735,10 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
             z[i] = fma2(e[i], y[i], z[i]);
             e[i] = mul2(fma2(y[i], both(-c1), mul2(gain[i], e[i])), both(r1));
         }
-        if (a.dx) store8<TX, MODE>(po, pl, x);
-        if (a.dy) store8<TY, MODE>(pq, pl, e);
-        po += a.width;
-        pq += a.width;
+        if (a.dx && there(r)) store8<TX, MODE>(po, pl, x);
+        if (a.dy && there(r)) store8<TY, MODE>(pq, pl, e);
+        po += SUBS * a.width;
+        pq += SUBS * a.width;
         // the last of the unit's rows with this gate row: its sum goes out
         if (a.gate_part && r + 1 == gate_end) {
             Pair w[4];
@@ -746,6 +762,15 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
 #pragma unroll
         for (int i = 0; i < 4; ++i) z[i] = mul2(w[i], z[i]);  // dgate
     }
+    // the sums of the rows side by side
+#pragma unroll
+    for (int o = 32 / SUBS; o < 32; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            dpre[i] = add2(dpre[i], __shfl_xor_sync(FULL, dpre[i], o));
+            dpost[i] = add2(dpost[i], __shfl_xor_sync(FULL, dpost[i], o));
+            z[i] = add2(z[i], __shfl_xor_sync(FULL, z[i], o));
+        }
     if constexpr (WIDE) cg::this_cluster().sync();  // no block leaves while a fellow may write its slots
     // The block's groups join their sums in order, through the ring (whose copies
     // are done: the last waits left only empty groups); one row of each is written.
@@ -763,7 +788,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
                     f[0].x += p.x; f[0].y += p.y; f[1].x += p.z; f[1].y += p.w;
                     f[2].x += q.x; f[2].y += q.y; f[3].x += q.z; f[3].y += q.w;
                 }
-                if (g + 1 < a.shape.groups) {
+                if (sub) {
+                } else if (g + 1 < a.shape.groups) {
                     same[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
                     same[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
                 } else {
@@ -896,6 +922,17 @@ bool lies(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % es
 bool lies8(const void* p) { return reinterpret_cast<uintptr_t>(p) % 8 == 0; }
 bool row_aligned(const void* p, int64_t ld, int dtype) { return !p || (aligned16(p) && ld * esize_of(dtype) % 16 == 0); }
 
+// Rows that a warp has side by side.  A row of at most 128 columns (float32, in
+// either array: 64) leaves half of a warp's lanes idle, of 64 (16-bit types) three
+// quarters, so two or four share the warp, where one gate row serves them all
+// (forward, backward: bf16 100000x64 31 -> 12 and 46 -> 22 us, 200000x128 60 -> 39 and
+// 84 -> 62; float32 100000x64 48 -> 27 and 50 -> 37).
+int rows_a_warp(int64_t width, int x_dtype, bool vec, bool one_gate) {
+    if (!vec || !one_gate) return 1;
+    if (x_dtype == SFFN_F32) return width <= 64 ? 2 : 1;
+    return width <= 64 ? 4 : width <= 128 ? 2 : 1;
+}
+
 template <class F>
 int by_types(int x_dtype, int y_dtype, F&& f) {
     using std::integral_constant;
@@ -931,13 +968,17 @@ extern "C" int sffn_residual_norm(const void* x, int x_dtype, int64_t x_ld, cons
                      row_aligned(pre, width, pre_dtype) && row_aligned(post, width, post_dtype) &&
                      row_aligned(gate, width, gate_dtype);
     const bool ringed = vec && (x_dtype != SFFN_F32 || y_dtype != SFFN_F32);
-    const Shape s = ringed ? shape_of(rows, width, 4, 1) : shape_of(rows, width, 1, 2);
+    const int subs = rows_a_warp(width, x_dtype, vec, !gate || gate_rows >= rows);
+    const Shape s = ringed ? shape_of(rows, width, 4 * subs, 1) : shape_of(rows, width, 1, 2);
     const NormArgs a{x, y, x_ld, y_ld, rows, (int)width, s, pre, post, gate, pre_dtype, post_dtype, gate_dtype,
                      gate_rows, post_norm, scale, eps, x_new, h, stats, status_dev};
     return by_types(x_dtype, y_dtype, [&](auto tx, auto ty) -> int {
         constexpr int TX = decltype(tx)::value, TY = decltype(ty)::value;
-        SFFN_CUDA_TRY(launch(s.parts > 1 ? (vec ? norm_kernel<TX, TY, true, true> : norm_kernel<TX, TY, false, true>)
-                                         : (vec ? norm_kernel<TX, TY, true, false> : norm_kernel<TX, TY, false, false>), s,
+        constexpr int FEW = TX == SFFN_F32 ? 2 : 4;
+        SFFN_CUDA_TRY(launch(s.parts > 1 ? (vec ? norm_kernel<TX, TY, true, true, 1> : norm_kernel<TX, TY, false, true, 1>)
+                             : subs == 4 ? norm_kernel<TX, TY, true, false, FEW>
+                             : subs == 2 ? norm_kernel<TX, TY, true, false, 2>
+                                         : (vec ? norm_kernel<TX, TY, true, false, 1> : norm_kernel<TX, TY, false, false, 1>), s,
                              ringed ? STAGES<TX, TY> * FWD_ROWS<TX, TY, true> * (BYTES<TX> + BYTES<TY>) * s.threads() : 0,
                              static_cast<cudaStream_t>(stream), a));
         return SFFN_OK;
@@ -982,6 +1023,7 @@ extern "C" int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, 
                      row_aligned(dx, width, x_dtype) && row_aligned(dy, width, y_dtype) &&
                      row_aligned(pre, width, pre_dtype) && row_aligned(post, width, post_dtype) &&
                      row_aligned(gate, width, gate_dtype);
+    const int subs = rows_a_warp(width, x_dtype, vec, shared_gate);
     float* part = static_cast<float*>(workspace);
     const int64_t sets = s.blocks / s.parts;
     float* gate_part = (dgate || dpost) && !shared_gate ? part + sets * 3 * width : nullptr;
@@ -991,8 +1033,11 @@ extern "C" int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, 
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int rc = by_types(x_dtype, y_dtype, [&](auto tx, auto ty) -> int {
         constexpr int TX = decltype(tx)::value, TY = decltype(ty)::value;
-        SFFN_CUDA_TRY(launch(s.parts > 1 ? (vec ? norm_bwd_kernel<TX, TY, true, true> : norm_bwd_kernel<TX, TY, false, true>)
-                                         : (vec ? norm_bwd_kernel<TX, TY, true, false> : norm_bwd_kernel<TX, TY, false, false>), s,
+        constexpr int FEW = TX == SFFN_F32 ? 2 : 4;
+        SFFN_CUDA_TRY(launch(s.parts > 1 ? (vec ? norm_bwd_kernel<TX, TY, true, true, 1> : norm_bwd_kernel<TX, TY, false, true, 1>)
+                             : subs == 4 ? norm_bwd_kernel<TX, TY, true, false, FEW>
+                             : subs == 2 ? norm_bwd_kernel<TX, TY, true, false, 2>
+                                         : (vec ? norm_bwd_kernel<TX, TY, true, false, 1> : norm_bwd_kernel<TX, TY, false, false, 1>), s,
                              vec || BWD_RING<TX, TY, false> ? BWD_STAGES<TX, TY> * 2 * (BYTES<TX> + BYTES<TY>) * s.threads()
                                                         : s.warps * 32 * 32,
                              st, a));

@@ -126,6 +126,19 @@ def params(D, seed=0, dtype=F32):
 
 
 @pytest.mark.parametrize("xt,yt", PAIRS)
+@pytest.mark.parametrize("rows,D", [(1, 8), (2, 64), (7, 128), (3, 40), (3001, 64), (2999, 128), (1026, 120), (12345, 16)])
+def test_narrow_rows(xt, yt, rows, D):
+    """Several rows to a warp, the last of them behind the end."""
+    x, y = randn(rows, D, seed=5, scale=2.0, dtype=xt), randn(rows, D, seed=6, dtype=yt)
+    pre, post, gate = params(D)
+    x[rows // 2] = 0
+    check(x, y, pre, post, gate, post_norm=True, scale=0.5)
+    check(x, None, pre, out_dtype=yt)
+    if rows % 3 == 0:  # a gate row for each third
+        check(x, y, pre, post, randn(3, D, seed=8), post_norm=True)
+
+
+@pytest.mark.parametrize("xt,yt", PAIRS)
 @pytest.mark.parametrize("rows,D", [(1, 1), (2, 7), (3, 8), (5, 31), (1, 64), (40, 100), (3000, 256), (7, 257), (33, 768),
                                     (2, 1001), (700, 1024), (5, 2056), (9, 4096), (3, 4097), (2, 5000), (310, 8192),
                                     (2, 8200), (3, 12345), (400, 16384), (1, 16383)])
