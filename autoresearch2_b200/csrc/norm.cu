@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
     constexpr int S = BWD_STAGES<TX, TY>, ROW = 2 * (BYTES<TX> + BYTES<TY>);
     constexpr bool ringed = BWD_RING<TX, TY, VEC>;
     constexpr int MODE = mode_of(TX, TY, VEC);
-    extern __shared__ float4 ring[];  // and, at the end, [warps * 32][2]: the join of the block's groups
+    extern __shared__ float4 ring[];  // and, at the end, [groups][warps * 32][2]: the join of the block's groups
     __shared__ float4 slots[SLOTS];
     __shared__ uint64_t filled[WIDE ? 2 : 1];
     using bx = typename Elt<TX>::bits;
@@ -772,34 +772,39 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
             z[i] = add2(z[i], __shfl_xor_sync(FULL, z[i], o));
         }
     if constexpr (WIDE) cg::this_cluster().sync();  // no block leaves while a fellow may write its slots
-    // The block's groups join their sums in order, through the ring (whose copies
+    // The block's groups join their sums, in order, through the ring (whose copies
     // are done: the last waits left only empty groups); one row of each is written.
+    // All threads add, a column's groups in order (one group after the other, with a
+    // barrier each: 3000x128 13.2 us instead of 9.7, 32768x768 60.3 instead of 59.2).
     __syncthreads();
-    float4* same = ring + (warp * 32 + lane) * 2;  // one place for the same columns of every group
+    const int groups = a.shape.groups, spread = warps * 32 * 2;  // float4 of a group
     auto put = [&](int which, Pair* d) {
         if (!((a.want >> which) & 1) || (which == 2 && a.gate_part)) return;
-        for (int g = 0; g < a.shape.groups; ++g) {
-            if (group == g) {
-                float2 f[4];
+        float4* mine = ring + group * spread + (warp * 32 + lane) * 2;
+        if (groups > 1) {
+            float2 f[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) f[i] = unpair(d[i]);
-                if (g) {
-                    const float4 p = same[0], q = same[1];
-                    f[0].x += p.x; f[0].y += p.y; f[1].x += p.z; f[1].y += p.w;
-                    f[2].x += q.x; f[2].y += q.y; f[3].x += q.z; f[3].y += q.w;
+            for (int i = 0; i < 4; ++i) f[i] = unpair(d[i]);
+            mine[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+            mine[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
+            __syncthreads();
+            for (int e = threadIdx.x; e < spread; e += threads) {
+                float4 f = ring[e];
+                for (int g = 1; g < groups; ++g) {
+                    const float4 p = ring[g * spread + e];
+                    f.x += p.x; f.y += p.y; f.z += p.z; f.w += p.w;
                 }
-                if (sub) {
-                } else if (g + 1 < a.shape.groups) {
-                    same[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
-                    same[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) d[i] = pair(f[i].x, f[i].y);
-                    store8<SFFN_F32, MODE>(a.part + (block * 3 + which) * a.width, pl, d);
-                }
+                ring[e] = f;
             }
             __syncthreads();
+            if (group) return;
+            const float4 p = mine[0], q = mine[1];
+            d[0] = pair(p.x, p.y);
+            d[1] = pair(p.z, p.w);
+            d[2] = pair(q.x, q.y);
+            d[3] = pair(q.z, q.w);
         }
+        if (!sub) store8<SFFN_F32, MODE>(a.part + (block * 3 + which) * a.width, pl, d);
     };
     put(0, dpre);
     put(1, dpost);
@@ -925,8 +930,8 @@ bool row_aligned(const void* p, int64_t ld, int dtype) { return !p || (aligned16
 // Rows that a warp has side by side.  A row of at most 128 columns (float32, in
 // either array: 64) leaves half of a warp's lanes idle, of 64 (16-bit types) three
 // quarters, so two or four share the warp, where one gate row serves them all
-// (forward, backward: bf16 100000x64 31 -> 12 and 46 -> 22 us, 200000x128 60 -> 39 and
-// 84 -> 62; float32 100000x64 48 -> 27 and 50 -> 37).
+// (forward, backward: bf16 100000x64 31 -> 12 and 46 -> 18 us, 200000x128 60 -> 39 and
+// 84 -> 60; float32 100000x64 48 -> 27 and 50 -> 33).
 int rows_a_warp(int64_t width, int x_dtype, bool vec, bool one_gate) {
     if (!vec || !one_gate) return 1;
     if (x_dtype == SFFN_F32) return width <= 64 ? 2 : 1;
@@ -1039,7 +1044,7 @@ extern "C" int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, 
                              : subs == 2 ? norm_bwd_kernel<TX, TY, true, false, 2>
                                          : (vec ? norm_bwd_kernel<TX, TY, true, false, 1> : norm_bwd_kernel<TX, TY, false, false, 1>), s,
                              vec || BWD_RING<TX, TY, false> ? BWD_STAGES<TX, TY> * 2 * (BYTES<TX> + BYTES<TY>) * s.threads()
-                                                        : s.warps * 32 * 32,
+                                                        : s.threads() * 32,
                              st, a));
         return SFFN_OK;
     });
@@ -1051,7 +1056,7 @@ extern "C" int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, 
         const int64_t ny = 3 + gates < 65535 ? 3 + gates : 65535;
         // Where the columns fill the SMs 8 threads add one up (the whole backward of
         // 8192x8192 with 8 gate rows: 237 us, with 32 threads 273); fewer columns take
-        // 32, whose loads are in flight together (32768x768: 61 us, with 8 threads 63).
+        // 32, whose loads are in flight together (32768x768: 2 us less than with 8).
         const dim3 grid((unsigned)((width + 31) / 32), (unsigned)ny);
         if ((int64_t)grid.x * grid.y >= 4 * SMS) norm_join_kernel<8><<<grid, dim3(32, 8), 0, st>>>(j);
         else norm_join_kernel<32><<<grid, dim3(32, 32), 0, st>>>(j);
