@@ -2,6 +2,7 @@
 Python functions and the C entry points refuse before any device call, the
 shapes torch.compile traces with, and the launch accounting."""
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -241,3 +242,14 @@ def test_gate_groups():
     x = torch.empty(4, 6, 8)
     for shape, groups in (((8,), 1), ((1, 8), 1), ((3, 8), 3), ((4, 1, 8), 4), ((4, 6, 8), 24), ((1, 1, 8), 1)):
         assert norms._gate_groups(torch.empty(*shape), x) == groups
+
+
+def test_a_thread_is_bound_once_and_to_no_other_device(monkeypatch):
+    calls = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "set_device", calls.append)
+    for index, want in ((0, []), (1, [torch.device("cuda", 1)])):
+        monkeypatch.setattr(_lib, "_thread", threading.local())
+        for _ in range(3):
+            _lib.bind_thread(torch.device("cuda", index))
+        assert calls == want
