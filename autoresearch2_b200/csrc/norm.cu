@@ -332,7 +332,8 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t barrier, int rank, fl
 // In a cluster each warp stores its sums to every block's slots (st.async), and
 // an mbarrier of each set counts the bytes: unlike the cluster's own barrier that
 // does not wait until the rows' stores to global memory are acknowledged (float32
-// 8192x8192 with bf16: 181 -> 155 us forward, 314 -> 273 us backward).  The wait is
+// 8192x8192 with bf16: 181 -> 155 us forward, 314 -> 273 us backward).  The wait
+// acquires at the cluster's scope, since other blocks stored what it waits for, and is
 // bounded: when it runs out it sets SFFN_STATUS_WAIT_TIMEOUT and no later one waits.
 template <int N, bool WIDE, int SUBS>
 struct RowSums {
@@ -384,7 +385,7 @@ struct RowSums {
             if (threadIdx.x == 0) mbar_arrive_expect_tx(full, parts * warps * POW * 4);
             if (lane % (32 / POW) == 0)
                 for (int i = 0; i < parts; ++i) send(smem_u32(mine), smem_u32(full), i, w[0]);
-            if (!gave_up && !mbar_wait_bounded(full, (phase >> which) & 1)) {
+            if (!gave_up && !mbar_wait_bounded<true>(full, (phase >> which) & 1)) {
                 gave_up = true;
                 atomicOr(status, SFFN_STATUS_WAIT_TIMEOUT);
             }
