@@ -43,8 +43,9 @@ def _check_backward(x, y, dx_new, dh, stats, out_dtype):
     for name, t, like, dtype in (("dx_new", dx_new, x, x.dtype), ("dh", dh, x, out_dtype)):
         if t is not None and (t.shape != like.shape or t.dtype != dtype or t.device != x.device):
             raise ValueError(f"{name} must be {dtype} of shape {tuple(like.shape)} on {x.device}")
-    if stats.numel() != 2 * (x.numel() // x.shape[-1]) or stats.dtype != torch.float32 or not stats.is_contiguous():
-        raise ValueError("stats are the forward's")
+    if (stats.numel() != 2 * (x.numel() // x.shape[-1]) or stats.dtype != torch.float32 or not stats.is_contiguous()
+            or stats.device != x.device):
+        raise ValueError(f"stats are the forward's: float32, contiguous, two a row, on {x.device}")
 
 
 def _empty(t, dtype=None):
