@@ -1260,6 +1260,12 @@ Plan plan_rows(int64_t rows, int64_t vocab, int dtype, int least, int wide) {
     return {vectors <= 2048 ? least : wide, 1};
 }
 
+// Dynamic shared memory that distill_kernel may take: the bit lists of 1,400,000
+// classes in one part come to 219,040 bytes, beside 2 KB of its own.  Calls set
+// this one limit whatever they need themselves, since it is every host thread's:
+// a smaller one could come between another thread's set and launch.
+constexpr size_t DISTILL_SMEM = 220 * 1024;
+
 // Launches kernel over rows x parts blocks, the parts of a row as a cluster.
 template <class Args>
 cudaError_t launch_rows(void (*kernel)(Args), const Plan& p, int64_t rows, size_t smem, cudaStream_t st, const Args& a) {
@@ -1388,6 +1394,7 @@ extern "C" int sffn_distill_topk(const void* logits, int dtype, int64_t rows, in
     const int64_t share = vocab / p.parts + 64;
     const size_t vectors = (share * esize_of(dtype) / 16 + 32 * p.threads) / (32 * p.threads) * p.threads;
     const size_t smem = bucket ? ((share + 31) / 32 + vectors) * 4 : 0;
+    if (smem > DISTILL_SMEM) return SFFN_ERR_TOO_LARGE;
     SFFN_BIND(scope, logits);
     const DistillArgs a{logits, {inner, s_outer, s_inner}, rows, (int)vocab, ids, id_bytes, scores, score_dtype,
                         k, bucket, inv_t, loss, stats, status_dev, p.parts};
@@ -1396,7 +1403,7 @@ extern "C" int sffn_distill_topk(const void* logits, int dtype, int64_t rows, in
     auto* kernel = p.threads == 512 ? distill_kernel<DT, 512> : p.threads == 128 ? distill_kernel<DT, 128> \
                                                                  : distill_kernel<DT, 32>;             \
     if (smem > 32 * 1024)                                                                                \
-        SFFN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
+        SFFN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DISTILL_SMEM)); \
     SFFN_CUDA_TRY(launch_rows(kernel, p, rows, smem, st, a))
     SFFN_BY_DTYPE(dtype, SFFN_CALL);
 #undef SFFN_CALL

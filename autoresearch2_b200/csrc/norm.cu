@@ -886,10 +886,15 @@ Shape shape_of(int64_t rows, int64_t width, int at_a_time, int blocks_per_sm) {
     return s;
 }
 
+// `smem_a_thread` bytes of dynamic shared memory.  The limit that a kernel carries
+// is its device's and every host thread's, so it is always set to what the largest
+// block takes: a smaller value, of a call with fewer threads, could come between
+// another thread's set and launch.
 template <class Args>
-cudaError_t launch(void (*kernel)(Args), const Shape& s, int smem, cudaStream_t st, const Args& a) {
+cudaError_t launch(void (*kernel)(Args), const Shape& s, int smem_a_thread, cudaStream_t st, const Args& a) {
+    const int smem = smem_a_thread * s.threads(), most = smem_a_thread * MAX_WARPS * 32;
     if (smem > 32 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
@@ -985,7 +990,7 @@ extern "C" int sffn_residual_norm(const void* x, int x_dtype, int64_t x_ld, cons
                              : subs == 4 ? norm_kernel<TX, TY, true, false, FEW>
                              : subs == 2 ? norm_kernel<TX, TY, true, false, 2>
                                          : (vec ? norm_kernel<TX, TY, true, false, 1> : norm_kernel<TX, TY, false, false, 1>), s,
-                             ringed ? STAGES<TX, TY> * FWD_ROWS<TX, TY, true> * (BYTES<TX> + BYTES<TY>) * s.threads() : 0,
+                             ringed ? STAGES<TX, TY> * FWD_ROWS<TX, TY, true> * (BYTES<TX> + BYTES<TY>) : 0,
                              static_cast<cudaStream_t>(stream), a));
         return SFFN_OK;
     });
@@ -1044,8 +1049,7 @@ extern "C" int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, 
                              : subs == 4 ? norm_bwd_kernel<TX, TY, true, false, FEW>
                              : subs == 2 ? norm_bwd_kernel<TX, TY, true, false, 2>
                                          : (vec ? norm_bwd_kernel<TX, TY, true, false, 1> : norm_bwd_kernel<TX, TY, false, false, 1>), s,
-                             vec || BWD_RING<TX, TY, false> ? BWD_STAGES<TX, TY> * 2 * (BYTES<TX> + BYTES<TY>) * s.threads()
-                                                        : s.threads() * 32,
+                             vec || BWD_RING<TX, TY, false> ? BWD_STAGES<TX, TY> * 2 * (BYTES<TX> + BYTES<TY>) : 32,
                              st, a));
         return SFFN_OK;
     });
