@@ -8,6 +8,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libsparseffn.so")
@@ -260,6 +261,20 @@ def require_cuda(*tensors):
     for t in tensors:
         if not (isinstance(t, torch.Tensor) and t.is_cuda):
             raise ValueError("autoresearch2_b200 runs on CUDA tensors only (no CPU path)")
+
+
+def tracked(*tensors):
+    """Whether autograd has to see a call on these tensors (or None): one of them
+    requires a gradient, or a forward-mode level is open, in which a tensor may
+    carry a tangent that data_ptr() would drop in silence (autograd.Function
+    refuses it)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def once_differentiable(name):

@@ -10,8 +10,9 @@
 Both take logits [..., V] in float32, bfloat16 or float16 (rows of any stride
 whose last dimension is dense; two leading strides are read in place, more
 are copied), compute in float32, and carry their gradient with respect to the
-logits.  Nothing of the logits' size is written in the forward, and only the
-gradient in the backward.
+logits (once, and in reverse mode: forward-mode tangents are refused).  Nothing
+of the logits' size is written in the forward, and only the gradient in the
+backward.
 """
 import math
 from typing import NamedTuple, Optional
@@ -188,7 +189,7 @@ def token_logprobs(logits, targets=None, top_k=0, temperature=1.0, ignore_index=
     _check_score(logits, targets, top_k, temperature)
     if torch.compiler.is_compiling():
         r = torch.ops.sparseffn.token_logprobs(logits, targets, top_k, temperature, ignore_index)
-    elif torch.is_grad_enabled() and logits.requires_grad:
+    elif _lib.tracked(logits):
         r = _TokenLogprobs.apply(logits, targets, top_k, temperature, ignore_index)
     else:
         r = _score_forward(logits, targets, top_k, temperature, ignore_index, keep=False)
@@ -281,6 +282,6 @@ def distill_topk(logits, teacher_ids, teacher_scores, temperature=1.0, tail="ren
         raise ValueError("no gradient flows to teacher_scores: detach them")
     if torch.compiler.is_compiling():
         return torch.ops.sparseffn.distill_topk(logits, teacher_ids, teacher_scores, temperature, tail)[0]
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _lib.tracked(logits):
         return _DistillTopk.apply(logits, teacher_ids, teacher_scores, temperature, tail)
     return _distill_forward(logits, teacher_ids, teacher_scores, temperature, tail, keep=False)[0]

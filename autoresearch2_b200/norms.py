@@ -10,7 +10,8 @@ x is the residual stream, y the output of the block that was fed h, and the
 new h feeds the next block: one kernel reads x and y and writes x_new and h.
 The backward recomputes x_new from x and y (no copy of either is kept) and
 gives every gradient in one pass plus a small join of the weight gradients,
-whose order of addition is fixed: equal inputs give equal bits.
+whose order of addition is fixed: equal inputs give equal bits.  Forward-mode
+tangents and second derivatives are refused.
 """
 import math
 
@@ -208,7 +209,7 @@ def residual_norm(x, y=None, pre_weight=None, post_weight=None, gate=None, post_
     args = (x, y, pre_weight, post_weight, gate, groups, bool(post_norm), float(residual_scale), float(eps), out_dtype)
     if torch.compiler.is_compiling():
         x_new, h, _ = torch.ops.sparseffn.residual_norm(*args)
-    elif torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:5]):
+    elif _lib.tracked(*args[:5]):
         x_new, h = _ResidualNorm.apply(*args)
     else:
         x_new, h, _ = _forward(*args, False)
