@@ -152,20 +152,28 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     return r;
 }
 
+// The largest of the values that these lanes of a warp bring, NaN left out.
+__device__ __forceinline__ float max_of_lanes(unsigned lanes, float x) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "r"(lanes));
+    return r;
+}
+
 // The running (m, s, w) of one thread, exponents in units of log 2: c = log2(e) / T.
-// s and w are kept as pairs (even and odd elements).  m need not be the largest
-// element: it is raised only past `limit`, where an exponent would pass SLACK, so
-// after a row's first vector hardly ever; e^d then reaches 2^32, whose sum over
-// any row is far inside float32.
-constexpr float SLACK = 32.0f;
+// s and w are kept as pairs (even and odd elements).  m is an element of the row and
+// none of the thread's own lies above it.  So a row's peak counts exactly 1 in s and
+// 0 in w, a peaked row's small terms keep their digits, and s >= 1, ln p <= 0, H >= 0.
+// (With m up to 2^32 behind, ln s and w / s came near 20 and their difference H lost
+// five digits where it was 0.02.)  A warp's lanes raise m together, to the largest of
+// their 32 vectors: about ln n times in n vectors of a lane, where lanes that raised
+// each for itself would hold the warp up at most vectors.
 // Without W (distillation, which wants no entropy) no w is kept, nor are exponents
 // held above -inf for it: 16384x50304 bf16 with the bucket 307 us instead of 332.
 template <bool W>
 struct Soft {
-    float m = LOWEST, limit = LOWEST;
+    float m = LOWEST;
     uint64_t s = 0, w = 0;
     __device__ __forceinline__ void raise(float to, float c) {
-        limit = to + SLACK / c;
         const float by = fmaxf((m - to) * c, D_MIN);
         const float f = ex2(by);
         if (W) w = mul2(fma2(s, pair(by, by), w), pair(f, f));
@@ -183,8 +191,12 @@ struct Soft {
         s = add2(s, e);
         if (W) w = fma2(e, pair(d0, d1), w);
     }
+    // Before a vector whose largest element is `top`, by those `lanes` of a warp.
+    __device__ __forceinline__ void reach(unsigned lanes, float top, float c) {
+        if (__any_sync(lanes, top > m)) raise(fmaxf(m, max_of_lanes(lanes, top)), c);
+    }
     __device__ __forceinline__ void one(float x, float c) {
-        if (x > limit) raise(x, c);
+        if (x > m) raise(x, c);
         add(x, -INFINITY, c);
     }
 };
@@ -272,17 +284,19 @@ __device__ __forceinline__ void entries(int k, F&& f) {
 // is used: DEEP of them (by blocks of 128, 8 instead of 4: 16384x50304 bf16 scored
 // in 282 us instead of 290, distilled, w kept, in 330 instead of 354), but
 // AHEAD beside the search of the alternatives, whose registers 8 would spill (8192
-// rows of it, k = 64: 257 us instead of 216).  edit(x, index) may replace elements:
-// a single one, and those of a vector where marks(iteration) has bit u set;
-// seen(u, max, which) is told each vector's largest (u: its place among those;
-// which: the vector, or -2 - index for a single element, with u = 0).  AGAIN: some
-// are read again.
+// rows of it, k = 64: 257 us instead of 216).  A warp whose lanes have all of them
+// runs without a check of each (16384x50304 bf16 250 us, with checks and the lanes
+// that pass them 281; distilled with the bucket 283 and 314).  edit(x, index) may
+// replace elements: a single one, and those of a vector where marks(iteration) has
+// bit u set; seen(u, max, which) is told each vector's largest (u: its place among
+// those; which: the vector, or -2 - index for a single element, with u = 0).  AGAIN:
+// some are read again.
 constexpr int AHEAD = 4, DEEP = 8;
 template <int DT, int NT, bool AGAIN, bool W, class Marks, class Edit, class Seen>
 __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, float c, Soft<W>& soft, Marks&& marks, Edit&& edit,
                                        Seen&& seen) {
     constexpr int N = Row<DT>::N, LOADS = AGAIN ? AHEAD : DEEP;
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, lane = t & 31;
     auto single = [&](int i) {
         float x[1] = {load1<DT>(row, i)};
         edit(x, i, std::integral_constant<int, 1>());
@@ -291,24 +305,27 @@ __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, floa
     };
     if (t < cut.head) single(t);
     const uint4* q = cut.vectors(row);
-    int iteration = 0;
-    for (int v0 = t; v0 < cut.nvec; v0 += NT * LOADS) {
+    int iteration = 0, v0 = t;
+    // WHOLE: all lanes of the warp have all LOADS vectors
+    auto go = [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
         uint4 raw[LOADS];
 #pragma unroll
         for (int u = 0; u < LOADS; ++u)
-            if (v0 + u * NT < cut.nvec) raw[u] = AGAIN ? __ldg(q + v0 + u * NT) : load_once(q + v0 + u * NT);
+            if (WHOLE || v0 + u * NT < cut.nvec) raw[u] = AGAIN ? __ldg(q + v0 + u * NT) : load_once(q + v0 + u * NT);
         const uint32_t marked = marks(iteration++);
         auto use = [&](auto place) {
             constexpr int u = decltype(place)::value;
             const int v = v0 + u * NT;
-            if (v >= cut.nvec) return;
+            if (!WHOLE && v >= cut.nvec) return;
             float x[N];
             unpack<DT>(raw[u], x);
             if ((marked >> u) & 1) edit(x, cut.at(v), std::integral_constant<int, N>());
             float top = x[0];
 #pragma unroll
             for (int j = 1; j < N; ++j) top = fmaxf(top, x[j]);
-            if (__any_sync(__activemask(), top > soft.limit) && top > soft.limit) soft.raise(top, c);
+            const int with = WHOLE ? 32 : cut.nvec - (v - lane);  // lanes, the first ones, with a vector here
+            soft.reach(with >= 32 ? FULL : (1u << with) - 1, top, c);
 #pragma unroll
             for (int j = 0; j < N; j += 2) soft.add(x[j], x[j + 1], c);
             seen(place, top, v);
@@ -323,7 +340,11 @@ __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, floa
             use(std::integral_constant<int, 6>());
             use(std::integral_constant<int, 7>());
         }
-    }
+        v0 += NT * LOADS;
+    };
+    const int whole = cut.nvec - (LOADS - 1) * NT - 31 + lane;  // the same v0 of its first lane for all of a warp
+    while (v0 < whole) go(std::true_type());
+    while (v0 < cut.nvec) go(std::false_type());
     if (t < cut.tail) single(cut.tail_at + t);
 }
 
