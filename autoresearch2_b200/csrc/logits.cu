@@ -968,8 +968,12 @@ __global__ void __launch_bounds__(NT, NT < 128 ? 32 : 1280 / NT) score_bwd_kerne
 //   L = sum q_i (ln q_i - ln p_{id_i}) [+ q_r (ln q_r - ln p_r)]
 //   T dL/dx_j = p_j Q - sum_{i: id_i = j} q_i  on the list, Q = sum q [+ q_r]
 //             = p_j (Q - q_r / p_r)            off it
-// p_r = s_off / s with s_off summed over the classes off the list themselves:
-// 1 - sum p_i would lose all digits where the list holds nearly everything.
+// The classes off the list are summed themselves, from their own maximum m_off:
+//   ln p_r = (m_off - m) / T + ln s_off - ln s
+// needs no p_r, which underflows where the list's logits stand far above the rest's
+// (1 - sum p_i would lose all digits much sooner).  Such a row, with p_r below P_FAR,
+// has its gradient off the list as q_off,j (p_r Q - q_r), where q_off,j = p_j / p_r =
+// e^{(x_j - m_off) / T} / s_off.
 struct DistillArgs {
     const void* logits;
     RowMap map;
@@ -982,13 +986,19 @@ struct DistillArgs {
     int k, bucket;
     float inv_t;
     float* loss;
-    float* stats;  // [rows, 4]: m, s, the factor off the list, ln of renorm's sum or bucket's Q
+    // [rows, 4]; all zero in a row without loss:
+    //   renorm       m, s, 1, ln of the scores' sum
+    //   bucket       m, s, the factor of p_j off the list, Q
+    //   a far row    m_off, s_off, p_r - q_r, -s (Q is 1, and m the largest listed logit)
+    float* stats;
     uint32_t* status;
     int parts;
 };
 
 // A listed mass this near to one leaves no rest: less is the scores' own rounding.
 constexpr float REST_FLOOR = 1.0f / (1 << 20);
+// From 2^-60 up p_j and q_r / p_r are within float32's range together.
+constexpr float P_FAR = 1.0f / (1ll << 60);
 
 template <int DT, int NT>
 __global__ void __launch_bounds__(NT, blocks_per_sm(NT)) distill_kernel(const DistillArgs a) {
@@ -1134,10 +1144,10 @@ __global__ void __launch_bounds__(NT, blocks_per_sm(NT)) distill_kernel(const Di
         z = sum_of(z);
         ln_z = top + logf(z);
     }
-    float off = 0.f;
+    const float m_off = m, s_off = s;
+    float off = 0.f;  // s_off from the row's maximum
     bool all_listed = false;
     if (a.bucket) {
-        const float m_off = m, s_off = s;
         m = max_of(m_on);
         off = s_off * ex2(fmaxf((m_off - m) * c, D_MIN));
         float s_on = 0.f;
@@ -1167,8 +1177,15 @@ __global__ void __launch_bounds__(NT, blocks_per_sm(NT)) distill_kernel(const Di
             more = z + rest;
             factor = more;
             if (rest > 0.f) {
-                loss += rest * (logf(rest) - (logf(off) - ln_s));
-                if (off > 0.f) factor -= rest * s / off;
+                loss += rest * (logf(rest) - (s_off == 0.f ? -INFINITY : (m_off - m) * a.inv_t + logf(s_off) - ln_s));
+                if (s_off > 0.f && off < P_FAR * s) {
+                    factor = off / s - rest;
+                    more = -s;
+                    m = m_off;
+                    s = s_off;
+                } else if (off > 0.f) {
+                    factor -= rest * s / off;
+                }
             }
         }
         a.loss[r] = loss;
@@ -1213,16 +1230,23 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const DistillBwdArgs a)
         return;
     }
     const float g = a.g_loss[r] * a.inv_t, factor = a.stats[4 * r + 2], more = a.stats[4 * r + 3];
-    const float Q = a.bucket ? more : 1.f, ln_z = a.bucket ? 0.f : more;
+    const bool far = a.bucket && more < 0.f;
+    const float Q = a.bucket && !far ? more : 1.f, ln_z = a.bucket ? 0.f : more;
     entries<NT>(a.k, [&](int e) {
         const int64_t j = load_index(a.ids, r * a.k + e, a.id_bytes);
         const bool ok = j >= 0 && j < a.vocab;
         ids[e] = ok ? (int)j : -1;
         qs[e] = ok ? expf(load_code(a.scores, r * a.k + e, a.score_code) - ln_z) : 0.f;
     });
-    const Weigh<DT> weigh(a.stats[4 * r], s, a.inv_t);
+    Weigh<DT> weigh(a.stats[4 * r], s, a.inv_t);
     weigh.template row<NT, false>(row + begin, out + begin, n, g * factor, 0.f);
     __syncthreads();
+    if (far) {  // the listed places, whatever the reference off the list left there
+        float m = a.stats[4 * r];
+        for (int e = t & 31; e < a.k; e += 32)
+            if (ids[e] >= 0) m = fmaxf(m, Elt<DT>::to_f(row[ids[e]]));
+        weigh = Weigh<DT>(max_of_lanes(FULL, m), -more, a.inv_t);
+    }
     entries<NT>(a.k, [&](int e) {
         const int id = ids[e];
         if (id < begin || id >= begin + n) return;

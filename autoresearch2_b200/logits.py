@@ -274,7 +274,9 @@ def distill_topk(logits, teacher_ids, teacher_scores, temperature=1.0, tail="ren
 
     A row without an entry of positive weight (ids all -1, scores all -inf)
     has loss 0 and gradient 0.  An id listed twice counts with both weights.
-    Where the student gives a listed class no probability the loss is +inf.
+    Where the student gives a listed class no probability (a logit of -inf, not
+    one that is only far below) the loss is +inf; with "bucket" also where it
+    has -inf for every class off the list and a rest is left.
     Other ids outside [0, V) count as absent and set the library's status word
     (check_status() reports it).  The loss carries no factor T^2."""
     _check_distill(logits, teacher_ids, teacher_scores, temperature, tail)

@@ -80,3 +80,80 @@ def test_a_small_rest_keeps_its_digits(rows, V, K, rest):
     tol = soft * (ln_pr.exp() + r) * (2 * e + 8 * U)
     within(g[outside], grad[outside], tol[outside])
     assert float((tol[outside] / grad[outside].abs()).median()) < 1e-3
+
+
+def check_bucket(x, ids, scores, T):
+    """Loss and gradient.  A logarithm l of a probability is within (300 + n) u + 4 u |l|
+    (its sum's logarithm; its exponent's three roundings and the last difference), q = e^c
+    within (4 + |c|) u of itself; the terms' products and sums take 20 u of them."""
+    x = x.detach().requires_grad_()
+    got = sf.distill_topk(x, ids, scores, temperature=T, tail="bucket")
+    g, = torch.autograd.grad(got.sum(), x)
+    loss, grad, soft, ln_pr, r = definition(x, ids, scores, T)
+    lp = torch.log_softmax(x.detach().to(F64) / T, -1).gather(1, ids)
+    c = scores.to(F64)
+    q, n = c.exp(), additions(x.shape[-1])
+    e = (300 + n) * U
+    tol = (q * (e + 4 * U * lp.abs() + 4 * U * c.abs() + (24 + c.abs()) * U * (c - lp).abs())).sum(-1, keepdim=True)
+    ln_r = torch.where(r > 0, r.log(), 0.0)
+    tol = tol + r * (e + 4 * U * ln_pr.abs() + 24 * U * (ln_r - ln_pr).abs())
+    assert bool(loss.isfinite().all())
+    within(got, loss, tol[:, 0])
+    tol = soft * (ln_pr.exp() + r) * (2 * e + 8 * U)
+    on = lp.exp() * (2 * e + 4 * U * lp.abs()) + q * (8 + 2 * c.abs()) * U
+    within(g, grad, tol.scatter(1, ids, on) / T, x.dtype)
+    return got, g
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [1.0, 0.05])
+@pytest.mark.parametrize("gap", [20.0, 80.0, 90.0, 104.0, 300.0, 1000.0])
+@pytest.mark.parametrize("rows,V,K", [(5, 700, 6), (1200, 257, 20), (2, 50304, 64)])
+def test_students_far_from_the_rest(rows, V, K, gap, T, dtype):
+    """The listed classes stand `gap` nats above the others: the mass off the list is
+    far below float32's smallest, its logarithm and the shares in it are not."""
+    ids, scores = a_list(rows, V, K, 1e-3 if gap < 100 else 0.2, 7)
+    x = randn(rows, V, seed=9).scatter_(1, ids, gap + randn(rows, K, seed=10)) * T
+    check_bucket(x.to(dtype), ids, scores, T)
+
+
+@pytest.mark.parametrize("gap", [90.0, 500.0])
+def test_students_far_below_the_rest(gap):
+    """The other way about: the listed classes have nothing, and no term is lost."""
+    ids, scores = a_list(4, 900, 9, 0.01, 21)
+    x = randn(4, 900, seed=22).scatter_(1, ids, -gap + randn(4, 9, seed=23))
+    check_bucket(x, ids, scores, 1.0)
+
+
+def test_a_rest_that_the_student_cannot_have():
+    """Nothing but -inf off the list: +inf, gradients of the list's classes alone; a NaN
+    stays one."""
+    ids, scores = a_list(3, 200, 5, 0.1, 31)
+    x = torch.full((3, 200), -math.inf, device=DEV).scatter_(1, ids, randn(3, 5, seed=32))
+    x[1, ids[1, 2]] = math.nan
+    x[2] = -math.inf
+    x.requires_grad_()
+    got = sf.distill_topk(x, ids, scores, tail="bucket")
+    assert got[0] == math.inf and got[1].isnan() and got[2] == math.inf
+    g, = torch.autograd.grad(got.sum(), x)
+    outside = torch.ones(200, dtype=torch.bool, device=DEV)
+    outside[ids[0]] = False
+    p, q = torch.softmax(x.detach()[0].to(F64), -1)[ids[0]], scores[0].to(F64).exp()
+    assert bool((g[0][outside] == 0).all()) and bool((g[2] == 0).all())
+    within(g[0][ids[0]], p - q, 40 * U * (p + q))
+
+
+def test_gradient_of_a_far_student_against_differences():
+    """Central differences of the loss's own value 30 nats apart, h = 2^-6: the third
+    derivative of the loss is at most 6, and its rounding 60 (300 + n) u a difference."""
+    ids, scores = a_list(1, 12, 4, 0.25, 41)
+    x = randn(1, 12, seed=42).scatter_(1, ids, 30.0 + randn(1, 4, seed=43)).requires_grad_()
+    f = lambda z: float(sf.distill_topk(z, ids, scores, tail="bucket"))  # noqa: E731
+    g, = torch.autograd.grad(sf.distill_topk(x, ids, scores, tail="bucket").sum(), x)
+    base, h = x.detach(), 2.0 ** -6
+    want = torch.zeros_like(base, dtype=F64)
+    for j in range(12):
+        step = torch.zeros_like(base)
+        step[0, j] = h
+        want[0, j] = (f(base + step) - f(base - step)) / (2 * h)
+    within(g, want, torch.tensor(h * h + 60 * 340 * U / (2 * h), dtype=F64, device=DEV))
