@@ -12,8 +12,9 @@
 // With q = gate u, mean(v yh) = mean(q (dx' + r2 t)) - r2 mean(t xh) mean(q xh), so
 // the backward adds up all it needs of a row at once and waits once a row.
 // x' is recomputed from x and y, unrounded, for the bytes that reading it back
-// would take.  All arithmetic, the row statistics and the sums over rows are
-// float32 (two to an instruction); each output is rounded once.
+// would take.  All arithmetic, the row statistics and a block's sums over its rows are
+// float32 (two to an instruction), the sums over the blocks 64 bits; each output is
+// rounded once.
 //
 // Bound by memory: the forward moves four arrays of the stream's size, the
 // backward six, and two things keep it from memory's rate: the instructions a
@@ -813,7 +814,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) norm_bwd_kernel(const NormB
 }
 
 // Joins the partial sums: blockIdx.y 0..2 the weight gradients (blocks rows of
-// `part`), from 3 on a gate row each (the units that hold rows of it).
+// `part`), from 3 on a gate row each (the units that hold rows of it).  In 64 bits,
+// rounded once: these are the largest sums of all, of the fewest terms.
 struct JoinArgs {
     const float *part, *gate_part;
     int64_t blocks, units, per, gate_rows, rows;
@@ -824,7 +826,7 @@ struct JoinArgs {
 
 template <int JOIN_ROWS>  // threads of a column
 __global__ void __launch_bounds__(32 * JOIN_ROWS) norm_join_kernel(const JoinArgs a) {
-    __shared__ float s[JOIN_ROWS][32];
+    __shared__ double s[JOIN_ROWS][32];
     const int x = threadIdx.x, y = threadIdx.y;
     const int col = blockIdx.x * 32 + x;
     const int64_t gates = a.gate_part && a.dgate ? (a.rows + a.gate_rows - 1) / a.gate_rows : 0;
@@ -840,7 +842,7 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) norm_join_kernel(const JoinArg
             last = (min(a.rows, (g + 1) * a.gate_rows) - 1) / a.per;
             step = a.width;
         }
-        float v = 0.f;
+        double v = 0.0;
         if (col < a.width)
 #pragma unroll 4
             for (int64_t u = first + y; u <= last; u += JOIN_ROWS) v += from[u * step + col];
@@ -848,9 +850,10 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) norm_join_kernel(const JoinArg
         s[y][x] = v;
         __syncthreads();
         if (y == 0 && col < a.width) {
-            float total = 0.f;
+            double all = 0.0;
 #pragma unroll
-            for (int i = 0; i < JOIN_ROWS; ++i) total += s[i][x];
+            for (int i = 0; i < JOIN_ROWS; ++i) all += s[i][x];
+            const float total = (float)all;
             if (which == 0) store_code(a.dpre, col, a.pre_code, total);
             else if (which == 1) store_code(a.dpost, col, a.post_code, total);
             else store_code(a.dgate, (which == 2 ? 0 : which - 3) * a.width + col, a.gate_code, total);

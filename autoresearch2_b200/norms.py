@@ -202,8 +202,8 @@ def residual_norm(x, y=None, pre_weight=None, post_weight=None, gate=None, post_
     x's last two dimensions.
 
     Rows are read in place where one stride fits them all.  Arithmetic,
-    statistics and sums are float32, each output is rounded once; h comes from
-    the unrounded x_new."""
+    statistics and sums are float32 (the blocks' sums of a weight gradient 64
+    bits), each output is rounded once; h comes from the unrounded x_new."""
     out_dtype = _check(x, y, pre_weight, post_weight, gate, post_norm, residual_scale, eps, out_dtype)
     groups = _gate_groups(gate, x) if gate is not None and x.numel() else 1
     args = (x, y, pre_weight, post_weight, gate, groups, bool(post_norm), float(residual_scale), float(eps), out_dtype)
