@@ -178,7 +178,10 @@ class DistillStep:
 
     The teacher (a GPT of the same vocabulary) is run anew each step, without
     gradient; targets of -100 are left out of both parts.  With hard_weight 0
-    targets may be None."""
+    targets may be None.  Another target outside the vocabulary makes a loss
+    with a hard part NaN, adds no gradient and sets the status word, which
+    check_status() after a step reports.  The two parts' gradients are rounded
+    to the logits' type each, and their sum again."""
 
     def __init__(self, student, teacher, idx, targets=None, top_k=64, temperature=1.0, tail="bucket", hard_weight=0.0,
                  lr=3e-4):

@@ -185,7 +185,9 @@ def token_logprobs(logits, targets=None, top_k=0, temperature=1.0, ignore_index=
     empty).  Logits of -inf have probability 0; a row of nothing else has logp
     -inf, entropy 0, gradient 0.  A row holding NaN or +inf has NaN.  Another
     target outside [0, V) gives NaN and sets the library's status word
-    (check_status() reports it)."""
+    (check_status() reports it); its logp has no gradient (the row's entropy
+    and top_logp keep theirs), so that one bad target does not spoil the
+    weights before the status is looked at."""
     _check_score(logits, targets, top_k, temperature)
     if torch.compiler.is_compiling():
         r = torch.ops.sparseffn.token_logprobs(logits, targets, top_k, temperature, ignore_index)

@@ -565,7 +565,8 @@ int sffn_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t voc
 /* Gradient with respect to the logits: grad [rows, vocab] (row stride
  * grad_ld), of the logits' dtype, from the gradients of logp, entropy and
  * top_logp (each NULL for zero), with what the forward wrote.  Rows left out
- * and rows of -inf get zeros. */
+ * and rows of -inf get zeros; a target outside the vocabulary, whose logp is NaN,
+ * adds nothing to its row. */
 int sffn_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t inner,
                             int64_t s_outer, int64_t s_inner, const void* targets, int target_bytes,
                             int64_t ignore_index, const int64_t* top_ids, int top_k, float inv_t, const float* stats,
