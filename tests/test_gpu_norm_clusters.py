@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import autoresearch2_b200 as sf
-from test_gpu_norms import BF16, F32, check, params, randn
+from test_gpu_norms import BF16, F32, check, close, params, randn, want_norm
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -40,4 +40,28 @@ def test_equal_bits_time_after_time(D):
     assert all(bool(t.isfinite().all()) for t in first)
     for _ in range(20):
         assert all(torch.equal(p, q) for p, q in zip(first, once()))
+    sf.check_status()
+
+
+@pytest.mark.parametrize("rows,D,xt,yt", [(3000, 16384, BF16, BF16), (4000, 8193, F32, F32), (5003, 12000, F32, BF16)])
+def test_weight_gradients_of_many_rows(rows, D, xt, yt):
+    """Rows wider than 8192 go to 32 clusters at most, so a thread adds up rows / 32 of
+    them in float32 (fma: one rounding a term); the clusters' sums are joined in 64
+    bits.  Beside the terms' own C u M (test_gpu_norms) that is (rows / 32 + 2) u M."""
+    x, y = randn(rows, D, seed=1, dtype=xt), randn(rows, D, seed=2, dtype=yt)
+    pre, post, gate = params(D)
+    leaves = [t.requires_grad_() for t in (pre, post, gate)]
+    dxn, dh = randn(rows, D, seed=3, dtype=xt), randn(rows, D, seed=4, dtype=yt)
+    a, h = sf.residual_norm(x, y, pre, post, gate, True, 0.5)
+    got = torch.autograd.grad([a, h], leaves, [dxn, dh])
+    want = {name: [0.0, 0.0] for name in ("dpre", "dpost", "dgate")}
+    for at in range(0, rows, 500):
+        part = slice(at, at + 500)
+        g = gate.detach().expand(min(500, rows - at), D)
+        values = want_norm(x[part], y[part], pre, post, g, True, 0.5, 1e-6, dxn[part], dh[part])
+        for name, sums in want.items():
+            for i in range(2):
+                sums[i] = sums[i] + values[name][i].sum(0)
+    for g, name in zip(got, want):
+        close(g, *want[name], extra=rows / 32 + 2)
     sf.check_status()
