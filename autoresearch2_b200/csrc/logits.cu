@@ -281,21 +281,21 @@ __device__ __forceinline__ void entries(int k, F&& f) {
 }
 
 // One pass over the part: several vectors of a thread are loaded before the first
-// is used: DEEP of them (by blocks of 128, 8 instead of 4: 16384x50304 bf16 scored
-// in 282 us instead of 290, distilled, w kept, in 330 instead of 354), but
-// AHEAD beside the search of the alternatives, whose registers 8 would spill (8192
-// rows of it, k = 64: 257 us instead of 216).  A warp whose lanes have all of them
-// runs without a check of each (16384x50304 bf16 250 us, with checks and the lanes
-// that pass them 281; distilled with the bucket 283 and 314).  edit(x, index) may
-// replace elements: a single one, and those of a vector where marks(iteration) has
-// bit u set; seen(u, max, which) is told each vector's largest (u: its place among
-// those; which: the vector, or -2 - index for a single element, with u = 0).  AGAIN:
-// some are read again.
+// is used: DEEP of them while a warp has as many (4 instead of 8: 16384x50304 bf16
+// scored in 269 us instead of 251, distilled in 300 instead of 283), then AHEAD, and
+// from the start beside the search of the alternatives, whose registers 8 would
+// spill (8192 rows of it, k = 64: 257 us instead of 216).  A warp whose lanes have
+// all of them runs without a check of each (with checks, and the lanes that pass
+// them for each vector: 281 us and 314 with the bucket).  edit(x, index) may
+// replace elements: a single one, and those of a vector where marks(places) has bit
+// u set; seen(u, max, which) is told each vector's largest (u: its place among those;
+// which: the vector, or -2 - index for a single element, with u = 0).  AGAIN: some
+// are read again.
 constexpr int AHEAD = 4, DEEP = 8;
 template <int DT, int NT, bool AGAIN, bool W, class Marks, class Edit, class Seen>
 __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, float c, Soft<W>& soft, Marks&& marks, Edit&& edit,
                                        Seen&& seen) {
-    constexpr int N = Row<DT>::N, LOADS = AGAIN ? AHEAD : DEEP;
+    constexpr int N = Row<DT>::N;
     const int t = threadIdx.x, lane = t & 31;
     auto single = [&](int i) {
         float x[1] = {load1<DT>(row, i)};
@@ -305,15 +305,16 @@ __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, floa
     };
     if (t < cut.head) single(t);
     const uint4* q = cut.vectors(row);
-    int iteration = 0, v0 = t;
-    // WHOLE: all lanes of the warp have all LOADS vectors
-    auto go = [&](auto whole) {
+    int v0 = t, places = 0;  // before v0, of each thread
+    // COUNT vectors of each thread.  WHOLE: all lanes of the warp have them all.
+    auto go = [&](auto count, auto whole) {
+        constexpr int COUNT = decltype(count)::value;
         constexpr bool WHOLE = decltype(whole)::value;
-        uint4 raw[LOADS];
+        uint4 raw[COUNT];
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u)
+        for (int u = 0; u < COUNT; ++u)
             if (WHOLE || v0 + u * NT < cut.nvec) raw[u] = AGAIN ? __ldg(q + v0 + u * NT) : load_once(q + v0 + u * NT);
-        const uint32_t marked = marks(iteration++);
+        const uint32_t marked = marks(places);
         auto use = [&](auto place) {
             constexpr int u = decltype(place)::value;
             const int v = v0 + u * NT;
@@ -334,17 +335,20 @@ __device__ __forceinline__ void stream(const void* row, const Cut<DT>& cut, floa
         use(std::integral_constant<int, 1>());
         use(std::integral_constant<int, 2>());
         use(std::integral_constant<int, 3>());
-        if constexpr (LOADS == DEEP) {
+        if constexpr (COUNT == DEEP) {
             use(std::integral_constant<int, 4>());
             use(std::integral_constant<int, 5>());
             use(std::integral_constant<int, 6>());
             use(std::integral_constant<int, 7>());
         }
-        v0 += NT * LOADS;
+        v0 += NT * COUNT;
+        places += COUNT;
     };
-    const int whole = cut.nvec - (LOADS - 1) * NT - 31 + lane;  // the same v0 of its first lane for all of a warp
-    while (v0 < whole) go(std::true_type());
-    while (v0 < cut.nvec) go(std::false_type());
+    // (v0 - lane, by which a whole warp goes, is its first lane's)
+    if constexpr (!AGAIN)
+        while (v0 - lane + (DEEP - 1) * NT + 31 < cut.nvec) go(std::integral_constant<int, DEEP>(), std::true_type());
+    while (v0 - lane + (AHEAD - 1) * NT + 31 < cut.nvec) go(std::integral_constant<int, AHEAD>(), std::true_type());
+    while (v0 < cut.nvec) go(std::integral_constant<int, AHEAD>(), std::false_type());
     if (t < cut.tail) single(cut.tail_at + t);
 }
 
@@ -1072,12 +1076,9 @@ __global__ void __launch_bounds__(NT, blocks_per_sm(NT)) distill_kernel(const Di
         });
     }
     Soft<false> soft;
-    static_assert(32 % DEEP == 0, "an iteration's marks lie in one word");
+    static_assert(32 % DEEP == 0 && DEEP % AHEAD == 0, "the marks of vectors loaded together lie in one word");
     stream<DT, NT, false>(row, cut, c, soft,
-                          [&](int iteration) {
-                              const int i = iteration * DEEP;
-                              return a.bucket ? marked_vectors[i / 32 * NT + t] >> (i % 32) : 0u;
-                          },
+                          [&](int places) { return a.bucket ? marked_vectors[places / 32 * NT + t] >> (places % 32) : 0u; },
                           [&](float* v, int i, auto count) {
                               if (!a.bucket) return;
                               constexpr int n = decltype(count)::value;
@@ -1324,7 +1325,12 @@ Plan plan_rows(int64_t rows, int64_t vocab, int dtype, int least, int wide) {
 // a smaller one could come between another thread's set and launch.
 constexpr size_t DISTILL_SMEM = 220 * 1024;
 
-// Launches kernel over rows x parts blocks, the parts of a row as a cluster.
+// Launches kernel over rows x parts blocks, the parts of a row as a cluster.  Where the
+// blocks of an SM could take more than 164 KB of shared memory (bit lists, 3 KB more a
+// block), 164 KB are asked for: the rest is L1, where the loads in flight land.  With as
+// many blocks as 228 KB hold, 1000x131072 float32 takes 102 us instead of 80, 1024x262144
+// 217 instead of 180 (2048x262144 bf16, 205, takes 223); smaller lists need less than
+// 164 KB and keep more L1 without (32768x8192 bf16 143 us, with 163).
 template <class Args>
 cudaError_t launch_rows(void (*kernel)(Args), const Plan& p, int64_t rows, size_t smem, cudaStream_t st, const Args& a) {
     cudaLaunchConfig_t cfg = {};
@@ -1332,12 +1338,18 @@ cudaError_t launch_rows(void (*kernel)(Args), const Plan& p, int64_t rows, size_
     cfg.blockDim = dim3((unsigned)p.threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)p.parts;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    if (p.parts > 1) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[cfg.numAttrs].val.clusterDim.x = (unsigned)p.parts;
+        at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    if (smem <= 128 * 1024 && (smem + 3072) * (blocks_per_sm(p.threads) + 1) > 164 * 1024) {
+        at[cfg.numAttrs].id = cudaLaunchAttributePreferredSharedMemoryCarveout;
+        at[cfg.numAttrs++].val.sharedMemCarveout = 72;  // per cent of 228 KB
+    }
     cfg.attrs = at;
-    cfg.numAttrs = p.parts > 1 ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
