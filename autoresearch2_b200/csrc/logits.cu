@@ -1178,8 +1178,13 @@ __global__ void __launch_bounds__(NT, blocks_per_sm(NT)) distill_kernel(const Di
             more = z + rest;
             factor = more;
             if (rest > 0.f) {
-                loss += rest * (logf(rest) - (s_off == 0.f ? -INFINITY : (m_off - m) * a.inv_t + logf(s_off) - ln_s));
-                if (s_off > 0.f && off < P_FAR * s) {
+                // One logarithm of q_r / p_r where that can be had: ln off and ln s are near ln V
+                // each, and where the student is near the teacher their last bits are the loss.
+                const bool far = s_off > 0.f && off < P_FAR * s;
+                const float ln_ratio = far ? logf(rest) - ((m_off - m) * a.inv_t + logf(s_off) - ln_s)
+                                           : s_off == 0.f ? INFINITY : logf(rest * (s / off));
+                loss += rest * ln_ratio;
+                if (far) {
                     factor = off / s - rest;
                     more = -s;
                     m = m_off;

@@ -157,3 +157,19 @@ def test_gradient_of_a_far_student_against_differences():
         step[0, j] = h
         want[0, j] = (f(base + step) - f(base - step)) / (2 * h)
     within(g, want, torch.tensor(h * h + 60 * 340 * U / (2 * h), dtype=F64, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_student_near_its_teacher(dtype):
+    """Equal logits: s = V and s_off = V - K are exact, ln p = -ln V, and the loss, some
+    10^-4 and less, turns on ln(q_r / p_r) near 0.  Its argument has three roundings, the
+    rest one, the logarithm and the product one each: 6 u.  The listed classes have a
+    share near K / V of the terms, each within 60 u (ln V, c and their difference)."""
+    for V in list(range(300, 320)) + [1000 + 37 * i for i in range(20)] + [20011 * i for i in range(1, 8)]:
+        K = 4
+        x = torch.zeros(3, V, device=DEV, dtype=dtype)
+        ids = torch.arange(K, device=DEV).repeat(3, 1) * 7
+        scores = (torch.tensor([[0.9], [1.0], [1.2]], device=DEV, dtype=F64) / V).log().float().expand(3, K).contiguous()
+        got = sf.distill_topk(x, ids, scores, tail="bucket")
+        loss = definition(x, ids, scores)[0]
+        within(got, loss, torch.tensor(6 * U + 1.2 * K / V * 60 * U, dtype=F64, device=DEV))
