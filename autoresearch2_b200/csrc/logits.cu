@@ -168,7 +168,7 @@ __device__ __forceinline__ float max_of_lanes(unsigned lanes, float x) {
 // their 32 vectors: about ln n times in n vectors of a lane, where lanes that raised
 // each for itself would hold the warp up at most vectors.
 // Without W (distillation, which wants no entropy) no w is kept, nor are exponents
-// held above -inf for it: 16384x50304 bf16 with the bucket 307 us instead of 332.
+// held above -inf for it (16384x50304 bf16 with the bucket: 8% of its time).
 template <bool W>
 struct Soft {
     float m = LOWEST;
@@ -1128,7 +1128,7 @@ __global__ void __launch_bounds__(NT, blocks_per_sm(NT)) distill_kernel(const Di
     if (a.bucket) {
         // The rest is a difference of numbers near one and may be 2^-20 itself: the sum
         // and its terms take 64 bits (a float32 sum of 128 terms leaves 3% of a rest of 1e-5
-        // in doubt).  32768x1024 bf16, k = 64: 63 us, in float32 60.
+        // in doubt).  32768x1024 bf16, k = 64: 3 us of 59.
         double listed = 0.0;
 #pragma unroll 1
         for (int e = t; e < a.k; e += 32)
@@ -1302,11 +1302,13 @@ int bwd_threads(int64_t per, int dtype) {
 // where one large block would wait for its own end, and the smaller the block, the
 // less a row costs beside its stream.  So it has `least` threads where the row is
 // at most 32 KB or a thread's loads are one go, else `wide`.  Scores: 32 and 64
-// (bf16, beside 128: 32768x1024 28 us and 74, 32768x8192 96 and 128; 16384x50304
-// 271 and 283; but float32 16384x16384 166 and 158).  Distillation: 32 and 128
-// (both with w still kept: 32768x1024 53 us and 109, 32768x8192 159 and 198; 64
-// threads would gain nothing at 16384x50304, and at 131072 classes their bit lists
-// leave room for few blocks: 276 us and 175).  With alternatives: 128, for the runs.
+// (bf16, beside 128: 32768x1024 27 us and 71, 32768x8192 89 and 117; 16384x16640 94
+// and 100, 2000x32000 27.2 and 28.3; from there on the two are even or 128 ahead:
+// 16384x50304 250 and 249, 12000x32000 130 and 127, 4096x131072 170 and 167, float32
+// 16384x16384 160 and 153).  Distillation with the bucket: 32 and 128 (32768x1024
+// 59 us and 104, 32768x8192 143 and 174; 64 threads would gain nothing at 16384x50304,
+// and at 131072 classes their bit lists leave room for few blocks: 226 us and 173).
+// With alternatives: 128, for the runs.
 // With fewer rows, a cluster of up to eight blocks of 128 takes a row, each a part
 // of at least 2048 elements; where even those leave SMs half idle and a thread
 // more than four vectors to read, the blocks have 512 threads.
