@@ -294,8 +294,8 @@ def status_word(device):
         idx = torch.cuda.current_device()
     t = _status.get(idx)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=f"cuda:{idx}")
-        _status[idx] = t
+        # (setdefault: of two threads that come here at once, both get the first one's)
+        t = _status.setdefault(idx, torch.zeros(1, dtype=torch.int32, device=f"cuda:{idx}"))
     return t
 
 
