@@ -1352,7 +1352,7 @@ cudaError_t launch_rows(void (*kernel)(Args), const Plan& p, int64_t rows, size_
         at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
         ++cfg.numAttrs;
     }
-    if (smem <= 128 * 1024 && (smem + 3072) * (blocks_per_sm(p.threads) + 1) > 164 * 1024) {
+    if (smem <= 128 * 1024 && (smem + 3 * 1024) * (blocks_per_sm(p.threads) + 1) > 164 * 1024) {
         at[cfg.numAttrs].id = cudaLaunchAttributePreferredSharedMemoryCarveout;
         at[cfg.numAttrs++].val.sharedMemCarveout = 72;  // per cent of 228 KB
     }
