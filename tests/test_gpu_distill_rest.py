@@ -173,3 +173,24 @@ def test_a_student_near_its_teacher(dtype):
         got = sf.distill_topk(x, ids, scores, tail="bucket")
         loss = definition(x, ids, scores)[0]
         within(got, loss, torch.tensor(6 * U + 1.2 * K / V * 60 * U, dtype=F64, device=DEV))
+
+
+@pytest.mark.parametrize("rows,V,dtype", [(600, 1400000, torch.bfloat16), (600, 700001, torch.bfloat16), (593, 1000000, torch.float32),
+                                          (200, 1400000, torch.bfloat16), (3, 1400000, torch.float32)])
+def test_the_longest_lists_of_bits(rows, V, dtype):
+    """Up to the largest vocabulary, with one block to a row and with several."""
+    K, check = 32, 3
+    ids, scores = (t.repeat(-(-rows // check), 1)[:rows].contiguous() for t in a_list(check, V, K, 0.3, 51))
+    ids[:, 0], ids[:, 1] = 0, V - 1
+    x = torch.empty(rows, V, device=DEV, dtype=dtype)
+    for at in range(0, rows, check):
+        x[at:at + check] = randn(min(check, rows - at), V, seed=at % 9)
+    got = sf.distill_topk(x, ids, scores, tail="bucket")
+    for at in (0, rows - check):
+        part = slice(at, at + check)
+        loss, *_ = definition(x[part], ids[part], scores[part])
+        lp = torch.log_softmax(x[part].to(F64), -1).gather(1, ids[part])
+        c, e = scores[part].to(F64), (300 + additions(V)) * U
+        tol = (c.exp() * (e + 30 * U * (lp.abs() + c.abs() + 1))).sum(-1) + e + 40 * U
+        within(got[part], loss, tol)
+    assert bool(got.isfinite().all())
