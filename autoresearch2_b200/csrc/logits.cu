@@ -991,7 +991,7 @@ struct DistillArgs {
     float inv_t;
     float* loss;
     // [rows, 4]; all zero in a row without loss:
-    //   renorm       m, s, 1, ln of the scores' sum
+    //   renorm       m, s, the largest score, ln of the scores' sum from it
     //   bucket       m, s, the factor of p_j off the list, Q
     //   a far row    m_off, s_off, p_r - q_r, -s (Q is 1, and m the largest listed logit)
     float* stats;
@@ -1124,8 +1124,11 @@ __global__ void __launch_bounds__(NT, blocks_per_sm(NT)) distill_kernel(const Di
         top = fmaxf(top, score[i]);
         m_on = fmaxf(m_on, x[i]);
     }
+    // q_i = e^{c_i - top} / z: the scores may be logits of any size, and top + ln z as one
+    // number would cost q as many digits as top has before its point.
     float z = 0.f, rest = 0.f, ln_z = 0.f;
     if (a.bucket) {
+        top = 0.f;
         // The rest is a difference of numbers near one and may be 2^-20 itself: the sum
         // and its terms take 64 bits (a float32 sum of 128 terms leaves 3% of a rest of 1e-5
         // in doubt).  32768x1024 bf16, k = 64: 3 us of 59.
@@ -1143,7 +1146,7 @@ __global__ void __launch_bounds__(NT, blocks_per_sm(NT)) distill_kernel(const Di
         for (int i = 0; i < PER; ++i)
             if (score[i] != -INFINITY) z += expf(score[i] - top);
         z = sum_of(z);
-        ln_z = top + logf(z);
+        ln_z = logf(z);
     }
     const float m_off = m, s_off = s;
     float off = 0.f;  // s_off from the row's maximum
@@ -1166,13 +1169,13 @@ __global__ void __launch_bounds__(NT, blocks_per_sm(NT)) distill_kernel(const Di
     float loss = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const float ln_q = score[i] - ln_z, q = on[i] ? expf(ln_q) : 0.f;
+        const float ln_q = (score[i] - top) - ln_z, q = on[i] ? expf(ln_q) : 0.f;
         const float ln_p = s == 0.f ? -INFINITY : (x[i] - m) * a.inv_t - ln_s;
         if (q != 0.f) loss += q * (ln_q - ln_p);
     }
     loss = sum_of(loss);
     if (t == 0) {
-        float factor = 1.f, more = ln_z;
+        float factor = top, more = ln_z;
         if (a.bucket) {
             if (rest < REST_FLOOR || all_listed) rest = 0.f;
             more = z + rest;
@@ -1235,14 +1238,15 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const DistillBwdArgs a)
         zero_row<NT>(out + begin, (int64_t)n * sizeof(bits));
         return;
     }
-    const float g = a.g_loss[r] * a.inv_t, factor = a.stats[4 * r + 2], more = a.stats[4 * r + 3];
+    const float g = a.g_loss[r] * a.inv_t, third = a.stats[4 * r + 2], more = a.stats[4 * r + 3];
     const bool far = a.bucket && more < 0.f;
-    const float Q = a.bucket && !far ? more : 1.f, ln_z = a.bucket ? 0.f : more;
+    const float Q = a.bucket && !far ? more : 1.f, factor = a.bucket ? third : 1.f;
+    const float top = a.bucket ? 0.f : third, ln_z = a.bucket ? 0.f : more;
     entries<NT>(a.k, [&](int e) {
         const int64_t j = load_index(a.ids, r * a.k + e, a.id_bytes);
         const bool ok = j >= 0 && j < a.vocab;
         ids[e] = ok ? (int)j : -1;
-        qs[e] = ok ? expf(load_code(a.scores, r * a.k + e, a.score_code) - ln_z) : 0.f;
+        qs[e] = ok ? expf((load_code(a.scores, r * a.k + e, a.score_code) - top) - ln_z) : 0.f;
     });
     Weigh<DT> weigh(a.stats[4 * r], s, a.inv_t);
     weigh.template row<NT, false>(row + begin, out + begin, n, g * factor, 0.f);
