@@ -110,6 +110,19 @@ SIGNATURES = {
     "sffn_residual_norm_bwd": (_int, [_vp, _int, _i64, _vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _int, _vp,
                                       _int, _i64, _int, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                                       _vp, _vp]),
+    "sffn_fp8_pack": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "sffn_fp8_unpack": (_int, [_vp, _i64, _vp, _i64, _i64, _int, _vp, _i64, _vp]),
+    "sffn_fp8_mm": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp, _vp]),
+    "sffn_glu_up": (_int, [_int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _int, _vp, _vp, _i64,
+                           _vp, _vp, _vp, _vp]),
+    "sffn_glu_dgrad": (_int, [_int, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _int, _vp, _vp, _i64, _vp, _vp, _vp, _vp,
+                              _i64, _vp, _i64, _vp, _vp]),
+    "sffn_gemm16_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "sffn_gemm16": (_int, [_int, _vp, _i64, _int, _vp, _i64, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64,
+                           _vp, _sz, _vp, _vp]),
+    "sffn_few_rows_mm": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "sffn_few_rows_glu": (_int, [_int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "sffn_few_rows_fp8": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp]),
 }
 
 _lib = None
@@ -146,7 +159,9 @@ LAUNCHING = {"sffn_sp24_compress": 1, "sffn_gemm_sp24": 1, "sffn_sp24_overflow_a
              "sffn_split_bf16x3": 1, "sffn_gemm_bf16_f32out": 1, "sffn_tile_copy_slots": 1,
              "sffn_gemm_bf16_f32acc": 1, "sffn_gemm_tf32": 1, "sffn_gemm_relu": 1,
              "sffn_round_tf32": 1, "sffn_token_logprobs": 1, "sffn_token_logprobs_bwd": 1, "sffn_distill_topk": 1,
-             "sffn_distill_topk_bwd": 1, "sffn_residual_norm": 1, "sffn_residual_norm_bwd": 1}
+             "sffn_distill_topk_bwd": 1, "sffn_residual_norm": 1, "sffn_residual_norm_bwd": 1,
+             "sffn_fp8_pack": 1, "sffn_fp8_unpack": 1, "sffn_fp8_mm": 1, "sffn_glu_up": 1, "sffn_glu_dgrad": 1,
+             "sffn_gemm16": 1, "sffn_few_rows_mm": 1, "sffn_few_rows_glu": 1, "sffn_few_rows_fp8": 1}
 launch_count = 0
 
 # Per-entry-point CUDA event pairs, recorded while a KernelTimer is active.
@@ -184,12 +199,15 @@ def _launches(name, args):
     """Kernels one successful call launched: LAUNCHING's count, except where
     it depends on the arguments (the float32-output GEMM runs one launch per
     K chunk of 1024; the tile pack without vals stops after count and scan;
-    the block norm's backward joins the weight gradients, if any, in a second)."""
+    the block norm's backward joins the weight gradients, if any, in a second;
+    the 16-bit product with a workspace joins its parts)."""
     if name == "sffn_gemm_bf16_f32out":
         return -(-int(args[10]) // 1024)
     if name == "sffn_tile_pack":
         v = args[9]
         return 2 if v is None or getattr(v, "value", v) in (None, 0) else 3
+    if name == "sffn_gemm16":
+        return 2 if args[18] else 1
     if name == "sffn_residual_norm_bwd":
         return 2 if any(getattr(v, "value", v) for v in args[22:25]) else 1
     return LAUNCHING.get(name, 0)

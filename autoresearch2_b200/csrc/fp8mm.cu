@@ -1,0 +1,365 @@
+// Product of two matrices in the 8-bit block format (fp8.cuh):
+// C[M, N] = A[M, K] B[N, K]^T, both with one power-of-two scale for each 128
+// elements of a row, C in 16 bits.
+//
+// tcgen05.mma kind::mxf8f6f4 with block scaling: the tensor cores multiply each
+// 32 products' sum by 2^(ea + eb) as they accumulate in float32, at the full
+// 8-bit rate; the four 32-wide steps of a 128-wide k-block use the same scale
+// byte.  One scale tile (128 rows x 4 blocks, 512 bytes) holds four k-blocks'
+// scales, which the instruction's scale-id field picks.
+//
+// CTA pairs, persistent over 256 x 256 tiles; each CTA loads its 128 rows of A
+// and of B (128 bytes of K a stage), its A scale tile and the two of B.
+//   warps 0-5    TMA issuers, one per (A / B / scales, even / odd k-block): one
+//                thread's copies complete one after another
+//   warp 6       MMA issuer (leader): three tcgen05.cp bring the stage's scales
+//                to tensor memory, four tcgen05.mma follow
+//   warp 7       allocates tensor memory
+//   warps 8-15   epilogue, two warpgroups of 128 columns.  The accumulator takes
+//                256 of 512 columns and the scales need some, so there is one:
+//                the epilogue frees it fast, as 16-bit pairs in 128 spare
+//                columns, and stores from there while the next tile runs.
+// The 256 x 256 tile is as large as tensor memory allows: at 8 bits a stage's
+// 32 KB a CTA feed 512 cycles of MMA, about what L2 can deliver.
+#include <string.h>
+
+#include <algorithm>
+
+#include "fp8.cuh"
+#include "sm100.cuh"
+#include "tmap.cuh"
+
+namespace sffn {
+namespace {
+
+constexpr int X_STAGES = 6;  // even: the issuers take alternate k-blocks
+constexpr int X_THREADS = 512;
+constexpr int X_OPERAND = 128 * 128;             // bytes of one operand a stage and CTA
+constexpr int X_STAGE = 2 * X_OPERAND;
+constexpr int X_SCALES = 3 * 512;                // A's tile, B's two
+constexpr int X_SMEM = X_STAGES * (X_STAGE + X_SCALES) + 8 * 2048 + 1024;
+constexpr int X_PACK_COL = 256;                  // 64 columns per warpgroup
+constexpr int X_SCALE_COL = 384;                 // 12 columns per stage: 4 of A, 8 of B
+static_assert(X_SCALE_COL + 12 * X_STAGES <= 512, "tensor memory columns");
+static_assert(X_SMEM <= 232448, "shared memory");
+
+struct MmArgs {
+    int M, N, K;
+    int tiles_m, tiles_n;  // of 128 rows, of 256 columns
+    int tiles_b;           // 128-row tiles of B
+    int bt;                // scale tiles across K
+    uint16_t* out;
+    long long ldc;
+    int vec_out;
+    uint32_t* status;
+};
+
+// kind::mxf8f6f4: e4m3 operands (format 0), K-major, ue8m0 scales (bit 23); the
+// scale bytes used by A (bits 29, 30) and B (bits 4, 5).
+__device__ constexpr uint32_t idesc_mx(int M, int N) {
+    return ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_mx_pair(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(ad), "l"(bd), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+// 32 rows of 16 bytes -> 4 tensor-memory columns, the same in each quarter of
+// the lanes; in each CTA of the pair from its own shared memory.
+__device__ __forceinline__ void cp_scales_pair(uint32_t taddr, uint64_t sdesc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+
+// The warp's 32 rows x 32 columns (lane = row) to its staging buffer and from
+// there by one bulk-tensor store (64-byte swizzle).
+__device__ __forceinline__ void stage_store(const CUtensorMap* tmap, unsigned char* sbuf, int lane, const uint32_t (&w)[16],
+                                            int col, int row0) {
+    if (lane == 0) bulk_wait_group_read0();
+    __syncwarp();
+    const uint32_t rb = smem_u32(sbuf) + (uint32_t)lane * 64u;
+    const int sw = (lane >> 1) & 3;
+#pragma unroll
+    for (int ch = 0; ch < 4; ++ch)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rb + 16u * (uint32_t)(ch ^ sw)), "r"(w[4 * ch]),
+                     "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3])
+                     : "memory");
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        tma_store_2d(tmap, sbuf, col, row0);
+        bulk_commit_group();
+    }
+}
+
+template <int DT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
+    fp8_mm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                  const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
+                  const __grid_constant__ CUtensorMap tmC, const MmArgs args) {
+    constexpr uint32_t IDESC = idesc_mx(256, 256);
+    extern __shared__ __align__(1024) unsigned char x_smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(x_smem_raw) + 1023) &
+                                                           ~static_cast<uintptr_t>(1023));
+    unsigned char* sscales = smem + X_STAGES * X_STAGE;
+    __shared__ __align__(8) uint64_t full_bar[X_STAGES], empty_bar[X_STAGES];
+    __shared__ __align__(8) uint64_t tfull_bar, tempty_bar;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles_mp = (args.tiles_m + 1) / 2;
+    const int ntiles = tiles_mp * args.tiles_n;
+    const int nkb = (args.K + 127) / 128;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int first_tile = (int)cluster_id_x();
+    const int tile_stride = (int)cluster_count_x();
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < X_STAGES; ++s) {
+            mbar_init(&full_bar[s], 1);   // the leader's arrive.expect_tx, for both CTAs' bytes
+            mbar_init(&empty_bar[s], 1);  // one multicast commit a use
+        }
+        mbar_init(&tfull_bar, 1);
+        mbar_init(&tempty_bar, 16);  // the 8 epilogue warps of both CTAs
+        s_abort = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tmA);
+        prefetch_tmap(&tmB);
+        prefetch_tmap(&tmSA);
+        prefetch_tmap(&tmSB);
+    }
+    if (warp == 7) {
+        tmem_alloc_pair(&s_tmem, 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = s_tmem;
+
+    if (warp < 6) {
+        // ------------------------------------------------------ producers --
+        const int op = warp % 3;   // 0: A, 1: B, 2: scales
+        const int par = warp / 3;  // even / odd k-blocks
+        if (lane == 0) {
+            int armed[X_STAGES] = {0};
+            long long kc = 0;
+            bool stop = false;
+            for (int tile = first_tile; tile < ntiles && !stop && !s_abort; tile += tile_stride) {
+                int pm, tn;
+                pair_raster(tile, tiles_mp, args.tiles_n, pm, tn);
+                const int arow = (pm * 2 + (int)rank) * 128;
+                const int brow = tn * 256 + (int)rank * 128;
+                // tiles past the end take the last one's scales: their rows' values are zero
+                const int ta = min(pm * 2 + (int)rank, args.tiles_m - 1);
+                const int tb0 = min(tn * 2, args.tiles_b - 1), tb1 = min(tn * 2 + 1, args.tiles_b - 1);
+                for (int kb = 0; kb < nkb; ++kb, ++kc) {
+                    if ((int)(kc & 1) != par) continue;
+                    const int stage = (int)(kc % X_STAGES);
+                    const uint32_t phase = (uint32_t)((kc / X_STAGES) & 1);
+                    if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u)) {
+                        atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
+                        s_abort = 1;
+                        stop = true;
+                        break;
+                    }
+                    unsigned char* sa = smem + stage * X_STAGE;
+                    if (op == 0) {
+                        if (leader) {
+                            mbar_arrive_expect_tx(&full_bar[stage], 2 * (X_STAGE + X_SCALES));
+                            ++armed[stage];
+                        }
+                        tma_load_2d_pair(sa, &tmA, kb * 128, arow, &full_bar[stage]);
+                    } else if (op == 1) {
+                        tma_load_2d_pair(sa + X_OPERAND, &tmB, kb * 128, brow, &full_bar[stage]);
+                    } else {
+                        unsigned char* ss = sscales + stage * X_SCALES;
+                        const int kt = kb >> 2;
+                        tma_load_2d_pair(ss, &tmSA, 0, (ta * args.bt + kt) * 32, &full_bar[stage]);
+                        tma_load_2d_pair(ss + 512, &tmSB, 0, (tb0 * args.bt + kt) * 32, &full_bar[stage]);
+                        tma_load_2d_pair(ss + 1024, &tmSB, 0, (tb1 * args.bt + kt) * 32, &full_bar[stage]);
+                    }
+                }
+            }
+            // once the last phases armed here complete, no copy is still landing in either CTA
+            if (leader && op == 0)
+                for (int s = 0; s < X_STAGES; ++s)
+                    if (armed[s]) (void)mbar_wait_bounded(&full_bar[s], (uint32_t)(armed[s] - 1) & 1u);
+        }
+        __syncwarp();
+    } else if (warp == 6) {
+        // ----------------------------------------------------------- MMA --
+        if (lane == 0 && leader) {
+            int stage = 0, it = 0;
+            uint32_t phase = 0;
+            for (int tile = first_tile; tile < ntiles && !s_abort; tile += tile_stride, ++it) {
+                if (!mbar_wait_bounded(&tempty_bar, ((uint32_t)it & 1u) ^ 1u)) {
+                    atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
+                    s_abort = 1;
+                    break;
+                }
+                tc_fence_after();
+                bool ready = mbar_try_wait(&full_bar[stage], phase), fail = false;
+                for (int kb = 0; kb < nkb; ++kb) {
+                    if (!ready && !mbar_wait_bounded(&full_bar[stage], phase)) {
+                        atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
+                        s_abort = 1;
+                        fail = true;
+                        break;
+                    }
+                    const uint32_t sa = smem_u32(smem + stage * X_STAGE), sb = sa + X_OPERAND;
+                    const uint32_t ss = smem_u32(sscales + stage * X_SCALES);
+                    // the stage's own columns: free since the MMAs of its last use
+                    const uint32_t ta = tmem_base + X_SCALE_COL + 12u * (uint32_t)stage, tb = ta + 4u;
+                    cp_scales_pair(ta, smem_desc_rows16(ss));
+                    cp_scales_pair(tb, smem_desc_rows16(ss + 512));
+                    cp_scales_pair(tb + 4u, smem_desc_rows16(ss + 1024));
+                    const uint32_t id = (uint32_t)kb & 3u;
+                    const uint32_t idesc = IDESC | (id << 4) | (id << 29);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        mma_mx_pair(tmem_base, umma_desc_sw128(sa + 32 * j, 16, 1024), umma_desc_sw128(sb + 32 * j, 16, 1024),
+                                    idesc, ta, tb, (kb | j) != 0 ? 1u : 0u);
+                    tc_commit_pair_multicast(&empty_bar[stage], 0x3);
+                    if (++stage == X_STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                    ready = kb + 1 < nkb && mbar_try_wait(&full_bar[stage], phase);
+                }
+                if (fail) break;
+                tc_commit_pair_multicast(&tfull_bar, 0x3);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 8) {
+        // ------------------------------------------------------ epilogue --
+        const int ew = warp & 3, wg = (warp - 8) >> 2;
+        unsigned char* sbuf = sscales + X_STAGES * X_SCALES + (warp - 8) * 2048;
+        const uint32_t tempty_leader = leader_smem_addr(&tempty_bar);
+        const uint32_t lane_base = tmem_base + ((uint32_t)(ew * 32) << 16);
+        int it = 0;
+        for (int tile = first_tile; tile < ntiles; tile += tile_stride, ++it) {
+            int pm, tn;
+            pair_raster(tile, tiles_mp, args.tiles_n, pm, tn);
+            const int row0 = (pm * 2 + (int)rank) * 128 + ew * 32, col0 = tn * 256 + wg * 128;
+            const bool ok = __all_sync(FULL, mbar_wait_bounded(&tfull_bar, (uint32_t)it & 1u));
+            if (!ok || __any_sync(FULL, s_abort != 0)) {
+                if (lane == 0 && !ok) atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
+                break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t r[32], w[16];
+                tmem_ld32(lane_base + (uint32_t)(wg * 128 + c * 32), r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int q = 0; q < 16; ++q)
+                    w[q] = pack16x2<DT>(__uint_as_float(r[2 * q]), __uint_as_float(r[2 * q + 1]));
+                tmem_st16(lane_base + (uint32_t)(X_PACK_COL + wg * 64 + c * 16), w);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(tempty_leader);
+            if (row0 >= args.M) continue;
+#pragma unroll 1
+            for (int c = 0; c < 4 && col0 + c * 32 < args.N; ++c) {
+                uint32_t w[16];
+                tmem_ld16(lane_base + (uint32_t)(X_PACK_COL + wg * 64 + c * 16), w);
+                tmem_wait_ld();
+                const int col = col0 + c * 32;
+                if (args.vec_out) {
+                    stage_store(&tmC, sbuf, lane, w, col, row0);
+                } else if (row0 + lane < args.M) {
+                    uint16_t* row = args.out + (long long)(row0 + lane) * args.ldc;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (col + j < args.N) row[col + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+                }
+            }
+        }
+        if (lane == 0) bulk_wait_group0();
+        __syncwarp();
+    }
+    // neither CTA leaves while the other can touch its shared or tensor memory
+    tc_fence_before();
+    cluster_sync();
+    if (warp == 7) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+template <int DT>
+int launch_mm(const void* a, long long lda, const void* as, const void* b, long long ldb, const void* bs, MmArgs args,
+              cudaStream_t st) {
+    CUtensorMap ta, tb, tsa, tsb, tc;
+    memset(&tc, 0, sizeof(tc));
+    const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const auto u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
+    const auto sw = CU_TENSOR_MAP_SWIZZLE_128B, none = CU_TENSOR_MAP_SWIZZLE_NONE;
+    if (int rc = tmap_2d(&ta, u8, 1, a, args.K, args.M, lda, 128, 128, sw)) return rc;
+    if (int rc = tmap_2d(&tb, u8, 1, b, args.K, args.N, ldb, 128, 128, sw)) return rc;
+    // scale tiles as rows of 16 bytes, 32 rows a tile
+    if (int rc = tmap_2d(&tsa, u32, 4, as, 4, (long long)args.tiles_m * args.bt * 32, 4, 4, 32, none)) return rc;
+    if (int rc = tmap_2d(&tsb, u32, 4, bs, 4, (long long)args.tiles_b * args.bt * 32, 4, 4, 32, none)) return rc;
+    if (args.vec_out)
+        if (int rc = tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, args.out, args.N, args.M, args.ldc, 32, 32,
+                             CU_TENSOR_MAP_SWIZZLE_64B))
+            return rc;
+    auto k = fp8_mm_kernel<DT>;
+    SFFN_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, X_SMEM));
+    static const int pairs = resident_pairs(k, X_THREADS, X_SMEM);
+    const long long ntiles = (long long)((args.tiles_m + 1) / 2) * args.tiles_n;
+    const int clusters = (int)std::min<long long>(ntiles, pairs);
+    k<<<clusters * 2, X_THREADS, X_SMEM, st>>>(ta, tb, tsa, tsb, tc, args);
+    SFFN_CHECK_LAUNCH();
+    return SFFN_OK;
+}
+
+}  // namespace
+}  // namespace sffn
+
+using namespace sffn;
+
+extern "C" int sffn_fp8_mm(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb,
+                           const void* b_scales, int64_t M, int64_t N, int64_t K, void* C, int c_dtype, int64_t ldc,
+                           uint32_t* status_dev, void* stream) {
+    if (c_dtype != SFFN_BF16 && c_dtype != SFFN_F16) return SFFN_ERR_DTYPE;
+    if (M < 0 || N < 0 || K <= 0) return SFFN_ERR_ARG;
+    if (M == 0 || N == 0) return SFFN_OK;
+    if (!a || !a_scales || !b || !b_scales || !C || !status_dev || lda < K || ldb < K || ldc < N) return SFFN_ERR_ARG;
+    // coordinates and scale rows are 32-bit in the tensor maps
+    if (M > 0x7FFFFF00 || N > 0x7FFFFF00 || K > 0x7FFFFF00 || (M + 127) / 128 * fp8_block_tiles(K) * 32 > 0x7FFFFFFF ||
+        (N + 127) / 128 * fp8_block_tiles(K) * 32 > 0x7FFFFFFF || (M + 255) / 256 * ((N + 255) / 256) > 0x3FFFFFFF)
+        return SFFN_ERR_TOO_LARGE;
+    if (!aligned16(a) || !aligned16(b) || !aligned16(a_scales) || !aligned16(b_scales) || lda % 16 || ldb % 16 ||
+        reinterpret_cast<uintptr_t>(C) % 2)
+        return SFFN_ERR_ALIGN;
+    DeviceScope scope;
+    if (int rc = scope.bind_same(a, {a_scales, b, b_scales, C, status_dev})) return rc;
+    if (!sm100_sms()) return SFFN_ERR_DEVICE;
+    MmArgs args{};
+    args.M = (int)M;
+    args.N = (int)N;
+    args.K = (int)K;
+    args.tiles_m = (int)((M + 127) / 128);
+    args.tiles_n = (int)((N + 255) / 256);
+    args.tiles_b = (int)((N + 127) / 128);
+    args.bt = (int)fp8_block_tiles(K);
+    args.out = static_cast<uint16_t*>(C);
+    args.ldc = ldc;
+    args.vec_out = aligned16(C) && ldc % 8 == 0;
+    args.status = status_dev;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return c_dtype == SFFN_BF16 ? launch_mm<SFFN_BF16>(a, lda, a_scales, b, ldb, b_scales, args, st)
+                                : launch_mm<SFFN_F16>(a, lda, a_scales, b, ldb, b_scales, args, st);
+}

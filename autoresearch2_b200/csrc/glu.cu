@@ -1,0 +1,792 @@
+// The gated feed-forward block h = act(x Wg^T) * (x Wu^T), y = h W2^T, and the
+// products of its backward, in bfloat16 or float16 on the tcgen05 tensor cores.
+//
+// One kernel: CTA pairs (tcgen05.mma.cta_group::2, 256 x 256 tiles, float32
+// accumulation in tensor memory, two accumulators), persistent over tiles;
+// operands by TMA in a ring of 64-wide k-blocks, either major order, so no
+// operand is transposed.
+//   warps 0,2 / 3,12  issuers of A / B (even / odd k-blocks)
+//   warp 1            MMA issuer (leader CTA)
+//   warp 2            also tensor memory
+//   warps 4-11        epilogue, two warpgroups; thread = accumulator row
+// Epilogues:
+//   STORE  C in 16 bits; or, split over K, float32 parts that a second kernel
+//          adds in order (few tiles and a long K: weight gradients).  K may run
+//          on into a second pair of operands: dx = dg Wg + du Wu is one product.
+//   UP     the pair's B rows are 128 of Wg (leader's shared memory) and the
+//          same 128 of Wu (peer's), so the accumulator holds g and u of 128
+//          columns side by side: h is formed here from the unrounded g and u,
+//          and g and u are kept for the backward in 16 bits or in the 8-bit
+//          block format (a tile's 128 columns are one block).
+//   DGRAD  dh = dy W2; reads g and u as they were kept and writes
+//          dg = dh u act'(g), du = dh act(g) and h = act(g) u (for dW2): dh
+//          itself is never stored.
+#include <string.h>
+
+#include <algorithm>
+
+#include "act.cuh"
+#include "fp8.cuh"
+#include "sm100.cuh"
+#include "tmap.cuh"
+
+namespace sffn {
+namespace {
+
+enum { P_STORE = 0, P_UP = 1, P_DGRAD = 2 };
+enum { KEEP_NONE = 0, KEEP_16 = 1, KEEP_8 = 2 };
+
+constexpr int P_BK = 64;
+constexpr int P_THREADS = 416;
+constexpr int P_OPERAND = 128 * P_BK * 2;  // bytes of one operand a stage and CTA
+constexpr int P_STAGE = 2 * P_OPERAND;
+// The fused epilogues stage three matrices a warp instead of one; their rings
+// have four stages to make room.  Even counts: the issuers take alternate
+// k-blocks.
+template <int EPI>
+constexpr int p_stages() { return EPI == P_STORE ? 6 : 4; }
+template <int EPI>
+constexpr int p_bufs() { return EPI == P_STORE ? 1 : 3; }
+template <int EPI>
+constexpr int p_smem() { return p_stages<EPI>() * P_STAGE + 8 * p_bufs<EPI>() * 2048 + 1024; }
+static_assert(p_smem<P_STORE>() <= 227 * 1024 - 6144 && p_smem<P_UP>() <= 227 * 1024 - 6144, "shared memory");
+
+struct PairArgs {
+    int M, N;
+    int tiles_m, tiles_n;  // of 128 rows; of 256 accumulator columns (UP: 128 columns of h)
+    int nkb1, nkb;         // k-blocks of the first pair of operands, and of both
+    int splits, per_split;
+    uint16_t* out;  // STORE
+    long long ldc;
+    int vec_out;
+    float* part;  // STORE, splits > 1: [splits][M][ldp]
+    long long ldp;
+    int keep;
+    const uint16_t *g, *u;  // DGRAD, KEEP_16: rows ldk apart
+    uint8_t *g8, *u8;       // KEEP_8: values (rows ldk apart) and scale tiles
+    uint8_t *gs, *us;
+    long long ldk;
+    int bt;  // scale tiles across a row
+    uint32_t* status;
+};
+
+template <int DT>
+__device__ constexpr uint32_t idesc16(bool a_mn, bool b_mn) {
+    const uint32_t f = DT == SFFN_BF16 ? 1u : 0u;  // both operands of one type
+    return (1u << 4) | (f << 7) | (f << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+           ((uint32_t)(256 >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+}
+
+// The warp's 32 rows x 32 columns (lane = row) into a staging buffer, in the
+// 64-byte swizzle of the store's tensor map.
+__device__ __forceinline__ void stage32(unsigned char* sbuf, int lane, const uint32_t (&w)[16]) {
+    const uint32_t rb = smem_u32(sbuf) + (uint32_t)lane * 64u;
+    const int sw = (lane >> 1) & 3;
+#pragma unroll
+    for (int ch = 0; ch < 4; ++ch)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rb + 16u * (uint32_t)(ch ^ sw)), "r"(w[4 * ch]),
+                     "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3])
+                     : "memory");
+}
+// Before the staging buffers are written again: their stores have read them.
+__device__ __forceinline__ void stage_free(int lane) {
+    if (lane == 0) bulk_wait_group_read0();
+    __syncwarp();
+}
+
+template <int DT, bool A_MN, bool B_MN, int EPI, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2,
+                const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmC2,
+                const __grid_constant__ CUtensorMap tmC3, const PairArgs args) {
+    constexpr int NST = p_stages<EPI>();
+    constexpr uint32_t IDESC = idesc16<DT>(A_MN, B_MN);
+    constexpr uint32_t MN_LBO = P_BK * 128;  // MN-major: 64-element blocks of 64 K rows x 128 bytes
+    constexpr int TILE_N = EPI == P_UP ? 128 : 256;
+    extern __shared__ __align__(1024) unsigned char p_smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p_smem_raw) + 1023) &
+                                                           ~static_cast<uintptr_t>(1023));
+    __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST];
+    __shared__ __align__(8) uint64_t tfull_bar[2], tempty_bar[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort, s_dead;
+    __shared__ uint2 s_amax[EPI == P_UP ? 2 : 1][2][128];  // UP: [tile parity][warpgroup][row], of g and u
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles_mp = (args.tiles_m + 1) / 2;
+    const int ntasks = tiles_mp * args.tiles_n * args.splits;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int first_task = (int)cluster_id_x();
+    const int task_stride = (int)cluster_count_x();
+    // the tile of a task and its k-blocks
+    auto locate = [&](int task, int& pm, int& tn, int& kb0, int& kb1) {
+        int sp = 0;
+        if (EPI == P_STORE && args.splits > 1) {
+            sp = task % args.splits;
+            task /= args.splits;
+        }
+        pair_raster(task, tiles_mp, args.tiles_n, pm, tn);
+        kb0 = sp * args.per_split;
+        kb1 = min(args.nkb, kb0 + args.per_split);
+        return sp;
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NST; ++s) {
+            mbar_init(&full_bar[s], 1);   // the leader's arrive.expect_tx, for both CTAs' bytes
+            mbar_init(&empty_bar[s], 1);  // one multicast commit a use
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&tfull_bar[a], 1);
+            mbar_init(&tempty_bar[a], 16);  // the epilogue warps of both CTAs
+        }
+        s_abort = s_dead = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tmA);
+        prefetch_tmap(&tmB);
+    }
+    if (warp == 2) {
+        tmem_alloc_pair(&s_tmem, 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = s_tmem;
+
+    if (warp == 0 || warp == 2 || warp == 3 || warp == 12) {
+        // ----------------------------------------------------- producers --
+        // Four issuing threads, one per (operand, k-block parity): one thread's
+        // copies complete one after another.  B's bytes may land before the A
+        // issuer arms the barrier; its transaction count goes below zero
+        // meanwhile, and the phase cannot complete before the arrival.
+        const bool loads_a = warp == 0 || warp == 2;
+        const int par = (warp == 0 || warp == 3) ? 0 : 1;
+        if (lane == 0) {
+            int armed[NST] = {0};
+            long long kc = 0;
+            bool stop = false;
+            for (int task = first_task; task < ntasks && !stop && !s_abort; task += task_stride) {
+                int pm, tn, kb0, kb1;
+                locate(task, pm, tn, kb0, kb1);
+                const int arow = (pm * 2 + (int)rank) * 128;
+                const int brow = EPI == P_UP ? tn * 128 : tn * 256 + (int)rank * 128;
+                for (int kb = kb0; kb < kb1; ++kb, ++kc) {
+                    if ((int)(kc & 1) != par) continue;
+                    const int stage = (int)(kc % NST);
+                    const uint32_t phase = (uint32_t)((kc / NST) & 1);
+                    if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u)) {
+                        atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
+                        s_abort = 1;
+                        stop = true;
+                        break;
+                    }
+                    unsigned char* sa = smem + stage * P_STAGE;
+                    const bool second = EPI == P_STORE && kb >= args.nkb1;
+                    const int k = (second ? kb - args.nkb1 : kb) * P_BK;
+                    if (loads_a) {
+                        if (leader) {
+                            mbar_arrive_expect_tx(&full_bar[stage], 2 * P_STAGE);
+                            ++armed[stage];
+                        }
+                        const CUtensorMap* ma = second ? &tmA2 : &tmA;
+                        if constexpr (!A_MN) {
+                            tma_load_2d_pair(sa, ma, k, arow, &full_bar[stage]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                tma_load_2d_pair(sa + j * MN_LBO, ma, arow + j * 64, k, &full_bar[stage]);
+                        }
+                    } else {
+                        unsigned char* sb = sa + P_OPERAND;
+                        const CUtensorMap* mb = EPI == P_UP ? (leader ? &tmB : &tmB2) : second ? &tmB2 : &tmB;
+                        if constexpr (!B_MN) {
+                            tma_load_2d_pair(sb, mb, k, brow, &full_bar[stage]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                tma_load_2d_pair(sb + j * MN_LBO, mb, brow + j * 64, k, &full_bar[stage]);
+                        }
+                    }
+                }
+            }
+            // once the last phases armed here complete, no copy is still landing in either CTA
+            if (leader && loads_a)
+                for (int s = 0; s < NST; ++s)
+                    if (armed[s]) (void)mbar_wait_bounded(&full_bar[s], (uint32_t)(armed[s] - 1) & 1u);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ----------------------------------------------------------- MMA --
+        if (lane == 0 && leader) {
+            int stage = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            for (int task = first_task; task < ntasks && !s_abort; task += task_stride) {
+                int pm, tn, kb0, kb1;
+                locate(task, pm, tn, kb0, kb1);
+                if (!mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1u)) {
+                    atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
+                    s_abort = 1;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem_base + (uint32_t)(acc * 256);
+                bool ready = mbar_try_wait(&full_bar[stage], phase), fail = false;
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!ready && !mbar_wait_bounded(&full_bar[stage], phase)) {
+                        atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
+                        s_abort = 1;
+                        fail = true;
+                        break;
+                    }
+                    const uint32_t sa = smem_u32(smem + stage * P_STAGE), sb = sa + P_OPERAND;
+#pragma unroll
+                    for (int k = 0; k < P_BK / 16; ++k) {
+                        const uint64_t ad = A_MN ? umma_desc_sw128(sa + k * 2048, MN_LBO, 1024)
+                                                 : umma_desc_sw128(sa + k * 32, 16, 1024);
+                        const uint64_t bd = B_MN ? umma_desc_sw128(sb + k * 2048, MN_LBO, 1024)
+                                                 : umma_desc_sw128(sb + k * 32, 16, 1024);
+                        tc_mma_f16_pair(d, ad, bd, IDESC, ((kb - kb0) | k) != 0 ? 1u : 0u);
+                    }
+                    tc_commit_pair_multicast(&empty_bar[stage], 0x3);
+                    if (++stage == NST) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                    ready = kb + 1 < kb1 && mbar_try_wait(&full_bar[stage], phase);
+                }
+                if (fail) break;
+                tc_commit_pair_multicast(&tfull_bar[acc], 0x3);
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4 && warp < 12) {
+        // ------------------------------------------------------ epilogue --
+        const int wg = (warp - 4) >> 2, ew = warp & 3;
+        unsigned char* sbuf = smem + NST * P_STAGE + (warp - 4) * (p_bufs<EPI>() * 2048);
+        const uint32_t tempty_leader[2] = {leader_smem_addr(&tempty_bar[0]), leader_smem_addr(&tempty_bar[1])};
+        int acc = 0, it = 0;
+        uint32_t acc_phase = 0;
+        for (int task = first_task; task < ntasks; task += task_stride, ++it) {
+            int pm, tn, kb0, kb1;
+            const int sp = locate(task, pm, tn, kb0, kb1);
+            const int row0 = (pm * 2 + (int)rank) * 128 + ew * 32;  // first row of this warp
+            const int row = row0 + lane;
+            const bool row_ok = row < args.M;
+            const int gcol0 = tn * TILE_N + wg * (TILE_N / 2);  // first column of this warpgroup
+            const bool ok = __all_sync(FULL, mbar_wait_bounded(&tfull_bar[acc], acc_phase));
+            if (!ok && lane == 0) atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
+            bool dead = !ok || __any_sync(FULL, s_abort != 0);
+            // The epilogue warps meet below (UP keeping 8 bits): all of them go on or
+            // none.  s_dead is theirs alone, written before the first barrier and
+            // read between the two.
+            if constexpr (EPI == P_UP) {
+                if (args.keep == KEEP_8) {
+                    if (dead && lane == 0) s_dead = 1;
+                    named_bar_sync(1, 256);
+                    dead = *reinterpret_cast<volatile int*>(&s_dead) != 0;
+                    named_bar_sync(1, 256);
+                }
+            }
+            if (dead) break;
+            tc_fence_after();
+            const uint32_t tbase = tmem_base + ((uint32_t)(ew * 32) << 16) + (uint32_t)(acc * 256 + wg * (TILE_N / 2));
+
+            if constexpr (EPI == P_STORE) {
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    const int col = gcol0 + c * 32;
+                    if (row0 >= args.M || col >= args.N) break;  // warp-uniform
+                    uint32_t r[32];
+                    tmem_ld32(tbase + c * 32, r);
+                    tmem_wait_ld();
+                    if (args.splits > 1) {
+                        // float32 parts: each lane its row's 128 contiguous bytes
+                        if (row_ok) {
+                            float* p = args.part + ((long long)sp * args.M + row) * args.ldp + col;
+#pragma unroll
+                            for (int q = 0; q < 8; ++q)
+                                if (col + 4 * q < args.ldp)  // ldp is a multiple of 4
+                                    reinterpret_cast<uint4*>(p)[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+                        }
+                        continue;
+                    }
+                    uint32_t w[16];
+#pragma unroll
+                    for (int q = 0; q < 16; ++q)
+                        w[q] = pack16x2<DT>(__uint_as_float(r[2 * q]), __uint_as_float(r[2 * q + 1]));
+                    if (args.vec_out) {
+                        stage_free(lane);
+                        stage32(sbuf, lane, w);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&tmC, sbuf, col, row0);
+                            bulk_commit_group();
+                        }
+                    } else if (row_ok) {
+                        uint16_t* p = args.out + (long long)row * args.ldc;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (col + j < args.N) p[col + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+                    }
+                }
+            } else if constexpr (EPI == P_UP) {
+                uint32_t gmax = 0, umax = 0;
+                const bool warp_live = row0 < args.M;
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    const int col = gcol0 + c * 32;
+                    if (!warp_live || col >= args.N) break;
+                    uint32_t g[32], u[32], w[16];
+                    tmem_ld32(tbase + c * 32, g);
+                    tmem_ld32(tbase + 128 + c * 32, u);
+                    tmem_wait_ld();
+                    stage_free(lane);
+                    float unused;
+#pragma unroll
+                    for (int q = 0; q < 16; ++q)
+                        w[q] = pack16x2<DT>(glu_act<ACT, false>(__uint_as_float(g[2 * q]), unused) * __uint_as_float(u[2 * q]),
+                                            glu_act<ACT, false>(__uint_as_float(g[2 * q + 1]), unused) *
+                                                __uint_as_float(u[2 * q + 1]));
+                    stage32(sbuf, lane, w);
+                    if (args.keep == KEEP_16) {
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) w[q] = pack16x2<DT>(__uint_as_float(g[2 * q]), __uint_as_float(g[2 * q + 1]));
+                        stage32(sbuf + 2048, lane, w);
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) w[q] = pack16x2<DT>(__uint_as_float(u[2 * q]), __uint_as_float(u[2 * q + 1]));
+                        stage32(sbuf + 4096, lane, w);
+                    } else if (args.keep == KEEP_8) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            gmax = max(gmax, finite_mag(__uint_as_float(g[j])));
+                            umax = max(umax, finite_mag(__uint_as_float(u[j])));
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmC, sbuf, col, row0);
+                        if (args.keep == KEEP_16) {
+                            tma_store_2d(&tmC2, sbuf + 2048, col, row0);
+                            tma_store_2d(&tmC3, sbuf + 4096, col, row0);
+                        }
+                        bulk_commit_group();
+                    }
+                }
+                if (args.keep == KEEP_8) {
+                    // the block of 128 columns spans both warpgroups (columns past N are zero)
+                    s_amax[it & 1][wg][ew * 32 + lane] = make_uint2(gmax, umax);
+                    named_bar_sync(1, 256);
+                    const uint2 other = s_amax[it & 1][wg ^ 1][ew * 32 + lane];
+                    const int ge = fp8_exponent(max(gmax, other.x)), ue = fp8_exponent(max(umax, other.y));
+                    if (row_ok) {
+                        const long long at = fp8_scale_at(row, tn, args.bt);
+                        if (wg == 0) args.gs[at] = (uint8_t)(ge + 127);
+                        else args.us[at] = (uint8_t)(ue + 127);
+                    }
+                    const float ginv = two_to(-ge), uinv = two_to(-ue);
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        const int col = gcol0 + (c >> 1) * 32;
+                        if (!warp_live || col >= args.N) break;
+                        const bool is_u = c & 1;
+                        uint32_t r[32];
+                        tmem_ld32(tbase + (is_u ? 128 : 0) + (c >> 1) * 32, r);
+                        tmem_wait_ld();
+                        uint32_t w[8];
+                        const float inv = is_u ? uinv : ginv;
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)
+                            w[q] = fp8_pack4(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]),
+                                             __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]), inv);
+                        if (row_ok) {  // a whole 32-byte sector
+                            uint4* p = reinterpret_cast<uint4*>((is_u ? args.u8 : args.g8) + (long long)row * args.ldk + col);
+                            p[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                            p[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                    }
+                }
+            } else {  // P_DGRAD
+                float gscale = 1.f, uscale = 1.f;
+                if (args.keep == KEEP_8 && row_ok && gcol0 < args.N) {
+                    const long long at = fp8_scale_at(row, gcol0 >> 7, args.bt);
+                    gscale = fp8_scale(args.gs[at]);
+                    uscale = fp8_scale(args.us[at]);
+                }
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    const int col = gcol0 + c * 32;
+                    if (row0 >= args.M || col >= args.N) break;
+                    uint32_t gw[16], uw[16];  // 16-bit pairs, or 8 words of four bytes
+                    if (args.keep == KEEP_8) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            uint4 a = make_uint4(0, 0, 0, 0), b = a;
+                            if (row_ok) {
+                                a = __ldcs(reinterpret_cast<const uint4*>(args.g8 + (long long)row * args.ldk + col) + i);
+                                b = __ldcs(reinterpret_cast<const uint4*>(args.u8 + (long long)row * args.ldk + col) + i);
+                            }
+                            gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
+                            uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint4 a = make_uint4(0, 0, 0, 0), b = a;
+                            if (row_ok) {
+                                a = __ldcs(reinterpret_cast<const uint4*>(args.g + (long long)row * args.ldk + col) + i);
+                                b = __ldcs(reinterpret_cast<const uint4*>(args.u + (long long)row * args.ldk + col) + i);
+                            }
+                            gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
+                            uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
+                        }
+                    }
+                    uint32_t r[32], wg_[16], wu_[16], wh_[16];
+                    tmem_ld32(tbase + c * 32, r);
+                    tmem_wait_ld();
+                    auto quad = [&](int q, const float (&g)[4], const float (&u)[4]) {  // elements 4q .. 4q + 3
+                        float dg[4], du[4], h[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float dh = __uint_as_float(r[4 * q + j]);
+                            float d;
+                            const float a = glu_act<ACT, true>(g[j], d);
+                            dg[j] = dh * u[j] * d;
+                            du[j] = dh * a;
+                            h[j] = a * u[j];
+                        }
+                        wg_[2 * q] = pack16x2<DT>(dg[0], dg[1]), wg_[2 * q + 1] = pack16x2<DT>(dg[2], dg[3]);
+                        wu_[2 * q] = pack16x2<DT>(du[0], du[1]), wu_[2 * q + 1] = pack16x2<DT>(du[2], du[3]);
+                        wh_[2 * q] = pack16x2<DT>(h[0], h[1]), wh_[2 * q + 1] = pack16x2<DT>(h[2], h[3]);
+                    };
+                    if (args.keep == KEEP_8) {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {
+                            float g[4], u[4];
+                            fp8_unpack4(gw[q], g);
+                            fp8_unpack4(uw[q], u);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) g[j] *= gscale, u[j] *= uscale;
+                            quad(q, g, u);
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {
+                            const float2 g0 = unpack16x2<DT>(gw[2 * q]), g1 = unpack16x2<DT>(gw[2 * q + 1]);
+                            const float2 u0 = unpack16x2<DT>(uw[2 * q]), u1 = unpack16x2<DT>(uw[2 * q + 1]);
+                            const float g[4] = {g0.x, g0.y, g1.x, g1.y}, u[4] = {u0.x, u0.y, u1.x, u1.y};
+                            quad(q, g, u);
+                        }
+                    }
+                    stage_free(lane);
+                    stage32(sbuf, lane, wg_);
+                    stage32(sbuf + 2048, lane, wu_);
+                    stage32(sbuf + 4096, lane, wh_);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmC, sbuf, col, row0);
+                        tma_store_2d(&tmC2, sbuf + 2048, col, row0);
+                        tma_store_2d(&tmC3, sbuf + 4096, col, row0);
+                        bulk_commit_group();
+                    }
+                }
+            }
+            // this accumulator back to the leader's MMA warp
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(tempty_leader[acc]);
+            if (++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1u;
+            }
+        }
+        if (lane == 0) bulk_wait_group0();
+        __syncwarp();
+    }
+    // neither CTA leaves while the other can touch its shared or tensor memory
+    tc_fence_before();
+    cluster_sync();
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+// C = the parts of a product split over K, added in their order.
+template <int DT>
+__global__ void __launch_bounds__(256)
+    join_parts_kernel(const float* __restrict__ part, int splits, long long M, int N, long long ldp, uint16_t* __restrict__ out,
+                      long long ldc, int vec) {
+    const long long quads = ldp / 4, n = M * quads;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const long long row = i / quads;
+        const int col = (int)(i - row * quads) * 4;
+        const float4* p = reinterpret_cast<const float4*>(part + row * ldp + col);
+        float4 s = __ldcs(p);
+        for (int k = 1; k < splits; ++k) {
+            const float4 v = __ldcs(p + k * (M * quads));
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        uint16_t* o = out + row * ldc + col;
+        const uint2 w = make_uint2(pack16x2<DT>(s.x, s.y), pack16x2<DT>(s.z, s.w));
+        if (vec && col + 4 <= N) {
+            *reinterpret_cast<uint2*>(o) = w;
+        } else {
+            if (col < N) o[0] = (uint16_t)w.x;
+            if (col + 1 < N) o[1] = (uint16_t)(w.x >> 16);
+            if (col + 2 < N) o[2] = (uint16_t)w.y;
+            if (col + 3 < N) o[3] = (uint16_t)(w.y >> 16);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host ----
+struct Operand {
+    const void* p;
+    long long ld;
+};
+
+// Map of a 16-bit operand [rows][K] (K-major) or [K][rows] (MN-major): boxes of
+// 64 k x 128 rows, or 64 rows x 64 k.
+int operand_map(CUtensorMap* m, const Operand& o, bool mn, long long rows, long long K) {
+    const auto t = CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    const auto sw = CU_TENSOR_MAP_SWIZZLE_128B;
+    return mn ? tmap_2d(m, t, 2, o.p, rows, K, o.ld, 64, P_BK, sw) : tmap_2d(m, t, 2, o.p, K, rows, o.ld, P_BK, 128, sw);
+}
+int store_map(CUtensorMap* m, const void* p, long long rows, long long cols, long long ld) {
+    return tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p, cols, rows, ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+bool operand_ok(const void* p, long long ld) { return aligned16(p) && ld % 8 == 0; }
+
+template <int DT, bool A_MN, bool B_MN, int EPI, int ACT>
+int launch_pair(const CUtensorMap (&m)[7], const PairArgs& args, cudaStream_t st) {
+    auto k = pair_kernel<DT, A_MN, B_MN, EPI, ACT>;
+    constexpr int smem = p_smem<EPI>();
+    SFFN_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static const int pairs = resident_pairs(k, P_THREADS, smem);
+    const long long tasks = (long long)((args.tiles_m + 1) / 2) * args.tiles_n * args.splits;
+    const int clusters = (int)std::min<long long>(tasks, pairs);
+    k<<<clusters * 2, P_THREADS, smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], args);
+    SFFN_CHECK_LAUNCH();
+    return SFFN_OK;
+}
+
+constexpr int P_PAIRS = 74;  // CTA pairs of a B200
+
+// How many parts K is split into: a product of few tiles leaves pairs idle, so
+// its k-blocks are dealt to more of them.  Costs are counted in k-blocks of one
+// pair (about 0.27 us at 256 x 256 x 64): the rounds of tasks times a part's
+// blocks, 4 to fill the pipeline, and for parts their float32 traffic (8 bytes
+// an element and part through HBM: 0.011 us a tile and part over 74 pairs) and
+// the second kernel (3 us).
+int split_of(long long tiles, long long nkb) {
+    long long best = 0;
+    int best_s = 1;
+    for (int s = 1; s <= 32 && s <= nkb; ++s) {
+        const long long per = (nkb + s - 1) / s;
+        if ((nkb + per - 1) / per != s) continue;
+        const long long rounds = (tiles * s + P_PAIRS - 1) / P_PAIRS;
+        const long long cost = 100 * rounds * (per + 4) + (s > 1 ? 1100 + 30 * tiles * s : 0);
+        if (s == 1 || cost < best) best = cost, best_s = s;
+    }
+    return best_s;
+}
+long long tiles_of(long long M, long long N) { return (M + 255) / 256 * ((N + 255) / 256); }
+long long kblocks(long long K) { return (K + P_BK - 1) / P_BK; }
+long long part_ld(long long N) { return (N + 3) / 4 * 4; }
+
+bool sizes_ok(long long M, long long N, long long K) {
+    const long long most = 0x7FFFFF00;
+    return M <= most && N <= most && K <= most && tiles_of(M, N) <= 0x1FFFFFF;
+}
+
+template <int DT>
+int gemm16(const Operand& A, bool a_mn, const Operand& B, bool b_mn, const Operand& A2, const Operand& B2, long long K2,
+           long long M, long long N, long long K, void* C, long long ldc, void* ws, size_t ws_bytes, uint32_t* status,
+           cudaStream_t st) {
+    PairArgs a{};
+    a.M = (int)M;
+    a.N = (int)N;
+    a.tiles_m = (int)((M + 127) / 128);
+    a.tiles_n = (int)((N + 255) / 256);
+    a.nkb1 = (int)kblocks(K);
+    a.nkb = a.nkb1 + (K2 ? (int)kblocks(K2) : 0);
+    a.splits = split_of(tiles_of(M, N), a.nkb);
+    a.ldp = part_ld(N);
+    if (a.splits > 1 && (!ws || ws_bytes < (size_t)a.splits * (size_t)M * (size_t)a.ldp * 4)) return SFFN_ERR_WORKSPACE;
+    a.per_split = (a.nkb + a.splits - 1) / a.splits;
+    a.part = static_cast<float*>(ws);
+    a.out = static_cast<uint16_t*>(C);
+    a.ldc = ldc;
+    a.vec_out = aligned16(C) && ldc % 8 == 0;
+    a.status = status;
+    CUtensorMap m[7];
+    memset(m, 0, sizeof(m));
+    if (int rc = operand_map(&m[0], A, a_mn, M, K)) return rc;
+    if (int rc = operand_map(&m[1], B, b_mn, N, K)) return rc;
+    if (K2) {
+        if (int rc = operand_map(&m[2], A2, a_mn, M, K2)) return rc;
+        if (int rc = operand_map(&m[3], B2, b_mn, N, K2)) return rc;
+    }
+    if (a.vec_out && a.splits == 1)
+        if (int rc = store_map(&m[4], C, M, N, ldc)) return rc;
+    int rc = !a_mn && !b_mn ? launch_pair<DT, false, false, P_STORE, 0>(m, a, st)
+             : !a_mn        ? launch_pair<DT, false, true, P_STORE, 0>(m, a, st)
+             : b_mn         ? launch_pair<DT, true, true, P_STORE, 0>(m, a, st)
+                            : launch_pair<DT, true, false, P_STORE, 0>(m, a, st);
+    if (rc || a.splits == 1) return rc;
+    const long long quads = M * (a.ldp / 4);
+    const int grid = (int)std::min<long long>((quads + 255) / 256, 148 * 8);
+    join_parts_kernel<DT><<<grid, 256, 0, st>>>(a.part, a.splits, M, (int)N, a.ldp, a.out, ldc,
+                                                 reinterpret_cast<uintptr_t>(C) % 8 == 0 && ldc % 4 == 0);
+    SFFN_CHECK_LAUNCH();
+    return SFFN_OK;
+}
+
+template <int DT, int EPI, bool B_MN>
+int launch_act(int act, const CUtensorMap (&m)[7], const PairArgs& a, cudaStream_t st) {
+    switch (act) {
+        case GLU_RELU: return launch_pair<DT, false, B_MN, EPI, GLU_RELU>(m, a, st);
+        case GLU_RELU2: return launch_pair<DT, false, B_MN, EPI, GLU_RELU2>(m, a, st);
+        case GLU_SILU: return launch_pair<DT, false, B_MN, EPI, GLU_SILU>(m, a, st);
+        default: return launch_pair<DT, false, B_MN, EPI, GLU_GELU>(m, a, st);
+    }
+}
+
+// Arguments the two fused products share; F columns of h, D of x and y.
+int check_glu(int dtype, int act, int keep, long long T, long long D, long long F, const void* g, const void* u, long long ldk,
+              const void* gs, const void* us, const void* status) {
+    if (dtype != SFFN_BF16 && dtype != SFFN_F16) return SFFN_ERR_DTYPE;
+    if (act < GLU_RELU || act > GLU_GELU || keep < KEEP_NONE || keep > KEEP_8 || T < 0 || D <= 0 || F <= 0 || !status)
+        return SFFN_ERR_ARG;
+    if (!sizes_ok(T, F, D) || T * fp8_block_tiles(F) > 0x7FFFFFFF) return SFFN_ERR_TOO_LARGE;
+    if (keep == KEEP_NONE) return SFFN_OK;
+    if (!g || !u || ldk < F || (keep == KEEP_8 && (!gs || !us))) return SFFN_ERR_ARG;
+    // whole 32-column chunks of the kept rows are written and read
+    if (!aligned16(g) || !aligned16(u) || ldk % 32) return SFFN_ERR_ALIGN;
+    return SFFN_OK;
+}
+
+PairArgs glu_args(long long T, long long F, long long D, int tile_n, int keep, const void* g, const void* u, long long ldk,
+                  const void* gs, const void* us, uint32_t* status) {
+    PairArgs a{};
+    a.M = (int)T;
+    a.N = (int)F;
+    a.tiles_m = (int)((T + 127) / 128);
+    a.tiles_n = (int)((F + tile_n - 1) / tile_n);
+    a.nkb = a.nkb1 = a.per_split = (int)kblocks(D);
+    a.splits = 1;
+    a.keep = keep;
+    if (keep == KEEP_8) {
+        a.g8 = static_cast<uint8_t*>(const_cast<void*>(g));
+        a.u8 = static_cast<uint8_t*>(const_cast<void*>(u));
+        a.gs = static_cast<uint8_t*>(const_cast<void*>(gs));
+        a.us = static_cast<uint8_t*>(const_cast<void*>(us));
+    } else {
+        a.g = static_cast<const uint16_t*>(g);
+        a.u = static_cast<const uint16_t*>(u);
+    }
+    a.ldk = ldk;
+    a.bt = (int)fp8_block_tiles(F);
+    a.status = status;
+    return a;
+}
+
+}  // namespace
+}  // namespace sffn
+
+using namespace sffn;
+
+extern "C" size_t sffn_gemm16_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t K2) {
+    if (M <= 0 || N <= 0 || K <= 0 || K2 < 0 || !sizes_ok(M, N, K) || !sizes_ok(M, N, K2)) return 0;
+    const int s = split_of(tiles_of(M, N), kblocks(K) + (K2 ? kblocks(K2) : 0));
+    return s > 1 ? (size_t)s * (size_t)M * (size_t)part_ld(N) * 4 : 0;
+}
+
+extern "C" int sffn_gemm16(int dtype, const void* A, int64_t lda, int a_mn, const void* B, int64_t ldb, int b_mn,
+                           const void* A2, int64_t lda2, const void* B2, int64_t ldb2, int64_t K2, int64_t M, int64_t N,
+                           int64_t K, void* C, int64_t ldc, void* workspace, size_t workspace_bytes, uint32_t* status_dev,
+                           void* stream) {
+    if (dtype != SFFN_BF16 && dtype != SFFN_F16) return SFFN_ERR_DTYPE;
+    if (M < 0 || N < 0 || K <= 0 || K2 < 0 || !status_dev) return SFFN_ERR_ARG;
+    if (M == 0 || N == 0) return SFFN_OK;
+    if (!sizes_ok(M, N, K) || !sizes_ok(M, N, K2)) return SFFN_ERR_TOO_LARGE;
+    if (!A || !B || !C || ldc < N || lda < (a_mn ? M : K) || ldb < (b_mn ? N : K) ||
+        (K2 && (!A2 || !B2 || lda2 < (a_mn ? M : K2) || ldb2 < (b_mn ? N : K2))))
+        return SFFN_ERR_ARG;
+    if (!operand_ok(A, lda) || !operand_ok(B, ldb) || (K2 && (!operand_ok(A2, lda2) || !operand_ok(B2, ldb2))) ||
+        reinterpret_cast<uintptr_t>(C) % 2 || (workspace && !aligned16(workspace)))
+        return SFFN_ERR_ALIGN;
+    DeviceScope scope;
+    if (int rc = scope.bind_same(A, {B, K2 ? A2 : nullptr, K2 ? B2 : nullptr, C, workspace, status_dev})) return rc;
+    if (!sm100_sms()) return SFFN_ERR_DEVICE;
+    const Operand a{A, lda}, b{B, ldb}, a2{A2, lda2}, b2{B2, ldb2};
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return dtype == SFFN_BF16
+               ? gemm16<SFFN_BF16>(a, a_mn != 0, b, b_mn != 0, a2, b2, K2, M, N, K, C, ldc, workspace, workspace_bytes, status_dev, st)
+               : gemm16<SFFN_F16>(a, a_mn != 0, b, b_mn != 0, a2, b2, K2, M, N, K, C, ldc, workspace, workspace_bytes, status_dev, st);
+}
+
+extern "C" int sffn_glu_up(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
+                           int64_t ldwu, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, int keep, void* g, void* u,
+                           int64_t ldk, void* g_scales, void* u_scales, uint32_t* status_dev, void* stream) {
+    if (int rc = check_glu(dtype, act, keep, T, D, F, g, u, ldk, g_scales, u_scales, status_dev)) return rc;
+    if (T == 0) return SFFN_OK;
+    if (!x || !wg || !wu || !h || ldx < D || ldwg < D || ldwu < D || ldh < F) return SFFN_ERR_ARG;
+    if (!operand_ok(x, ldx) || !operand_ok(wg, ldwg) || !operand_ok(wu, ldwu) || !operand_ok(h, ldh))
+        return SFFN_ERR_ALIGN;
+    DeviceScope scope;
+    if (int rc = scope.bind_same(x, {wg, wu, h, g, u, g_scales, u_scales, status_dev})) return rc;
+    if (!sm100_sms()) return SFFN_ERR_DEVICE;
+    const PairArgs a = glu_args(T, F, D, 128, keep, g, u, ldk, g_scales, u_scales, status_dev);
+    CUtensorMap m[7];
+    memset(m, 0, sizeof(m));
+    if (int rc = operand_map(&m[0], {x, ldx}, false, T, D)) return rc;
+    if (int rc = operand_map(&m[1], {wg, ldwg}, false, F, D)) return rc;
+    if (int rc = operand_map(&m[3], {wu, ldwu}, false, F, D)) return rc;
+    if (int rc = store_map(&m[4], h, T, F, ldh)) return rc;
+    if (keep == KEEP_16) {
+        if (int rc = store_map(&m[5], g, T, F, ldk)) return rc;
+        if (int rc = store_map(&m[6], u, T, F, ldk)) return rc;
+    }
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return dtype == SFFN_BF16 ? launch_act<SFFN_BF16, P_UP, false>(act, m, a, st)
+                              : launch_act<SFFN_F16, P_UP, false>(act, m, a, st);
+}
+
+extern "C" int sffn_glu_dgrad(int dtype, int act, const void* dy, int64_t lddy, const void* w2, int64_t ldw2, int64_t T,
+                              int64_t D, int64_t F, int keep, const void* g, const void* u, int64_t ldk,
+                              const void* g_scales, const void* u_scales, void* dg, void* du, int64_t ldd, void* h,
+                              int64_t ldh, uint32_t* status_dev, void* stream) {
+    if (keep == KEEP_NONE) return SFFN_ERR_ARG;
+    if (int rc = check_glu(dtype, act, keep, T, D, F, g, u, ldk, g_scales, u_scales, status_dev)) return rc;
+    if (T == 0) return SFFN_OK;
+    if (!dy || !w2 || !dg || !du || !h || lddy < D || ldw2 < F || ldd < F || ldh < F) return SFFN_ERR_ARG;
+    if (!operand_ok(dy, lddy) || !operand_ok(w2, ldw2) || !operand_ok(dg, ldd) || !operand_ok(du, ldd) ||
+        !operand_ok(h, ldh))
+        return SFFN_ERR_ALIGN;
+    DeviceScope scope;
+    if (int rc = scope.bind_same(dy, {w2, g, u, g_scales, u_scales, dg, du, h, status_dev})) return rc;
+    if (!sm100_sms()) return SFFN_ERR_DEVICE;
+    const PairArgs a = glu_args(T, F, D, 256, keep, g, u, ldk, g_scales, u_scales, status_dev);
+    CUtensorMap m[7];
+    memset(m, 0, sizeof(m));
+    if (int rc = operand_map(&m[0], {dy, lddy}, false, T, D)) return rc;
+    if (int rc = operand_map(&m[1], {w2, ldw2}, true, F, D)) return rc;
+    if (int rc = store_map(&m[4], dg, T, F, ldd)) return rc;
+    if (int rc = store_map(&m[5], du, T, F, ldd)) return rc;
+    if (int rc = store_map(&m[6], h, T, F, ldh)) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return dtype == SFFN_BF16 ? launch_act<SFFN_BF16, P_DGRAD, true>(act, m, a, st)
+                              : launch_act<SFFN_F16, P_DGRAD, true>(act, m, a, st);
+}

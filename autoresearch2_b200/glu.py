@@ -1,0 +1,142 @@
+"""The gated feed-forward block, forward and backward.
+
+    gated_ffn(x, Wg, Wu, W2, activation="silu", checkpoint=None)
+
+    g = x Wg^T, u = x Wu^T, h = act(g) * u, y = h W2^T
+
+One kernel computes both projections, the activation and the product; g and u
+never make a trip through memory on the way to h.  The backward works from x, g
+and u as the forward kept them -- in the inputs' type, or with
+checkpoint="fp8" in the 8-bit block format of fp8.py, half the bytes:
+
+    dh = dy W2, dg = dh * u * act'(g), du = dh * act(g)
+    dW2 = dy^T (act(g) * u), dWg = dg^T x, dWu = du^T x, dx = dg Wg + du Wu
+
+dh's kernel reads g and u and writes dg, du and act(g) * u; dx is one product
+over both pairs.  Products sum in float32; h, dg and du are rounded to the
+inputs' type, in which the tensor cores read them.
+"""
+import torch
+
+from . import _lib, fp8
+from ._lib import address as ptr
+from ._lib import call, stream_handle
+from .parallel import submit_grad
+
+__all__ = ["ACTIVATIONS", "gated_ffn"]
+
+ACTIVATIONS = {"relu": 0, "relu2": 1, "silu": 2, "gelu": 3}
+KEEP = {None: 1, "fp8": 2}
+CHUNK = 32  # columns: kept rows are padded to whole ones
+
+
+def _forward(x, Wg, Wu, W2, act, keep):
+    """(y, g, u, g_tiles, u_tiles, x_values, x_tiles): keep 0 keeps nothing, 1 g
+    and u in x's type, 2 all three in 8 bits; what is not kept is None."""
+    x2, Wg, Wu, W2 = map(fp8._rows, (x, Wg, Wu, W2))
+    T, D = x2.shape
+    F, dev, code = Wg.shape[0], x.device, _lib._DTYPES[x.dtype]
+    g = u = gt = ut = xv = xt = None
+    if keep == 2:
+        g, u = (fp8._empty_values(T, F, dev, CHUNK) for _ in range(2))
+        gt, ut = (fp8._empty_tiles(T, F, dev) for _ in range(2))
+        xv, xt = fp8._pack(x2)
+    elif keep == 1:
+        g, u = (x2.new_empty((T, fp8._cdiv(F, CHUNK) * CHUNK))[:, :F] for _ in range(2))
+    if T == 0:
+        return x.new_empty((*x.shape[:-1], D)), g, u, gt, ut, xv, xt
+    ldk = fp8._cdiv(F, CHUNK) * CHUNK
+    ldh = fp8._cdiv(F, 8) * 8
+    h = x2.new_empty((T, ldh))[:, :F]
+    if keep == 0 and T <= fp8.FEW_ROWS:
+        call("sffn_few_rows_glu", code, act, x2.data_ptr(), fp8._ld(x2), Wg.data_ptr(), fp8._ld(Wg), Wu.data_ptr(),
+             fp8._ld(Wu), T, D, F, h.data_ptr(), ldh, stream_handle(dev))
+    else:
+        (xa, ldx), (Wg, ldg), (Wu, ldu) = map(fp8._aligned, (x2, Wg, Wu))
+        call("sffn_glu_up", code, act, xa.data_ptr(), ldx, Wg.data_ptr(), ldg, Wu.data_ptr(), ldu, T, D, F, h.data_ptr(), ldh,
+             keep, ptr(g), ptr(u), ldk, ptr(gt), ptr(ut), _lib.status_word(dev).data_ptr(), stream_handle(dev))
+    return fp8._linear(h, W2).view(x.shape), g, u, gt, ut, xv, xt
+
+
+def _backward(dy, x, Wg, Wu, W2, g, u, gt, ut, xv, xt, act, want):
+    """Gradients of (x, Wg, Wu, W2); None where `want` is false.  x is None with 8-bit checkpoints."""
+    _lib.bind_thread(dy.device)
+    dy2, Wg, Wu, W2 = map(fp8._rows, (dy, Wg, Wu, W2))
+    T, D = dy2.shape
+    F, dev, code = Wg.shape[0], dy.device, _lib._DTYPES[dy.dtype]
+    dx = dWg = dWu = dW2 = None
+    if T == 0:
+        zeros = [w.new_zeros(w.shape) if n else None for w, n in zip((Wg, Wu, W2), want[1:])]
+        return (dy.new_empty(dy.shape) if want[0] else None, *zeros)
+    keep = 2 if xv is not None else 1
+    ld, ldk = fp8._cdiv(F, 8) * 8, fp8._cdiv(F, CHUNK) * CHUNK
+    d = dy2.new_empty((T, 2 * ld))  # dg | du, so that their weight gradients are one product
+    dg, du = d[:, :F], d[:, ld:ld + F]
+    h = dy2.new_empty((T, ld))[:, :F]
+    dya, lddy = fp8._aligned(dy2)
+    W2a, ldw2 = fp8._aligned(W2)
+    call("sffn_glu_dgrad", code, act, dya.data_ptr(), lddy, W2a.data_ptr(), ldw2, T, D, F, keep, g.data_ptr(), u.data_ptr(),
+         ldk, ptr(gt), ptr(ut), dg.data_ptr(), du.data_ptr(), 2 * ld, h.data_ptr(), ld, _lib.status_word(dev).data_ptr(),
+         stream_handle(dev))
+    if want[3]:
+        dW2 = submit_grad(fp8._mm_into(W2.new_empty((D, F)), dya, True, h, True))
+    del h
+    if want[1] or want[2]:
+        xk = fp8._unpack(xv, xt, (T, D), dy.dtype) if keep == 2 else fp8._rows(x)
+        if want[1] and want[2]:
+            dW = fp8._mm_into(Wg.new_empty((2 * ld, D)), d, True, xk, True)
+            dWg, dWu = dW[:F], dW[ld:ld + F]
+        elif want[1]:
+            dWg = fp8._mm_into(Wg.new_empty((F, D)), dg, True, xk, True)
+        else:
+            dWu = fp8._mm_into(Wu.new_empty((F, D)), du, True, xk, True)
+        submit_grad(dWg)
+        submit_grad(dWu)
+        del xk
+    if want[0]:
+        dx = fp8._mm_into(dy2.new_empty((T, D)), dg, False, Wg, True, (du, Wu)).view(dy.shape)
+    return dx, dWg, dWu, dW2
+
+
+class _GatedFFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, Wg, Wu, W2, act, keep):
+        y, *kept = _forward(x, Wg, Wu, W2, act, keep)
+        ctx.save_for_backward(x if keep == 1 else None, Wg, Wu, W2, *kept)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        _lib.once_differentiable("gated_ffn")
+        return *_backward(dy, *ctx.saved_tensors, ctx.act, ctx.needs_input_grad[:4]), None, None
+
+
+def _check(x, Wg, Wu, W2):
+    D = x.shape[-1] if x.dim() else 0
+    F = Wg.shape[0] if Wg.dim() else 0
+    fp8._check_weights(x, Wg=(Wg, (F, D)), Wu=(Wu, (F, D)), W2=(W2, (D, F)))
+
+
+def gated_ffn(x, Wg, Wu, W2, activation="silu", checkpoint=None):
+    """y [..., D] of x [..., D], Wg and Wu [F, D], W2 [D, F] (nn.Linear layout),
+    all bfloat16 or all float16.
+
+    activation: "silu", "gelu" (exact), "relu" or "relu2".  checkpoint=None keeps
+    x, x Wg^T and x Wu^T for the backward in their type, "fp8" in 8 bits; the
+    output is the same.  Nothing is kept where no gradient is wanted; calls of up
+    to 32 rows then take the few-row kernels.  Weight gradients are handed to an
+    attached parallel.GradAllReduce as they are produced.  Differentiable once,
+    in reverse mode."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+    if checkpoint not in KEEP:
+        raise ValueError(f"checkpoint must be None or 'fp8', got {checkpoint!r}")
+    _check(x, Wg, Wu, W2)
+    act, keep = ACTIVATIONS[activation], KEEP[checkpoint]
+    tracked = _lib.tracked(x, Wg, Wu, W2)
+    if torch.compiler.is_compiling():
+        return torch.ops.sparseffn.gated_ffn(x, Wg, Wu, W2, act, keep if tracked else 0)[0]
+    if tracked:
+        return _GatedFFN.apply(x, Wg, Wu, W2, act, keep)
+    return _forward(x, Wg, Wu, W2, act, 0)[0]

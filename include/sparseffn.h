@@ -625,6 +625,82 @@ int sffn_residual_norm_bwd(const void* x, int x_dtype, int64_t x_ld, const void*
                            void* dpre, void* dpost, void* dgate, void* workspace, size_t workspace_bytes,
                            uint32_t* status_dev, void* stream);
 
+/* ---- 8-bit blocks --------------------------------------------------------
+ * e4m3 values with one power-of-two scale for each 128 elements of a row: 2^e
+ * with the smallest integer e such that the block's largest finite magnitude is
+ * at most 448 * 2^e, e >= -118 (e = 0 for a block of zeros); infinities and NaN
+ * become NaN.  Values [rows, width], rows `ldv` bytes apart (a multiple of 16).
+ * Scales: bytes e + 127, in tiles of 128 rows x 4 blocks, 512 bytes each:
+ * [rows/128][blocks/4][row % 32][row % 128 / 32][block % 4], rounded up.  No
+ * counterpart in the reference.
+ */
+
+/* x [rows, width] of dtype, row stride ld elements (any alignment).  Bytes of
+ * the values' rows beyond the 16 that hold the last element are not written;
+ * every scale byte is (0 where the tiles are padded). */
+int sffn_fp8_pack(const void* x, int dtype, int64_t rows, int64_t width, int64_t ld, void* values, int64_t ldv,
+                  void* scales, void* stream);
+
+/* The reverse, into out [rows, width] of dtype; finite values beyond the type's
+ * range become its largest. */
+int sffn_fp8_unpack(const void* values, int64_t ldv, const void* scales, int64_t rows, int64_t width, int dtype,
+                    void* out, int64_t ldo, void* stream);
+
+/* C [M, N] (SFFN_BF16 or SFFN_F16) = A [M, K] B [N, K]^T, both in 8-bit blocks,
+ * on the block-scaled tensor cores. */
+int sffn_fp8_mm(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb, const void* b_scales,
+                int64_t M, int64_t N, int64_t K, void* C, int c_dtype, int64_t ldc, uint32_t* status_dev,
+                void* stream);
+
+/* ---- gated feed-forward block -------------------------------------------- */
+
+enum { /* activations */
+    SFFN_GLU_RELU = 0,
+    SFFN_GLU_RELU2 = 1,
+    SFFN_GLU_SILU = 2,
+    SFFN_GLU_GELU = 3 /* x * Phi(x) */
+};
+enum { /* how g and u are kept for the backward */
+    SFFN_KEEP_NONE = 0,
+    SFFN_KEEP_16 = 1, /* in the operands' dtype    */
+    SFFN_KEEP_8 = 2   /* in 8-bit blocks, as above */
+};
+
+/* g = x wg^T, u = x wu^T, h [T, F] = act(g) * u from the unrounded g and u, and
+ * g and u kept as `keep` says: rows ldk elements apart (a multiple of 32; whole
+ * groups of 32 columns of 8-bit values are written), their scale tiles for
+ * SFFN_KEEP_8.  x [T, D], wg and wu [F, D]; every matrix 16-byte aligned with
+ * row strides of a multiple of 8 elements; dtype SFFN_BF16 or SFFN_F16. */
+int sffn_glu_up(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
+                int64_t ldwu, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, int keep, void* g, void* u,
+                int64_t ldk, void* g_scales, void* u_scales, uint32_t* status_dev, void* stream);
+
+/* dh = dy w2 (dy [T, D], w2 [D, F]) and, from g and u as kept,
+ * dg = dh * u * act'(g), du = dh * act(g) (row stride ldd), h = act(g) * u. */
+int sffn_glu_dgrad(int dtype, int act, const void* dy, int64_t lddy, const void* w2, int64_t ldw2, int64_t T,
+                   int64_t D, int64_t F, int keep, const void* g, const void* u, int64_t ldk, const void* g_scales,
+                   const void* u_scales, void* dg, void* du, int64_t ldd, void* h, int64_t ldh, uint32_t* status_dev,
+                   void* stream);
+
+/* C [M, N] = A B^T (+ A2 B2^T over K2 when K2 > 0), 16-bit operands and result
+ * of one dtype, float32 sums.  A is [M, K], with a_mn [K, M]; B [N, K] or
+ * [K, N].  Products of few tiles and a long K are split over K: their float32
+ * parts go to the workspace (NULL where sffn_gemm16_workspace_bytes is 0). */
+size_t sffn_gemm16_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t K2);
+int sffn_gemm16(int dtype, const void* A, int64_t lda, int a_mn, const void* B, int64_t ldb, int b_mn, const void* A2,
+                int64_t lda2, const void* B2, int64_t ldb2, int64_t K2, int64_t M, int64_t N, int64_t K, void* C,
+                int64_t ldc, void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream);
+
+/* Products of at most 32 rows with long weights (any alignment): out [T, N] =
+ * x w^T; h [T, F] = act(x wg^T) * (x wu^T); and x w^T in 8-bit blocks. */
+int sffn_few_rows_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t T, int64_t N, int64_t K,
+                     void* out, int64_t ldo, void* stream);
+int sffn_few_rows_glu(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
+                      int64_t ldwu, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, void* stream);
+int sffn_few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw,
+                      const void* w_scales, int64_t T, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
+                      void* stream);
+
 /* ---- bounded waits ------------------------------------------------------ */
 
 /* Test hook, no counterpart in the reference.  Runs one of this library's
