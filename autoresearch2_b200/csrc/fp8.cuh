@@ -53,13 +53,14 @@ __device__ __forceinline__ float fp8_scale(uint32_t byte) {
 }
 
 // Four values scaled by 2^-e as four e4m3 bytes.  No finite value saturates
-// (the scale sees to that), an infinity becomes a NaN.
+// (the scale sees to that), an infinity becomes a NaN; FINITE: there is none.
+template <bool FINITE>
 __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float inv) {
     const float inf = __uint_as_float(0x7F800000u), nan = __uint_as_float(0x7FFFFFFFu);
-    a = fabsf(a) < inf ? a * inv : nan;
-    b = fabsf(b) < inf ? b * inv : nan;
-    c = fabsf(c) < inf ? c * inv : nan;
-    d = fabsf(d) < inf ? d * inv : nan;
+    a = FINITE || fabsf(a) < inf ? a * inv : nan;
+    b = FINITE || fabsf(b) < inf ? b * inv : nan;
+    c = FINITE || fabsf(c) < inf ? c * inv : nan;
+    d = FINITE || fabsf(d) < inf ? d * inv : nan;
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);

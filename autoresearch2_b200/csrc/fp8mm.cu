@@ -21,12 +21,13 @@
 //                columns, and stores from there while the next tile runs.
 // The 256 x 256 tile is as large as tensor memory allows: at 8 bits a stage's
 // 32 KB a CTA feed 512 cycles of MMA, about what L2 can deliver.
+#include <cuda.h>
 #include <string.h>
 
 #include <algorithm>
 
 #include "fp8.cuh"
-#include "sm100.cuh"
+#include "stage.cuh"
 #include "tmap.cuh"
 
 namespace sffn {
@@ -73,27 +74,6 @@ __device__ __forceinline__ void mma_mx_pair(uint32_t d, uint64_t ad, uint64_t bd
 // the lanes; in each CTA of the pair from its own shared memory.
 __device__ __forceinline__ void cp_scales_pair(uint32_t taddr, uint64_t sdesc) {
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
-}
-
-// The warp's 32 rows x 32 columns (lane = row) to its staging buffer and from
-// there by one bulk-tensor store (64-byte swizzle).
-__device__ __forceinline__ void stage_store(const CUtensorMap* tmap, unsigned char* sbuf, int lane, const uint32_t (&w)[16],
-                                            int col, int row0) {
-    if (lane == 0) bulk_wait_group_read0();
-    __syncwarp();
-    const uint32_t rb = smem_u32(sbuf) + (uint32_t)lane * 64u;
-    const int sw = (lane >> 1) & 3;
-#pragma unroll
-    for (int ch = 0; ch < 4; ++ch)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rb + 16u * (uint32_t)(ch ^ sw)), "r"(w[4 * ch]),
-                     "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3])
-                     : "memory");
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-        tma_store_2d(tmap, sbuf, col, row0);
-        bulk_commit_group();
-    }
 }
 
 template <int DT>
@@ -278,11 +258,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
                 const int col = col0 + c * 32;
                 if (args.vec_out) {
                     stage_store(&tmC, sbuf, lane, w, col, row0);
-                } else if (row0 + lane < args.M) {
-                    uint16_t* row = args.out + (long long)(row0 + lane) * args.ldc;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (col + j < args.N) row[col + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+                } else {
+                    stage_store_plain(args.out, args.ldc, args.M, args.N, sbuf, lane, w, col, row0);
                 }
             }
         }
@@ -345,7 +322,7 @@ extern "C" int sffn_fp8_mm(const void* a, int64_t lda, const void* a_scales, con
         reinterpret_cast<uintptr_t>(C) % 2)
         return SFFN_ERR_ALIGN;
     DeviceScope scope;
-    if (int rc = scope.bind_same(a, {a_scales, b, b_scales, C, status_dev})) return rc;
+    if (int rc = scope.bind(a)) return rc;
     if (!sm100_sms()) return SFFN_ERR_DEVICE;
     MmArgs args{};
     args.M = (int)M;

@@ -21,13 +21,14 @@
 //   DGRAD  dh = dy W2; reads g and u as they were kept and writes
 //          dg = dh u act'(g), du = dh act(g) and h = act(g) u (for dW2): dh
 //          itself is never stored.
+#include <cuda.h>
 #include <string.h>
 
 #include <algorithm>
 
 #include "act.cuh"
 #include "fp8.cuh"
-#include "sm100.cuh"
+#include "stage.cuh"
 #include "tmap.cuh"
 
 namespace sffn {
@@ -75,23 +76,6 @@ __device__ constexpr uint32_t idesc16(bool a_mn, bool b_mn) {
     const uint32_t f = DT == SFFN_BF16 ? 1u : 0u;  // both operands of one type
     return (1u << 4) | (f << 7) | (f << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
            ((uint32_t)(256 >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
-}
-
-// The warp's 32 rows x 32 columns (lane = row) into a staging buffer, in the
-// 64-byte swizzle of the store's tensor map.
-__device__ __forceinline__ void stage32(unsigned char* sbuf, int lane, const uint32_t (&w)[16]) {
-    const uint32_t rb = smem_u32(sbuf) + (uint32_t)lane * 64u;
-    const int sw = (lane >> 1) & 3;
-#pragma unroll
-    for (int ch = 0; ch < 4; ++ch)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rb + 16u * (uint32_t)(ch ^ sw)), "r"(w[4 * ch]),
-                     "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3])
-                     : "memory");
-}
-// Before the staging buffers are written again: their stores have read them.
-__device__ __forceinline__ void stage_free(int lane) {
-    if (lane == 0) bulk_wait_group_read0();
-    __syncwarp();
 }
 
 template <int DT, bool A_MN, bool B_MN, int EPI, int ACT>
@@ -321,21 +305,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
 #pragma unroll
                     for (int q = 0; q < 16; ++q)
                         w[q] = pack16x2<DT>(__uint_as_float(r[2 * q]), __uint_as_float(r[2 * q + 1]));
-                    if (args.vec_out) {
-                        stage_free(lane);
-                        stage32(sbuf, lane, w);
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tma_store_2d(&tmC, sbuf, col, row0);
-                            bulk_commit_group();
-                        }
-                    } else if (row_ok) {
-                        uint16_t* p = args.out + (long long)row * args.ldc;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (col + j < args.N) p[col + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-                    }
+                    if (args.vec_out) stage_store(&tmC, sbuf, lane, w, col, row0);
+                    else stage_store_plain(args.out, args.ldc, args.M, args.N, sbuf, lane, w, col, row0);
                 }
             } else if constexpr (EPI == P_UP) {
                 uint32_t gmax = 0, umax = 0;
@@ -366,8 +337,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     } else if (args.keep == KEEP_8) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            gmax = max(gmax, finite_mag(__uint_as_float(g[j])));
-                            umax = max(umax, finite_mag(__uint_as_float(u[j])));
+                            gmax = max(gmax, g[j] & 0x7FFFFFFFu);
+                            umax = max(umax, u[j] & 0x7FFFFFFFu);
                         }
                     }
                     fence_proxy_async_smem();
@@ -382,6 +353,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     }
                 }
                 if (args.keep == KEEP_8) {
+                    // rare: infinities and NaN do not count
+                    if (__any_sync(FULL, max(gmax, umax) >= 0x7F800000u)) {
+                        gmax = umax = 0;
+#pragma unroll 1
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t g[32], u[32];
+                            tmem_ld32(tbase + c * 32, g);
+                            tmem_ld32(tbase + 128 + c * 32, u);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                gmax = max(gmax, finite_mag(__uint_as_float(g[j])));
+                                umax = max(umax, finite_mag(__uint_as_float(u[j])));
+                            }
+                        }
+                    }
                     // the block of 128 columns spans both warpgroups (columns past N are zero)
                     s_amax[it & 1][wg][ew * 32 + lane] = make_uint2(gmax, umax);
                     named_bar_sync(1, 256);
@@ -405,7 +392,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                         const float inv = is_u ? uinv : ginv;
 #pragma unroll
                         for (int q = 0; q < 8; ++q)
-                            w[q] = fp8_pack4(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]),
+                            w[q] = fp8_pack4<false>(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]),
                                              __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]), inv);
                         if (row_ok) {  // a whole 32-byte sector
                             uint4* p = reinterpret_cast<uint4*>((is_u ? args.u8 : args.g8) + (long long)row * args.ldk + col);
@@ -728,7 +715,7 @@ extern "C" int sffn_gemm16(int dtype, const void* A, int64_t lda, int a_mn, cons
         reinterpret_cast<uintptr_t>(C) % 2 || (workspace && !aligned16(workspace)))
         return SFFN_ERR_ALIGN;
     DeviceScope scope;
-    if (int rc = scope.bind_same(A, {B, K2 ? A2 : nullptr, K2 ? B2 : nullptr, C, workspace, status_dev})) return rc;
+    if (int rc = scope.bind(A)) return rc;
     if (!sm100_sms()) return SFFN_ERR_DEVICE;
     const Operand a{A, lda}, b{B, ldb}, a2{A2, lda2}, b2{B2, ldb2};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -746,7 +733,7 @@ extern "C" int sffn_glu_up(int dtype, int act, const void* x, int64_t ldx, const
     if (!operand_ok(x, ldx) || !operand_ok(wg, ldwg) || !operand_ok(wu, ldwu) || !operand_ok(h, ldh))
         return SFFN_ERR_ALIGN;
     DeviceScope scope;
-    if (int rc = scope.bind_same(x, {wg, wu, h, g, u, g_scales, u_scales, status_dev})) return rc;
+    if (int rc = scope.bind(x)) return rc;
     if (!sm100_sms()) return SFFN_ERR_DEVICE;
     const PairArgs a = glu_args(T, F, D, 128, keep, g, u, ldk, g_scales, u_scales, status_dev);
     CUtensorMap m[7];
@@ -776,7 +763,7 @@ extern "C" int sffn_glu_dgrad(int dtype, int act, const void* dy, int64_t lddy, 
         !operand_ok(h, ldh))
         return SFFN_ERR_ALIGN;
     DeviceScope scope;
-    if (int rc = scope.bind_same(dy, {w2, g, u, g_scales, u_scales, dg, du, h, status_dev})) return rc;
+    if (int rc = scope.bind(dy)) return rc;
     if (!sm100_sms()) return SFFN_ERR_DEVICE;
     const PairArgs a = glu_args(T, F, D, 256, keep, g, u, ldk, g_scales, u_scales, status_dev);
     CUtensorMap m[7];

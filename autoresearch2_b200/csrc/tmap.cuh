@@ -7,6 +7,8 @@
 
 #include <stdio.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace sffn {
@@ -60,13 +62,19 @@ inline int tmap_2d(CUtensorMap* m, CUtensorMapDataType type, int esize, const vo
     return SFFN_OK;
 }
 
-// The current device's multiprocessors; 0 unless it is sm_100.
+// The current device's multiprocessors; 0 unless it is sm_100.  Asked of the
+// driver once a device.
 inline int sm100_sms() {
+    static std::atomic<int> known[64];  // sms + 1, 0: not asked yet
     int dev = 0, major = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess || major != 10 ||
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev < 64)
+        if (const int k = known[dev].load(std::memory_order_relaxed)) return k - 1;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         return 0;
+    if (major != 10) sms = 0;
+    if (dev < 64) known[dev].store(sms + 1, std::memory_order_relaxed);
     return sms;
 }
 

@@ -11,6 +11,9 @@ Values are rounded once, to nearest, ties to even; infinities and NaN become
 NaN.  A power of two adds no rounding, dequantised values are exact in bfloat16
 and float32, and the tensor cores apply such scales themselves.
 """
+import ctypes
+import functools
+
 import torch
 
 from . import _lib
@@ -82,7 +85,7 @@ class Fp8Tensor:
 
 
 def _tile_shape(rows, width):
-    return _cdiv(rows, 128), _cdiv(_cdiv(width, BLOCK), 4), 32, 4, 4
+    return (rows + 127) // 128, (width + 511) // 512, 32, 4, 4
 
 
 def _stride(values):
@@ -92,7 +95,10 @@ def _stride(values):
 
 def _rows(t):
     """t as [rows, width] with dense rows (a view where the strides allow one)."""
-    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.is_contiguous():
+        return t
     rows, width = t.shape
     dense = (width == 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= width)
     return t if dense else t.contiguous()
@@ -100,25 +106,46 @@ def _rows(t):
 
 def _ld(t):
     """Elements between the rows of a matrix with dense rows."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, width = t.shape
+    return t.stride(0) if rows > 1 else width
 
 
-def _aligned(t):
-    """A 16-bit matrix with rows on 16 bytes, as TMA reads them, and its row
-    stride: t, or a copy with padded rows."""
-    ld = t.stride(0)
-    if t.shape[0] == 1:
-        ld = _cdiv(t.shape[1], 8) * 8
-    if ld % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t, ld
-    ld = _cdiv(t.shape[1], 8) * 8
-    out = t.new_empty((t.shape[0], ld))
-    out[:, :t.shape[1]] = t
-    return out[:, :t.shape[1]], ld
+def _align(*mats):
+    """[(matrix, row stride)] of up to four 16-bit matrices of one type with dense
+    rows, as TMA reads them: rows on 16 bytes.  Those that are not are copied, all
+    of them by one kernel."""
+    out, copies = [], None
+    for t in mats:
+        rows, cols = t.shape
+        ld = t.stride(0) if rows > 1 else (cols + 7) // 8 * 8
+        if ld % 8 or t.data_ptr() % 16:
+            copies = copies or []
+            copies.append((len(out), t, rows, cols, (cols + 7) // 8 * 8))
+        out.append((t, ld))
+    if copies:
+        t = copies[0][1]
+        buf = t.new_empty(sum(rows * ldd for _, _, rows, _, ldd in copies))
+        desc, at = (ctypes.c_int64 * (6 * len(copies)))(), 0
+        for k, (i, t, rows, cols, ldd) in enumerate(copies):
+            to = buf.as_strided((rows, cols), (ldd, 1), at)
+            desc[6 * k:6 * k + 6] = t.data_ptr(), rows, cols, _ld(t), to.data_ptr(), ldd
+            out[i] = to, ldd
+            at += rows * ldd
+        call("sffn_pad_rows16", len(copies), ctypes.addressof(desc), stream_handle(buf.device))
+    return out
+
+
+def _empty_rows(t, rows, cols, multiple):
+    """[rows, cols] of t's type, its rows padded to a multiple of so many elements."""
+    ld = -(-cols // multiple) * multiple
+    out = t.new_empty((rows, ld))
+    return out if ld == cols else out[:, :cols]
 
 
 def _empty_values(rows, width, device, multiple=16):
-    return torch.empty((rows, _cdiv(width, multiple) * multiple), dtype=E4M3, device=device)[:, :width]
+    ld = -(-width // multiple) * multiple
+    out = torch.empty((rows, ld), dtype=E4M3, device=device)
+    return out if ld == width else out[:, :width]
 
 
 def _empty_tiles(rows, width, device):
@@ -129,19 +156,21 @@ def _pack(x):
     """(values, scale tiles) of x [..., width]."""
     x2 = _rows(x)
     rows, width = x2.shape
-    values, tiles = _empty_values(rows, width, x.device), _empty_tiles(rows, width, x.device)
+    dev = x.device
+    values, tiles = _empty_values(rows, width, dev), _empty_tiles(rows, width, dev)
     if rows:
         call("sffn_fp8_pack", x2.data_ptr(), _lib._DTYPES[x.dtype], rows, width, _ld(x2), values.data_ptr(),
-             _stride(values), tiles.data_ptr(), stream_handle(x.device))
+             -(-width // 16) * 16, tiles.data_ptr(), stream_handle(dev))
     return values, tiles
 
 
-def _unpack(values, tiles, shape, dtype):
-    out = torch.empty(shape, dtype=dtype, device=values.device)
-    rows, width = values.shape
+def _unpack(values, tiles, out, width):
+    """Into out, whose rows are dense; returns it."""
+    rows = values.shape[0]
     if rows:
-        call("sffn_fp8_unpack", values.data_ptr(), _stride(values), tiles.data_ptr(), rows, width, _lib._DTYPES[dtype],
-             out.data_ptr(), width, stream_handle(values.device))
+        ldo = out.stride(0) if out.dim() == 2 and rows > 1 else width
+        call("sffn_fp8_unpack", values.data_ptr(), _stride(values), tiles.data_ptr(), rows, width, _lib._DTYPES[out.dtype],
+             out.data_ptr(), ldo, stream_handle(values.device))
     return out
 
 
@@ -162,7 +191,9 @@ def fp8_pack(x):
     _check_pack(x)
     _refuse_grad("fp8_pack", x)
     values, tiles = torch.ops.sparseffn.fp8_pack(x) if torch.compiler.is_compiling() else _pack(x)
-    return Fp8Tensor(values, tiles, x.shape)
+    q = Fp8Tensor.__new__(Fp8Tensor)
+    q.values, q.scale_tiles, q.shape = values, tiles, x.shape
+    return q
 
 
 def fp8_unpack(q, dtype=torch.bfloat16):
@@ -173,7 +204,7 @@ def fp8_unpack(q, dtype=torch.bfloat16):
         raise TypeError(f"unsupported dtype {dtype}; expected float32, bfloat16 or float16")
     if torch.compiler.is_compiling():
         return torch.ops.sparseffn.fp8_unpack(q.values, q.scale_tiles, q.shape, dtype)
-    return _unpack(q.values, q.scale_tiles, q.shape, dtype)
+    return _unpack(q.values, q.scale_tiles, torch.empty(q.shape, dtype=dtype, device=q.values.device), q.shape[-1])
 
 
 # ---------------------------------------------------------------------------
@@ -231,48 +262,53 @@ def fp8_matmul(a, b, out_dtype=None):
     else:
         _check_product(a.values, b.values, out_dtype)
         out = _matmul(a.values, a.scale_tiles, b.values, b.scale_tiles, out_dtype)
-    return out.view(*a.shape[:-1], b.shape[0])
+    return out if len(a.shape) == 2 else out.view(*a.shape[:-1], b.shape[0])
 
 
 # ---------------------------------------------------------------------------
 # 16-bit products on the tensor cores
 # ---------------------------------------------------------------------------
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(M, N, K, K2):
+    return _lib.load().sffn_gemm16_workspace_bytes(M, N, K, K2)
+
+
 def _mm_into(out, A, a_mn, B, b_mn, second=None):
-    """out [M, N] = A B^T; A is [M, K], or with a_mn [K, M]; B [N, K] or [K, N];
-    plus second = (A2, B2), likewise, added within the product."""
+    """out [M, N] = A B^T; A is [M, K], or with a_mn [K, M]; B [N, K] or [K, N]; plus
+    second = (A2, B2), likewise, added within the product.  Each operand as _align
+    gives it, a pair of matrix and row stride."""
     M, N = out.shape
-    A, lda = _aligned(A)
-    B, ldb = _aligned(B)
-    K = A.shape[0] if a_mn else A.shape[1]
+    (A, lda), (B, ldb) = A, B
+    K, dev = A.shape[0 if a_mn else 1], out.device
     A2 = B2 = None
     lda2 = ldb2 = K2 = 0
     if second is not None:
-        (A2, lda2), (B2, ldb2) = map(_aligned, second)
-        K2 = A2.shape[0] if a_mn else A2.shape[1]
-    ws_bytes = _lib.load().sffn_gemm16_workspace_bytes(M, N, K, K2)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=out.device) if ws_bytes else None
-    call("sffn_gemm16", _lib._DTYPES[out.dtype], A.data_ptr(), lda, int(a_mn), B.data_ptr(), ldb, int(b_mn), ptr(A2), lda2,
-         ptr(B2), ldb2, K2, M, N, K, out.data_ptr(), _ld(out), ptr(ws), ws_bytes, _lib.status_word(out.device).data_ptr(),
-         stream_handle(out.device))
+        (A2, lda2), (B2, ldb2) = second
+        K2 = A2.shape[0 if a_mn else 1]
+    ws_bytes = _workspace_bytes(M, N, K, K2)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    call("sffn_gemm16", _lib._DTYPES[out.dtype], A.data_ptr(), lda, a_mn, B.data_ptr(), ldb, b_mn, ptr(A2), lda2, ptr(B2),
+         ldb2, K2, M, N, K, out.data_ptr(), _ld(out), ptr(ws), ws_bytes, _lib.status_word(dev).data_ptr(), stream_handle(dev))
     return out
 
 
-def _linear(x, W):
-    """x [T, K] W [N, K]^T in their type."""
+def _few_rows(x, W):
+    """x [T, K] W [N, K]^T for T <= FEW_ROWS, in their type."""
     T, N = x.shape[0], W.shape[0]
     out = x.new_empty((T, N))
-    if T == 0:
-        return out
-    if T <= FEW_ROWS:
+    if T:
         call("sffn_few_rows_mm", _lib._DTYPES[x.dtype], x.data_ptr(), _ld(x), W.data_ptr(), _ld(W), T, N, x.shape[1],
              out.data_ptr(), N, stream_handle(x.device))
-        return out
-    return _mm_into(out, x, False, W, False)
+    return out
 
 
 # ---------------------------------------------------------------------------
 # A linear layer that keeps its input in 8 bits
 # ---------------------------------------------------------------------------
+def _fits(x, w, rows, cols):
+    return w.dtype is x.dtype and w.is_cuda and w.device == x.device and w.shape == (rows, cols)
+
+
 def _check_weights(x, **weights):
     """x [..., D] against weights {name: (tensor, shape)}: CUDA, one 16-bit type, one device."""
     ts = [w for w, _ in weights.values()]
@@ -290,10 +326,24 @@ def _check_weights(x, **weights):
             raise ValueError(f"{name} must be {shape}, got {tuple(w.shape)}")
 
 
+def _check_linear(x, W):
+    if not (isinstance(x, torch.Tensor) and isinstance(W, torch.Tensor) and x.is_cuda and x.dim() and W.dim() == 2
+            and x.dtype in OUT_TYPES and x.shape[-1] and W.shape[0] and _fits(x, W, W.shape[0], x.shape[-1])):
+        _lib.require_cuda(x, W)
+        _check_weights(x, W=(W, (W.shape[0] if W.dim() else 0, x.shape[-1] if x.dim() else 0)))
+
+
 def _linear_forward(x, W, keep):
     """(y, values, tiles) -- the last two None without keep."""
-    x2 = _rows(x)
-    y = _linear(x2, _rows(W)).view(*x.shape[:-1], W.shape[0])
+    x2, W2 = _rows(x), _rows(W)
+    if x2.shape[0] <= FEW_ROWS:
+        y = _few_rows(x2, W2)
+    else:
+        A, B = _align(x2, W2)
+        x2 = A[0]
+        y = _mm_into(x2.new_empty((x2.shape[0], W2.shape[0])), A, 0, B, 0)
+    if x.dim() != 2:
+        y = y.view(*x.shape[:-1], W.shape[0])
     return (y, *_pack(x2)) if keep else (y, None, None)
 
 
@@ -301,19 +351,15 @@ def _linear_backward(dy, W, values, tiles, x_shape, want_x, want_W):
     _lib.bind_thread(dy.device)
     dy2, width = _rows(dy), x_shape[-1]
     dx = dW = None
+    if dy2.shape[0] == 0:
+        return dy.new_empty(x_shape) if want_x else None, submit_grad(W.new_zeros(W.shape)) if want_W else None
+    A, *B = _align(dy2, _rows(W)) if want_x else _align(dy2)
     if want_W:
-        dW = W.new_empty((dy2.shape[1], width))
-        if dy2.shape[0]:
-            kept = _unpack(values, tiles, values.shape, dy.dtype)
-            _mm_into(dW, dy2, True, kept, True)
-            del kept
-        else:
-            dW.zero_()
-        submit_grad(dW)
+        kept = _unpack(values, tiles, _empty_rows(dy2, dy2.shape[0], width, 8), width)
+        dW = submit_grad(_mm_into(dy2.new_empty((dy2.shape[1], width)), A, 1, *_align(kept), 1))
+        del kept
     if want_x:
-        dx = dy.new_empty(x_shape)
-        if dy2.shape[0]:
-            _mm_into(dx.view(-1, width), dy2, False, _rows(W), True)
+        dx = _mm_into(dy2.new_empty((dy2.shape[0], width)), A, 0, *B, 1).view(x_shape)
     return dx, dW
 
 
@@ -338,7 +384,7 @@ def ckpt_linear(x, W):
     Between forward and backward only W and x in 8 bits are kept (half a 16-bit
     x): the output and x's gradient are those of a linear layer, the weight's
     gradient is dy^T times the kept x.  Differentiable once, in reverse mode."""
-    _check_weights(x, W=(W, (W.shape[0] if W.dim() else 0, x.shape[-1] if x.dim() else 0)))
+    _check_linear(x, W)
     if torch.compiler.is_compiling():
         return torch.ops.sparseffn.ckpt_linear(x, W)[0]
     if _lib.tracked(x, W):

@@ -33,68 +33,83 @@ CHUNK = 32  # columns: kept rows are padded to whole ones
 def _forward(x, Wg, Wu, W2, act, keep):
     """(y, g, u, g_tiles, u_tiles, x_values, x_tiles): keep 0 keeps nothing, 1 g
     and u in x's type, 2 all three in 8 bits; what is not kept is None."""
-    x2, Wg, Wu, W2 = map(fp8._rows, (x, Wg, Wu, W2))
+    x2, Wg, Wu, W2 = fp8._rows(x), fp8._rows(Wg), fp8._rows(Wu), fp8._rows(W2)
     T, D = x2.shape
     F, dev, code = Wg.shape[0], x.device, _lib._DTYPES[x.dtype]
     g = u = gt = ut = xv = xt = None
+    if keep == 0 and 0 < T <= fp8.FEW_ROWS:
+        h, y = x2.new_empty((T, (F + 7) // 8 * 8)), x2.new_empty((T, D))
+        call("sffn_few_rows_ffn", code, act, x2.data_ptr(), fp8._ld(x2), Wg.data_ptr(), fp8._ld(Wg), Wu.data_ptr(),
+             fp8._ld(Wu), W2.data_ptr(), fp8._ld(W2), T, D, F, h.data_ptr(), h.shape[1], y.data_ptr(), D, stream_handle(dev))
+        return y if x.dim() == 2 else y.view(x.shape), g, u, gt, ut, xv, xt
     if keep == 2:
         g, u = (fp8._empty_values(T, F, dev, CHUNK) for _ in range(2))
         gt, ut = (fp8._empty_tiles(T, F, dev) for _ in range(2))
-        xv, xt = fp8._pack(x2)
     elif keep == 1:
-        g, u = (x2.new_empty((T, fp8._cdiv(F, CHUNK) * CHUNK))[:, :F] for _ in range(2))
+        g, u = (fp8._empty_rows(x2, T, F, CHUNK) for _ in range(2))
     if T == 0:
-        return x.new_empty((*x.shape[:-1], D)), g, u, gt, ut, xv, xt
-    ldk = fp8._cdiv(F, CHUNK) * CHUNK
-    ldh = fp8._cdiv(F, 8) * 8
-    h = x2.new_empty((T, ldh))[:, :F]
-    if keep == 0 and T <= fp8.FEW_ROWS:
-        call("sffn_few_rows_glu", code, act, x2.data_ptr(), fp8._ld(x2), Wg.data_ptr(), fp8._ld(Wg), Wu.data_ptr(),
-             fp8._ld(Wu), T, D, F, h.data_ptr(), ldh, stream_handle(dev))
+        if keep == 2:
+            xv, xt = fp8._pack(x2)
+        return x.new_empty(x.shape), g, u, gt, ut, xv, xt
+    if T <= fp8.FEW_ROWS:  # kept, so the tensor cores' tiles: W2's product is the few-row kernel's
+        xa, ga, ua = fp8._align(x2, Wg, Wu)
     else:
-        (xa, ldx), (Wg, ldg), (Wu, ldu) = map(fp8._aligned, (x2, Wg, Wu))
-        call("sffn_glu_up", code, act, xa.data_ptr(), ldx, Wg.data_ptr(), ldg, Wu.data_ptr(), ldu, T, D, F, h.data_ptr(), ldh,
-             keep, ptr(g), ptr(u), ldk, ptr(gt), ptr(ut), _lib.status_word(dev).data_ptr(), stream_handle(dev))
-    return fp8._linear(h, W2).view(x.shape), g, u, gt, ut, xv, xt
+        xa, ga, ua, W2a = fp8._align(x2, Wg, Wu, W2)
+    h = fp8._empty_rows(x2, T, F, 8)
+    ldh = (F + 7) // 8 * 8
+    call("sffn_glu_up", code, act, xa[0].data_ptr(), xa[1], ga[0].data_ptr(), ga[1], ua[0].data_ptr(), ua[1], T, D, F,
+         h.data_ptr(), ldh, keep, ptr(g), ptr(u), -(-F // CHUNK) * CHUNK, ptr(gt), ptr(ut),
+         _lib.status_word(dev).data_ptr(), stream_handle(dev))
+    if T <= fp8.FEW_ROWS:
+        y = fp8._few_rows(h, W2)
+    else:
+        y = fp8._mm_into(x2.new_empty((T, D)), (h, ldh), 0, W2a, 0)
+    if keep == 2:
+        xv, xt = fp8._pack(xa[0])
+    return y if x.dim() == 2 else y.view(x.shape), g, u, gt, ut, xv, xt
 
 
 def _backward(dy, x, Wg, Wu, W2, g, u, gt, ut, xv, xt, act, want):
     """Gradients of (x, Wg, Wu, W2); None where `want` is false.  x is None with 8-bit checkpoints."""
     _lib.bind_thread(dy.device)
-    dy2, Wg, Wu, W2 = map(fp8._rows, (dy, Wg, Wu, W2))
+    dy2, Wg, Wu, W2 = fp8._rows(dy), fp8._rows(Wg), fp8._rows(Wu), fp8._rows(W2)
     T, D = dy2.shape
     F, dev, code = Wg.shape[0], dy.device, _lib._DTYPES[dy.dtype]
     dx = dWg = dWu = dW2 = None
     if T == 0:
-        zeros = [w.new_zeros(w.shape) if n else None for w, n in zip((Wg, Wu, W2), want[1:])]
-        return (dy.new_empty(dy.shape) if want[0] else None, *zeros)
+        return (dy.new_empty(dy.shape) if want[0] else None,
+                *(submit_grad(w.new_zeros(w.shape)) if n else None for w, n in zip((Wg, Wu, W2), want[1:])))
     keep = 2 if xv is not None else 1
-    ld, ldk = fp8._cdiv(F, 8) * 8, fp8._cdiv(F, CHUNK) * CHUNK
-    d = dy2.new_empty((T, 2 * ld))  # dg | du, so that their weight gradients are one product
-    dg, du = d[:, :F], d[:, ld:ld + F]
-    h = dy2.new_empty((T, ld))[:, :F]
-    dya, lddy = fp8._aligned(dy2)
-    W2a, ldw2 = fp8._aligned(W2)
-    call("sffn_glu_dgrad", code, act, dya.data_ptr(), lddy, W2a.data_ptr(), ldw2, T, D, F, keep, g.data_ptr(), u.data_ptr(),
-         ldk, ptr(gt), ptr(ut), dg.data_ptr(), du.data_ptr(), 2 * ld, h.data_ptr(), ld, _lib.status_word(dev).data_ptr(),
-         stream_handle(dev))
+    ld = (F + 7) // 8 * 8
+    d, h = dy2.new_empty((T, 2 * ld)), fp8._empty_rows(dy2, T, F, 8)  # d: dg | du, their weights' gradient is one product
+    dg, du = (d[:, :F], 2 * ld), (d[:, ld:ld + F], 2 * ld)
+    if want[0]:
+        dya, W2a, ga, ua = fp8._align(dy2, W2, Wg, Wu)
+    else:
+        dya, W2a = fp8._align(dy2, W2)
+    call("sffn_glu_dgrad", code, act, dya[0].data_ptr(), dya[1], W2a[0].data_ptr(), W2a[1], T, D, F, keep, g.data_ptr(),
+         u.data_ptr(), -(-F // CHUNK) * CHUNK, ptr(gt), ptr(ut), dg[0].data_ptr(), du[0].data_ptr(), 2 * ld, h.data_ptr(), ld,
+         _lib.status_word(dev).data_ptr(), stream_handle(dev))
     if want[3]:
-        dW2 = submit_grad(fp8._mm_into(W2.new_empty((D, F)), dya, True, h, True))
+        dW2 = submit_grad(fp8._mm_into(dy2.new_empty((D, F)), dya, 1, (h, ld), 1))
     del h
     if want[1] or want[2]:
-        xk = fp8._unpack(xv, xt, (T, D), dy.dtype) if keep == 2 else fp8._rows(x)
+        if keep == 2:
+            xk = fp8._unpack(xv, xt, fp8._empty_rows(dy2, T, D, 8), D), (D + 7) // 8 * 8
+        else:
+            xk, = fp8._align(fp8._rows(x))
         if want[1] and want[2]:
-            dW = fp8._mm_into(Wg.new_empty((2 * ld, D)), d, True, xk, True)
+            dW = fp8._mm_into(dy2.new_empty((2 * ld, D)), (d, 2 * ld), 1, xk, 1)
             dWg, dWu = dW[:F], dW[ld:ld + F]
         elif want[1]:
-            dWg = fp8._mm_into(Wg.new_empty((F, D)), dg, True, xk, True)
+            dWg = fp8._mm_into(dy2.new_empty((F, D)), dg, 1, xk, 1)
         else:
-            dWu = fp8._mm_into(Wu.new_empty((F, D)), du, True, xk, True)
+            dWu = fp8._mm_into(dy2.new_empty((F, D)), du, 1, xk, 1)
         submit_grad(dWg)
         submit_grad(dWu)
         del xk
     if want[0]:
-        dx = fp8._mm_into(dy2.new_empty((T, D)), dg, False, Wg, True, (du, Wu)).view(dy.shape)
+        dx = fp8._mm_into(dy2.new_empty((T, D)), dg, 0, ga, 1, (du, ua)).view(dy.shape)
     return dx, dWg, dWu, dW2
 
 
@@ -113,9 +128,12 @@ class _GatedFFN(torch.autograd.Function):
 
 
 def _check(x, Wg, Wu, W2):
+    _lib.require_cuda(x, Wg, Wu, W2)
     D = x.shape[-1] if x.dim() else 0
     F = Wg.shape[0] if Wg.dim() else 0
-    fp8._check_weights(x, Wg=(Wg, (F, D)), Wu=(Wu, (F, D)), W2=(W2, (D, F)))
+    if not (x.dtype in fp8.OUT_TYPES and D and F and fp8._fits(x, Wg, F, D) and fp8._fits(x, Wu, F, D)
+            and fp8._fits(x, W2, D, F)):
+        fp8._check_weights(x, Wg=(Wg, (F, D)), Wu=(Wu, (F, D)), W2=(W2, (D, F)))
 
 
 def gated_ffn(x, Wg, Wu, W2, activation="silu", checkpoint=None):

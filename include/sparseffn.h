@@ -652,6 +652,12 @@ int sffn_fp8_mm(const void* a, int64_t lda, const void* a_scales, const void* b,
                 int64_t M, int64_t N, int64_t K, void* C, int c_dtype, int64_t ldc, uint32_t* status_dev,
                 void* stream);
 
+/* Copies up to four 16-bit matrices to rows on 16 bytes.  desc: six numbers a
+ * matrix -- source address, rows, columns, row stride, destination address (on
+ * 16 bytes), its row stride (a multiple of 8); what the last 8 columns written of
+ * a row have beyond it is zero. */
+int sffn_pad_rows16(int count, const int64_t* desc, void* stream);
+
 /* ---- gated feed-forward block -------------------------------------------- */
 
 enum { /* activations */
@@ -697,6 +703,10 @@ int sffn_few_rows_mm(int dtype, const void* x, int64_t ldx, const void* w, int64
                      void* out, int64_t ldo, void* stream);
 int sffn_few_rows_glu(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
                       int64_t ldwu, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, void* stream);
+/* sffn_few_rows_glu and then y [T, D] = h w2^T, in one call. */
+int sffn_few_rows_ffn(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
+                      int64_t ldwu, const void* w2, int64_t ldw2, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh,
+                      void* y, int64_t ldy, void* stream);
 int sffn_few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw,
                       const void* w_scales, int64_t T, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
                       void* stream);

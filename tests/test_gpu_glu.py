@@ -21,7 +21,7 @@ import pytest
 import torch
 
 import autoresearch2_b200 as sf
-from autoresearch2_b200 import fp8, glu
+from autoresearch2_b200 import glu
 from test_gpu_fp8 import want_blocks
 
 pytestmark = pytest.mark.gpu
@@ -68,6 +68,10 @@ def check(name, got, want, tol):
     tol = tol + half(got.dtype) * want.abs() + tiny(got.dtype)
     bad = ~(err <= tol)
     assert not bad.any(), f"{name}: {int(bad.sum())} of {bad.numel()} off, worst {float((err / tol).max()):.3g} of the tolerance"
+
+
+def unpacked(values, tiles, dtype):
+    return sf.fp8_unpack(sf.Fp8Tensor(values, tiles), dtype)
 
 
 def inputs(T, D, F, dtype, seed=0):
@@ -149,17 +153,17 @@ def test_training(T, D, F, dtype, checkpoint):
             check("u", u, wu, Eu)
             kept = x.detach()
         else:
-            kept = fp8._unpack(xv, xt, (T, D), F32)
+            kept = unpacked(xv, xt, F32)
             assert torch.equal(kept.to(F64), want_blocks(x.detach())[0])
-            kept = fp8._unpack(xv, xt, (T, D), dtype)
+            kept = unpacked(xv, xt, dtype)
             for v, t, w, E in ((g, gt, wg, Eg), (u, ut, wu, Eu)):
-                got = fp8._unpack(v, t, (T, F), F32).to(F64)
+                got = unpacked(v, t, F32).to(F64)
                 # half a step of e4m3 of the value, or half the smallest of the block's scale (448 -> 2^-9:
                 # 2^-10 / 224 of the block's largest at most)
                 top = torch.nn.functional.pad(w.abs() + E, (0, -F % 128)).view(T, -1, 128).amax(-1)
                 floor = (top * 2 ** -10 / 224).repeat_interleave(128, 1)[:, :F]
                 assert ((got - w).abs() <= torch.maximum(w.abs() * 2 ** -4, floor) * (1 + 2 ** -8) + 2 * E).all()
-            g, u = fp8._unpack(g, gt, (T, F), F32), fp8._unpack(u, ut, (T, F), F32)
+            g, u = unpacked(g, gt, F32), unpacked(u, ut, F32)
         check_backward(grads, dy, kept, Wg, Wu, W2, g, u, name)
         again = torch.autograd.grad(sf.gated_ffn(x, Wg, Wu, W2, name, checkpoint=checkpoint), leaves, dy)
         assert all(torch.equal(a, b) for a, b in zip(grads, again))
