@@ -120,12 +120,12 @@ SIGNATURES = {
     "sffn_gemm16_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
     "sffn_gemm16": (_int, [_int, _vp, _i64, _int, _vp, _i64, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64,
                            _vp, _sz, _vp, _vp]),
-    "sffn_few_rows_mm": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
-    "sffn_few_rows_glu": (_int, [_int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "sffn_few_rows_mm": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "sffn_few_rows_glu": (_int, [_int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "sffn_few_rows_ffn": (_int, [_int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp,
-                                 _i64, _vp]),
+                                 _i64, _vp, _vp]),
     "sffn_pad_rows16": (_int, [_int, _vp, _vp]),
-    "sffn_few_rows_fp8": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp]),
+    "sffn_few_rows_fp8": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp, _vp]),
 }
 
 _lib = None

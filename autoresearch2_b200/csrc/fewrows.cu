@@ -5,24 +5,33 @@
 // Bound by reading the weights once.  A tensor-core tile of 128 or 256 rows of
 // x would leave most multiprocessors without a tile; here the weights are the
 // rows of mma.sync (m16n8k16, float32 accumulation) and the tokens its columns.
-// One block a multiprocessor takes 16 rows of W at a time (of Wg and Wu each),
-// all its 16 warps on them in alternate 128-byte pieces, and adds their sums in
-// shared memory in a fixed order.  The whole multiprocessor on one group of rows
-// keeps the groups short, so that the last ones end together.  Weights come by
-// cp.async, 192 KB of them under way on a multiprocessor, across the ends of
-// groups; a thread copies the very bytes it multiplies, so that only its own
-// copies need waiting for.  The k index within a piece is permuted, alike for W
-// and x, so that these are 16 contiguous bytes of a row.
+// A block a multiprocessor, up to 16 rows of W (of Wg and Wu) at a time:
+//   warp 16       copies 1 KB of each of these rows and of x a stage, by one TMA box
+//                 a matrix
+//   warps 0-15    multiply, 128 bytes of the stage's rows each, eight warps on a
+//                 stage and eight on the next
+//   warps 17-19   add the warps' sums in a fixed order and store, meanwhile
+// Tried and slower on 16 rows x (14336 x 4096) x 2: a bulk copy for each row (1 KB
+// each: the copy engine's rate, 94 us), weights by each warp's own loads and x from
+// L2 (its latency, and warps that drift apart fetch scattered 128-byte pieces:
+// 69 us).  Groups have equally many rows, so that the last ones end together.  The k index
+// within a piece is permuted, alike for W and x, so that a lane's fragments are
+// 16 contiguous bytes of a row.
+#include <cuda.h>
+#include <string.h>
+
 #include "act.cuh"
 #include "fp8.cuh"
+#include "sm100.cuh"
 #include "tmap.cuh"
 
 namespace sffn {
 namespace {
 
 constexpr int S_MAX_ROWS = 32;
-constexpr int S_WARPS = 16;
-constexpr int S_PIECE = 128;  // bytes of a row a warp takes at a time: one block of 8-bit values, 64 16-bit ones
+constexpr int S_WARPS = 16;                // that multiply
+constexpr int S_ADDERS = 3;                // that add and store
+constexpr int S_THREADS = (S_WARPS + 1 + S_ADDERS) * 32;
 enum { S_PLAIN = 0, S_GATED = 1 };
 
 struct FewArgs {
@@ -34,8 +43,10 @@ struct FewArgs {
     const uint8_t* xs;  // scale tiles (8-bit operands)
     const uint8_t* ws;
     int bt;
+    int per;  // rows of W a group
     uint16_t* out;
     long long ldo;
+    uint32_t* status;
 };
 
 template <int DT>
@@ -74,74 +85,151 @@ __device__ __forceinline__ uint32_t scale_byte(const uint8_t* s, long long row, 
     return __ldg(s + fp8_scale_at(row, block, bt));
 }
 
-// Pieces of the weights under way: 64 bytes a thread and matrix each.
+// A stage in shared memory: rows of 1 KB, 16 of each matrix, then NT * 8 of x (rows
+// and tokens past the last one hold anything: their sums are not stored).
+constexpr int S_ROW = 1024, S_PIECE = 128;
 template <int MATS, int NT>
-constexpr int few_depth() { return MATS == 1 ? 6 : NT == 4 ? 2 : 3; }
+struct FewStage {
+    static constexpr int BYTES = (MATS * 16 + NT * 8) * S_ROW;
+    static constexpr int SUMS = S_WARPS * NT * 8 * (MATS * 16 + 1) * 4;
+    static constexpr int FIT = (232448 - 1024 - SUMS) / BYTES;
+    // An even count: each stage then belongs to one half of the warps, and a warp
+    // has waited for every earlier use of the stage it waits for.  (Were the halves
+    // to take turns, one could find the phase before last complete and take it for
+    // its own, when copies land out of order.)
+    static constexpr int DEPTH = FIT >= 8 ? 8 : FIT & ~1;
+    static_assert(DEPTH >= 2, "stages");
+};
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {  // zeros after `bytes`
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// A lane's two vectors of a row's piece, from each half of 64 bytes.  Rows are 1 KB
+// apart, so lanes of odd rows read the halves in the other order: a
+// quarter-warp's eight then meet different banks.
+__device__ __forceinline__ void load_halves(const unsigned char* row, int gid, uint4 (&v)[2]) {
+    const int odd = gid & 1;
+    const uint4 a = *reinterpret_cast<const uint4*>(row + odd * 64), b = *reinterpret_cast<const uint4*>(row + (odd ^ 1) * 64);
+    v[0] = odd ? b : a;
+    v[1] = odd ? a : b;
 }
 
 // DT: type of x and W (FP8: both in 8 bits) and OT of the output; NT tiles of 8
 // tokens.
 template <int DT, int OT, bool FP8, int MODE, int ACT, int NT, bool VEC>
-__global__ void __launch_bounds__(S_WARPS * 32, 1) few_rows_kernel(const FewArgs a) {
+__global__ void __launch_bounds__(S_THREADS, 1)
+    few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW2,
+                    const __grid_constant__ CUtensorMap tmX, const FewArgs a) {
     constexpr int MATS = MODE == S_GATED ? 2 : 1;
     constexpr int ROWS = MATS * 16;  // rows of sums
     constexpr int ESIZE = FP8 ? 1 : 2;
-    constexpr int DEPTH = few_depth<MATS, NT>();
-    constexpr int VECS = MATS * 4;  // 16-byte vectors of weights a thread takes of a piece
-    extern __shared__ __align__(16) unsigned char few_smem[];
-    // [DEPTH][VECS][threads] vectors, then [S_WARPS][NT * 8][ROWS + 1] sums
-    uint4* ring = reinterpret_cast<uint4*>(few_smem);
-    float* red = reinterpret_cast<float*>(few_smem + DEPTH * VECS * S_WARPS * 32 * 16);
+    using St = FewStage<MATS, NT>;
+    constexpr int STAGE = St::BYTES, DEPTH = St::DEPTH;
+    extern __shared__ __align__(128) unsigned char few_smem[];
+    float* red = reinterpret_cast<float*>(few_smem + (VEC ? DEPTH * STAGE : 0));  // [S_WARPS][NT * 8][ROWS + 1]
+    __shared__ __align__(8) uint64_t full_bar[DEPTH], empty_bar[DEPTH];  // a stage's rows have come; are read
+    __shared__ __align__(8) uint64_t sums_bar, free_bar;                 // the warps' sums are written; are read
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int gid = lane >> 2, tig = lane & 3;
     const long long bytes = (long long)a.K * ESIZE;
-    const int pieces = (int)((bytes + S_PIECE - 1) / S_PIECE);
-    const int mine = pieces > warp ? (pieces - warp + S_WARPS - 1) / S_WARPS : 0;
-    const int groups = (a.N + 15) / 16;
+    const long long whole = bytes & ~15LL;  // copied; a row's last few bytes are read where they are multiplied
+    const int chunks = (int)((bytes + S_ROW - 1) / S_ROW);
+    const int groups = (a.N + a.per - 1) / a.per;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < DEPTH; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], S_WARPS / 2);
+        }
+        mbar_init(&sums_bar, S_WARPS);
+        mbar_init(&free_bar, S_ADDERS);
+        fence_mbar_init();
+    }
+    __syncthreads();
 
+    if (warp == S_WARPS) {
+        // -------------------------------------------------------- copies --
+        if (VEC && lane == 0) {
+            const uint32_t count = (uint32_t)(a.per * MATS + a.T) * S_ROW;  // whole boxes: zeros past the edges
+            int stage = 0;
+            uint32_t phase = 1;
+            for (int group = blockIdx.x; group < groups; group += gridDim.x)
+                for (int c = 0; c < chunks; ++c) {
+                    if (!mbar_wait_bounded(&empty_bar[stage], phase)) {
+                        atomicOr(a.status, SFFN_STATUS_WAIT_TIMEOUT);
+                        // no copy lands after the block has left
+                        for (int s = 0; s < DEPTH; ++s) (void)mbar_wait_bounded(&full_bar[s], (s < stage ? phase : phase ^ 1u) ^ 1u);
+                        return;
+                    }
+                    unsigned char* to = few_smem + stage * STAGE;
+                    mbar_arrive_expect_tx(&full_bar[stage], count);
+                    tma_load_2d(to, &tmW, c * (S_ROW / 4), group * a.per, &full_bar[stage]);
+                    if constexpr (MATS == 2) tma_load_2d(to + 16 * S_ROW, &tmW2, c * (S_ROW / 4), group * a.per, &full_bar[stage]);
+                    tma_load_2d(to + ROWS * S_ROW, &tmX, c * (S_ROW / 4), 0, &full_bar[stage]);
+                    if (++stage == DEPTH) stage = 0, phase ^= 1u;
+                }
+        }
+        return;
+    }
+    if (warp > S_WARPS) {
+        // -------------------------------------------------------- adders --
+        uint32_t phase = 0;
+        for (int group = blockIdx.x; group < groups; group += gridDim.x, phase ^= 1u) {
+            if (!__all_sync(FULL, mbar_wait_bounded(&sums_bar, phase))) {
+                if (lane == 0) atomicOr(a.status, SFFN_STATUS_WAIT_TIMEOUT);
+                return;
+            }
+            const int n0 = group * a.per, rows = min(a.per, a.N - n0);
+            for (int i = (warp - S_WARPS - 1) * 32 + lane; i < 16 * a.T; i += S_ADDERS * 32) {
+                const int t = i >> 4, r = i & 15;
+                float sum[MATS];
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) {
+                    float v[S_WARPS];
+#pragma unroll
+                    for (int w = 0; w < S_WARPS; ++w) v[w] = red[(w * (NT * 8) + t) * (ROWS + 1) + m * 16 + r];
+#pragma unroll
+                    for (int o = S_WARPS / 2; o > 0; o >>= 1)
+#pragma unroll
+                        for (int w = 0; w < o; ++w) v[w] += v[w + o];
+                    sum[m] = v[0];
+                }
+                if (r < rows) {
+                    float v = sum[0], unused;
+                    if constexpr (MODE == S_GATED) v = glu_act<ACT, false>(sum[0], unused) * sum[1];
+                    a.out[(long long)t * a.ldo + n0 + r] = Elt<OT>::from_f(v);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&free_bar);
+        }
+        return;
+    }
+
+    // ------------------------------------------------------------ products --
     const uint8_t* xrow[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) xrow[t] = static_cast<const uint8_t*>(a.x) + (long long)min(t * 8 + gid, a.T - 1) * a.ldx * ESIZE;
-
-    // the copies run DEPTH - 1 pieces ahead: of piece ci of group cg, into slot cs
-    int cg = mine ? (int)blockIdx.x : groups, ci = 0, cs = 0;
-    auto copy = [&] {
-        if (cg < groups) {
-            const long long k0 = ((long long)warp + (long long)ci * S_WARPS) * S_PIECE + tig * 16;
-            uint4* slot = ring + (cs * VECS) * (S_WARPS * 32) + threadIdx.x;
+    // row h * 8 + gid of a group (past the group's end: any, its sums are not stored)
+    auto row_of = [&](int group, int h) { return (long long)min(group * a.per + h * 8 + gid, a.N - 1); };
+    uint32_t we[2], xe[NT][2];
+    auto fetch_scales = [&](int group, int c) {
+        const int block = c * (S_WARPS / 2) + (warp & 7);
+        if ((long long)block * FP8_BLOCK >= bytes) return;  // not used
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                // rows past the end read the last one; their sums are not stored
-                const long long n = min(cg * 16 + h * 8 + gid, a.N - 1);
+        for (int h = 0; h < 2; ++h) we[h] = scale_byte(a.ws, row_of(group, h), block, a.bt);
 #pragma unroll
-                for (int m = 0; m < MATS; ++m) {
-                    const uint8_t* row = static_cast<const uint8_t*>(a.w[m]) + n * a.ldw[m] * ESIZE;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        uint4* to = slot + ((m * 2 + h) * 2 + q) * (S_WARPS * 32);
-                        const long long k = k0 + q * 64, left = bytes - k;
-                        if constexpr (VEC)
-                            cp_async16((uint32_t)__cvta_generic_to_shared(to), left > 0 ? row + k : row,
-                                       left >= 16 ? 16u : left > 0 ? (uint32_t)left : 0u);
-                        else
-                            *to = load_piece<false, ESIZE, true>(row, k, bytes);
-                    }
-                }
-            }
-            if (++ci == mine) ci = 0, cg += gridDim.x;
-            cs = cs + 1 == DEPTH ? 0 : cs + 1;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+            for (int h = 0; h < 2; ++h) xe[t][h] = scale_byte(a.xs, min(t * 8 + tig * 2 + h, a.T - 1), block, a.bt);
     };
-    int slot_at = 0;
-
-#pragma unroll
-    for (int d = 0; d < DEPTH - 1; ++d) copy();
+    // this warp's stages: every other one of the block's, from warp / 8 on
+    int it = 0;
+    uint32_t free_phase = 1;  // the first use finds the sums' place free
+    int sg = blockIdx.x, sc = warp >> 3;  // the piece whose scales are loaded
+    auto next_scales = [&] {
+        while (sc >= chunks) sc -= chunks, sg += gridDim.x;
+        if (sg < groups) fetch_scales(sg, sc);
+        sc += 2;
+    };
+    if constexpr (FP8) next_scales();
     for (int group = blockIdx.x; group < groups; group += gridDim.x) {
-        const int n0 = group * 16;
         float acc[MATS][NT][4];
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
@@ -150,84 +238,105 @@ __global__ void __launch_bounds__(S_WARPS * 32, 1) few_rows_kernel(const FewArgs
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[m][t][j] = 0.f;
 #pragma unroll 1
-        for (int i = 0; i < mine; ++i) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 2) : "memory");
-            uint4 w[MATS][2][2], x[2][NT];
-            const long long xk = ((long long)warp + (long long)i * S_WARPS) * S_PIECE + tig * 16;
-            if constexpr (FP8 || NT <= 2) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) x[q][t] = load_piece<VEC, ESIZE, false>(xrow[t], xk + q * 64, bytes);
+        for (int c = 0; c < chunks; ++c, ++it) {
+            if ((it & 1) != (warp >> 3)) continue;
+            const int stage = it % DEPTH;
+            if constexpr (VEC) {
+                if (!__all_sync(FULL, mbar_wait_bounded(&full_bar[stage], (uint32_t)(it / DEPTH) & 1u))) {
+                    if (lane == 0) atomicOr(a.status, SFFN_STATUS_WAIT_TIMEOUT);
+                    return;
+                }
             }
+            const int off = (warp & 7) * S_PIECE + tig * 16;  // of this lane's first vector in the rows
+            const long long k = (long long)c * S_ROW + off;
+            const unsigned char* slot = few_smem + stage * STAGE + gid * S_ROW + off;
+            if ((long long)c * S_ROW + (warp & 7) * S_PIECE < bytes) {
+                float part[FP8 ? NT : 1][4];
+                if constexpr (FP8) {
 #pragma unroll
-            for (int v = 0; v < VECS; ++v) w[v >> 2][(v >> 1) & 1][v & 1] = ring[(slot_at * VECS + v) * (S_WARPS * 32) + threadIdx.x];
-            slot_at = slot_at + 1 == DEPTH ? 0 : slot_at + 1;
-            copy();  // into the slot read in the last step
-            if constexpr (!FP8) {
+                    for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
+                        for (int j = 0; j < 4; ++j) part[t][j] = 0.f;
+                }
+                uint4 w[MATS][2][2], x[NT][2];  // [][half of the rows][half of the piece]
+                auto direct = [&](const uint8_t* row, uint4(&v)[2]) {
+                    v[0] = load_piece<false, ESIZE, true>(row, k, bytes);
+                    v[1] = load_piece<false, ESIZE, true>(row, k + 64, bytes);
+                };
+                const bool ring = VEC && k + 80 <= whole;
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        if constexpr (NT > 2) x[q][t] = load_piece<VEC, ESIZE, false>(xrow[t], xk + q * 64, bytes);
+                for (int m = 0; m < MATS; ++m)
 #pragma unroll
-                        for (int m = 0; m < MATS; ++m) {
-                            const uint4 w0 = w[m][0][q], w1 = w[m][1][q], xb = x[q][t];
-                            mma16816<DT>(acc[m][t], w0.x, w1.x, w0.y, w1.y, xb.x, xb.y);
-                            mma16816<DT>(acc[m][t], w0.z, w1.z, w0.w, w1.w, xb.z, xb.w);
+                    for (int h = 0; h < 2; ++h) {
+                        if (ring) load_halves(slot + (m * 16 + h * 8) * S_ROW, gid, w[m][h]);
+                        else direct(static_cast<const uint8_t*>(a.w[m]) + row_of(group, h) * a.ldw[m] * ESIZE, w[m][h]);
+                    }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if (ring) load_halves(slot + (ROWS + t * 8) * S_ROW, gid, x[t]);
+                    else direct(xrow[t], x[t]);
+                }
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    if constexpr (!FP8) {
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int m = 0; m < MATS; ++m) {
+                                const uint4 w0 = w[m][0][q], w1 = w[m][1][q], xv = x[t][q];
+                                mma16816<DT>(acc[m][t], w0.x, w1.x, w0.y, w1.y, xv.x, xv.y);
+                                mma16816<DT>(acc[m][t], w0.z, w1.z, w0.w, w1.w, xv.z, xv.w);
+                            }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            auto halves = [&](const uint4& u, uint32_t& lo, uint32_t& hi) {
+                                const uint32_t v = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
+                                const __half2 l = fp8_half2(v), h = fp8_half2(v >> 16);
+                                lo = *reinterpret_cast<const uint32_t*>(&l);
+                                hi = *reinterpret_cast<const uint32_t*>(&h);
+                            };
+                            uint32_t w0l, w0h, w1l, w1h;
+                            halves(w[0][0][q], w0l, w0h);
+                            halves(w[0][1][q], w1l, w1h);
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                uint32_t xl, xh;
+                                halves(x[t][q], xl, xh);
+                                mma16816<SFFN_F16>(part[t], w0l, w1l, w0h, w1h, xl, xh);
+                            }
                         }
                     }
-            } else {
-                // one block of 128: the sum of its products, then its two scales
-                const int block = warp + i * S_WARPS;
-                int we[2], xe[NT][2];
+                }
+                if constexpr (FP8) {
+                    // one block of 128: the sum of its products times its two scales,
+                    // 2^(ew + ex) in two factors, since one of the scales may leave the
+                    // range of a float where the product of both does not
 #pragma unroll
-                for (int h = 0; h < 2; ++h) we[h] = (int)scale_byte(a.ws, min(n0 + h * 8 + gid, a.N - 1), block, a.bt);
+                    for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) xe[t][h] = (int)scale_byte(a.xs, min(t * 8 + tig * 2 + h, a.T - 1), block, a.bt);
-                float part[NT][4];
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) part[t][j] = 0.f;
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        auto halves = [&](const uint4& u, uint32_t& lo, uint32_t& hi) {
-                            const uint32_t v = c == 0 ? u.x : c == 1 ? u.y : c == 2 ? u.z : u.w;
-                            const __half2 l = fp8_half2(v), h = fp8_half2(v >> 16);
-                            lo = *reinterpret_cast<const uint32_t*>(&l);
-                            hi = *reinterpret_cast<const uint32_t*>(&h);
-                        };
-                        uint32_t w0l, w0h, w1l, w1h;
-                        halves(w[0][0][q], w0l, w0h);
-                        halves(w[0][1][q], w1l, w1h);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            uint32_t xl, xh;
-                            halves(x[q][t], xl, xh);
-                            mma16816<SFFN_F16>(part[t], w0l, w1l, w0h, w1h, xl, xh);
+                        for (int j = 0; j < 4; ++j) {
+                            const int wb = (int)we[j >> 1], xb = (int)xe[t][j & 1];
+                            const int e = wb + xb - 254, e1 = e >> 1;
+                            float s1 = two_to(max(e1, -126));
+                            const float s2 = two_to(max(e - e1, -126));
+                            if (wb == 255 || xb == 255) s1 = __uint_as_float(0x7FFFFFFFu);
+                            acc[0][t][j] += part[t][j] * s1 * s2;
                         }
-                    }
-                // 2^(ew + ex) in two factors: one of the scales may leave the range
-                // of a float where the product of both does not
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int wb = we[j >> 1], xb = xe[t][j & 1];
-                        const int e = wb + xb - 254, e1 = e >> 1;
-                        float s1 = two_to(max(e1, -126));
-                        const float s2 = two_to(max(e - e1, -126));
-                        if (wb == 255 || xb == 255) s1 = __uint_as_float(0x7FFFFFFFu);
-                        acc[0][t][j] += part[t][j] * s1 * s2;
-                    }
+                }
+            }
+            if constexpr (FP8) next_scales();
+            if constexpr (VEC) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty_bar[stage]);
             }
         }
-        // the warps' sums, token x row of W
+        // this warp's sums, token x row of W, once the last ones are read
+        if (!__all_sync(FULL, mbar_wait_bounded(&free_bar, free_phase))) {
+            if (lane == 0) atomicOr(a.status, SFFN_STATUS_WAIT_TIMEOUT);
+            return;
+        }
+        free_phase ^= 1u;
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
 #pragma unroll
@@ -235,36 +344,41 @@ __global__ void __launch_bounds__(S_WARPS * 32, 1) few_rows_kernel(const FewArgs
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     red[(warp * (NT * 8) + t * 8 + tig * 2 + (j & 1)) * (ROWS + 1) + m * 16 + (j >> 1) * 8 + gid] = acc[m][t][j];
-        __syncthreads();
-        for (int i = threadIdx.x; i < 16 * a.T; i += S_WARPS * 32) {
-            const int t = i >> 4, r = i & 15;
-            float sum[MATS];
-#pragma unroll
-            for (int m = 0; m < MATS; ++m) {
-                sum[m] = 0.f;
-#pragma unroll
-                for (int w = 0; w < S_WARPS; ++w) sum[m] += red[(w * (NT * 8) + t) * (ROWS + 1) + m * 16 + r];
-            }
-            if (n0 + r < a.N) {
-                float v = sum[0], unused;
-                if constexpr (MODE == S_GATED) v = glu_act<ACT, false>(sum[0], unused) * sum[1];
-                a.out[(long long)t * a.ldo + n0 + r] = Elt<OT>::from_f(v);
-            }
-        }
-        __syncthreads();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sums_bar);
     }
 }
 
 template <int DT, int OT, bool FP8, int MODE, int ACT, int NT, bool VEC>
-int launch_few_nt(const FewArgs& a, cudaStream_t st) {
+int launch_few_nt(FewArgs a, cudaStream_t st) {
     auto k = few_rows_kernel<DT, OT, FP8, MODE, ACT, NT, VEC>;
     constexpr int MATS = MODE == S_GATED ? 2 : 1;
-    constexpr int smem = few_depth<MATS, NT>() * MATS * 4 * S_WARPS * 32 * 16 + S_WARPS * NT * 8 * (MATS * 16 + 1) * 4;
-    static_assert(smem <= 232448, "shared memory");
-    SFFN_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    using St = FewStage<MATS, NT>;
+    constexpr int smem = (VEC ? St::DEPTH * St::BYTES : 0) + St::SUMS;
+    static_assert(smem <= 232448 - 1024, "shared memory");
+    static SmemOnce once;
+    SFFN_CUDA_TRY(once.set(k, smem));
     const int sms = sm100_sms();
     if (!sms) return SFFN_ERR_DEVICE;
-    k<<<min((a.N + 15) / 16, sms), S_WARPS * 32, smem, st>>>(a);
+    const long long rounds = ((a.N + 15) / 16 + sms - 1) / sms;
+    a.per = (int)((a.N + sms * rounds - 1) / (sms * rounds));
+    CUtensorMap m[3];
+    memset(m, 0, sizeof(m));
+    if constexpr (VEC) {  // rows as 4-byte elements, whole 16-byte vectors of them
+        constexpr int ES = FP8 ? 1 : 2;
+        const auto u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
+        const auto none = CU_TENSOR_MAP_SWIZZLE_NONE;
+        const long long inner = (long long)a.K * ES / 16 * 4;
+        if (inner) {
+            for (int i = 0; i < MATS; ++i)
+                if (int rc = tmap_2d(&m[i], u32, 4, a.w[i], inner, a.N, a.ldw[i] * ES / 4, S_ROW / 4, a.per, none)) return rc;
+            if (int rc = tmap_2d(&m[2], u32, 4, a.x, inner, a.T, a.ldx * ES / 4, S_ROW / 4, a.T, none)) return rc;
+        } else {
+            return launch_few_nt<DT, OT, FP8, MODE, ACT, NT, false>(a, st);  // rows of less than 16 bytes
+        }
+    }
+    const int groups = (a.N + a.per - 1) / a.per;
+    k<<<groups < sms ? groups : sms, S_THREADS, smem, st>>>(m[0], m[1], m[2], a);
     SFFN_CHECK_LAUNCH();
     return SFFN_OK;
 }
@@ -298,22 +412,24 @@ int check_few(long long T, long long N, long long K) {
 
 using namespace sffn;
 
-extern "C" int sffn_few_rows_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t T, int64_t N,
-                                int64_t K, void* out, int64_t ldo, void* stream) {
+namespace sffn {
+namespace {
+int few_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t T, int64_t N, int64_t K, void* out,
+           int64_t ldo, uint32_t* status_dev, cudaStream_t st, DeviceScope& scope) {
     if (dtype != SFFN_BF16 && dtype != SFFN_F16) return SFFN_ERR_DTYPE;
     if (int rc = check_few(T, N, K)) return rc;
     if (T == 0 || N == 0) return SFFN_OK;
-    if (!x || !w || !out || ldx < K || ldw < K || ldo < N) return SFFN_ERR_ARG;
+    if (!x || !w || !out || !status_dev || ldx < K || ldw < K || ldo < N) return SFFN_ERR_ARG;
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) & 1) return SFFN_ERR_ALIGN;
-    DeviceScope scope;
-    if (int rc = scope.bind(x)) return rc;
+    if (scope.device() < 0)
+        if (int rc = scope.bind(x)) return rc;
     FewArgs a{};
+    a.status = status_dev;
     a.T = (int)T, a.N = (int)N, a.K = (int)K;
     a.x = x, a.ldx = ldx;
     a.w[0] = w, a.ldw[0] = ldw;
     a.out = static_cast<uint16_t*>(out), a.ldo = ldo;
     const bool vec = rows16(x, ldx, 2) && rows16(w, ldw, 2);
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == SFFN_BF16)
         return vec ? launch_few<SFFN_BF16, SFFN_BF16, false, S_PLAIN, 0, true>(a, st)
                    : launch_few<SFFN_BF16, SFFN_BF16, false, S_PLAIN, 0, false>(a, st);
@@ -321,48 +437,67 @@ extern "C" int sffn_few_rows_mm(int dtype, const void* x, int64_t ldx, const voi
                : launch_few<SFFN_F16, SFFN_F16, false, S_PLAIN, 0, false>(a, st);
 }
 
-extern "C" int sffn_few_rows_glu(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
-                                 int64_t ldwu, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, void* stream) {
+int few_glu(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
+            int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, uint32_t* status_dev, cudaStream_t st, DeviceScope& scope) {
     if (dtype != SFFN_BF16 && dtype != SFFN_F16) return SFFN_ERR_DTYPE;
     if (int rc = check_few(T, F, D)) return rc;
     if (act < GLU_RELU || act > GLU_GELU) return SFFN_ERR_ARG;
     if (T == 0 || F == 0) return SFFN_OK;
-    if (!x || !wg || !wu || !h || ldx < D || ldwg < D || ldwu < D || ldh < F) return SFFN_ERR_ARG;
+    if (!x || !wg || !wu || !h || !status_dev || ldx < D || ldwg < D || ldwu < D || ldh < F) return SFFN_ERR_ARG;
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(wg) | reinterpret_cast<uintptr_t>(wu) |
          reinterpret_cast<uintptr_t>(h)) & 1)
         return SFFN_ERR_ALIGN;
-    DeviceScope scope;
-    if (int rc = scope.bind(x)) return rc;
+    if (scope.device() < 0)
+        if (int rc = scope.bind(x)) return rc;
     FewArgs a{};
+    a.status = status_dev;
     a.T = (int)T, a.N = (int)F, a.K = (int)D;
     a.x = x, a.ldx = ldx;
     a.w[0] = wg, a.ldw[0] = ldwg;
     a.w[1] = wu, a.ldw[1] = ldwu;
     a.out = static_cast<uint16_t*>(h), a.ldo = ldh;
     const bool vec = rows16(x, ldx, 2) && rows16(wg, ldwg, 2) && rows16(wu, ldwu, 2);
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == SFFN_BF16) return vec ? launch_gated<SFFN_BF16, true>(act, a, st) : launch_gated<SFFN_BF16, false>(act, a, st);
     return vec ? launch_gated<SFFN_F16, true>(act, a, st) : launch_gated<SFFN_F16, false>(act, a, st);
+}
+}  // namespace
+}  // namespace sffn
+
+extern "C" int sffn_few_rows_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t T, int64_t N,
+                                int64_t K, void* out, int64_t ldo, uint32_t* status_dev, void* stream) {
+    DeviceScope scope;
+    return few_mm(dtype, x, ldx, w, ldw, T, N, K, out, ldo, status_dev, reinterpret_cast<cudaStream_t>(stream), scope);
+}
+
+extern "C" int sffn_few_rows_glu(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
+                                 int64_t ldwu, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, uint32_t* status_dev,
+                                 void* stream) {
+    DeviceScope scope;
+    return few_glu(dtype, act, x, ldx, wg, ldwg, wu, ldwu, T, D, F, h, ldh, status_dev, reinterpret_cast<cudaStream_t>(stream),
+                   scope);
 }
 
 extern "C" int sffn_few_rows_ffn(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
                                  int64_t ldwu, const void* w2, int64_t ldw2, int64_t T, int64_t D, int64_t F, void* h,
-                                 int64_t ldh, void* y, int64_t ldy, void* stream) {
-    if (int rc = sffn_few_rows_glu(dtype, act, x, ldx, wg, ldwg, wu, ldwu, T, D, F, h, ldh, stream)) return rc;
-    return sffn_few_rows_mm(dtype, h, ldh, w2, ldw2, T, D, F, y, ldy, stream);
+                                 int64_t ldh, void* y, int64_t ldy, uint32_t* status_dev, void* stream) {
+    DeviceScope scope;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (int rc = few_glu(dtype, act, x, ldx, wg, ldwg, wu, ldwu, T, D, F, h, ldh, status_dev, st, scope)) return rc;
+    return few_mm(dtype, h, ldh, w2, ldw2, T, D, F, y, ldy, status_dev, st, scope);
 }
 
 extern "C" int sffn_few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw,
                                  const void* w_scales, int64_t T, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
-                                 void* stream) {
+                                 uint32_t* status_dev, void* stream) {
     if (out_dtype != SFFN_BF16 && out_dtype != SFFN_F16) return SFFN_ERR_DTYPE;
     if (int rc = check_few(T, N, K)) return rc;
     if (T == 0 || N == 0) return SFFN_OK;
-    if (!x || !x_scales || !w || !w_scales || !out || ldx < K || ldw < K || ldo < N) return SFFN_ERR_ARG;
+    if (!x || !x_scales || !w || !w_scales || !out || !status_dev || ldx < K || ldw < K || ldo < N) return SFFN_ERR_ARG;
     if (!rows16(x, ldx, 1) || !rows16(w, ldw, 1) || reinterpret_cast<uintptr_t>(out) % 2) return SFFN_ERR_ALIGN;
     DeviceScope scope;
     if (int rc = scope.bind(x)) return rc;
     FewArgs a{};
+    a.status = status_dev;
     a.T = (int)T, a.N = (int)N, a.K = (int)K;
     a.x = x, a.ldx = ldx;
     a.w[0] = w, a.ldw[0] = ldw;

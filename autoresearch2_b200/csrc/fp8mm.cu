@@ -222,6 +222,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
         // ------------------------------------------------------ epilogue --
         const int ew = warp & 3, wg = (warp - 8) >> 2;
         unsigned char* sbuf = sscales + X_STAGES * X_SCALES + (warp - 8) * 2048;
+        StageRing<1> ring(sbuf);
         const uint32_t tempty_leader = leader_smem_addr(&tempty_bar);
         const uint32_t lane_base = tmem_base + ((uint32_t)(ew * 32) << 16);
         int it = 0;
@@ -257,7 +258,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
                 tmem_wait_ld();
                 const int col = col0 + c * 32;
                 if (args.vec_out) {
-                    stage_store(&tmC, sbuf, lane, w, col, row0);
+                    ring.store(&tmC, lane, w, col, row0);
                 } else {
                     stage_store_plain(args.out, args.ldc, args.M, args.N, sbuf, lane, w, col, row0);
                 }
@@ -293,7 +294,8 @@ int launch_mm(const void* a, long long lda, const void* as, const void* b, long 
                              CU_TENSOR_MAP_SWIZZLE_64B))
             return rc;
     auto k = fp8_mm_kernel<DT>;
-    SFFN_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, X_SMEM));
+    static SmemOnce once;
+    SFFN_CUDA_TRY(once.set(k, X_SMEM));
     static const int pairs = resident_pairs(k, X_THREADS, X_SMEM);
     const long long ntiles = (long long)((args.tiles_m + 1) / 2) * args.tiles_n;
     const int clusters = (int)std::min<long long>(ntiles, pairs);

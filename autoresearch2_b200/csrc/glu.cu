@@ -41,16 +41,16 @@ constexpr int P_BK = 64;
 constexpr int P_THREADS = 416;
 constexpr int P_OPERAND = 128 * P_BK * 2;  // bytes of one operand a stage and CTA
 constexpr int P_STAGE = 2 * P_OPERAND;
-// The fused epilogues stage three matrices a warp instead of one; their rings
-// have four stages to make room.  Even counts: the issuers take alternate
-// k-blocks.
+// The fused epilogues store three matrices instead of one and have more staging
+// buffers a warp; their operand rings have four stages to make room.  Even
+// counts: the issuers take alternate k-blocks.
 template <int EPI>
 constexpr int p_stages() { return EPI == P_STORE ? 6 : 4; }
 template <int EPI>
-constexpr int p_bufs() { return EPI == P_STORE ? 1 : 3; }
+constexpr int p_bufs() { return EPI == P_STORE ? 2 : 5; }
 template <int EPI>
 constexpr int p_smem() { return p_stages<EPI>() * P_STAGE + 8 * p_bufs<EPI>() * 2048 + 1024; }
-static_assert(p_smem<P_STORE>() <= 227 * 1024 - 6144 && p_smem<P_UP>() <= 227 * 1024 - 6144, "shared memory");
+static_assert(p_smem<P_STORE>() <= 227 * 1024 - 1024 && p_smem<P_UP>() <= 227 * 1024 - 6144, "shared memory");
 
 struct PairArgs {
     int M, N;
@@ -254,7 +254,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         // ------------------------------------------------------ epilogue --
         const int wg = (warp - 4) >> 2, ew = warp & 3;
         unsigned char* sbuf = smem + NST * P_STAGE + (warp - 4) * (p_bufs<EPI>() * 2048);
+        StageRing<p_bufs<EPI>()> ring(sbuf);
         const uint32_t tempty_leader[2] = {leader_smem_addr(&tempty_bar[0]), leader_smem_addr(&tempty_bar[1])};
+        // DGRAD: 32 columns of g and u as kept, 16-bit pairs or 8 words of four bytes,
+        // loaded 32 columns ahead
+        uint32_t gw[EPI == P_DGRAD ? 16 : 1], uw[EPI == P_DGRAD ? 16 : 1];
+        auto load_kept = [&](int row, bool row_ok, int col) {
+            if constexpr (EPI == P_DGRAD) {
+                if (!row_ok || col >= args.N) return;  // not used
+                const long long at = (long long)row * args.ldk + col;
+                const uint4* gp = args.keep == KEEP_8 ? reinterpret_cast<const uint4*>(args.g8 + at) : reinterpret_cast<const uint4*>(args.g + at);
+                const uint4* up = args.keep == KEEP_8 ? reinterpret_cast<const uint4*>(args.u8 + at) : reinterpret_cast<const uint4*>(args.u + at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i < 2 || args.keep == KEEP_16) {
+                        const uint4 a = __ldcs(gp + i), b = __ldcs(up + i);
+                        gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
+                        uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
+                    }
+                }
+            }
+        };
         int acc = 0, it = 0;
         uint32_t acc_phase = 0;
         for (int task = first_task; task < ntasks; task += task_stride, ++it) {
@@ -264,6 +284,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             const int row = row0 + lane;
             const bool row_ok = row < args.M;
             const int gcol0 = tn * TILE_N + wg * (TILE_N / 2);  // first column of this warpgroup
+            float2 scales_ahead = make_float2(1.f, 1.f);
+            if constexpr (EPI == P_DGRAD) {  // while the products still run
+                if (args.keep == KEEP_8 && row_ok && gcol0 < args.N) {
+                    const long long at = fp8_scale_at(row, gcol0 >> 7, args.bt);
+                    scales_ahead = make_float2(fp8_scale(args.gs[at]), fp8_scale(args.us[at]));
+                }
+                load_kept(row, row_ok, gcol0);
+            }
             const bool ok = __all_sync(FULL, mbar_wait_bounded(&tfull_bar[acc], acc_phase));
             if (!ok && lane == 0) atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
             bool dead = !ok || __any_sync(FULL, s_abort != 0);
@@ -305,7 +333,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
 #pragma unroll
                     for (int q = 0; q < 16; ++q)
                         w[q] = pack16x2<DT>(__uint_as_float(r[2 * q]), __uint_as_float(r[2 * q + 1]));
-                    if (args.vec_out) stage_store(&tmC, sbuf, lane, w, col, row0);
+                    if (args.vec_out) ring.store(&tmC, lane, w, col, row0);
                     else stage_store_plain(args.out, args.ldc, args.M, args.N, sbuf, lane, w, col, row0);
                 }
             } else if constexpr (EPI == P_UP) {
@@ -319,37 +347,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     tmem_ld32(tbase + c * 32, g);
                     tmem_ld32(tbase + 128 + c * 32, u);
                     tmem_wait_ld();
-                    stage_free(lane);
                     float unused;
 #pragma unroll
                     for (int q = 0; q < 16; ++q)
                         w[q] = pack16x2<DT>(glu_act<ACT, false>(__uint_as_float(g[2 * q]), unused) * __uint_as_float(u[2 * q]),
                                             glu_act<ACT, false>(__uint_as_float(g[2 * q + 1]), unused) *
                                                 __uint_as_float(u[2 * q + 1]));
-                    stage32(sbuf, lane, w);
+                    ring.store(&tmC, lane, w, col, row0);
                     if (args.keep == KEEP_16) {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) w[q] = pack16x2<DT>(__uint_as_float(g[2 * q]), __uint_as_float(g[2 * q + 1]));
-                        stage32(sbuf + 2048, lane, w);
+                        ring.store(&tmC2, lane, w, col, row0);
 #pragma unroll
                         for (int q = 0; q < 16; ++q) w[q] = pack16x2<DT>(__uint_as_float(u[2 * q]), __uint_as_float(u[2 * q + 1]));
-                        stage32(sbuf + 4096, lane, w);
+                        ring.store(&tmC3, lane, w, col, row0);
                     } else if (args.keep == KEEP_8) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
                             gmax = max(gmax, g[j] & 0x7FFFFFFFu);
                             umax = max(umax, u[j] & 0x7FFFFFFFu);
                         }
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_2d(&tmC, sbuf, col, row0);
-                        if (args.keep == KEEP_16) {
-                            tma_store_2d(&tmC2, sbuf + 2048, col, row0);
-                            tma_store_2d(&tmC3, sbuf + 4096, col, row0);
-                        }
-                        bulk_commit_group();
                     }
                 }
                 if (args.keep == KEEP_8) {
@@ -402,40 +419,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     }
                 }
             } else {  // P_DGRAD
-                float gscale = 1.f, uscale = 1.f;
-                if (args.keep == KEEP_8 && row_ok && gcol0 < args.N) {
-                    const long long at = fp8_scale_at(row, gcol0 >> 7, args.bt);
-                    gscale = fp8_scale(args.gs[at]);
-                    uscale = fp8_scale(args.us[at]);
-                }
+                const float gscale = scales_ahead.x, uscale = scales_ahead.y;
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     const int col = gcol0 + c * 32;
                     if (row0 >= args.M || col >= args.N) break;
-                    uint32_t gw[16], uw[16];  // 16-bit pairs, or 8 words of four bytes
-                    if (args.keep == KEEP_8) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            uint4 a = make_uint4(0, 0, 0, 0), b = a;
-                            if (row_ok) {
-                                a = __ldcs(reinterpret_cast<const uint4*>(args.g8 + (long long)row * args.ldk + col) + i);
-                                b = __ldcs(reinterpret_cast<const uint4*>(args.u8 + (long long)row * args.ldk + col) + i);
-                            }
-                            gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
-                            uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint4 a = make_uint4(0, 0, 0, 0), b = a;
-                            if (row_ok) {
-                                a = __ldcs(reinterpret_cast<const uint4*>(args.g + (long long)row * args.ldk + col) + i);
-                                b = __ldcs(reinterpret_cast<const uint4*>(args.u + (long long)row * args.ldk + col) + i);
-                            }
-                            gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
-                            uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
-                        }
-                    }
                     uint32_t r[32], wg_[16], wu_[16], wh_[16];
                     tmem_ld32(tbase + c * 32, r);
                     tmem_wait_ld();
@@ -473,18 +461,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                             quad(q, g, u);
                         }
                     }
-                    stage_free(lane);
-                    stage32(sbuf, lane, wg_);
-                    stage32(sbuf + 2048, lane, wu_);
-                    stage32(sbuf + 4096, lane, wh_);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_2d(&tmC, sbuf, col, row0);
-                        tma_store_2d(&tmC2, sbuf + 2048, col, row0);
-                        tma_store_2d(&tmC3, sbuf + 4096, col, row0);
-                        bulk_commit_group();
-                    }
+                    if (c < 3) load_kept(row, row_ok, col + 32);
+                    ring.store(&tmC, lane, wg_, col, row0);
+                    ring.store(&tmC2, lane, wu_, col, row0);
+                    ring.store(&tmC3, lane, wh_, col, row0);
                 }
             }
             // this accumulator back to the leader's MMA warp
@@ -559,7 +539,8 @@ template <int DT, bool A_MN, bool B_MN, int EPI, int ACT>
 int launch_pair(const CUtensorMap (&m)[7], const PairArgs& args, cudaStream_t st) {
     auto k = pair_kernel<DT, A_MN, B_MN, EPI, ACT>;
     constexpr int smem = p_smem<EPI>();
-    SFFN_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static SmemOnce once;
+    SFFN_CUDA_TRY(once.set(k, smem));
     static const int pairs = resident_pairs(k, P_THREADS, smem);
     const long long tasks = (long long)((args.tiles_m + 1) / 2) * args.tiles_n * args.splits;
     const int clusters = (int)std::min<long long>(tasks, pairs);

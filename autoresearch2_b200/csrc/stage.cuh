@@ -18,25 +18,32 @@ __device__ __forceinline__ void stage32(unsigned char* sbuf, int lane, const uin
                      : "memory");
 }
 
-// Before staging buffers are written again: this warp's stores have read them.
-__device__ __forceinline__ void stage_free(int lane) {
-    if (lane == 0) bulk_wait_group_read0();
-    __syncwarp();
-}
+// A warp's R staging buffers, used in turn: each store is a bulk group of its own,
+// and a buffer is written again once the store that used it has read it, with
+// the R - 1 later ones still under way.  (Waiting for the last store each time
+// made the epilogue, not the products, the bound of a 768-wide K.)
+template <int R>
+struct StageRing {
+    unsigned char* base;
+    int at = 0;
+    __device__ __forceinline__ explicit StageRing(unsigned char* p) : base(p) {}
 
-// The block by one bulk-tensor store (whole 64-byte row segments; clipped at the
-// tensor's edges).
-__device__ __forceinline__ void stage_store(const CUtensorMap* tmap, unsigned char* sbuf, int lane, const uint32_t (&w)[16],
-                                            int col, int row0) {
-    stage_free(lane);
-    stage32(sbuf, lane, w);
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-        tma_store_2d(tmap, sbuf, col, row0);
-        bulk_commit_group();
+    // The block by one bulk-tensor store (whole 64-byte row segments; clipped at the
+    // tensor's edges).
+    __device__ __forceinline__ void store(const CUtensorMap* tmap, int lane, const uint32_t (&w)[16], int col, int row0) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(R - 1) : "memory");
+        __syncwarp();
+        unsigned char* sbuf = base + at * 2048;
+        at = at + 1 == R ? 0 : at + 1;
+        stage32(sbuf, lane, w);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(tmap, sbuf, col, row0);
+            bulk_commit_group();
+        }
     }
-}
+};
 
 // The same where the rows' stride or start suit no tensor map: lane = column,
 // row by row.  (A lane writing its own row, 2 bytes of 32 rows an instruction,

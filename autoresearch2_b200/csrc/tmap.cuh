@@ -78,6 +78,21 @@ inline int sm100_sms() {
     return sms;
 }
 
+// A kernel's shared-memory limit, raised once a device.
+struct SmemOnce {
+    std::atomic<uint64_t> done{0};
+    template <typename K>
+    cudaError_t set(K kernel, int smem) {
+        int dev = 0;
+        if (const cudaError_t e = cudaGetDevice(&dev)) return e;
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+        return e;
+    }
+};
+
 // CTA pairs of this kernel that are resident at once (one CTA fills an SM).
 template <typename K>
 int resident_pairs(K kernel, int threads, int smem) {

@@ -219,7 +219,7 @@ def _matmul(av, at, bv, bt, out_dtype):
         return out
     if M <= FEW_ROWS:
         call("sffn_few_rows_fp8", av.data_ptr(), _stride(av), at.data_ptr(), bv.data_ptr(), _stride(bv), bt.data_ptr(), M, N,
-             K, out.data_ptr(), _lib._DTYPES[out_dtype], N, stream_handle(dev))
+             K, out.data_ptr(), _lib._DTYPES[out_dtype], N, _lib.status_word(dev).data_ptr(), stream_handle(dev))
     else:
         call("sffn_fp8_mm", av.data_ptr(), _stride(av), at.data_ptr(), bv.data_ptr(), _stride(bv), bt.data_ptr(), M, N, K,
              out.data_ptr(), _lib._DTYPES[out_dtype], N, _lib.status_word(dev).data_ptr(), stream_handle(dev))
@@ -298,7 +298,7 @@ def _few_rows(x, W):
     out = x.new_empty((T, N))
     if T:
         call("sffn_few_rows_mm", _lib._DTYPES[x.dtype], x.data_ptr(), _ld(x), W.data_ptr(), _ld(W), T, N, x.shape[1],
-             out.data_ptr(), N, stream_handle(x.device))
+             out.data_ptr(), N, _lib.status_word(x.device).data_ptr(), stream_handle(x.device))
     return out
 
 

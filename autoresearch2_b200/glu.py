@@ -40,7 +40,8 @@ def _forward(x, Wg, Wu, W2, act, keep):
     if keep == 0 and 0 < T <= fp8.FEW_ROWS:
         h, y = x2.new_empty((T, (F + 7) // 8 * 8)), x2.new_empty((T, D))
         call("sffn_few_rows_ffn", code, act, x2.data_ptr(), fp8._ld(x2), Wg.data_ptr(), fp8._ld(Wg), Wu.data_ptr(),
-             fp8._ld(Wu), W2.data_ptr(), fp8._ld(W2), T, D, F, h.data_ptr(), h.shape[1], y.data_ptr(), D, stream_handle(dev))
+             fp8._ld(Wu), W2.data_ptr(), fp8._ld(W2), T, D, F, h.data_ptr(), h.shape[1], y.data_ptr(), D,
+             _lib.status_word(dev).data_ptr(), stream_handle(dev))
         return y if x.dim() == 2 else y.view(x.shape), g, u, gt, ut, xv, xt
     if keep == 2:
         g, u = (fp8._empty_values(T, F, dev, CHUNK) for _ in range(2))

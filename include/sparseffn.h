@@ -700,16 +700,17 @@ int sffn_gemm16(int dtype, const void* A, int64_t lda, int a_mn, const void* B, 
 /* Products of at most 32 rows with long weights (any alignment): out [T, N] =
  * x w^T; h [T, F] = act(x wg^T) * (x wu^T); and x w^T in 8-bit blocks. */
 int sffn_few_rows_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t T, int64_t N, int64_t K,
-                     void* out, int64_t ldo, void* stream);
+                     void* out, int64_t ldo, uint32_t* status_dev, void* stream);
 int sffn_few_rows_glu(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
-                      int64_t ldwu, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, void* stream);
+                      int64_t ldwu, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, uint32_t* status_dev,
+                      void* stream);
 /* sffn_few_rows_glu and then y [T, D] = h w2^T, in one call. */
 int sffn_few_rows_ffn(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
                       int64_t ldwu, const void* w2, int64_t ldw2, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh,
-                      void* y, int64_t ldy, void* stream);
+                      void* y, int64_t ldy, uint32_t* status_dev, void* stream);
 int sffn_few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw,
                       const void* w_scales, int64_t T, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
-                      void* stream);
+                      uint32_t* status_dev, void* stream);
 
 /* ---- bounded waits ------------------------------------------------------ */
 

@@ -135,6 +135,17 @@ def test_forward(T, D, F, dtype):
     sf.check_status()
 
 
+@pytest.mark.parametrize("T,D,F", [(1, 3000, 5003), (8, 600, 2500), (16, 2600, 4096), (27, 2500, 7001), (32, 515, 9000)])
+def test_forward_of_few_rows_and_long_weights(T, D, F):
+    """Several groups of weight rows a multiprocessor, in both projections; many
+    calls under way at once."""
+    x, Wg, Wu, W2, _ = inputs(T, D, F, BF16)
+    ys = [sf.gated_ffn(x, Wg, Wu, W2) for _ in range(20)]
+    check_forward(ys[0], x, Wg, Wu, W2, "silu")
+    assert all(torch.equal(ys[0], y) for y in ys[1:])
+    sf.check_status()
+
+
 @pytest.mark.parametrize("checkpoint", [None, "fp8"])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("T,D,F", SIZES)
