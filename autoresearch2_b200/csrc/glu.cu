@@ -47,10 +47,12 @@ constexpr int P_STAGE = 2 * P_OPERAND;
 template <int EPI>
 constexpr int p_stages() { return EPI == P_STORE ? 6 : 4; }
 template <int EPI>
-constexpr int p_bufs() { return EPI == P_STORE ? 2 : 5; }
+constexpr int p_bufs() { return EPI == P_STORE ? 2 : EPI == P_UP ? 5 : 4; }
+constexpr int P_KEPT = 4096;  // DGRAD: a warp's 32 x 32 of g and of u as kept
 template <int EPI>
-constexpr int p_smem() { return p_stages<EPI>() * P_STAGE + 8 * p_bufs<EPI>() * 2048 + 1024; }
-static_assert(p_smem<P_STORE>() <= 227 * 1024 - 1024 && p_smem<P_UP>() <= 227 * 1024 - 6144, "shared memory");
+constexpr int p_smem() { return p_stages<EPI>() * P_STAGE + 8 * (p_bufs<EPI>() * 2048 + (EPI == P_DGRAD ? P_KEPT : 0)) + 1024; }
+static_assert(p_smem<P_STORE>() <= 227 * 1024 - 1024 && p_smem<P_UP>() <= 227 * 1024 - 6144 &&
+              p_smem<P_DGRAD>() <= 227 * 1024 - 1024, "shared memory");
 
 struct PairArgs {
     int M, N;
@@ -63,10 +65,7 @@ struct PairArgs {
     float* part;  // STORE, splits > 1: [splits][M][ldp]
     long long ldp;
     int keep;
-    const uint16_t *g, *u;  // DGRAD, KEEP_16: rows ldk apart
-    uint8_t *g8, *u8;       // KEEP_8: values (rows ldk apart) and scale tiles
-    uint8_t *gs, *us;
-    long long ldk;
+    uint8_t *gs, *us;  // KEEP_8: scale tiles of g and u
     int bt;  // scale tiles across a row
     uint32_t* status;
 };
@@ -83,7 +82,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2,
                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmC2,
-                const __grid_constant__ CUtensorMap tmC3, const PairArgs args) {
+                const __grid_constant__ CUtensorMap tmC3, const __grid_constant__ CUtensorMap tmG,
+                const __grid_constant__ CUtensorMap tmU, const PairArgs args) {
     constexpr int NST = p_stages<EPI>();
     constexpr uint32_t IDESC = idesc16<DT>(A_MN, B_MN);
     constexpr uint32_t MN_LBO = P_BK * 128;  // MN-major: 64-element blocks of 64 K rows x 128 bytes
@@ -93,6 +93,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                                                            ~static_cast<uintptr_t>(1023));
     __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST];
     __shared__ __align__(8) uint64_t tfull_bar[2], tempty_bar[2];
+    __shared__ __align__(8) uint64_t kept_bar[8];  // DGRAD: each epilogue warp's g and u have come
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_dead;
     __shared__ uint2 s_amax[EPI == P_UP ? 2 : 1][2][128];  // UP: [tile parity][warpgroup][row], of g and u
@@ -107,9 +108,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     // the tile of a task and its k-blocks
     auto locate = [&](int task, int& pm, int& tn, int& kb0, int& kb1) {
         int sp = 0;
+        // all tiles of one part of K run together: they share its operands in L2
+        // (2304 x 768 of 32768 in 5 parts: 113 -> 106 us)
         if (EPI == P_STORE && args.splits > 1) {
-            sp = task % args.splits;
-            task /= args.splits;
+            const int tiles = tiles_mp * args.tiles_n;
+            sp = task / tiles;
+            task -= sp * tiles;
         }
         pair_raster(task, tiles_mp, args.tiles_n, pm, tn);
         kb0 = sp * args.per_split;
@@ -126,6 +130,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             mbar_init(&tfull_bar[a], 1);
             mbar_init(&tempty_bar[a], 16);  // the epilogue warps of both CTAs
         }
+        for (int w = 0; w < 8; ++w) mbar_init(&kept_bar[w], 1);
         s_abort = s_dead = 0;
         fence_mbar_init();
         prefetch_tmap(&tmA);
@@ -256,25 +261,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         unsigned char* sbuf = smem + NST * P_STAGE + (warp - 4) * (p_bufs<EPI>() * 2048);
         StageRing<p_bufs<EPI>()> ring(sbuf);
         const uint32_t tempty_leader[2] = {leader_smem_addr(&tempty_bar[0]), leader_smem_addr(&tempty_bar[1])};
-        // DGRAD: 32 columns of g and u as kept, 16-bit pairs or 8 words of four bytes,
-        // loaded 32 columns ahead
-        uint32_t gw[EPI == P_DGRAD ? 16 : 1], uw[EPI == P_DGRAD ? 16 : 1];
-        auto load_kept = [&](int row, bool row_ok, int col) {
-            if constexpr (EPI == P_DGRAD) {
-                if (!row_ok || col >= args.N) return;  // not used
-                const long long at = (long long)row * args.ldk + col;
-                const uint4* gp = args.keep == KEEP_8 ? reinterpret_cast<const uint4*>(args.g8 + at) : reinterpret_cast<const uint4*>(args.g + at);
-                const uint4* up = args.keep == KEEP_8 ? reinterpret_cast<const uint4*>(args.u8 + at) : reinterpret_cast<const uint4*>(args.u + at);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (i < 2 || args.keep == KEEP_16) {
-                        const uint4 a = __ldcs(gp + i), b = __ldcs(up + i);
-                        gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
-                        uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
-                    }
-                }
+        // DGRAD: 32 columns of g and u as kept come by TMA, 32 ahead (each lane's own
+        // loads, of 32 rows an instruction, took half of the kernel's time)
+        unsigned char* kept = smem + NST * P_STAGE + 8 * (p_bufs<EPI>() * 2048) + (warp - 4) * P_KEPT;
+        uint64_t* kbar = &kept_bar[warp - 4];
+        const uint32_t kept_bytes = args.keep == KEEP_8 ? 1024u : 2048u;  // of one matrix
+        uint32_t kept_phase = 0;
+        auto fetch_kept = [&](int col, int row0) {  // the last ones are in registers
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive_expect_tx(kbar, 2 * kept_bytes);
+                tma_load_2d(kept, &tmG, col, row0, kbar);
+                tma_load_2d(kept + 2048, &tmU, col, row0, kbar);
             }
         };
+        bool kept_due = false;  // a fetch is under way
         int acc = 0, it = 0;
         uint32_t acc_phase = 0;
         for (int task = first_task; task < ntasks; task += task_stride, ++it) {
@@ -290,7 +291,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     const long long at = fp8_scale_at(row, gcol0 >> 7, args.bt);
                     scales_ahead = make_float2(fp8_scale(args.gs[at]), fp8_scale(args.us[at]));
                 }
-                load_kept(row, row_ok, gcol0);
+                if (row0 < args.M && gcol0 < args.N) {
+                    fetch_kept(gcol0, row0);
+                    kept_due = true;
+                }
             }
             const bool ok = __all_sync(FULL, mbar_wait_bounded(&tfull_bar[acc], acc_phase));
             if (!ok && lane == 0) atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
@@ -357,10 +361,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     if (args.keep == KEEP_16) {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) w[q] = pack16x2<DT>(__uint_as_float(g[2 * q]), __uint_as_float(g[2 * q + 1]));
-                        ring.store(&tmC2, lane, w, col, row0);
+                        ring.store(&tmG, lane, w, col, row0);
 #pragma unroll
                         for (int q = 0; q < 16; ++q) w[q] = pack16x2<DT>(__uint_as_float(u[2 * q]), __uint_as_float(u[2 * q + 1]));
-                        ring.store(&tmC3, lane, w, col, row0);
+                        ring.store(&tmU, lane, w, col, row0);
                     } else if (args.keep == KEEP_8) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
@@ -371,7 +375,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                 }
                 if (args.keep == KEEP_8) {
                     // rare: infinities and NaN do not count
-                    if (__any_sync(FULL, max(gmax, umax) >= 0x7F800000u)) {
+                    const bool finite = !__any_sync(FULL, max(gmax, umax) >= 0x7F800000u);
+                    if (!finite) {
                         gmax = umax = 0;
 #pragma unroll 1
                         for (int c = 0; c < 2; ++c) {
@@ -396,26 +401,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                         if (wg == 0) args.gs[at] = (uint8_t)(ge + 127);
                         else args.us[at] = (uint8_t)(ue + 127);
                     }
-                    const float ginv = two_to(-ge), uinv = two_to(-ue);
+                    // 64 columns of g, then of u, a lane's 64 bytes as 32 16-bit values are
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        const int col = gcol0 + (c >> 1) * 32;
-                        if (!warp_live || col >= args.N) break;
-                        const bool is_u = c & 1;
-                        uint32_t r[32];
-                        tmem_ld32(tbase + (is_u ? 128 : 0) + (c >> 1) * 32, r);
-                        tmem_wait_ld();
-                        uint32_t w[8];
-                        const float inv = is_u ? uinv : ginv;
+                    for (int m = 0; m < 2; ++m) {
+                        if (!warp_live || gcol0 >= args.N) break;
+                        const float inv = two_to(m ? -ue : -ge);
+                        uint32_t w[16];
 #pragma unroll
-                        for (int q = 0; q < 8; ++q)
-                            w[q] = fp8_pack4<false>(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]),
-                                             __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]), inv);
-                        if (row_ok) {  // a whole 32-byte sector
-                            uint4* p = reinterpret_cast<uint4*>((is_u ? args.u8 : args.g8) + (long long)row * args.ldk + col);
-                            p[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                            p[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t r[32];
+                            tmem_ld32(tbase + m * 128 + c * 32, r);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) {
+                                const float v0 = __uint_as_float(r[4 * q]), v1 = __uint_as_float(r[4 * q + 1]);
+                                const float v2 = __uint_as_float(r[4 * q + 2]), v3 = __uint_as_float(r[4 * q + 3]);
+                                w[c * 8 + q] = finite ? fp8_pack4<true>(v0, v1, v2, v3, inv) : fp8_pack4<false>(v0, v1, v2, v3, inv);
+                            }
                         }
+                        ring.store(m ? &tmU : &tmG, lane, w, gcol0, row0);
                     }
                 }
             } else {  // P_DGRAD
@@ -424,6 +428,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                 for (int c = 0; c < 4; ++c) {
                     const int col = gcol0 + c * 32;
                     if (row0 >= args.M || col >= args.N) break;
+                    if (!__all_sync(FULL, mbar_wait_bounded(kbar, kept_phase))) {
+                        if (lane == 0) atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
+                        dead = true;
+                        break;
+                    }
+                    kept_phase ^= 1u;
+                    kept_due = false;
+                    uint32_t gw[16], uw[16];  // this row's: 16-bit pairs, or 8 words of four bytes
+                    if (args.keep == KEEP_8) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint4 a = *reinterpret_cast<const uint4*>(kept + lane * 32 + 16 * i);
+                            const uint4 b = *reinterpret_cast<const uint4*>(kept + 2048 + lane * 32 + 16 * i);
+                            gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
+                            uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = lane * 64 + 16 * (i ^ ((lane >> 1) & 3));
+                            const uint4 a = *reinterpret_cast<const uint4*>(kept + at);
+                            const uint4 b = *reinterpret_cast<const uint4*>(kept + 2048 + at);
+                            gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
+                            uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
+                        }
+                    }
+                    if (c < 3 && col + 32 < args.N) {
+                        fetch_kept(col + 32, row0);
+                        kept_due = true;
+                    }
                     uint32_t r[32], wg_[16], wu_[16], wh_[16];
                     tmem_ld32(tbase + c * 32, r);
                     tmem_wait_ld();
@@ -461,12 +495,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                             quad(q, g, u);
                         }
                     }
-                    if (c < 3) load_kept(row, row_ok, col + 32);
                     ring.store(&tmC, lane, wg_, col, row0);
                     ring.store(&tmC2, lane, wu_, col, row0);
                     ring.store(&tmC3, lane, wh_, col, row0);
                 }
             }
+            if (EPI == P_DGRAD && dead) break;
             // this accumulator back to the leader's MMA warp
             tc_fence_before();
             __syncwarp();
@@ -476,6 +510,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                 acc_phase ^= 1u;
             }
         }
+        if (EPI == P_DGRAD && kept_due) (void)mbar_wait_bounded(kbar, kept_phase);  // left early: it has landed
         if (lane == 0) bulk_wait_group0();
         __syncwarp();
     }
@@ -533,10 +568,18 @@ int store_map(CUtensorMap* m, const void* p, long long rows, long long cols, lon
     return tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p, cols, rows, ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
+// Maps of g or u as kept, to write (UP) and to read (DGRAD): 64 bytes of 32 rows,
+// or 32 bytes in 8 bits where DGRAD reads 32 columns.
+int kept_map(CUtensorMap* m, int keep, const void* p, long long T, long long F, long long ldk, bool read) {
+    if (keep == KEEP_16) return store_map(m, p, T, F, ldk);
+    return tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p, F, T, ldk, read ? 32 : 64, 32,
+                   read ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 bool operand_ok(const void* p, long long ld) { return aligned16(p) && ld % 8 == 0; }
 
 template <int DT, bool A_MN, bool B_MN, int EPI, int ACT>
-int launch_pair(const CUtensorMap (&m)[7], const PairArgs& args, cudaStream_t st) {
+int launch_pair(const CUtensorMap (&m)[9], const PairArgs& args, cudaStream_t st) {
     auto k = pair_kernel<DT, A_MN, B_MN, EPI, ACT>;
     constexpr int smem = p_smem<EPI>();
     static SmemOnce once;
@@ -544,7 +587,7 @@ int launch_pair(const CUtensorMap (&m)[7], const PairArgs& args, cudaStream_t st
     static const int pairs = resident_pairs(k, P_THREADS, smem);
     const long long tasks = (long long)((args.tiles_m + 1) / 2) * args.tiles_n * args.splits;
     const int clusters = (int)std::min<long long>(tasks, pairs);
-    k<<<clusters * 2, P_THREADS, smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], args);
+    k<<<clusters * 2, P_THREADS, smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7], m[8], args);
     SFFN_CHECK_LAUNCH();
     return SFFN_OK;
 }
@@ -598,7 +641,7 @@ int gemm16(const Operand& A, bool a_mn, const Operand& B, bool b_mn, const Opera
     a.ldc = ldc;
     a.vec_out = aligned16(C) && ldc % 8 == 0;
     a.status = status;
-    CUtensorMap m[7];
+    CUtensorMap m[9];
     memset(m, 0, sizeof(m));
     if (int rc = operand_map(&m[0], A, a_mn, M, K)) return rc;
     if (int rc = operand_map(&m[1], B, b_mn, N, K)) return rc;
@@ -622,7 +665,7 @@ int gemm16(const Operand& A, bool a_mn, const Operand& B, bool b_mn, const Opera
 }
 
 template <int DT, int EPI, bool B_MN>
-int launch_act(int act, const CUtensorMap (&m)[7], const PairArgs& a, cudaStream_t st) {
+int launch_act(int act, const CUtensorMap (&m)[9], const PairArgs& a, cudaStream_t st) {
     switch (act) {
         case GLU_RELU: return launch_pair<DT, false, B_MN, EPI, GLU_RELU>(m, a, st);
         case GLU_RELU2: return launch_pair<DT, false, B_MN, EPI, GLU_RELU2>(m, a, st);
@@ -640,13 +683,11 @@ int check_glu(int dtype, int act, int keep, long long T, long long D, long long 
     if (!sizes_ok(T, F, D) || T * fp8_block_tiles(F) > 0x7FFFFFFF) return SFFN_ERR_TOO_LARGE;
     if (keep == KEEP_NONE) return SFFN_OK;
     if (!g || !u || ldk < F || (keep == KEEP_8 && (!gs || !us))) return SFFN_ERR_ARG;
-    // whole 32-column chunks of the kept rows are written and read
-    if (!aligned16(g) || !aligned16(u) || ldk % 32) return SFFN_ERR_ALIGN;
+    if (!aligned16(g) || !aligned16(u) || ldk % (keep == KEEP_8 ? 16 : 8)) return SFFN_ERR_ALIGN;
     return SFFN_OK;
 }
 
-PairArgs glu_args(long long T, long long F, long long D, int tile_n, int keep, const void* g, const void* u, long long ldk,
-                  const void* gs, const void* us, uint32_t* status) {
+PairArgs glu_args(long long T, long long F, long long D, int tile_n, int keep, const void* gs, const void* us, uint32_t* status) {
     PairArgs a{};
     a.M = (int)T;
     a.N = (int)F;
@@ -655,16 +696,8 @@ PairArgs glu_args(long long T, long long F, long long D, int tile_n, int keep, c
     a.nkb = a.nkb1 = a.per_split = (int)kblocks(D);
     a.splits = 1;
     a.keep = keep;
-    if (keep == KEEP_8) {
-        a.g8 = static_cast<uint8_t*>(const_cast<void*>(g));
-        a.u8 = static_cast<uint8_t*>(const_cast<void*>(u));
-        a.gs = static_cast<uint8_t*>(const_cast<void*>(gs));
-        a.us = static_cast<uint8_t*>(const_cast<void*>(us));
-    } else {
-        a.g = static_cast<const uint16_t*>(g);
-        a.u = static_cast<const uint16_t*>(u);
-    }
-    a.ldk = ldk;
+    a.gs = static_cast<uint8_t*>(const_cast<void*>(gs));
+    a.us = static_cast<uint8_t*>(const_cast<void*>(us));
     a.bt = (int)fp8_block_tiles(F);
     a.status = status;
     return a;
@@ -716,16 +749,16 @@ extern "C" int sffn_glu_up(int dtype, int act, const void* x, int64_t ldx, const
     DeviceScope scope;
     if (int rc = scope.bind(x)) return rc;
     if (!sm100_sms()) return SFFN_ERR_DEVICE;
-    const PairArgs a = glu_args(T, F, D, 128, keep, g, u, ldk, g_scales, u_scales, status_dev);
-    CUtensorMap m[7];
+    const PairArgs a = glu_args(T, F, D, 128, keep, g_scales, u_scales, status_dev);
+    CUtensorMap m[9];
     memset(m, 0, sizeof(m));
     if (int rc = operand_map(&m[0], {x, ldx}, false, T, D)) return rc;
     if (int rc = operand_map(&m[1], {wg, ldwg}, false, F, D)) return rc;
     if (int rc = operand_map(&m[3], {wu, ldwu}, false, F, D)) return rc;
     if (int rc = store_map(&m[4], h, T, F, ldh)) return rc;
-    if (keep == KEEP_16) {
-        if (int rc = store_map(&m[5], g, T, F, ldk)) return rc;
-        if (int rc = store_map(&m[6], u, T, F, ldk)) return rc;
+    if (keep != KEEP_NONE) {
+        if (int rc = kept_map(&m[7], keep, g, T, F, ldk, false)) return rc;
+        if (int rc = kept_map(&m[8], keep, u, T, F, ldk, false)) return rc;
     }
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return dtype == SFFN_BF16 ? launch_act<SFFN_BF16, P_UP, false>(act, m, a, st)
@@ -746,14 +779,16 @@ extern "C" int sffn_glu_dgrad(int dtype, int act, const void* dy, int64_t lddy, 
     DeviceScope scope;
     if (int rc = scope.bind(dy)) return rc;
     if (!sm100_sms()) return SFFN_ERR_DEVICE;
-    const PairArgs a = glu_args(T, F, D, 256, keep, g, u, ldk, g_scales, u_scales, status_dev);
-    CUtensorMap m[7];
+    const PairArgs a = glu_args(T, F, D, 256, keep, g_scales, u_scales, status_dev);
+    CUtensorMap m[9];
     memset(m, 0, sizeof(m));
     if (int rc = operand_map(&m[0], {dy, lddy}, false, T, D)) return rc;
     if (int rc = operand_map(&m[1], {w2, ldw2}, true, F, D)) return rc;
     if (int rc = store_map(&m[4], dg, T, F, ldd)) return rc;
     if (int rc = store_map(&m[5], du, T, F, ldd)) return rc;
     if (int rc = store_map(&m[6], h, T, F, ldh)) return rc;
+    if (int rc = kept_map(&m[7], keep, g, T, F, ldk, true)) return rc;
+    if (int rc = kept_map(&m[8], keep, u, T, F, ldk, true)) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return dtype == SFFN_BF16 ? launch_act<SFFN_BF16, P_DGRAD, true>(act, m, a, st)
                               : launch_act<SFFN_F16, P_DGRAD, true>(act, m, a, st);

@@ -27,7 +27,10 @@ __all__ = ["ACTIVATIONS", "gated_ffn"]
 
 ACTIVATIONS = {"relu": 0, "relu2": 1, "silu": 2, "gelu": 3}
 KEEP = {None: 1, "fp8": 2}
-CHUNK = 32  # columns: kept rows are padded to whole ones
+
+
+def _kept_ld(F, keep):
+    return (F + 15) // 16 * 16 if keep == 2 else (F + 7) // 8 * 8
 
 
 def _forward(x, Wg, Wu, W2, act, keep):
@@ -44,10 +47,10 @@ def _forward(x, Wg, Wu, W2, act, keep):
              _lib.status_word(dev).data_ptr(), stream_handle(dev))
         return y if x.dim() == 2 else y.view(x.shape), g, u, gt, ut, xv, xt
     if keep == 2:
-        g, u = (fp8._empty_values(T, F, dev, CHUNK) for _ in range(2))
+        g, u = (fp8._empty_values(T, F, dev) for _ in range(2))
         gt, ut = (fp8._empty_tiles(T, F, dev) for _ in range(2))
     elif keep == 1:
-        g, u = (fp8._empty_rows(x2, T, F, CHUNK) for _ in range(2))
+        g, u = (fp8._empty_rows(x2, T, F, 8) for _ in range(2))
     if T == 0:
         if keep == 2:
             xv, xt = fp8._pack(x2)
@@ -59,7 +62,7 @@ def _forward(x, Wg, Wu, W2, act, keep):
     h = fp8._empty_rows(x2, T, F, 8)
     ldh = (F + 7) // 8 * 8
     call("sffn_glu_up", code, act, xa[0].data_ptr(), xa[1], ga[0].data_ptr(), ga[1], ua[0].data_ptr(), ua[1], T, D, F,
-         h.data_ptr(), ldh, keep, ptr(g), ptr(u), -(-F // CHUNK) * CHUNK, ptr(gt), ptr(ut),
+         h.data_ptr(), ldh, keep, ptr(g), ptr(u), _kept_ld(F, keep), ptr(gt), ptr(ut),
          _lib.status_word(dev).data_ptr(), stream_handle(dev))
     if T <= fp8.FEW_ROWS:
         y = fp8._few_rows(h, W2)
@@ -89,7 +92,7 @@ def _backward(dy, x, Wg, Wu, W2, g, u, gt, ut, xv, xt, act, want):
     else:
         dya, W2a = fp8._align(dy2, W2)
     call("sffn_glu_dgrad", code, act, dya[0].data_ptr(), dya[1], W2a[0].data_ptr(), W2a[1], T, D, F, keep, g.data_ptr(),
-         u.data_ptr(), -(-F // CHUNK) * CHUNK, ptr(gt), ptr(ut), dg[0].data_ptr(), du[0].data_ptr(), 2 * ld, h.data_ptr(), ld,
+         u.data_ptr(), _kept_ld(F, keep), ptr(gt), ptr(ut), dg[0].data_ptr(), du[0].data_ptr(), 2 * ld, h.data_ptr(), ld,
          _lib.status_word(dev).data_ptr(), stream_handle(dev))
     if want[3]:
         dW2 = submit_grad(fp8._mm_into(dy2.new_empty((D, F)), dya, 1, (h, ld), 1))

@@ -673,9 +673,8 @@ enum { /* how g and u are kept for the backward */
 };
 
 /* g = x wg^T, u = x wu^T, h [T, F] = act(g) * u from the unrounded g and u, and
- * g and u kept as `keep` says: rows ldk elements apart (a multiple of 32; whole
- * groups of 32 columns of 8-bit values are written), their scale tiles for
- * SFFN_KEEP_8.  x [T, D], wg and wu [F, D]; every matrix 16-byte aligned with
+ * g and u kept as `keep` says: rows ldk elements apart (a multiple of 16 bytes),
+ * their scale tiles for SFFN_KEEP_8 (bytes of padding are not written).  x [T, D], wg and wu [F, D]; every matrix 16-byte aligned with
  * row strides of a multiple of 8 elements; dtype SFFN_BF16 or SFFN_F16. */
 int sffn_glu_up(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
                 int64_t ldwu, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, int keep, void* g, void* u,
