@@ -10,11 +10,13 @@
 //
 // CTA pairs, persistent over 256 x 256 tiles; each CTA loads its 128 rows of A
 // and of B (128 bytes of K a stage), its A scale tile and the two of B.
-//   warps 0-5    TMA issuers, one per (A / B / scales, even / odd k-block): one
-//                thread's copies complete one after another
-//   warp 6       MMA issuer (leader): three tcgen05.cp bring the stage's scales
-//                to tensor memory, four tcgen05.mma follow
-//   warp 7       allocates tensor memory
+//   warps 0-5    TMA issuers of A and B, three each for every third k-block: one
+//                thread's copies complete one after another, about one per trip to
+//                L2, and a stage is multiplied in half of such a trip
+//   warp 6       MMA issuer (leader): at every fourth k-block three tcgen05.cp bring
+//                the next four's scales to tensor memory; four tcgen05.mma a stage
+//   warp 7       allocates tensor memory and issues the copies of the scales, two for
+//                four k-blocks
 //   warps 8-15   epilogue, two warpgroups of 128 columns.  The accumulator takes
 //                256 of 512 columns and the scales need some, so there is one:
 //                the epilogue frees it fast, as 16-bit pairs in 128 spare
@@ -33,7 +35,8 @@
 namespace sffn {
 namespace {
 
-constexpr int X_STAGES = 6;  // even: the issuers take alternate k-blocks
+constexpr int X_ISSUERS = 3;  // of each operand
+constexpr int X_STAGES = 6;   // a multiple: a stage belongs to one issuer
 constexpr int X_THREADS = 512;
 constexpr int X_OPERAND = 128 * 128;             // bytes of one operand a stage and CTA
 constexpr int X_STAGE = 2 * X_OPERAND;
@@ -68,6 +71,14 @@ __device__ __forceinline__ void mma_mx_pair(uint32_t d, uint64_t ad, uint64_t bd
         "setp.ne.b32 p, %6, 0;\n\t"
         "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
         "l"(ad), "l"(bd), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+// A 3-D box for a CTA pair, completing on the leader's barrier.
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const void* tmap, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(leader_smem_addr(bar))
         : "memory");
 }
 // 32 rows of 16 bytes -> 4 tensor-memory columns, the same in each quarter of
@@ -123,24 +134,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
     tc_fence_after();
     const uint32_t tmem_base = s_tmem;
 
-    if (warp < 6) {
+    if (warp < 6 || warp == 7) {
         // ------------------------------------------------------ producers --
-        const int op = warp % 3;   // 0: A, 1: B, 2: scales
-        const int par = warp / 3;  // even / odd k-blocks
+        const int op = warp == 7 ? 2 : warp / X_ISSUERS;  // 0: A, 1: B, 2: scales
         if (lane == 0) {
             int armed[X_STAGES] = {0};
             long long kc = 0;
+            int sgroup = 0;  // groups of up to four k-blocks with one tile of scales so far
             bool stop = false;
             for (int tile = first_tile; tile < ntiles && !stop && !s_abort; tile += tile_stride) {
                 int pm, tn;
                 pair_raster(tile, tiles_mp, args.tiles_n, pm, tn);
                 const int arow = (pm * 2 + (int)rank) * 128;
                 const int brow = tn * 256 + (int)rank * 128;
-                // tiles past the end take the last one's scales: their rows' values are zero
-                const int ta = min(pm * 2 + (int)rank, args.tiles_m - 1);
-                const int tb0 = min(tn * 2, args.tiles_b - 1), tb1 = min(tn * 2 + 1, args.tiles_b - 1);
                 for (int kb = 0; kb < nkb; ++kb, ++kc) {
-                    if ((int)(kc & 1) != par) continue;
+                    if (op == 2 ? (kb & 3) != 0 : (int)(kc % X_ISSUERS) != warp % X_ISSUERS) continue;
                     const int stage = (int)(kc % X_STAGES);
                     const uint32_t phase = (uint32_t)((kc / X_STAGES) & 1);
                     if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u)) {
@@ -152,18 +160,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
                     unsigned char* sa = smem + stage * X_STAGE;
                     if (op == 0) {
                         if (leader) {
-                            mbar_arrive_expect_tx(&full_bar[stage], 2 * (X_STAGE + X_SCALES));
+                            mbar_arrive_expect_tx(&full_bar[stage], 2 * (X_STAGE + ((kb & 3) == 0 ? X_SCALES : 0)));
                             ++armed[stage];
                         }
                         tma_load_2d_pair(sa, &tmA, kb * 128, arow, &full_bar[stage]);
                     } else if (op == 1) {
                         tma_load_2d_pair(sa + X_OPERAND, &tmB, kb * 128, brow, &full_bar[stage]);
                     } else {
-                        unsigned char* ss = sscales + stage * X_SCALES;
-                        const int kt = kb >> 2;
-                        tma_load_2d_pair(ss, &tmSA, 0, (ta * args.bt + kt) * 32, &full_bar[stage]);
-                        tma_load_2d_pair(ss + 512, &tmSB, 0, (tb0 * args.bt + kt) * 32, &full_bar[stage]);
-                        tma_load_2d_pair(ss + 1024, &tmSB, 0, (tb1 * args.bt + kt) * 32, &full_bar[stage]);
+                        // Slots are as many as stages and a group has a k-block at
+                        // least: the slot's last group lies a whole ring back, its
+                        // tcgen05.cp before the commit waited for above.
+                        unsigned char* ss = sscales + sgroup * X_SCALES;
+                        tma_load_3d_pair(ss, &tmSA, 0, (kb >> 2) * 32, pm * 2 + (int)rank, &full_bar[stage]);
+                        tma_load_3d_pair(ss + 512, &tmSB, 0, (kb >> 2) * 32, tn * 2, &full_bar[stage]);
+                        sgroup = sgroup + 1 == X_STAGES ? 0 : sgroup + 1;
                     }
                 }
             }
@@ -176,7 +186,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
     } else if (warp == 6) {
         // ----------------------------------------------------------- MMA --
         if (lane == 0 && leader) {
-            int stage = 0, it = 0;
+            int stage = 0, it = 0, sgroup = -1;
             uint32_t phase = 0;
             for (int tile = first_tile; tile < ntiles && !s_abort; tile += tile_stride, ++it) {
                 if (!mbar_wait_bounded(&tempty_bar, ((uint32_t)it & 1u) ^ 1u)) {
@@ -194,12 +204,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
                         break;
                     }
                     const uint32_t sa = smem_u32(smem + stage * X_STAGE), sb = sa + X_OPERAND;
-                    const uint32_t ss = smem_u32(sscales + stage * X_SCALES);
-                    // the stage's own columns: free since the MMAs of its last use
-                    const uint32_t ta = tmem_base + X_SCALE_COL + 12u * (uint32_t)stage, tb = ta + 4u;
-                    cp_scales_pair(ta, smem_desc_rows16(ss));
-                    cp_scales_pair(tb, smem_desc_rows16(ss + 512));
-                    cp_scales_pair(tb + 4u, smem_desc_rows16(ss + 1024));
+                    if ((kb & 3) == 0) sgroup = sgroup + 1 == X_STAGES ? 0 : sgroup + 1;
+                    // the group's own columns, free as its shared memory is
+                    const uint32_t ta = tmem_base + X_SCALE_COL + 12u * (uint32_t)sgroup, tb = ta + 4u;
+                    if ((kb & 3) == 0) {
+                        const uint32_t ss = smem_u32(sscales + sgroup * X_SCALES);
+                        cp_scales_pair(ta, smem_desc_rows16(ss));
+                        cp_scales_pair(tb, smem_desc_rows16(ss + 512));
+                        cp_scales_pair(tb + 4u, smem_desc_rows16(ss + 1024));
+                    }
                     const uint32_t id = (uint32_t)kb & 3u;
                     const uint32_t idesc = IDESC | (id << 4) | (id << 29);
 #pragma unroll
@@ -276,19 +289,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
     }
 }
 
+// Scale tiles [tiles][32 * bt] rows of 16 bytes; boxes of one block tile's 32 rows
+// in `count` row tiles (zeros past the last one, whose values are zero too).
+int scale_map(CUtensorMap* m, const void* p, long long tiles, long long bt, int count) {
+    const auto fn = tmap_encoder();
+    const cuuint64_t dims[3] = {4, (cuuint64_t)(bt * 32), (cuuint64_t)tiles};
+    const cuuint64_t strides[2] = {16, (cuuint64_t)(bt * 512)};
+    const cuuint32_t box[3] = {4, 32, (cuuint32_t)count}, estr[3] = {1, 1, 1};
+    if (!fn || fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(p), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+        set_error_text("cuTensorMapEncodeTiled failed for the scale tiles");
+        return SFFN_ERR_CUDA;
+    }
+    return SFFN_OK;
+}
+
 template <int DT>
 int launch_mm(const void* a, long long lda, const void* as, const void* b, long long ldb, const void* bs, MmArgs args,
               cudaStream_t st) {
     CUtensorMap ta, tb, tsa, tsb, tc;
     memset(&tc, 0, sizeof(tc));
     const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    const auto u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
-    const auto sw = CU_TENSOR_MAP_SWIZZLE_128B, none = CU_TENSOR_MAP_SWIZZLE_NONE;
+    const auto sw = CU_TENSOR_MAP_SWIZZLE_128B;
     if (int rc = tmap_2d(&ta, u8, 1, a, args.K, args.M, lda, 128, 128, sw)) return rc;
     if (int rc = tmap_2d(&tb, u8, 1, b, args.K, args.N, ldb, 128, 128, sw)) return rc;
-    // scale tiles as rows of 16 bytes, 32 rows a tile
-    if (int rc = tmap_2d(&tsa, u32, 4, as, 4, (long long)args.tiles_m * args.bt * 32, 4, 4, 32, none)) return rc;
-    if (int rc = tmap_2d(&tsb, u32, 4, bs, 4, (long long)args.tiles_b * args.bt * 32, 4, 4, 32, none)) return rc;
+    if (int rc = scale_map(&tsa, as, args.tiles_m, args.bt, 1)) return rc;
+    if (int rc = scale_map(&tsb, bs, args.tiles_b, args.bt, 2)) return rc;
     if (args.vec_out)
         if (int rc = tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, args.out, args.N, args.M, args.ldc, 32, 32,
                              CU_TENSOR_MAP_SWIZZLE_64B))

@@ -93,7 +93,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                                                            ~static_cast<uintptr_t>(1023));
     __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST];
     __shared__ __align__(8) uint64_t tfull_bar[2], tempty_bar[2];
-    __shared__ __align__(8) uint64_t kept_bar[8];  // DGRAD: each epilogue warp's g and u have come
+    __shared__ __align__(8) uint64_t kept_bar[8][2];  // DGRAD: each epilogue warp's g and u have come
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_dead;
     __shared__ uint2 s_amax[EPI == P_UP ? 2 : 1][2][128];  // UP: [tile parity][warpgroup][row], of g and u
@@ -130,7 +130,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             mbar_init(&tfull_bar[a], 1);
             mbar_init(&tempty_bar[a], 16);  // the epilogue warps of both CTAs
         }
-        for (int w = 0; w < 8; ++w) mbar_init(&kept_bar[w], 1);
+        for (int w = 0; w < 16; ++w) mbar_init(&kept_bar[w >> 1][w & 1], 1);
         s_abort = s_dead = 0;
         fence_mbar_init();
         prefetch_tmap(&tmA);
@@ -261,21 +261,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         unsigned char* sbuf = smem + NST * P_STAGE + (warp - 4) * (p_bufs<EPI>() * 2048);
         StageRing<p_bufs<EPI>()> ring(sbuf);
         const uint32_t tempty_leader[2] = {leader_smem_addr(&tempty_bar[0]), leader_smem_addr(&tempty_bar[1])};
-        // DGRAD: 32 columns of g and u as kept come by TMA, 32 ahead (each lane's own
-        // loads, of 32 rows an instruction, took half of the kernel's time)
+        // DGRAD: 32 columns of g and u as kept come by TMA, one such chunk ahead in 16
+        // bits and two in 8, across tiles (each lane's own loads, of 32 rows an
+        // instruction, took half of the kernel's time)
         unsigned char* kept = smem + NST * P_STAGE + 8 * (p_bufs<EPI>() * 2048) + (warp - 4) * P_KEPT;
-        uint64_t* kbar = &kept_bar[warp - 4];
+        uint64_t* kbar = kept_bar[warp - 4];
+        const int slots = args.keep == KEEP_8 ? 2 : 1;
         const uint32_t kept_bytes = args.keep == KEEP_8 ? 1024u : 2048u;  // of one matrix
-        uint32_t kept_phase = 0;
-        auto fetch_kept = [&](int col, int row0) {  // the last ones are in registers
+        int f_task = first_task, f_chunk = 0, k_slot = 0;  // the next chunk to fetch; the slot of the next one to read
+        uint32_t k_phase = 0, k_due = 0;                   // a bit a slot: its phase; a fetch is under way
+        auto fetch_kept = [&](int slot) {                  // what the slot held is in registers
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive_expect_tx(kbar, 2 * kept_bytes);
-                tma_load_2d(kept, &tmG, col, row0, kbar);
-                tma_load_2d(kept + 2048, &tmU, col, row0, kbar);
+            while (f_task < ntasks) {
+                int pm, tn, kb0, kb1;
+                locate(f_task, pm, tn, kb0, kb1);
+                const int row0 = (pm * 2 + (int)rank) * 128 + ew * 32, col = tn * TILE_N + wg * (TILE_N / 2) + f_chunk * 32;
+                if (f_chunk < 4 && row0 < args.M && col < args.N) {
+                    if (lane == 0) {
+                        unsigned char* to = kept + slot * 2048;
+                        mbar_arrive_expect_tx(&kbar[slot], 2 * kept_bytes);
+                        tma_load_2d(to, &tmG, col, row0, &kbar[slot]);
+                        tma_load_2d(to + kept_bytes, &tmU, col, row0, &kbar[slot]);
+                    }
+                    k_due |= 1u << slot;
+                    ++f_chunk;
+                    return;
+                }
+                f_task += task_stride;
+                f_chunk = 0;
             }
         };
-        bool kept_due = false;  // a fetch is under way
+        if constexpr (EPI == P_DGRAD)
+            for (int i = 0; i < slots; ++i) fetch_kept(i);
         int acc = 0, it = 0;
         uint32_t acc_phase = 0;
         for (int task = first_task; task < ntasks; task += task_stride, ++it) {
@@ -290,10 +307,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                 if (args.keep == KEEP_8 && row_ok && gcol0 < args.N) {
                     const long long at = fp8_scale_at(row, gcol0 >> 7, args.bt);
                     scales_ahead = make_float2(fp8_scale(args.gs[at]), fp8_scale(args.us[at]));
-                }
-                if (row0 < args.M && gcol0 < args.N) {
-                    fetch_kept(gcol0, row0);
-                    kept_due = true;
                 }
             }
             const bool ok = __all_sync(FULL, mbar_wait_bounded(&tfull_bar[acc], acc_phase));
@@ -428,36 +441,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                 for (int c = 0; c < 4; ++c) {
                     const int col = gcol0 + c * 32;
                     if (row0 >= args.M || col >= args.N) break;
-                    if (!__all_sync(FULL, mbar_wait_bounded(kbar, kept_phase))) {
+                    if (!__all_sync(FULL, mbar_wait_bounded(&kbar[k_slot], (k_phase >> k_slot) & 1u))) {
                         if (lane == 0) atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
                         dead = true;
                         break;
                     }
-                    kept_phase ^= 1u;
-                    kept_due = false;
+                    k_phase ^= 1u << k_slot;
+                    k_due &= ~(1u << k_slot);
                     uint32_t gw[16], uw[16];  // this row's: 16-bit pairs, or 8 words of four bytes
                     if (args.keep == KEEP_8) {
+                        const unsigned char* at = kept + k_slot * 2048 + lane * 32;
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const uint4 a = *reinterpret_cast<const uint4*>(kept + lane * 32 + 16 * i);
-                            const uint4 b = *reinterpret_cast<const uint4*>(kept + 2048 + lane * 32 + 16 * i);
+                            const uint4 a = *reinterpret_cast<const uint4*>(at + 16 * i);
+                            const uint4 b = *reinterpret_cast<const uint4*>(at + 1024 + 16 * i);
                             gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
                             uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
                         }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int at = lane * 64 + 16 * (i ^ ((lane >> 1) & 3));
-                            const uint4 a = *reinterpret_cast<const uint4*>(kept + at);
-                            const uint4 b = *reinterpret_cast<const uint4*>(kept + 2048 + at);
+                            const unsigned char* at = kept + lane * 64 + 16 * (i ^ ((lane >> 1) & 3));
+                            const uint4 a = *reinterpret_cast<const uint4*>(at);
+                            const uint4 b = *reinterpret_cast<const uint4*>(at + 2048);
                             gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
                             uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
                         }
                     }
-                    if (c < 3 && col + 32 < args.N) {
-                        fetch_kept(col + 32, row0);
-                        kept_due = true;
-                    }
+                    fetch_kept(k_slot);
+                    k_slot = slots == 2 ? k_slot ^ 1 : 0;
                     uint32_t r[32], wg_[16], wu_[16], wh_[16];
                     tmem_ld32(tbase + c * 32, r);
                     tmem_wait_ld();
@@ -510,7 +522,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                 acc_phase ^= 1u;
             }
         }
-        if (EPI == P_DGRAD && kept_due) (void)mbar_wait_bounded(kbar, kept_phase);  // left early: it has landed
+        if constexpr (EPI == P_DGRAD)  // left early: what is under way lands first
+            for (int i = 0; i < 2; ++i)
+                if ((k_due >> i) & 1u) (void)mbar_wait_bounded(&kbar[i], (k_phase >> i) & 1u);
         if (lane == 0) bulk_wait_group0();
         __syncwarp();
     }
