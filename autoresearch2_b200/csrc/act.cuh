@@ -7,31 +7,87 @@ namespace sffn {
 
 enum { GLU_RELU = 0, GLU_RELU2 = 1, GLU_SILU = 2, GLU_GELU = 3 };
 
-// act(g) and act'(g).  SiLU: s = 1 / (1 + exp(-g)), the hardware's exp2 and
-// reciprocal (a few 2^-22 of the value: below a twentieth of a 16-bit
-// rounding).  GELU is the exact one; erfc keeps its relative precision where
-// 1 + erf would cancel.
+// Two float32 values, for the packed instructions: half the issue slots, which
+// bound the fused epilogues (35 instructions an element before).
+using Float2 = unsigned long long;
+__device__ __forceinline__ Float2 join2(float lo, float hi) {
+    Float2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 split2(Float2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ Float2 pair_mul(Float2 a, Float2 b) {
+    Float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Float2 pair_add(Float2 a, Float2 b) {
+    Float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Float2 pair_fma(Float2 a, Float2 b, Float2 c) {
+    Float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float exp2_approx(float x) {  // 2^x within 2 ulp; subnormals are 0
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {  // 1 / x within 1 ulp
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// act(g) and act'(g) of two elements.  SiLU: s = 1 / (1 + 2^(-g log2 e)) by the
+// hardware's exp2 and reciprocal, within 2^-21 max(|g|, 1) of the value: below a
+// twentieth of a 16-bit rounding.  GELU is the exact one; erfc keeps its relative
+// precision where 1 + erf would cancel.
 template <int ACT, bool GRAD>
-__device__ __forceinline__ float glu_act(float g, float& d) {
+__device__ __forceinline__ Float2 glu_act2(Float2 g, Float2& d) {
     if constexpr (ACT == GLU_SILU) {
-        const float s = __fdividef(1.f, 1.f + __expf(-g));
-        const float a = g * s;
-        if constexpr (GRAD) d = fmaf(a, 1.f - s, s);
+        const float2 t = split2(pair_mul(g, join2(-1.4426950408889634f, -1.4426950408889634f)));
+        const float2 e = split2(pair_add(join2(exp2_approx(t.x), exp2_approx(t.y)), join2(1.f, 1.f)));
+        const Float2 s = join2(rcp_approx(e.x), rcp_approx(e.y));
+        const Float2 a = pair_mul(g, s);
+        if constexpr (GRAD) d = pair_fma(a, pair_fma(s, join2(-1.f, -1.f), join2(1.f, 1.f)), s);
         return a;
-    } else if constexpr (ACT == GLU_GELU) {
-        const float c = 0.5f * erfcf(-0.70710678118654752f * g);
-        if constexpr (GRAD) d = fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), c);
-        return g * c;
     } else {
-        const float r = g > 0.f || g != g ? g : 0.f;  // NaN stays
-        if constexpr (ACT == GLU_RELU) {
-            if constexpr (GRAD) d = g > 0.f ? 1.f : g != g ? g : 0.f;
-            return r;
-        } else {
-            if constexpr (GRAD) d = 2.f * r;
-            return r * r;
-        }
+        const float2 v = split2(g);
+        float2 a, dd = make_float2(0.f, 0.f);
+        auto one = [](float x, float& dx) {
+            if constexpr (ACT == GLU_GELU) {
+                const float c = 0.5f * erfcf(-0.70710678118654752f * x);
+                if constexpr (GRAD) dx = fmaf(x * 0.39894228040143268f, __expf(-0.5f * x * x), c);
+                return x * c;
+            } else {
+                const float r = x > 0.f || x != x ? x : 0.f;  // NaN stays
+                if constexpr (ACT == GLU_RELU) {
+                    if constexpr (GRAD) dx = x > 0.f ? 1.f : x != x ? x : 0.f;
+                    return r;
+                } else {
+                    if constexpr (GRAD) dx = 2.f * r;
+                    return r * r;
+                }
+            }
+        };
+        a.x = one(v.x, dd.x);
+        a.y = one(v.y, dd.y);
+        if constexpr (GRAD) d = join2(dd.x, dd.y);
+        return join2(a.x, a.y);
     }
+}
+template <int ACT>
+__device__ __forceinline__ float glu_act(float g) {
+    Float2 unused;
+    return split2(glu_act2<ACT, false>(join2(g, g), unused)).x;
 }
 
 }  // namespace sffn

@@ -191,8 +191,8 @@ __global__ void __launch_bounds__(S_THREADS, 1)
                     sum[m] = v[0];
                 }
                 if (r < rows) {
-                    float v = sum[0], unused;
-                    if constexpr (MODE == S_GATED) v = glu_act<ACT, false>(sum[0], unused) * sum[1];
+                    float v = sum[0];
+                    if constexpr (MODE == S_GATED) v = glu_act<ACT>(sum[0]) * sum[1];
                     a.out[(long long)t * a.ldo + n0 + r] = Elt<OT>::from_f(v);
                 }
             }

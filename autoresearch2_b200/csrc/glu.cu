@@ -77,6 +77,13 @@ __device__ constexpr uint32_t idesc16(bool a_mn, bool b_mn) {
            ((uint32_t)(256 >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
 }
 
+// Four scaled values as four e4m3 bytes.
+__device__ __forceinline__ uint32_t fp8_four(Float2 lo, Float2 hi) {
+    const float2 a = split2(lo), b = split2(hi);
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
+           ((uint32_t)__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3) << 16);
+}
+
 template <int DT, bool A_MN, bool B_MN, int EPI, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -354,7 +361,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     else stage_store_plain(args.out, args.ldc, args.M, args.N, sbuf, lane, w, col, row0);
                 }
             } else if constexpr (EPI == P_UP) {
-                uint32_t gmax = 0, umax = 0;
+                float gtop = 0.f, utop = 0.f;
                 const bool warp_live = row0 < args.M;
 #pragma unroll 1
                 for (int c = 0; c < 2; ++c) {
@@ -364,12 +371,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     tmem_ld32(tbase + c * 32, g);
                     tmem_ld32(tbase + 128 + c * 32, u);
                     tmem_wait_ld();
-                    float unused;
 #pragma unroll
-                    for (int q = 0; q < 16; ++q)
-                        w[q] = pack16x2<DT>(glu_act<ACT, false>(__uint_as_float(g[2 * q]), unused) * __uint_as_float(u[2 * q]),
-                                            glu_act<ACT, false>(__uint_as_float(g[2 * q + 1]), unused) *
-                                                __uint_as_float(u[2 * q + 1]));
+                    for (int q = 0; q < 16; ++q) {
+                        Float2 unused;
+                        const Float2 gp = join2(__uint_as_float(g[2 * q]), __uint_as_float(g[2 * q + 1]));
+                        const Float2 up = join2(__uint_as_float(u[2 * q]), __uint_as_float(u[2 * q + 1]));
+                        const float2 h = split2(pair_mul(glu_act2<ACT, false>(gp, unused), up));
+                        w[q] = pack16x2<DT>(h.x, h.y);
+                    }
                     ring.store(&tmC, lane, w, col, row0);
                     if (args.keep == KEEP_16) {
 #pragma unroll
@@ -381,13 +390,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     } else if (args.keep == KEEP_8) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            gmax = max(gmax, g[j] & 0x7FFFFFFFu);
-                            umax = max(umax, u[j] & 0x7FFFFFFFu);
+                            gtop = fmaxf(gtop, fabsf(__uint_as_float(g[j])));  // NaN does not count
+                            utop = fmaxf(utop, fabsf(__uint_as_float(u[j])));
                         }
                     }
                 }
                 if (args.keep == KEEP_8) {
-                    // rare: infinities and NaN do not count
+                    uint32_t gmax = __float_as_uint(gtop), umax = __float_as_uint(utop);
+                    // rare: infinities do not count either
                     const bool finite = !__any_sync(FULL, max(gmax, umax) >= 0x7F800000u);
                     if (!finite) {
                         gmax = umax = 0;
@@ -429,7 +439,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                             for (int q = 0; q < 8; ++q) {
                                 const float v0 = __uint_as_float(r[4 * q]), v1 = __uint_as_float(r[4 * q + 1]);
                                 const float v2 = __uint_as_float(r[4 * q + 2]), v3 = __uint_as_float(r[4 * q + 3]);
-                                w[c * 8 + q] = finite ? fp8_pack4<true>(v0, v1, v2, v3, inv) : fp8_pack4<false>(v0, v1, v2, v3, inv);
+                                if (finite) {
+                                    const Float2 s2 = join2(inv, inv);
+                                    w[c * 8 + q] = fp8_four(pair_mul(join2(v0, v1), s2), pair_mul(join2(v2, v3), s2));
+                                } else {
+                                    w[c * 8 + q] = fp8_pack4<false>(v0, v1, v2, v3, inv);
+                                }
                             }
                         }
                         ring.store(m ? &tmU : &tmG, lane, w, gcol0, row0);
@@ -473,38 +488,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     uint32_t r[32], wg_[16], wu_[16], wh_[16];
                     tmem_ld32(tbase + c * 32, r);
                     tmem_wait_ld();
-                    auto quad = [&](int q, const float (&g)[4], const float (&u)[4]) {  // elements 4q .. 4q + 3
-                        float dg[4], du[4], h[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float dh = __uint_as_float(r[4 * q + j]);
-                            float d;
-                            const float a = glu_act<ACT, true>(g[j], d);
-                            dg[j] = dh * u[j] * d;
-                            du[j] = dh * a;
-                            h[j] = a * u[j];
-                        }
-                        wg_[2 * q] = pack16x2<DT>(dg[0], dg[1]), wg_[2 * q + 1] = pack16x2<DT>(dg[2], dg[3]);
-                        wu_[2 * q] = pack16x2<DT>(du[0], du[1]), wu_[2 * q + 1] = pack16x2<DT>(du[2], du[3]);
-                        wh_[2 * q] = pack16x2<DT>(h[0], h[1]), wh_[2 * q + 1] = pack16x2<DT>(h[2], h[3]);
+                    auto two = [&](int q, Float2 g, Float2 u) {  // elements 2q, 2q + 1
+                        Float2 d;
+                        const Float2 dh = join2(__uint_as_float(r[2 * q]), __uint_as_float(r[2 * q + 1]));
+                        const Float2 a = glu_act2<ACT, true>(g, d);
+                        const float2 dg = split2(pair_mul(pair_mul(dh, u), d)), du = split2(pair_mul(dh, a));
+                        const float2 h = split2(pair_mul(a, u));
+                        wg_[q] = pack16x2<DT>(dg.x, dg.y);
+                        wu_[q] = pack16x2<DT>(du.x, du.y);
+                        wh_[q] = pack16x2<DT>(h.x, h.y);
                     };
                     if (args.keep == KEEP_8) {
+                        const Float2 gs2 = join2(gscale, gscale), us2 = join2(uscale, uscale);
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) {
-                            float g[4], u[4];
-                            fp8_unpack4(gw[q], g);
-                            fp8_unpack4(uw[q], u);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) g[j] *= gscale, u[j] *= uscale;
-                            quad(q, g, u);
+                        for (int q = 0; q < 16; ++q) {
+                            const uint32_t sh = 16 * (q & 1);
+                            const float2 g = __half22float2(fp8_half2(gw[q >> 1] >> sh)), u = __half22float2(fp8_half2(uw[q >> 1] >> sh));
+                            two(q, pair_mul(join2(g.x, g.y), gs2), pair_mul(join2(u.x, u.y), us2));
                         }
                     } else {
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) {
-                            const float2 g0 = unpack16x2<DT>(gw[2 * q]), g1 = unpack16x2<DT>(gw[2 * q + 1]);
-                            const float2 u0 = unpack16x2<DT>(uw[2 * q]), u1 = unpack16x2<DT>(uw[2 * q + 1]);
-                            const float g[4] = {g0.x, g0.y, g1.x, g1.y}, u[4] = {u0.x, u0.y, u1.x, u1.y};
-                            quad(q, g, u);
+                        for (int q = 0; q < 16; ++q) {
+                            const float2 g = unpack16x2<DT>(gw[q]), u = unpack16x2<DT>(uw[q]);
+                            two(q, join2(g.x, g.y), join2(u.x, u.y));
                         }
                     }
                     ring.store(&tmC, lane, wg_, col, row0);
