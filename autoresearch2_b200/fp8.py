@@ -386,7 +386,7 @@ def ckpt_linear(x, W):
     gradient is dy^T times the kept x.  Differentiable once, in reverse mode."""
     _check_linear(x, W)
     if torch.compiler.is_compiling():
-        return torch.ops.sparseffn.ckpt_linear(x, W)[0]
+        return torch.ops.sparseffn.ckpt_linear(x, W, torch.is_grad_enabled() and W.requires_grad)[0]
     if _lib.tracked(x, W):
         return _CkptLinear.apply(x, W)
     return _linear_forward(x, W, False)[0]

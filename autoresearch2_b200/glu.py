@@ -73,8 +73,9 @@ def _forward(x, Wg, Wu, W2, act, keep):
     return y if x.dim() == 2 else y.view(x.shape), g, u, gt, ut, xv, xt
 
 
-def _backward(dy, x, Wg, Wu, W2, g, u, gt, ut, xv, xt, act, want):
-    """Gradients of (x, Wg, Wu, W2); None where `want` is false.  x is None with 8-bit checkpoints."""
+def _backward(dy, x, Wg, Wu, W2, g, u, gt, ut, xv, xt, act, want, apart=False):
+    """Gradients of (x, Wg, Wu, W2); None where `want` is false.  x is None with 8-bit
+    checkpoints.  apart: dWg and dWu do not share their storage."""
     _lib.bind_thread(dy.device)
     dy2, Wg, Wu, W2 = fp8._rows(dy), fp8._rows(Wg), fp8._rows(Wu), fp8._rows(W2)
     T, D = dy2.shape
@@ -102,19 +103,32 @@ def _backward(dy, x, Wg, Wu, W2, g, u, gt, ut, xv, xt, act, want):
             xk = fp8._unpack(xv, xt, fp8._empty_rows(dy2, T, D, 8), D), (D + 7) // 8 * 8
         else:
             xk, = fp8._align(fp8._rows(x))
-        if want[1] and want[2]:
+        if want[1] and want[2] and not apart:
             dW = fp8._mm_into(dy2.new_empty((2 * ld, D)), (d, 2 * ld), 1, xk, 1)
-            dWg, dWu = dW[:F], dW[ld:ld + F]
-        elif want[1]:
-            dWg = fp8._mm_into(dy2.new_empty((F, D)), dg, 1, xk, 1)
+            dWg, dWu = submit_grad(dW[:F]), submit_grad(dW[ld:ld + F])
         else:
-            dWu = fp8._mm_into(dy2.new_empty((F, D)), du, 1, xk, 1)
-        submit_grad(dWg)
-        submit_grad(dWu)
+            dWg = submit_grad(fp8._mm_into(dy2.new_empty((F, D)), dg, 1, xk, 1)) if want[1] else None
+            dWu = submit_grad(fp8._mm_into(dy2.new_empty((F, D)), du, 1, xk, 1)) if want[2] else None
         del xk
     if want[0]:
         dx = fp8._mm_into(dy2.new_empty((T, D)), dg, 0, ga, 1, (du, ua)).view(dy.shape)
     return dx, dWg, dWu, dW2
+
+
+def _check_kept(dy, x, F, g, u, gt, ut, xv, xt):
+    """The backward op's: what it is given is what a forward keeps."""
+    rows, D = dy.numel() // dy.shape[-1], dy.shape[-1]
+    if x is not None:
+        ok = x.shape == dy.shape and x.dtype == dy.dtype and x.device == dy.device and all(
+            t.shape == (rows, F) and t.dtype == dy.dtype and t.device == dy.device and t.data_ptr() % 16 == 0
+            and (rows <= 1 or t.stride() == (_kept_ld(F, 1), 1)) for t in (g, u))
+    else:
+        ok = True
+        for v, t, width in ((g, gt, F), (u, ut, F), (xv, xt, D)):
+            fp8.Fp8Tensor(v, t)
+            ok = ok and v.shape == (rows, width) and v.device == dy.device and (rows <= 1 or v.stride(0) == _kept_ld(width, 2))
+    if not ok:
+        raise ValueError("x, g and u are not as the forward kept them")
 
 
 class _GatedFFN(torch.autograd.Function):

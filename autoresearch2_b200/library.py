@@ -36,6 +36,14 @@ outputs' shapes and dtypes, so tracing needs no device.
         reference), with their autograd formulas over the ops named *_bwd;
         their functions call these ops while torch.compile traces.  Outputs
         that a call leaves out are empty tensors here.
+    sparseffn::fp8_pack(x) -> (values, scale_tiles)
+    sparseffn::fp8_unpack(values, scale_tiles, shape, dtype) -> x
+    sparseffn::fp8_matmul(a_values, a_tiles, b_values, b_tiles, out_dtype) -> a b^T
+    sparseffn::ckpt_linear(x, W, keep) -> (y, values, tiles)
+    sparseffn::gated_ffn(x, Wg, Wu, W2, act, keep)
+        -> (y, g, u, g_tiles, u_tiles, x_values, x_tiles)
+        the 8-bit blocks (fp8.py) and the gated block (glu.py), without
+        counterpart in the reference, the last two with autograd formulas
 
 The fused bf16 path (ffn._fused_ok, decided from dtypes, contiguity and
 shapes alone) keeps z in 128x128 tiles and returns per-row value offsets and
@@ -49,13 +57,14 @@ from torch import Tensor
 
 from . import bitshift
 from . import bitsparse as bs
-from . import ffn, logits, norms
+from . import ffn, fp8, glu, logits, norms
 
 __all__ = ["OPS"]
 
 OPS = ("bitsparse_pack", "bitsparse_unpack", "tile_pack", "tile_unpack", "ffn_fwd", "ffn_bwd",
        "codec15_compress", "codec15_uncompress", "token_logprobs", "token_logprobs_bwd", "distill_topk",
-       "distill_topk_bwd", "residual_norm", "residual_norm_bwd")
+       "distill_topk_bwd", "residual_norm", "residual_norm_bwd", "fp8_pack", "fp8_unpack", "fp8_matmul", "ckpt_linear",
+       "ckpt_linear_bwd", "gated_ffn", "gated_ffn_bwd")
 
 
 def _cdiv(a, b):
@@ -350,3 +359,160 @@ def _norm_bwd(ctx, dx_new, dh, _stats):
 
 
 residual_norm.register_autograd(_norm_bwd, setup_context=_norm_setup)
+
+
+# ---------------------------------------------------------------------------
+# 8-bit blocks
+# ---------------------------------------------------------------------------
+def _rows_of(x):
+    return x.numel() // x.shape[-1]
+
+
+def _fake_values(x, rows, width):
+    ld = _cdiv(width, 16) * 16
+    return x.new_empty_strided((rows, width), (ld, 1), dtype=fp8.E4M3)
+
+
+def _fake_tiles(x, rows, width):
+    return x.new_empty(fp8._tile_shape(rows, width), dtype=torch.uint8)
+
+
+def _check_blocks(values, tiles):
+    fp8.Fp8Tensor(values, tiles)  # refuses what does not fit
+
+
+@torch.library.custom_op("sparseffn::fp8_pack", mutates_args=())
+def fp8_pack(x: Tensor) -> tuple[Tensor, Tensor]:
+    fp8._check_pack(x)
+    return fp8._pack(x)
+
+
+@fp8_pack.register_fake
+def _(x):
+    return _fake_values(x, _rows_of(x), x.shape[-1]), _fake_tiles(x, _rows_of(x), x.shape[-1])
+
+
+@torch.library.custom_op("sparseffn::fp8_unpack", mutates_args=())
+def fp8_unpack(values: Tensor, tiles: Tensor, shape: list[int], dtype: torch.dtype) -> Tensor:
+    return fp8.fp8_unpack(fp8.Fp8Tensor(values, tiles, shape), dtype)
+
+
+@fp8_unpack.register_fake
+def _(values, tiles, shape, dtype):
+    return values.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("sparseffn::fp8_matmul", mutates_args=())
+def fp8_matmul(av: Tensor, at: Tensor, bv: Tensor, bt: Tensor, out_dtype: torch.dtype) -> Tensor:
+    _check_blocks(av, at)
+    _check_blocks(bv, bt)
+    fp8._check_product(av, bv, out_dtype)
+    return fp8._matmul(av, at, bv, bt, out_dtype)
+
+
+@fp8_matmul.register_fake
+def _(av, at, bv, bt, out_dtype):
+    return av.new_empty((av.shape[0], bv.shape[0]), dtype=out_dtype)
+
+
+@torch.library.custom_op("sparseffn::ckpt_linear", mutates_args=())
+def ckpt_linear(x: Tensor, W: Tensor, keep: bool) -> tuple[Tensor, Tensor, Tensor]:
+    fp8._check_linear(x, W)
+    return _or_empty(x, fp8._linear_forward(x, W, keep))
+
+
+@ckpt_linear.register_fake
+def _(x, W, keep):
+    rows, width = _rows_of(x), x.shape[-1]
+    kept = (_fake_values(x, rows, width), _fake_tiles(x, rows, width)) if keep else (x.new_empty(0), x.new_empty(0))
+    return (x.new_empty((*x.shape[:-1], W.shape[0])), *kept)
+
+
+@torch.library.custom_op("sparseffn::ckpt_linear_bwd", mutates_args=())
+def ckpt_linear_bwd(dy: Tensor, W: Tensor, values: Tensor, tiles: Tensor, x_shape: list[int], want_x: bool,
+                    want_W: bool) -> tuple[Tensor, Tensor]:
+    if tuple(dy.shape) != (*x_shape[:-1], W.shape[0]):
+        raise ValueError(f"dy must be {(*x_shape[:-1], W.shape[0])}, got {tuple(dy.shape)}")
+    fp8._check_weights(dy, W=(W, (dy.shape[-1], x_shape[-1])))
+    if want_W:
+        _check_blocks(values, tiles)
+        if values.shape != (dy.numel() // dy.shape[-1], x_shape[-1]) or values.device != dy.device:
+            raise ValueError("values are not the forward's")
+    return _or_empty(dy, fp8._linear_backward(dy, W, values, tiles, torch.Size(x_shape), want_x, want_W))
+
+
+@ckpt_linear_bwd.register_fake
+def _(dy, W, values, tiles, x_shape, want_x, want_W):
+    return dy.new_empty(x_shape if want_x else (0,)), W.new_empty(W.shape if want_W else (0,))
+
+
+def _linear_setup(ctx, inputs, output):
+    x, W, keep = inputs
+    ctx.save_for_backward(W, output[1], output[2])
+    ctx.x_shape, ctx.keep = x.shape, keep
+    ctx.mark_non_differentiable(output[1], output[2])
+    ctx.set_materialize_grads(False)
+
+
+def _linear_bwd(ctx, dy, _values, _tiles):
+    want_x, want_W = ctx.needs_input_grad[:2]
+    dx, dW = ckpt_linear_bwd(dy, *ctx.saved_tensors, list(ctx.x_shape), want_x, want_W)
+    return dx if want_x else None, dW if want_W else None, None
+
+
+ckpt_linear.register_autograd(_linear_bwd, setup_context=_linear_setup)
+
+
+# ---------------------------------------------------------------------------
+# Gated feed-forward block
+# ---------------------------------------------------------------------------
+@torch.library.custom_op("sparseffn::gated_ffn", mutates_args=())
+def gated_ffn(x: Tensor, Wg: Tensor, Wu: Tensor, W2: Tensor, act: int,
+              keep: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    glu._check(x, Wg, Wu, W2)
+    return _or_empty(x, glu._forward(x, Wg, Wu, W2, act, keep))
+
+
+@gated_ffn.register_fake
+def _(x, Wg, Wu, W2, act, keep):
+    rows, D, F = _rows_of(x), x.shape[-1], Wg.shape[0]
+    none = [x.new_empty(0) for _ in range(6)]
+    if keep == 1:
+        ld = _cdiv(F, 8) * 8
+        none[:2] = [x.new_empty_strided((rows, F), (ld, 1)) for _ in range(2)]
+    elif keep == 2:
+        none = [_fake_values(x, rows, F), _fake_values(x, rows, F), _fake_tiles(x, rows, F), _fake_tiles(x, rows, F),
+                _fake_values(x, rows, D), _fake_tiles(x, rows, D)]
+    return (x.new_empty(x.shape), *none)
+
+
+@torch.library.custom_op("sparseffn::gated_ffn_bwd", mutates_args=())
+def gated_ffn_bwd(dy: Tensor, x: Optional[Tensor], Wg: Tensor, Wu: Tensor, W2: Tensor, g: Tensor, u: Tensor, gt: Tensor,
+                  ut: Tensor, xv: Tensor, xt: Tensor, act: int,
+                  want: list[bool]) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    glu._check(dy, Wg, Wu, W2)
+    glu._check_kept(dy, x, Wg.shape[0], g, u, gt, ut, xv, xt)
+    kept = (g, u, gt, ut, xv, xt) if x is None else (g, u, None, None, None, None)
+    return _or_empty(dy, glu._backward(dy, x, Wg, Wu, W2, *kept, act, want, apart=True))
+
+
+@gated_ffn_bwd.register_fake
+def _(dy, x, Wg, Wu, W2, g, u, gt, ut, xv, xt, act, want):
+    return tuple(t.new_empty(t.shape if w else (0,)) for t, w in zip((dy, Wg, Wu, W2), want))
+
+
+def _gated_setup(ctx, inputs, output):
+    x, Wg, Wu, W2, act, keep = inputs
+    ctx.save_for_backward(x if keep == 1 else None, Wg, Wu, W2, *output[1:])
+    ctx.act = act
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.set_materialize_grads(False)
+
+
+def _gated_bwd(ctx, dy, *_kept):
+    want = list(ctx.needs_input_grad[:4])
+    grads = gated_ffn_bwd(dy, *ctx.saved_tensors, ctx.act, want)
+    return *(g if w else None for g, w in zip(grads, want)), None, None
+
+
+gated_ffn.register_autograd(_gated_bwd, setup_context=_gated_setup)

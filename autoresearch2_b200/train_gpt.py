@@ -36,6 +36,8 @@ def main(argv=None):
     ap.add_argument("--seq", type=int, default=1024)
     ap.add_argument("--dense", action="store_true", help="dense torch MLPs instead of the sparse FFN")
     ap.add_argument("--sandwich", action="store_true", help="norms and gates after the blocks as well (GPTConfig.sandwich)")
+    ap.add_argument("--gated", default=None, choices=("silu", "gelu", "relu", "relu2"), help="gated MLPs with this activation (GPTConfig.gated)")
+    ap.add_argument("--ckpt8", action="store_true", help="activations for the backward in 8 bits (GPTConfig.ckpt8; with --gated)")
     ap.add_argument("--distill", type=int, default=0, metavar="K",
                     help="train on the K top logits of a frozen dense teacher of the same shape (random weights, another seed)")
     ap.add_argument("--check", action="store_true")
@@ -49,7 +51,7 @@ def main(argv=None):
     if world > 1:
         dist.init_process_group("nccl", timeout=timedelta(seconds=120), device_id=device)
     cfg = GPTConfig(n_layer=args.layers, n_head=args.heads, n_embd=args.width, ffn_hidden=args.hidden,
-                    vocab=args.vocab, seq_len=args.seq, sandwich=args.sandwich)
+                    vocab=args.vocab, seq_len=args.seq, sandwich=args.sandwich, gated=args.gated, ckpt8=args.ckpt8)
     model = GPT(cfg, sparse=not args.dense, device=device)
     net = torch.nn.parallel.DistributedDataParallel(model, device_ids=[local]) if world > 1 else model
     idx, tgt = synthetic_batch(cfg, args.batch, device, seed=rank)
@@ -85,7 +87,8 @@ def main(argv=None):
     bs.check_status(device)
     tokens = world * args.batch * cfg.seq_len
     if rank == 0:
-        print(json.dumps({"harness": "gpt", "mlp": "dense" if args.dense else "sparse_relu2", "n_gpus": world,
+        print(json.dumps({"harness": "gpt", "mlp": ("dense " if args.dense else "") + f"gated_{args.gated}" if args.gated else "dense" if args.dense else "sparse_relu2",
+                          "ckpt8": args.ckpt8, "n_gpus": world,
                           "sandwich": args.sandwich, "distill_top_k": args.distill,
                           "tokens_per_s": round(tokens / (ms / 1e3), 1), "ms_per_step": round(ms, 3),
                           "tokens_per_step": tokens, "flops_per_token": flops_per_token(cfg),
