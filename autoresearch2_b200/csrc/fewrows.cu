@@ -80,17 +80,14 @@ __device__ __forceinline__ uint4 load_piece(const uint8_t* row, long long k, lon
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Byte of the scale tiles of one row, for every block.
-__device__ __forceinline__ uint32_t scale_byte(const uint8_t* s, long long row, int block, int bt) {
-    return __ldg(s + fp8_scale_at(row, block, bt));
-}
-
 // A stage in shared memory: rows of 1 KB, 16 of each matrix, then NT * 8 of x (rows
-// and tokens past the last one hold anything: their sums are not stored).
+// and tokens past the last one hold anything: their sums are not stored); 8-bit
+// operands' scale bytes of its eight blocks, 16 rows' of W and NT * 8 of x.
 constexpr int S_ROW = 1024, S_PIECE = 128;
-template <int MATS, int NT>
+template <bool FP8, int MATS, int NT>
 struct FewStage {
-    static constexpr int BYTES = (MATS * 16 + NT * 8) * S_ROW;
+    static constexpr int SCALES = (MATS * 16 + NT * 8) * S_ROW;  // where these are
+    static constexpr int BYTES = SCALES + (FP8 ? 512 : 0);
     static constexpr int SUMS = S_WARPS * NT * 8 * (MATS * 16 + 1) * 4;
     static constexpr int FIT = (232448 - 1024 - SUMS) / BYTES;
     // An even count: each stage then belongs to one half of the warps, and a warp
@@ -120,7 +117,7 @@ __global__ void __launch_bounds__(S_THREADS, 1)
     constexpr int MATS = MODE == S_GATED ? 2 : 1;
     constexpr int ROWS = MATS * 16;  // rows of sums
     constexpr int ESIZE = FP8 ? 1 : 2;
-    using St = FewStage<MATS, NT>;
+    using St = FewStage<FP8, MATS, NT>;
     constexpr int STAGE = St::BYTES, DEPTH = St::DEPTH;
     extern __shared__ __align__(128) unsigned char few_smem[];
     float* red = reinterpret_cast<float*>(few_smem + (VEC ? DEPTH * STAGE : 0));  // [S_WARPS][NT * 8][ROWS + 1]
@@ -134,7 +131,7 @@ __global__ void __launch_bounds__(S_THREADS, 1)
     const int groups = (a.N + a.per - 1) / a.per;
     if (threadIdx.x == 0) {
         for (int s = 0; s < DEPTH; ++s) {
-            mbar_init(&full_bar[s], 1);
+            mbar_init(&full_bar[s], VEC && FP8 ? 1 + 32 : 1);  // the boxes' bytes; each lane's scales
             mbar_init(&empty_bar[s], S_WARPS / 2);
         }
         mbar_init(&sums_bar, S_WARPS);
@@ -145,25 +142,50 @@ __global__ void __launch_bounds__(S_THREADS, 1)
 
     if (warp == S_WARPS) {
         // -------------------------------------------------------- copies --
-        if (VEC && lane == 0) {
+        if constexpr (VEC) {
             const uint32_t count = (uint32_t)(a.per * MATS + a.T) * S_ROW;  // whole boxes: zeros past the edges
+            // the scales of a stage's eight blocks: lane = half of them of a row of W or of x
+            auto copy_scales = [&](int group, int c, uint32_t to, uint64_t* bar) {
+                const int block = c * 8 + (lane & 1) * 4;
+                if (block < (int)fp8_blocks(a.K)) {
+                    auto copy = [&](const uint8_t* tiles, long long row, int place) {
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + place * 8 + (lane & 1) * 4),
+                                     "l"(tiles + fp8_scale_at(row, block, a.bt))
+                                     : "memory");
+                    };
+                    copy(a.ws, min(group * a.per + (lane >> 1), a.N - 1), lane >> 1);
+#pragma unroll
+                    for (int i = 0; i < (NT + 1) / 2; ++i) {
+                        const int t = i * 16 + (lane >> 1);
+                        if (t < NT * 8) copy(a.xs, min(t, a.T - 1), 16 + t);
+                    }
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+            };
             int stage = 0;
             uint32_t phase = 1;
             for (int group = blockIdx.x; group < groups; group += gridDim.x)
                 for (int c = 0; c < chunks; ++c) {
-                    if (!mbar_wait_bounded(&empty_bar[stage], phase)) {
-                        atomicOr(a.status, SFFN_STATUS_WAIT_TIMEOUT);
+                    if (!__all_sync(FULL, mbar_wait_bounded(&empty_bar[stage], phase))) {
+                        if (lane == 0) atomicOr(a.status, SFFN_STATUS_WAIT_TIMEOUT);
                         // no copy lands after the block has left
                         for (int s = 0; s < DEPTH; ++s) (void)mbar_wait_bounded(&full_bar[s], (s < stage ? phase : phase ^ 1u) ^ 1u);
                         return;
                     }
                     unsigned char* to = few_smem + stage * STAGE;
-                    mbar_arrive_expect_tx(&full_bar[stage], count);
-                    tma_load_2d(to, &tmW, c * (S_ROW / 4), group * a.per, &full_bar[stage]);
-                    if constexpr (MATS == 2) tma_load_2d(to + 16 * S_ROW, &tmW2, c * (S_ROW / 4), group * a.per, &full_bar[stage]);
-                    tma_load_2d(to + ROWS * S_ROW, &tmX, c * (S_ROW / 4), 0, &full_bar[stage]);
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&full_bar[stage], count);
+                        tma_load_2d(to, &tmW, c * (S_ROW / 4), group * a.per, &full_bar[stage]);
+                        if constexpr (MATS == 2) tma_load_2d(to + 16 * S_ROW, &tmW2, c * (S_ROW / 4), group * a.per, &full_bar[stage]);
+                        tma_load_2d(to + ROWS * S_ROW, &tmX, c * (S_ROW / 4), 0, &full_bar[stage]);
+                    }
+                    if constexpr (FP8) {
+                        __syncwarp();
+                        copy_scales(group, c, smem_u32(to + St::SCALES), &full_bar[stage]);
+                    }
                     if (++stage == DEPTH) stage = 0, phase ^= 1u;
                 }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
         return;
     }
@@ -208,27 +230,9 @@ __global__ void __launch_bounds__(S_THREADS, 1)
     for (int t = 0; t < NT; ++t) xrow[t] = static_cast<const uint8_t*>(a.x) + (long long)min(t * 8 + gid, a.T - 1) * a.ldx * ESIZE;
     // row h * 8 + gid of a group (past the group's end: any, its sums are not stored)
     auto row_of = [&](int group, int h) { return (long long)min(group * a.per + h * 8 + gid, a.N - 1); };
-    uint32_t we[2], xe[NT][2];
-    auto fetch_scales = [&](int group, int c) {
-        const int block = c * (S_WARPS / 2) + (warp & 7);
-        if ((long long)block * FP8_BLOCK >= bytes) return;  // not used
-#pragma unroll
-        for (int h = 0; h < 2; ++h) we[h] = scale_byte(a.ws, row_of(group, h), block, a.bt);
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) xe[t][h] = scale_byte(a.xs, min(t * 8 + tig * 2 + h, a.T - 1), block, a.bt);
-    };
     // this warp's stages: every other one of the block's, from warp / 8 on
     int it = 0;
     uint32_t free_phase = 1;  // the first use finds the sums' place free
-    int sg = blockIdx.x, sc = warp >> 3;  // the piece whose scales are loaded
-    auto next_scales = [&] {
-        while (sc >= chunks) sc -= chunks, sg += gridDim.x;
-        if (sg < groups) fetch_scales(sg, sc);
-        sc += 2;
-    };
-    if constexpr (FP8) next_scales();
     for (int group = blockIdx.x; group < groups; group += gridDim.x) {
         float acc[MATS][NT][4];
 #pragma unroll
@@ -309,23 +313,41 @@ __global__ void __launch_bounds__(S_THREADS, 1)
                     }
                 }
                 if constexpr (FP8) {
-                    // one block of 128: the sum of its products times its two scales,
-                    // 2^(ew + ex) in two factors, since one of the scales may leave the
-                    // range of a float where the product of both does not
+                    // one block of 128: the sum of its products times its two scales
+                    int we[2], xe[NT][2];
+                    if constexpr (VEC) {
+                        const unsigned char* at = few_smem + stage * STAGE + St::SCALES + (warp & 7);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) we[h] = at[(h * 8 + gid) * 8];
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) xe[t][h] = at[(16 + t * 8 + tig * 2 + h) * 8];
+                    } else {
+                        const int block = c * (S_WARPS / 2) + (warp & 7);
+                        auto byte = [&](const uint8_t* p, long long row) { return (int)__ldg(p + fp8_scale_at(row, block, a.bt)); };
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) we[h] = byte(a.ws, row_of(group, h));
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) xe[t][h] = byte(a.xs, min(t * 8 + tig * 2 + h, a.T - 1));
+                    }
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int wb = (int)we[j >> 1], xb = (int)xe[t][j & 1];
-                            const int e = wb + xb - 254, e1 = e >> 1;
-                            float s1 = two_to(max(e1, -126));
-                            const float s2 = two_to(max(e - e1, -126));
-                            if (wb == 255 || xb == 255) s1 = __uint_as_float(0x7FFFFFFFu);
-                            acc[0][t][j] += part[t][j] * s1 * s2;
+                            const int wb = we[j >> 1], xb = xe[t][j & 1], e = wb + xb - 127;  // 2^(e - 127)
+                            if (e >= 1 && e <= 254 && max(wb, xb) < 255) {
+                                acc[0][t][j] = fmaf(part[t][j], __uint_as_float((uint32_t)e << 23), acc[0][t][j]);
+                            } else {  // in two factors: the product may be in a float's range all the same
+                                const int f = e - 127, f1 = f >> 1;
+                                const float s1 = max(wb, xb) == 255 ? __uint_as_float(0x7FFFFFFFu) : two_to(max(f1, -126));
+                                acc[0][t][j] += part[t][j] * s1 * two_to(max(f - f1, -126));
+                            }
                         }
                 }
             }
-            if constexpr (FP8) next_scales();
             if constexpr (VEC) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty_bar[stage]);
@@ -353,7 +375,7 @@ template <int DT, int OT, bool FP8, int MODE, int ACT, int NT, bool VEC>
 int launch_few_nt(FewArgs a, cudaStream_t st) {
     auto k = few_rows_kernel<DT, OT, FP8, MODE, ACT, NT, VEC>;
     constexpr int MATS = MODE == S_GATED ? 2 : 1;
-    using St = FewStage<MATS, NT>;
+    using St = FewStage<FP8, MATS, NT>;
     constexpr int smem = (VEC ? St::DEPTH * St::BYTES : 0) + St::SUMS;
     static_assert(smem <= 232448 - 1024, "shared memory");
     static SmemOnce once;
