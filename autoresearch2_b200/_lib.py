@@ -4,6 +4,7 @@ The library is the only compute path: if it is missing, every operation
 raises instead of falling back to another implementation.
 """
 import ctypes
+import functools
 import os
 import threading
 
@@ -126,6 +127,15 @@ SIGNATURES = {
                                  _i64, _vp, _vp]),
     "sffn_pad_rows16": (_int, [_int, _vp, _vp]),
     "sffn_few_rows_fp8": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp, _vp]),
+    "sffn_ckpt_linear_workspace_bytes": (_sz, [_int, _int, _int, _i64, _i64, _i64]),
+    "sffn_ckpt_linear": (_int, [_int, _vp, _i64, _vp, _i64, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "sffn_ckpt_linear_bwd": (_int, [_int, _vp, _i64, _vp, _i64, _int, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _sz,
+                                    _vp, _vp]),
+    "sffn_gated_ffn_workspace_bytes": (_sz, [_int, _int, _int, _int, _i64, _i64, _i64]),
+    "sffn_gated_ffn": (_int, [_int, _int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _int, _i64, _i64, _i64, _vp, _vp,
+                              _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "sffn_gated_ffn_bwd": (_int, [_int, _int, _int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _int, _vp,
+                                  _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
 }
 
 _lib = None
@@ -165,7 +175,8 @@ LAUNCHING = {"sffn_sp24_compress": 1, "sffn_gemm_sp24": 1, "sffn_sp24_overflow_a
              "sffn_distill_topk_bwd": 1, "sffn_residual_norm": 1, "sffn_residual_norm_bwd": 1,
              "sffn_fp8_pack": 1, "sffn_fp8_unpack": 1, "sffn_fp8_mm": 1, "sffn_glu_up": 1, "sffn_glu_dgrad": 1,
              "sffn_gemm16": 1, "sffn_few_rows_mm": 1, "sffn_few_rows_glu": 1, "sffn_few_rows_fp8": 1,
-             "sffn_few_rows_ffn": 2, "sffn_pad_rows16": 1}
+             "sffn_few_rows_ffn": 2, "sffn_pad_rows16": 1, "sffn_ckpt_linear": 1, "sffn_ckpt_linear_bwd": 1,
+             "sffn_gated_ffn": 2, "sffn_gated_ffn_bwd": 1}
 launch_count = 0
 
 # Per-entry-point CUDA event pairs, recorded while a KernelTimer is active.
@@ -199,6 +210,45 @@ class KernelTimer:
         return out
 
 
+@functools.lru_cache(maxsize=4096)
+def _gemm16(M, N, K, K2=0):
+    return 2 if load().sffn_gemm16_workspace_bytes(M, N, K, K2) else 1
+
+
+def _linear_launches(_dtype, _x, _ldx, _W, _ldw, odd, T, N, K, _y, values, *_):
+    return (1 if T <= 32 else bool(odd) + _gemm16(T, N, K)) + bool(values)
+
+
+def _linear_bwd_launches(_dtype, _dy, _ldy, _W, _ldw, odd, _v, _ldv, _s, T, N, K, dx, dW, *_):
+    return (bool(odd & (3 if dx else 1)) + (1 + _gemm16(N, K, T) if dW else 0) + (_gemm16(T, K, N) if dx else 0))
+
+
+def _gated_launches(_dtype, _act, keep, _x, _ldx, _wg, _ldg, _wu, _ldu, _w2, _ld2, odd, T, D, F, *_):
+    if keep == 0 and T <= 32:
+        return 2
+    return bool(odd & (7 if T <= 32 else 15)) + 1 + (1 if T <= 32 else _gemm16(T, D, F)) + (keep == 2)
+
+
+def _gated_bwd_launches(_dtype, _act, keep, steps, *a):
+    odd, T, D, F, dx, dwg, dwu, dw2 = a[10], *a[17:24]
+    n = 0
+    if steps & 1:
+        n += bool(odd & (15 if dx else 9)) + 1
+    if steps & 2 and dw2:
+        n += _gemm16(D, F, T)
+    if steps & 4 and (dwg or dwu):
+        ld = (F + 7) // 8 * 8
+        joint = dwg and dwu == dwg + ld * D * 2
+        n += (1 if keep == 2 else bool(odd & 16)) + (_gemm16(2 * ld, D, T) if joint else (bool(dwg) + bool(dwu)) * _gemm16(F, D, T))
+    if steps & 8 and dx:
+        n += _gemm16(T, D, F, F)
+    return n
+
+
+_BLOCKS = {"sffn_ckpt_linear": _linear_launches, "sffn_ckpt_linear_bwd": _linear_bwd_launches,
+           "sffn_gated_ffn": _gated_launches, "sffn_gated_ffn_bwd": _gated_bwd_launches}
+
+
 def _launches(name, args):
     """Kernels one successful call launched: LAUNCHING's count, except where
     it depends on the arguments (the float32-output GEMM runs one launch per
@@ -212,6 +262,8 @@ def _launches(name, args):
         return 2 if v is None or getattr(v, "value", v) in (None, 0) else 3
     if name == "sffn_gemm16":
         return 2 if args[18] else 1
+    if name in _BLOCKS:
+        return _BLOCKS[name](*args)
     if name == "sffn_residual_norm_bwd":
         return 2 if any(getattr(v, "value", v) for v in args[22:25]) else 1
     return LAUNCHING.get(name, 0)

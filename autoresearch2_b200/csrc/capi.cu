@@ -66,7 +66,19 @@ unsigned long long current_context_id() {
     return id;
 }
 
+namespace {
+thread_local int g_outer_device = -1;  // of an entry point that is made of others
+}
+
+OuterScope::OuterScope(const DeviceScope& scope) : saved_(g_outer_device) { g_outer_device = scope.device(); }
+OuterScope::~OuterScope() { g_outer_device = saved_; }
+
 int DeviceScope::bind(const void* p) {
+    if (g_outer_device >= 0) {  // bound by the entry point around this one
+        if (!p) return SFFN_ERR_ARG;
+        dev_ = g_outer_device;
+        return SFFN_OK;
+    }
     const int d = device_of(p);
     if (d < 0) return SFFN_ERR_ARG;
     const CtxFns& f = ctx_fns();

@@ -69,6 +69,19 @@ class DeviceScope {
     int dev_ = -1;
 };
 
+// For the length of an entry point that calls others: its scope's device is theirs,
+// which they do not look up again.
+class OuterScope {
+  public:
+    explicit OuterScope(const DeviceScope& scope);
+    OuterScope(const OuterScope&) = delete;
+    OuterScope& operator=(const OuterScope&) = delete;
+    ~OuterScope();
+
+  private:
+    int saved_;
+};
+
 // One-line form for the entry points: `SFFN_BIND(scope, ptr)` declares a
 // DeviceScope named `scope` bound to ptr's device, returning on failure.
 #define SFFN_BIND(scope, p)                              \

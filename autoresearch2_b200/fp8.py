@@ -11,7 +11,6 @@ Values are rounded once, to nearest, ties to even; infinities and NaN become
 NaN.  A power of two adds no rounding, dequantised values are exact in bfloat16
 and float32, and the tensor cores apply such scales themselves.
 """
-import ctypes
 import functools
 
 import torch
@@ -19,13 +18,13 @@ import torch
 from . import _lib
 from ._lib import address as ptr
 from ._lib import call, stream_handle
-from .parallel import submit_grad
+from .parallel import current, submit_grad
 
 __all__ = ["BLOCK", "Fp8Tensor", "fp8_pack", "fp8_unpack", "fp8_matmul", "ckpt_linear"]
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
-FEW_ROWS = 32  # products of at most so many rows read the weights by the few-row kernel
+FEW_ROWS = 32  # products of at most so many rows read the weights by the few-row kernels
 OUT_TYPES = (torch.bfloat16, torch.float16)
 
 
@@ -110,29 +109,12 @@ def _ld(t):
     return t.stride(0) if rows > 1 else width
 
 
-def _align(*mats):
-    """[(matrix, row stride)] of up to four 16-bit matrices of one type with dense
-    rows, as TMA reads them: rows on 16 bytes.  Those that are not are copied, all
-    of them by one kernel."""
-    out, copies = [], None
-    for t in mats:
-        rows, cols = t.shape
-        ld = t.stride(0) if rows > 1 else (cols + 7) // 8 * 8
-        if ld % 8 or t.data_ptr() % 16:
-            copies = copies or []
-            copies.append((len(out), t, rows, cols, (cols + 7) // 8 * 8))
-        out.append((t, ld))
-    if copies:
-        t = copies[0][1]
-        buf = t.new_empty(sum(rows * ldd for _, _, rows, _, ldd in copies))
-        desc, at = (ctypes.c_int64 * (6 * len(copies)))(), 0
-        for k, (i, t, rows, cols, ldd) in enumerate(copies):
-            to = buf.as_strided((rows, cols), (ldd, 1), at)
-            desc[6 * k:6 * k + 6] = t.data_ptr(), rows, cols, _ld(t), to.data_ptr(), ldd
-            out[i] = to, ldd
-            at += rows * ldd
-        call("sffn_pad_rows16", len(copies), ctypes.addressof(desc), stream_handle(buf.device))
-    return out
+def _row_stride(t, bit):
+    """(row stride, bit if the matrix's rows are not on 16 bytes, as TMA reads them) of a
+    16-bit matrix with dense rows."""
+    rows, width = t.shape
+    ld = t.stride(0) if rows > 1 else width
+    return ld, bit if t.data_ptr() % 16 or (rows > 1 and ld % 8) else 0
 
 
 def _empty_rows(t, rows, cols, multiple):
@@ -266,43 +248,6 @@ def fp8_matmul(a, b, out_dtype=None):
 
 
 # ---------------------------------------------------------------------------
-# 16-bit products on the tensor cores
-# ---------------------------------------------------------------------------
-@functools.lru_cache(maxsize=4096)
-def _workspace_bytes(M, N, K, K2):
-    return _lib.load().sffn_gemm16_workspace_bytes(M, N, K, K2)
-
-
-def _mm_into(out, A, a_mn, B, b_mn, second=None):
-    """out [M, N] = A B^T; A is [M, K], or with a_mn [K, M]; B [N, K] or [K, N]; plus
-    second = (A2, B2), likewise, added within the product.  Each operand as _align
-    gives it, a pair of matrix and row stride."""
-    M, N = out.shape
-    (A, lda), (B, ldb) = A, B
-    K, dev = A.shape[0 if a_mn else 1], out.device
-    A2 = B2 = None
-    lda2 = ldb2 = K2 = 0
-    if second is not None:
-        (A2, lda2), (B2, ldb2) = second
-        K2 = A2.shape[0 if a_mn else 1]
-    ws_bytes = _workspace_bytes(M, N, K, K2)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    call("sffn_gemm16", _lib._DTYPES[out.dtype], A.data_ptr(), lda, a_mn, B.data_ptr(), ldb, b_mn, ptr(A2), lda2, ptr(B2),
-         ldb2, K2, M, N, K, out.data_ptr(), _ld(out), ptr(ws), ws_bytes, _lib.status_word(dev).data_ptr(), stream_handle(dev))
-    return out
-
-
-def _few_rows(x, W):
-    """x [T, K] W [N, K]^T for T <= FEW_ROWS, in their type."""
-    T, N = x.shape[0], W.shape[0]
-    out = x.new_empty((T, N))
-    if T:
-        call("sffn_few_rows_mm", _lib._DTYPES[x.dtype], x.data_ptr(), _ld(x), W.data_ptr(), _ld(W), T, N, x.shape[1],
-             out.data_ptr(), N, _lib.status_word(x.device).data_ptr(), stream_handle(x.device))
-    return out
-
-
-# ---------------------------------------------------------------------------
 # A linear layer that keeps its input in 8 bits
 # ---------------------------------------------------------------------------
 def _fits(x, w, rows, cols):
@@ -333,33 +278,59 @@ def _check_linear(x, W):
         _check_weights(x, W=(W, (W.shape[0] if W.dim() else 0, x.shape[-1] if x.dim() else 0)))
 
 
+@functools.lru_cache(maxsize=4096)
+def _linear_workspace(backward, odd, want, T, N, K):
+    return _lib.load().sffn_ckpt_linear_workspace_bytes(backward, odd, want, T, N, K)
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 def _linear_forward(x, W, keep):
     """(y, values, tiles) -- the last two None without keep."""
     x2, W2 = _rows(x), _rows(W)
-    if x2.shape[0] <= FEW_ROWS:
-        y = _few_rows(x2, W2)
-    else:
-        A, B = _align(x2, W2)
-        x2 = A[0]
-        y = _mm_into(x2.new_empty((x2.shape[0], W2.shape[0])), A, 0, B, 0)
-    if x.dim() != 2:
-        y = y.view(*x.shape[:-1], W.shape[0])
-    return (y, *_pack(x2)) if keep else (y, None, None)
+    T, K = x2.shape
+    N, dev = W2.shape[0], x.device
+    y = x2.new_empty((T, N))
+    values = tiles = None
+    if keep:
+        values, tiles = _empty_values(T, K, dev), _empty_tiles(T, K, dev)
+    if T:
+        (ldx, ox), (ldw, ow) = _row_stride(x2, 1), _row_stride(W2, 2)
+        n = _linear_workspace(0, ox | ow, 0, T, N, K)
+        ws = _workspace(n, dev)
+        call("sffn_ckpt_linear", _lib._DTYPES[x.dtype], x2.data_ptr(), ldx, W2.data_ptr(), ldw, ox | ow, T, N, K, y.data_ptr(),
+             ptr(values), ptr(tiles), ptr(ws), n, _lib.status_word(dev).data_ptr(), stream_handle(dev))
+    return (y if x.dim() == 2 else y.view(*x.shape[:-1], N)), values, tiles
 
 
 def _linear_backward(dy, W, values, tiles, x_shape, want_x, want_W):
-    _lib.bind_thread(dy.device)
-    dy2, width = _rows(dy), x_shape[-1]
-    dx = dW = None
-    if dy2.shape[0] == 0:
-        return dy.new_empty(x_shape) if want_x else None, submit_grad(W.new_zeros(W.shape)) if want_W else None
-    A, *B = _align(dy2, _rows(W)) if want_x else _align(dy2)
-    if want_W:
-        kept = _unpack(values, tiles, _empty_rows(dy2, dy2.shape[0], width, 8), width)
-        dW = submit_grad(_mm_into(dy2.new_empty((dy2.shape[1], width)), A, 1, *_align(kept), 1))
-        del kept
-    if want_x:
-        dx = _mm_into(dy2.new_empty((dy2.shape[0], width)), A, 0, *B, 1).view(x_shape)
+    dev = dy.device
+    _lib.bind_thread(dev)
+    dy2, W2 = _rows(dy), _rows(W)
+    T, N = dy2.shape
+    K = x_shape[-1]
+    dx = dy2.new_empty(x_shape) if want_x else None
+    if not T:
+        return dx, submit_grad(W.new_zeros((N, K))) if want_W else None
+    dW = dy2.new_empty((N, K)) if want_W else None
+    (ldy, oy), (ldw, ow) = _row_stride(dy2, 1), _row_stride(W2, 2)
+    dtype, status, stream = _lib._DTYPES[dy.dtype], _lib.status_word(dev).data_ptr(), stream_handle(dev)
+
+    def run(dx, dW):
+        n = _linear_workspace(1, oy | ow, (dx is not None) + 2 * (dW is not None), T, N, K)
+        ws = _workspace(n, dev)
+        call("sffn_ckpt_linear_bwd", dtype, dy2.data_ptr(), ldy, W2.data_ptr(), ldw, oy | ow, ptr(values),
+             _stride(values) if dW is not None else 0, ptr(tiles), T, N, K, ptr(dx), ptr(dW), ptr(ws), n, status, stream)
+
+    if want_x and want_W and current() is not None:  # dW's reduction beside dx
+        run(None, dW)
+        submit_grad(dW)
+        run(dx, None)
+    else:
+        run(dx, dW)
+        submit_grad(dW)
     return dx, dW
 
 

@@ -16,21 +16,29 @@ dh's kernel reads g and u and writes dg, du and act(g) * u; dx is one product
 over both pairs.  Products sum in float32; h, dg and du are rounded to the
 inputs' type, in which the tensor cores read them.
 """
+import functools
+
 import torch
 
 from . import _lib, fp8
 from ._lib import address as ptr
 from ._lib import call, stream_handle
-from .parallel import submit_grad
+from .parallel import current, submit_grad
 
 __all__ = ["ACTIVATIONS", "gated_ffn"]
 
 ACTIVATIONS = {"relu": 0, "relu2": 1, "silu": 2, "gelu": 3}
 KEEP = {None: 1, "fp8": 2}
+DGRAD, DW2, DWGU, DX = 1, 2, 4, 8  # steps of the backward
 
 
 def _kept_ld(F, keep):
     return (F + 15) // 16 * 16 if keep == 2 else (F + 7) // 8 * 8
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(backward, keep, odd, want, T, D, F):
+    return _lib.load().sffn_gated_ffn_workspace_bytes(backward, keep, odd, want, T, D, F)
 
 
 def _forward(x, Wg, Wu, W2, act, keep):
@@ -38,80 +46,72 @@ def _forward(x, Wg, Wu, W2, act, keep):
     and u in x's type, 2 all three in 8 bits; what is not kept is None."""
     x2, Wg, Wu, W2 = fp8._rows(x), fp8._rows(Wg), fp8._rows(Wu), fp8._rows(W2)
     T, D = x2.shape
-    F, dev, code = Wg.shape[0], x.device, _lib._DTYPES[x.dtype]
+    F, dev = Wg.shape[0], x.device
     g = u = gt = ut = xv = xt = None
-    if keep == 0 and 0 < T <= fp8.FEW_ROWS:
-        h, y = x2.new_empty((T, (F + 7) // 8 * 8)), x2.new_empty((T, D))
-        call("sffn_few_rows_ffn", code, act, x2.data_ptr(), fp8._ld(x2), Wg.data_ptr(), fp8._ld(Wg), Wu.data_ptr(),
-             fp8._ld(Wu), W2.data_ptr(), fp8._ld(W2), T, D, F, h.data_ptr(), h.shape[1], y.data_ptr(), D,
-             _lib.status_word(dev).data_ptr(), stream_handle(dev))
-        return y if x.dim() == 2 else y.view(x.shape), g, u, gt, ut, xv, xt
     if keep == 2:
-        g, u = (fp8._empty_values(T, F, dev) for _ in range(2))
-        gt, ut = (fp8._empty_tiles(T, F, dev) for _ in range(2))
+        g, u, xv = fp8._empty_values(T, F, dev), fp8._empty_values(T, F, dev), fp8._empty_values(T, D, dev)
+        gt, ut, xt = fp8._empty_tiles(T, F, dev), fp8._empty_tiles(T, F, dev), fp8._empty_tiles(T, D, dev)
     elif keep == 1:
-        g, u = (fp8._empty_rows(x2, T, F, 8) for _ in range(2))
-    if T == 0:
-        if keep == 2:
-            xv, xt = fp8._pack(x2)
-        return x.new_empty(x.shape), g, u, gt, ut, xv, xt
-    if T <= fp8.FEW_ROWS:  # kept, so the tensor cores' tiles: W2's product is the few-row kernel's
-        xa, ga, ua = fp8._align(x2, Wg, Wu)
-    else:
-        xa, ga, ua, W2a = fp8._align(x2, Wg, Wu, W2)
-    h = fp8._empty_rows(x2, T, F, 8)
-    ldh = (F + 7) // 8 * 8
-    call("sffn_glu_up", code, act, xa[0].data_ptr(), xa[1], ga[0].data_ptr(), ga[1], ua[0].data_ptr(), ua[1], T, D, F,
-         h.data_ptr(), ldh, keep, ptr(g), ptr(u), _kept_ld(F, keep), ptr(gt), ptr(ut),
-         _lib.status_word(dev).data_ptr(), stream_handle(dev))
-    if T <= fp8.FEW_ROWS:
-        y = fp8._few_rows(h, W2)
-    else:
-        y = fp8._mm_into(x2.new_empty((T, D)), (h, ldh), 0, W2a, 0)
-    if keep == 2:
-        xv, xt = fp8._pack(xa[0])
-    return y if x.dim() == 2 else y.view(x.shape), g, u, gt, ut, xv, xt
+        g, u = fp8._empty_rows(x2, T, F, 8), fp8._empty_rows(x2, T, F, 8)
+    y = x2.new_empty((T, D))
+    if T:
+        (ldx, ox), (ldg, og), (ldu, ou), (ld2, o2) = (fp8._row_stride(x2, 1), fp8._row_stride(Wg, 2),
+                                                      fp8._row_stride(Wu, 4), fp8._row_stride(W2, 8))
+        odd = ox | og | ou | o2
+        n = _workspace_bytes(0, keep, odd, 0, T, D, F)
+        ws = fp8._workspace(n, dev)
+        call("sffn_gated_ffn", _lib._DTYPES[x.dtype], act, keep, x2.data_ptr(), ldx, Wg.data_ptr(), ldg, Wu.data_ptr(), ldu,
+             W2.data_ptr(), ld2, odd, T, D, F, y.data_ptr(), ptr(g), ptr(u), ptr(gt), ptr(ut), ptr(xv), ptr(xt), ptr(ws), n,
+             _lib.status_word(dev).data_ptr(), stream_handle(dev))
+    return (y if x.dim() == 2 else y.view(x.shape)), g, u, gt, ut, xv, xt
 
 
 def _backward(dy, x, Wg, Wu, W2, g, u, gt, ut, xv, xt, act, want, apart=False):
     """Gradients of (x, Wg, Wu, W2); None where `want` is false.  x is None with 8-bit
     checkpoints.  apart: dWg and dWu do not share their storage."""
-    _lib.bind_thread(dy.device)
+    dev = dy.device
+    _lib.bind_thread(dev)
     dy2, Wg, Wu, W2 = fp8._rows(dy), fp8._rows(Wg), fp8._rows(Wu), fp8._rows(W2)
     T, D = dy2.shape
-    F, dev, code = Wg.shape[0], dy.device, _lib._DTYPES[dy.dtype]
+    F, keep = Wg.shape[0], 1 if xv is None else 2
     dx = dWg = dWu = dW2 = None
-    if T == 0:
-        return (dy.new_empty(dy.shape) if want[0] else None,
-                *(submit_grad(w.new_zeros(w.shape)) if n else None for w, n in zip((Wg, Wu, W2), want[1:])))
-    keep = 2 if xv is not None else 1
-    ld = (F + 7) // 8 * 8
-    d, h = dy2.new_empty((T, 2 * ld)), fp8._empty_rows(dy2, T, F, 8)  # d: dg | du, their weights' gradient is one product
-    dg, du = (d[:, :F], 2 * ld), (d[:, ld:ld + F], 2 * ld)
     if want[0]:
-        dya, W2a, ga, ua = fp8._align(dy2, W2, Wg, Wu)
+        dx = dy2.new_empty(dy.shape)
+    if not T:
+        return (dx, *(submit_grad(w.new_zeros(w.shape)) if n else None for w, n in zip((Wg, Wu, W2), want[1:])))
+    if want[1] and want[2] and not apart:  # one product, rows of dWu after F rounded up to 8 of dWg
+        ld = (F + 7) // 8 * 8
+        both = dy2.new_empty((2 * ld, D))
+        dWg, dWu = both[:F], both[ld:ld + F]
     else:
-        dya, W2a = fp8._align(dy2, W2)
-    call("sffn_glu_dgrad", code, act, dya[0].data_ptr(), dya[1], W2a[0].data_ptr(), W2a[1], T, D, F, keep, g.data_ptr(),
-         u.data_ptr(), _kept_ld(F, keep), ptr(gt), ptr(ut), dg[0].data_ptr(), du[0].data_ptr(), 2 * ld, h.data_ptr(), ld,
-         _lib.status_word(dev).data_ptr(), stream_handle(dev))
+        dWg, dWu = (dy2.new_empty((F, D)) if w else None for w in want[1:3])
     if want[3]:
-        dW2 = submit_grad(fp8._mm_into(dy2.new_empty((D, F)), dya, 1, (h, ld), 1))
-    del h
-    if want[1] or want[2]:
-        if keep == 2:
-            xk = fp8._unpack(xv, xt, fp8._empty_rows(dy2, T, D, 8), D), (D + 7) // 8 * 8
-        else:
-            xk, = fp8._align(fp8._rows(x))
-        if want[1] and want[2] and not apart:
-            dW = fp8._mm_into(dy2.new_empty((2 * ld, D)), (d, 2 * ld), 1, xk, 1)
-            dWg, dWu = submit_grad(dW[:F]), submit_grad(dW[ld:ld + F])
-        else:
-            dWg = submit_grad(fp8._mm_into(dy2.new_empty((F, D)), dg, 1, xk, 1)) if want[1] else None
-            dWu = submit_grad(fp8._mm_into(dy2.new_empty((F, D)), du, 1, xk, 1)) if want[2] else None
-        del xk
-    if want[0]:
-        dx = fp8._mm_into(dy2.new_empty((T, D)), dg, 0, ga, 1, (du, ua)).view(dy.shape)
+        dW2 = dy2.new_empty((D, F))
+    x2, (ldx, ox) = None, (0, 0)
+    if keep == 1:
+        x2 = fp8._rows(x)
+        ldx, ox = fp8._row_stride(x2, 16)
+    (ldy, oy), (ldg, og), (ldu, ou), (ld2, o2) = (fp8._row_stride(dy2, 1), fp8._row_stride(Wg, 2), fp8._row_stride(Wu, 4),
+                                                  fp8._row_stride(W2, 8))
+    odd = oy | og | ou | o2 | ox
+    n = _workspace_bytes(1, keep, odd, want[0] + 2 * want[1] + 4 * want[2] + 8 * want[3], T, D, F)
+    ws = fp8._workspace(n, dev)
+    code, status, stream = _lib._DTYPES[dy.dtype], _lib.status_word(dev).data_ptr(), stream_handle(dev)
+
+    def run(steps):
+        call("sffn_gated_ffn_bwd", code, act, keep, steps, dy2.data_ptr(), ldy, ptr(x2), ldx, Wg.data_ptr(), ldg, Wu.data_ptr(),
+             ldu, W2.data_ptr(), ld2, odd, g.data_ptr(), u.data_ptr(), ptr(gt), ptr(ut), ptr(xv), ptr(xt), T, D, F, ptr(dx),
+             ptr(dWg), ptr(dWu), ptr(dW2), ptr(ws), n, status, stream)
+
+    if current() is None:
+        run(DGRAD | DW2 | DWGU | DX)
+    else:  # each weight gradient's reduction beside what follows it
+        run(DGRAD | DW2)
+        submit_grad(dW2)
+        run(DWGU)
+        submit_grad(dWg)
+        submit_grad(dWu)
+        run(DX)
     return dx, dWg, dWu, dW2
 
 

@@ -711,6 +711,44 @@ int sffn_few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const vo
                       const void* w_scales, int64_t T, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
                       uint32_t* status_dev, void* stream);
 
+/* ckpt_linear: y [T, N] = x [T, K] W [N, K]^T and, unless `values` is NULL, x in 8-bit
+ * blocks (rows as wide as K rounded up to 16); backward dx = dy W and dW = dy^T times
+ * the kept x (each NULL: not wanted).  odd: bits of the operands whose rows are not
+ * on 16 bytes and are copied (forward 1 x, 2 W; backward 1 dy, 2 W).  One row:
+ * its stride is not read.  want: 1 dx, 2 dW. */
+size_t sffn_ckpt_linear_workspace_bytes(int backward, int odd, int want, int64_t T, int64_t N, int64_t K);
+int sffn_ckpt_linear(int dtype, const void* x, int64_t ldx, const void* W, int64_t ldw, int odd, int64_t T, int64_t N,
+                     int64_t K, void* y, void* values, void* scales, void* workspace, size_t workspace_bytes,
+                     uint32_t* status_dev, void* stream);
+int sffn_ckpt_linear_bwd(int dtype, const void* dy, int64_t lddy, const void* W, int64_t ldw, int odd, const void* values,
+                         int64_t ldv, const void* scales, int64_t T, int64_t N, int64_t K, void* dx, void* dW,
+                         void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream);
+
+enum { /* steps of the gated block's backward, on one workspace, in this order */
+    SFFN_GATED_DGRAD = 1,
+    SFFN_GATED_DW2 = 2,
+    SFFN_GATED_DWGU = 4,
+    SFFN_GATED_DX = 8
+};
+
+/* The gated block, all of a direction: y [T, D] = (act(x wg^T) * (x wu^T)) w2^T,
+ * keeping as sffn_glu_up does (rows of g and u as wide as F rounded up to 16 bytes)
+ * and, for SFFN_KEEP_8, x too; and the gradients (each NULL: not wanted; dwu
+ * right behind dwg's F rounded up to 8 rows makes the two one product, whose
+ * rows beyond F are written).  odd: bits of the operands whose rows are not on 16
+ * bytes (1 x, or dy in the backward, 2 wg, 4 wu, 8 w2, 16 x in the backward).
+ * want: 1 dx, 2 dwg, 4 dwu, 8 dw2. */
+size_t sffn_gated_ffn_workspace_bytes(int backward, int keep, int odd, int want, int64_t T, int64_t D, int64_t F);
+int sffn_gated_ffn(int dtype, int act, int keep, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
+                   int64_t ldwu, const void* w2, int64_t ldw2, int odd, int64_t T, int64_t D, int64_t F, void* y, void* g,
+                   void* u, void* g_scales, void* u_scales, void* x_values, void* x_scales, void* workspace,
+                   size_t workspace_bytes, uint32_t* status_dev, void* stream);
+int sffn_gated_ffn_bwd(int dtype, int act, int keep, int steps, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                       const void* wg, int64_t ldwg, const void* wu, int64_t ldwu, const void* w2, int64_t ldw2, int odd,
+                       const void* g, const void* u, const void* g_scales, const void* u_scales, const void* x_values,
+                       const void* x_scales, int64_t T, int64_t D, int64_t F, void* dx, void* dwg, void* dwu, void* dw2,
+                       void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream);
+
 /* ---- bounded waits ------------------------------------------------------ */
 
 /* Test hook, no counterpart in the reference.  Runs one of this library's

@@ -327,3 +327,41 @@ def test_workspace_and_launches(lib):
     assert _lib._launches("sffn_gemm16", a) == 1
     a[18] = n
     assert _lib._launches("sffn_gemm16", a) == 2 and _lib._launches("sffn_few_rows_ffn", []) == 2
+
+
+def test_launches_of_the_blocks():
+    f = _lib._launches
+    linear = lambda T, N, K, odd=0, keep=1: f("sffn_ckpt_linear", [1, 1, K, 1, K, odd, T, N, K, 1, keep, 1, 1, 0, 1, 0])  # noqa: E731
+    assert linear(8, 64, 64) == 2 and linear(8, 64, 64, 3, None) == 1 and linear(4096, 4096, 64) == 2 and linear(4096, 4096, 63, 1) == 3
+    bwd = lambda T, N, K, dx, dW, odd=0: f("sffn_ckpt_linear_bwd", [1, 1, N, 1, K, odd, 1, K, 1, T, N, K, dx, dW, 1, 0, 1, 0])  # noqa: E731
+    assert bwd(4096, 4096, 4096, 1, 1) == 3 and bwd(4096, 4096, 4096, None, 1, 2) == 2 and bwd(4096, 4096, 4096, 1, None, 2) == 2
+    assert bwd(32768, 768, 768, 1, 1) == 4  # the weight gradient in parts, joined
+    up = lambda keep, T, odd=0: f("sffn_gated_ffn", [1, 2, keep, 1, 64, 1, 64, 1, 64, 1, 64, odd, T, 64, 64])  # noqa: E731
+    assert up(0, 8) == 2 and up(0, 64) == 2 and up(1, 8) == 2 and up(2, 8) == 3 and up(2, 64, 1) == 4 and up(1, 8, 8) == 2
+    T, D, F = 4096, 4096, 4096
+    down = lambda keep, steps, dx, dwg, dwu, dw2, odd=0: f("sffn_gated_ffn_bwd", [  # noqa: E731
+        1, 2, keep, steps, 1, D, 1, D, 1, D, 1, D, 1, F, odd, 1, 1, 1, 1, 1, 1, T, D, F, dx, dwg, dwu, dw2, 1, 0, 1, 0])
+    assert down(1, 15, 1, 16, 16 + F * D * 2, 1) == 4 and down(2, 15, 1, 16, 16 + F * D * 2, 1) == 5
+    assert down(1, 15, 1, 16, 32, 1, 16) == 6 and down(1, 1, 1, 16, 32, 1) == 1 and down(1, 6, 1, None, None, 1) == 1
+
+
+def test_block_entries(lib):
+    w = lib.sffn_ckpt_linear_workspace_bytes
+    assert w(0, 0, 0, 64, 64, 64) == 0 and w(0, 3, 0, 8, 64, 64) == 0 and w(0, 1, 0, 64, 64, 63) == 64 * 64 * 2
+    assert w(1, 0, 1, 64, 64, 64) == 0 and w(1, 0, 2, 64, 64, 63) >= 64 * 64 * 2 and w(0, 0, 0, 0, 64, 64) == 0
+    ok = [1, P, 64, P, 64, 0, 100, 64, 64, P, P, P, None, 0, P, None]
+    f = lib.sffn_ckpt_linear
+    assert rc(f, ok, _0=0) == 2 and rc(f, ok, _6=0) == 1 and rc(f, ok, _1=None) == 1 and rc(f, ok, _14=None) == 1
+    assert rc(f, ok, _5=1) == 4 and rc(f, ok, _5=1, _12=P, _13=100) == 4 and rc(f, ok, _5=1, _12=ODD, _13=1 << 20) == 3
+    ok = [1, P, 64, P, 64, 0, P, 64, P, 100, 64, 64, P, P, P, 1 << 20, P, None]
+    f = lib.sffn_ckpt_linear_bwd
+    assert rc(f, ok, _0=0) == 2 and rc(f, ok, _9=0) == 1 and rc(f, ok, _14=None) == 4 and rc(f, ok, _15=100) == 4 and rc(f, ok, _1=None) == 1
+    w = lib.sffn_gated_ffn_workspace_bytes
+    assert w(0, 0, 0, 0, 64, 64, 64) == 64 * 64 * 2 and w(1, 1, 0, 15, 4096, 4096, 4096) == 3 * 4096 * 4096 * 2
+    assert w(1, 2, 0, 15, 4096, 4096, 4096) == 4 * 4096 * 4096 * 2 and w(0, 1, 0, 0, 64, 0, 64) == 0
+    ok = [1, 2, 1, P, 64, P, 64, P, 64, P, 64, 0, 100, 64, 64, P, P, P, None, None, None, None, P, 1 << 20, P, None]
+    f = lib.sffn_gated_ffn
+    assert rc(f, ok, _0=0) == 2 and rc(f, ok, _2=3) == 1 and rc(f, ok, _12=0) == 1 and rc(f, ok, _22=None) == 4 and rc(f, ok, _23=8) == 4
+    ok = [1, 2, 1, 15, P, 64, P, 64, P, 64, P, 64, P, 64, 0, P, P, None, None, None, None, 100, 64, 64, P, P, P, P, P, 1 << 24, P, None]
+    f = lib.sffn_gated_ffn_bwd
+    assert rc(f, ok, _0=0) == 2 and rc(f, ok, _2=0) == 1 and rc(f, ok, _21=0) == 1 and rc(f, ok, _28=None) == 4 and rc(f, ok, _29=8) == 4
