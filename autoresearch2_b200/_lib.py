@@ -216,7 +216,7 @@ def _gemm16(M, N, K, K2=0):
 
 
 def _linear_launches(_dtype, _x, _ldx, _W, _ldw, odd, T, N, K, _y, values, *_):
-    return (1 if T <= 32 else bool(odd) + _gemm16(T, N, K)) + bool(values)
+    return ((odd == 1) + 1 if T <= 32 else bool(odd) + _gemm16(T, N, K)) + bool(values)
 
 
 def _linear_bwd_launches(_dtype, _dy, _ldy, _W, _ldw, odd, _v, _ldv, _s, T, N, K, dx, dW, *_):
@@ -225,7 +225,7 @@ def _linear_bwd_launches(_dtype, _dy, _ldy, _W, _ldw, odd, _v, _ldv, _s, T, N, K
 
 def _gated_launches(_dtype, _act, keep, _x, _ldx, _wg, _ldg, _wu, _ldu, _w2, _ld2, odd, T, D, F, *_):
     if keep == 0 and T <= 32:
-        return 2
+        return 2 + (odd & 7 == 1)
     return bool(odd & (7 if T <= 32 else 15)) + 1 + (1 if T <= 32 else _gemm16(T, D, F)) + (keep == 2)
 
 

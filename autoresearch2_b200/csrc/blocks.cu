@@ -80,11 +80,13 @@ bool dtype16(int d) { return d == SFFN_BF16 || d == SFFN_F16; }
 int linear_fwd(int dtype, const void* x, long long ldx, const void* W, long long ldw, int odd, long long T, long long N,
                long long K, void* y, void* values, void* scales, Scratch& ws, uint32_t* status, void* stream, bool count) {
     Mat X = mat(x, ldx, T, K, odd & 1), V = mat(W, ldw, N, K, odd & 2);
+    Pads pads;
     if (T <= FEW) {
+        if (!(odd & 2)) pads.place(X, ws);  // few rows are copied for the fast way through many
         if (count) return SFFN_OK;
-        TRY(sffn_few_rows_mm(dtype, x, ldx, W, ldw, T, N, K, y, N, status, stream));
+        TRY(pads.run(stream));
+        TRY(sffn_few_rows_mm(dtype, X.p, X.ld, W, ldw, T, N, K, y, N, status, stream));
     } else {
-        Pads pads;
         pads.place(X, ws);
         pads.place(V, ws);
         if (!count) TRY(pads.run(stream));
@@ -123,10 +125,13 @@ int gated_fwd(int dtype, int act, int keep, const void* x, long long ldx, const 
         W2 = mat(w2, ld2, D, F, odd & 8);
     void* h = ws.take((size_t)T * up8(F) * 2);
     const Mat H = mat(h, up8(F), T, F, false);
-    if (keep == SFFN_KEEP_NONE && T <= FEW)
-        return count ? SFFN_OK
-                     : sffn_few_rows_ffn(dtype, act, x, ldx, wg, ldg, wu, ldu, w2, ld2, T, D, F, h, H.ld, y, D, status, stream);
     Pads pads;
+    if (keep == SFFN_KEEP_NONE && T <= FEW) {
+        if (!(odd & 6)) pads.place(X, ws);  // few rows are copied for the fast way through many
+        if (count) return SFFN_OK;
+        TRY(pads.run(stream));
+        return sffn_few_rows_ffn(dtype, act, X.p, X.ld, wg, ldg, wu, ldu, w2, ld2, T, D, F, h, H.ld, y, D, status, stream);
+    }
     pads.place(X, ws);
     pads.place(G, ws);
     pads.place(U, ws);

@@ -515,7 +515,9 @@ extern "C" int sffn_few_rows_fp8(const void* x, int64_t ldx, const void* x_scale
     if (int rc = check_few(T, N, K)) return rc;
     if (T == 0 || N == 0) return SFFN_OK;
     if (!x || !x_scales || !w || !w_scales || !out || !status_dev || ldx < K || ldw < K || ldo < N) return SFFN_ERR_ARG;
-    if (!rows16(x, ldx, 1) || !rows16(w, ldw, 1) || reinterpret_cast<uintptr_t>(out) % 2) return SFFN_ERR_ALIGN;
+    if (!rows16(x, ldx, 1) || !rows16(w, ldw, 1) || !aligned16(x_scales) || !aligned16(w_scales) ||
+        reinterpret_cast<uintptr_t>(out) % 2)
+        return SFFN_ERR_ALIGN;
     DeviceScope scope;
     if (int rc = scope.bind(x)) return rc;
     FewArgs a{};

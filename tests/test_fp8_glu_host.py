@@ -259,6 +259,7 @@ def test_product_entries(lib):
             assert rc(f, ok, **{f"_{i}": None}) == 1
         assert rc(f, ok, _1=32) == 1 and rc(f, ok, _4=32) == 1 and rc(f, ok, _11=7) == 1
         assert rc(f, ok, _1=56) == 3 and rc(f, ok, _0=ODD) == 3 and rc(f, ok, _3=ODD) == 3 and rc(f, ok, _9=vp((1 << 20) + 1)) == 3
+        assert rc(f, ok, _2=ODD) == 3 and rc(f, ok, _5=ODD) == 3
         assert rc(f, ok, _7=BIG, _11=BIG) == 8
     assert rc(lib.sffn_fp8_mm, [P, 48, P, P, 48, P, BIG, 8, 40, P, 1, 8, P, None]) == 8
 
@@ -332,12 +333,12 @@ def test_workspace_and_launches(lib):
 def test_launches_of_the_blocks():
     f = _lib._launches
     linear = lambda T, N, K, odd=0, keep=1: f("sffn_ckpt_linear", [1, 1, K, 1, K, odd, T, N, K, 1, keep, 1, 1, 0, 1, 0])  # noqa: E731
-    assert linear(8, 64, 64) == 2 and linear(8, 64, 64, 3, None) == 1 and linear(4096, 4096, 64) == 2 and linear(4096, 4096, 63, 1) == 3
+    assert linear(8, 64, 64) == 2 and linear(8, 64, 64, 1) == 3 and linear(8, 64, 64, 3, None) == 1 and linear(4096, 4096, 64) == 2 and linear(4096, 4096, 63, 1) == 3
     bwd = lambda T, N, K, dx, dW, odd=0: f("sffn_ckpt_linear_bwd", [1, 1, N, 1, K, odd, 1, K, 1, T, N, K, dx, dW, 1, 0, 1, 0])  # noqa: E731
     assert bwd(4096, 4096, 4096, 1, 1) == 3 and bwd(4096, 4096, 4096, None, 1, 2) == 2 and bwd(4096, 4096, 4096, 1, None, 2) == 2
     assert bwd(32768, 768, 768, 1, 1) == 4  # the weight gradient in parts, joined
     up = lambda keep, T, odd=0: f("sffn_gated_ffn", [1, 2, keep, 1, 64, 1, 64, 1, 64, 1, 64, odd, T, 64, 64])  # noqa: E731
-    assert up(0, 8) == 2 and up(0, 64) == 2 and up(1, 8) == 2 and up(2, 8) == 3 and up(2, 64, 1) == 4 and up(1, 8, 8) == 2
+    assert up(0, 8) == 2 and up(0, 8, 9) == 3 and up(0, 8, 3) == 2 and up(0, 64) == 2 and up(1, 8) == 2 and up(2, 8) == 3 and up(2, 64, 1) == 4 and up(1, 8, 8) == 2
     T, D, F = 4096, 4096, 4096
     down = lambda keep, steps, dx, dwg, dwu, dw2, odd=0: f("sffn_gated_ffn_bwd", [  # noqa: E731
         1, 2, keep, steps, 1, D, 1, D, 1, D, 1, D, 1, F, odd, 1, 1, 1, 1, 1, 1, T, D, F, dx, dwg, dwu, dw2, 1, 0, 1, 0])

@@ -200,6 +200,20 @@ def test_product_shapes_and_types():
     assert torch.equal(sf.fp8_matmul(x[0, 0], w), y[0, 0])
 
 
+@pytest.mark.parametrize("M", [2, 40])
+def test_misaligned_blocks_are_refused(M):
+    b = sf.fp8_pack(randn(64, 64))
+    q = sf.fp8_pack(randn(M, 64))
+    t = torch.zeros(q.scale_tiles.numel() + 2, dtype=torch.uint8, device=DEV)[2:].view(q.scale_tiles.shape)
+    v = torch.zeros(M * 80 + 1, dtype=torch.uint8, device=DEV)[1:].view(fp8.E4M3).view(M, 80)[:, :64]
+    with pytest.raises(sf._lib.SparseFFNError, match="misaligned"):
+        sf.fp8_matmul(sf.Fp8Tensor(q.values, t), b)
+    with pytest.raises(ValueError, match="start on 16 bytes"):
+        sf.fp8_matmul(sf.Fp8Tensor(v, q.scale_tiles), b)
+    with pytest.raises(sf._lib.SparseFFNError, match="misaligned"):
+        sf.fp8_unpack(sf.Fp8Tensor(v, q.scale_tiles))
+
+
 def test_product_beside_others_rows():
     """Nothing is written past the result, with rows that are not 16 bytes apart."""
     from autoresearch2_b200 import _lib

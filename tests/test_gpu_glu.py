@@ -235,6 +235,16 @@ def test_no_rows():
         assert y.shape == (0, 64) and not any(g.any() for g in grads)
 
 
+@pytest.mark.parametrize("T", [1, 9])
+def test_few_unaligned_rows_with_aligned_weights(T):
+    big, (_, Wg, Wu, W2, _) = randn(T, 100, seed=1, dtype=BF16), inputs(1, 96, 200, BF16)
+    x = big[:, 3:99]
+    assert torch.equal(sf.gated_ffn(x, Wg, Wu, W2), sf.gated_ffn(x.contiguous(), Wg, Wu, W2))
+    assert torch.equal(sf.ckpt_linear(x, Wg), sf.ckpt_linear(x.contiguous(), Wg))
+    W = randn(200, 99, seed=2, dtype=BF16)[:, 3:]
+    assert torch.equal(sf.ckpt_linear(x, W), sf.ckpt_linear(x.contiguous(), W.contiguous()))
+
+
 @pytest.mark.parametrize("T", [4, 150])
 def test_strided_operands(T):
     big = randn(2 * T, 200, seed=1, dtype=BF16)
