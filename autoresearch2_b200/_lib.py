@@ -113,7 +113,10 @@ SIGNATURES = {
                                       _vp, _vp]),
     "sffn_fp8_pack": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "sffn_fp8_unpack": (_int, [_vp, _i64, _vp, _i64, _i64, _int, _vp, _i64, _vp]),
-    "sffn_fp8_mm": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp, _vp]),
+    "sffn_fp8_mm_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "sffn_fp8_mm": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp, _sz, _vp, _vp]),
+    "sffn_fp8_linear_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "sffn_fp8_linear": (_int, [_vp, _int, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp, _sz, _vp, _vp]),
     "sffn_glu_up": (_int, [_int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _int, _vp, _vp, _i64,
                            _vp, _vp, _vp, _vp]),
     "sffn_glu_dgrad": (_int, [_int, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _int, _vp, _vp, _i64, _vp, _vp, _vp, _vp,
@@ -173,7 +176,7 @@ LAUNCHING = {"sffn_sp24_compress": 1, "sffn_gemm_sp24": 1, "sffn_sp24_overflow_a
              "sffn_gemm_bf16_f32acc": 1, "sffn_gemm_tf32": 1, "sffn_gemm_relu": 1,
              "sffn_round_tf32": 1, "sffn_token_logprobs": 1, "sffn_token_logprobs_bwd": 1, "sffn_distill_topk": 1,
              "sffn_distill_topk_bwd": 1, "sffn_residual_norm": 1, "sffn_residual_norm_bwd": 1,
-             "sffn_fp8_pack": 1, "sffn_fp8_unpack": 1, "sffn_fp8_mm": 1, "sffn_glu_up": 1, "sffn_glu_dgrad": 1,
+             "sffn_fp8_pack": 1, "sffn_fp8_unpack": 1, "sffn_fp8_mm": 1, "sffn_fp8_linear": 2, "sffn_glu_up": 1, "sffn_glu_dgrad": 1,
              "sffn_gemm16": 1, "sffn_few_rows_mm": 1, "sffn_few_rows_glu": 1, "sffn_few_rows_fp8": 1,
              "sffn_few_rows_ffn": 2, "sffn_pad_rows16": 1, "sffn_ckpt_linear": 1, "sffn_ckpt_linear_bwd": 1,
              "sffn_gated_ffn": 2, "sffn_gated_ffn_bwd": 1}
@@ -210,13 +213,16 @@ class KernelTimer:
         return out
 
 
+_FEW_ROWS = 16  # as in csrc/blocks.cu
+
+
 @functools.lru_cache(maxsize=4096)
 def _gemm16(M, N, K, K2=0):
     return 2 if load().sffn_gemm16_workspace_bytes(M, N, K, K2) else 1
 
 
 def _linear_launches(_dtype, _x, _ldx, _W, _ldw, odd, T, N, K, _y, values, *_):
-    return ((odd == 1) + 1 if T <= 32 else bool(odd) + _gemm16(T, N, K)) + bool(values)
+    return ((odd == 1) + 1 if T <= _FEW_ROWS else bool(odd) + _gemm16(T, N, K)) + bool(values)
 
 
 def _linear_bwd_launches(_dtype, _dy, _ldy, _W, _ldw, odd, _v, _ldv, _s, T, N, K, dx, dW, *_):
@@ -224,9 +230,9 @@ def _linear_bwd_launches(_dtype, _dy, _ldy, _W, _ldw, odd, _v, _ldv, _s, T, N, K
 
 
 def _gated_launches(_dtype, _act, keep, _x, _ldx, _wg, _ldg, _wu, _ldu, _w2, _ld2, odd, T, D, F, *_):
-    if keep == 0 and T <= 32:
+    if keep == 0 and T <= _FEW_ROWS:
         return 2 + (odd & 7 == 1)
-    return bool(odd & (7 if T <= 32 else 15)) + 1 + (1 if T <= 32 else _gemm16(T, D, F)) + (keep == 2)
+    return bool(odd & (7 if T <= _FEW_ROWS else 15)) + 1 + (1 if T <= _FEW_ROWS else _gemm16(T, D, F)) + (keep == 2)
 
 
 def _gated_bwd_launches(_dtype, _act, keep, steps, *a):
@@ -262,6 +268,10 @@ def _launches(name, args):
         return 2 if v is None or getattr(v, "value", v) in (None, 0) else 3
     if name == "sffn_gemm16":
         return 2 if args[18] else 1
+    if name == "sffn_fp8_mm":
+        return 2 if args[12] else 1
+    if name == "sffn_fp8_linear":
+        return 2 + (args[6] > _FEW_ROWS and load().sffn_fp8_mm_workspace_bytes(*args[6:9]) > 0)
     if name in _BLOCKS:
         return _BLOCKS[name](*args)
     if name == "sffn_residual_norm_bwd":

@@ -1,5 +1,5 @@
 // Products of few rows (single tokens, small batches) with long weights:
-// out[T, N] = x[T, K] W[N, K]^T for T <= 32, in 16 bits or in the 8-bit block
+// out[T, N] = x[T, K] W[N, K]^T for T <= 16, in 16 bits or in the 8-bit block
 // format, and the gated pair act(x Wg^T) * (x Wu^T).
 //
 // Bound by reading the weights once.  A tensor-core tile of 128 or 256 rows of
@@ -28,7 +28,7 @@
 namespace sffn {
 namespace {
 
-constexpr int S_MAX_ROWS = 32;
+constexpr int S_MAX_ROWS = 16;
 constexpr int S_WARPS = 16;                // that multiply
 constexpr int S_ADDERS = 3;                // that add and store
 constexpr int S_THREADS = (S_WARPS + 1 + S_ADDERS) * 32;
@@ -407,9 +407,7 @@ int launch_few_nt(FewArgs a, cudaStream_t st) {
 
 template <int DT, int OT, bool FP8, int MODE, int ACT, bool VEC>
 int launch_few(const FewArgs& a, cudaStream_t st) {
-    return a.T <= 8    ? launch_few_nt<DT, OT, FP8, MODE, ACT, 1, VEC>(a, st)
-           : a.T <= 16 ? launch_few_nt<DT, OT, FP8, MODE, ACT, 2, VEC>(a, st)
-                       : launch_few_nt<DT, OT, FP8, MODE, ACT, 4, VEC>(a, st);
+    return a.T <= 8 ? launch_few_nt<DT, OT, FP8, MODE, ACT, 1, VEC>(a, st) : launch_few_nt<DT, OT, FP8, MODE, ACT, 2, VEC>(a, st);
 }
 
 template <int DT, bool VEC>

@@ -26,9 +26,8 @@
 #include <cuda.h>
 #include <string.h>
 
-#include <algorithm>
-
 #include "fp8.cuh"
+#include "parts.cuh"
 #include "stage.cuh"
 #include "tmap.cuh"
 
@@ -55,6 +54,9 @@ struct MmArgs {
     uint16_t* out;
     long long ldc;
     int vec_out;
+    int splits, per_split;  // parts of K, k-blocks of each (a multiple of 4)
+    float* part;            // splits > 1: [splits][M][ldp]
+    long long ldp;
     uint32_t* status;
 };
 
@@ -104,12 +106,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tiles_mp = (args.tiles_m + 1) / 2;
-    const int ntiles = tiles_mp * args.tiles_n;
+    const int tiles = tiles_mp * args.tiles_n;
+    const int ntasks = tiles * args.splits;
     const int nkb = (args.K + 127) / 128;
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
-    const int first_tile = (int)cluster_id_x();
-    const int tile_stride = (int)cluster_count_x();
+    const int first_task = (int)cluster_id_x();
+    const int task_stride = (int)cluster_count_x();
+    // the tile of a task and its k-blocks; all tiles of one part of K run together
+    auto locate = [&](int task, int& pm, int& tn, int& kb0, int& kb1) {
+        const int sp = task / tiles;
+        pair_raster(task - sp * tiles, tiles_mp, args.tiles_n, pm, tn);
+        kb0 = sp * args.per_split;
+        kb1 = min(nkb, kb0 + args.per_split);
+        return sp;
+    };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < X_STAGES; ++s) {
@@ -142,12 +153,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
             long long kc = 0;
             int sgroup = 0;  // groups of up to four k-blocks with one tile of scales so far
             bool stop = false;
-            for (int tile = first_tile; tile < ntiles && !stop && !s_abort; tile += tile_stride) {
-                int pm, tn;
-                pair_raster(tile, tiles_mp, args.tiles_n, pm, tn);
+            for (int task = first_task; task < ntasks && !stop && !s_abort; task += task_stride) {
+                int pm, tn, kb0, kb1;
+                locate(task, pm, tn, kb0, kb1);
                 const int arow = (pm * 2 + (int)rank) * 128;
                 const int brow = tn * 256 + (int)rank * 128;
-                for (int kb = 0; kb < nkb; ++kb, ++kc) {
+                for (int kb = kb0; kb < kb1; ++kb, ++kc) {
                     if (op == 2 ? (kb & 3) != 0 : (int)(kc % X_ISSUERS) != warp % X_ISSUERS) continue;
                     const int stage = (int)(kc % X_STAGES);
                     const uint32_t phase = (uint32_t)((kc / X_STAGES) & 1);
@@ -188,7 +199,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
         if (lane == 0 && leader) {
             int stage = 0, it = 0, sgroup = -1;
             uint32_t phase = 0;
-            for (int tile = first_tile; tile < ntiles && !s_abort; tile += tile_stride, ++it) {
+            for (int task = first_task; task < ntasks && !s_abort; task += task_stride, ++it) {
+                int pm, tn, kb0, kb1;
+                locate(task, pm, tn, kb0, kb1);
                 if (!mbar_wait_bounded(&tempty_bar, ((uint32_t)it & 1u) ^ 1u)) {
                     atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
                     s_abort = 1;
@@ -196,7 +209,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
                 }
                 tc_fence_after();
                 bool ready = mbar_try_wait(&full_bar[stage], phase), fail = false;
-                for (int kb = 0; kb < nkb; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!ready && !mbar_wait_bounded(&full_bar[stage], phase)) {
                         atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
                         s_abort = 1;
@@ -218,13 +231,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         mma_mx_pair(tmem_base, umma_desc_sw128(sa + 32 * j, 16, 1024), umma_desc_sw128(sb + 32 * j, 16, 1024),
-                                    idesc, ta, tb, (kb | j) != 0 ? 1u : 0u);
+                                    idesc, ta, tb, ((kb - kb0) | j) != 0 ? 1u : 0u);
                     tc_commit_pair_multicast(&empty_bar[stage], 0x3);
                     if (++stage == X_STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
-                    ready = kb + 1 < nkb && mbar_try_wait(&full_bar[stage], phase);
+                    ready = kb + 1 < kb1 && mbar_try_wait(&full_bar[stage], phase);
                 }
                 if (fail) break;
                 tc_commit_pair_multicast(&tfull_bar, 0x3);
@@ -239,9 +252,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
         const uint32_t tempty_leader = leader_smem_addr(&tempty_bar);
         const uint32_t lane_base = tmem_base + ((uint32_t)(ew * 32) << 16);
         int it = 0;
-        for (int tile = first_tile; tile < ntiles; tile += tile_stride, ++it) {
-            int pm, tn;
-            pair_raster(tile, tiles_mp, args.tiles_n, pm, tn);
+        for (int task = first_task; task < ntasks; task += task_stride, ++it) {
+            int pm, tn, kb0, kb1;
+            const int sp = locate(task, pm, tn, kb0, kb1);
             const int row0 = (pm * 2 + (int)rank) * 128 + ew * 32, col0 = tn * 256 + wg * 128;
             const bool ok = __all_sync(FULL, mbar_wait_bounded(&tfull_bar, (uint32_t)it & 1u));
             if (!ok || __any_sync(FULL, s_abort != 0)) {
@@ -249,6 +262,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
                 break;
             }
             tc_fence_after();
+            if (args.splits > 1) {  // float32 parts: each lane its row's 128 contiguous bytes
+#pragma unroll 1
+                for (int c = 0; c < 4 && row0 < args.M && col0 + c * 32 < args.N; ++c) {
+                    uint32_t r[32];
+                    tmem_ld32(lane_base + (uint32_t)(wg * 128 + c * 32), r);
+                    tmem_wait_ld();
+                    if (row0 + lane < args.M) {
+                        float* p = args.part + ((long long)sp * args.M + row0 + lane) * args.ldp + col0 + c * 32;
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)
+                            if (col0 + c * 32 + 4 * q < args.ldp)  // ldp is a multiple of 4
+                                reinterpret_cast<uint4*>(p)[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(tempty_leader);
+                continue;
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t r[32], w[16];
@@ -316,7 +348,7 @@ int launch_mm(const void* a, long long lda, const void* as, const void* b, long 
     if (int rc = tmap_2d(&tb, u8, 1, b, args.K, args.N, ldb, 128, 128, sw)) return rc;
     if (int rc = scale_map(&tsa, as, args.tiles_m, args.bt, 1)) return rc;
     if (int rc = scale_map(&tsb, bs, args.tiles_b, args.bt, 2)) return rc;
-    if (args.vec_out)
+    if (args.vec_out && args.splits == 1)
         if (int rc = tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, args.out, args.N, args.M, args.ldc, 32, 32,
                              CU_TENSOR_MAP_SWIZZLE_64B))
             return rc;
@@ -324,11 +356,21 @@ int launch_mm(const void* a, long long lda, const void* as, const void* b, long 
     static SmemOnce once;
     SFFN_CUDA_TRY(once.set(k, X_SMEM));
     static const int pairs = resident_pairs(k, X_THREADS, X_SMEM);
-    const long long ntiles = (long long)((args.tiles_m + 1) / 2) * args.tiles_n;
-    const int clusters = (int)std::min<long long>(ntiles, pairs);
+    const long long tasks = (long long)((args.tiles_m + 1) / 2) * args.tiles_n * args.splits;
+    const int clusters = (int)std::min<long long>(tasks, pairs);
     k<<<clusters * 2, X_THREADS, X_SMEM, st>>>(ta, tb, tsa, tsb, tc, args);
     SFFN_CHECK_LAUNCH();
-    return SFFN_OK;
+    return args.splits > 1 ? join_parts<DT>(args.part, args.splits, args.M, args.N, args.out, args.ldc, st) : SFFN_OK;
+}
+
+// Parts of K: a 128-wide k-block of a pair takes about 0.45 us, four share a scale tile.
+int split8(long long M, long long N, long long K) { return split_of(M, N, (K + 127) / 128, 4, 0.45); }
+
+// Coordinates and scale rows are 32-bit in the tensor maps.
+bool mm_sizes_ok(long long M, long long N, long long K) {
+    const long long most = 0x7FFFFF00;
+    return M <= most && N <= most && K <= most && (M + 127) / 128 * fp8_block_tiles(K) * 32 <= 0x7FFFFFFF &&
+           (N + 127) / 128 * fp8_block_tiles(K) * 32 <= 0x7FFFFFFF && tiles_of(M, N) <= 0x1FFFFFF;
 }
 
 }  // namespace
@@ -336,20 +378,25 @@ int launch_mm(const void* a, long long lda, const void* as, const void* b, long 
 
 using namespace sffn;
 
+extern "C" size_t sffn_fp8_mm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || !mm_sizes_ok(M, N, K)) return 0;
+    const int s = split8(M, N, K);
+    return s > 1 ? (size_t)s * (size_t)M * (size_t)part_ld(N) * 4 : 0;
+}
+
 extern "C" int sffn_fp8_mm(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb,
                            const void* b_scales, int64_t M, int64_t N, int64_t K, void* C, int c_dtype, int64_t ldc,
-                           uint32_t* status_dev, void* stream) {
+                           void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream) {
     if (c_dtype != SFFN_BF16 && c_dtype != SFFN_F16) return SFFN_ERR_DTYPE;
     if (M < 0 || N < 0 || K <= 0) return SFFN_ERR_ARG;
     if (M == 0 || N == 0) return SFFN_OK;
     if (!a || !a_scales || !b || !b_scales || !C || !status_dev || lda < K || ldb < K || ldc < N) return SFFN_ERR_ARG;
-    // coordinates and scale rows are 32-bit in the tensor maps
-    if (M > 0x7FFFFF00 || N > 0x7FFFFF00 || K > 0x7FFFFF00 || (M + 127) / 128 * fp8_block_tiles(K) * 32 > 0x7FFFFFFF ||
-        (N + 127) / 128 * fp8_block_tiles(K) * 32 > 0x7FFFFFFF || (M + 255) / 256 * ((N + 255) / 256) > 0x3FFFFFFF)
-        return SFFN_ERR_TOO_LARGE;
+    if (!mm_sizes_ok(M, N, K)) return SFFN_ERR_TOO_LARGE;
     if (!aligned16(a) || !aligned16(b) || !aligned16(a_scales) || !aligned16(b_scales) || lda % 16 || ldb % 16 ||
-        reinterpret_cast<uintptr_t>(C) % 2)
+        reinterpret_cast<uintptr_t>(C) % 2 || !aligned16(workspace))
         return SFFN_ERR_ALIGN;
+    const size_t need = sffn_fp8_mm_workspace_bytes(M, N, K);
+    if (need && (!workspace || workspace_bytes < need)) return SFFN_ERR_WORKSPACE;
     DeviceScope scope;
     if (int rc = scope.bind(a)) return rc;
     if (!sm100_sms()) return SFFN_ERR_DEVICE;
@@ -364,6 +411,11 @@ extern "C" int sffn_fp8_mm(const void* a, int64_t lda, const void* a_scales, con
     args.out = static_cast<uint16_t*>(C);
     args.ldc = ldc;
     args.vec_out = aligned16(C) && ldc % 8 == 0;
+    args.splits = split8(M, N, K);
+    const int nkb = (int)((K + 127) / 128);
+    args.per_split = ((nkb + 3) / 4 + args.splits - 1) / args.splits * 4;
+    args.part = static_cast<float*>(workspace);
+    args.ldp = part_ld(N);
     args.status = status_dev;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return c_dtype == SFFN_BF16 ? launch_mm<SFFN_BF16>(a, lda, a_scales, b, ldb, b_scales, args, st)

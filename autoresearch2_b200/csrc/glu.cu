@@ -28,6 +28,7 @@
 
 #include "act.cuh"
 #include "fp8.cuh"
+#include "parts.cuh"
 #include "stage.cuh"
 #include "tmap.cuh"
 
@@ -543,34 +544,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     }
 }
 
-// C = the parts of a product split over K, added in their order.
-template <int DT>
-__global__ void __launch_bounds__(256)
-    join_parts_kernel(const float* __restrict__ part, int splits, long long M, int N, long long ldp, uint16_t* __restrict__ out,
-                      long long ldc, int vec) {
-    const long long quads = ldp / 4, n = M * quads;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const long long row = i / quads;
-        const int col = (int)(i - row * quads) * 4;
-        const float4* p = reinterpret_cast<const float4*>(part + row * ldp + col);
-        float4 s = __ldcs(p);
-        for (int k = 1; k < splits; ++k) {
-            const float4 v = __ldcs(p + k * (M * quads));
-            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-        }
-        uint16_t* o = out + row * ldc + col;
-        const uint2 w = make_uint2(pack16x2<DT>(s.x, s.y), pack16x2<DT>(s.z, s.w));
-        if (vec && col + 4 <= N) {
-            *reinterpret_cast<uint2*>(o) = w;
-        } else {
-            if (col < N) o[0] = (uint16_t)w.x;
-            if (col + 1 < N) o[1] = (uint16_t)(w.x >> 16);
-            if (col + 2 < N) o[2] = (uint16_t)w.y;
-            if (col + 3 < N) o[3] = (uint16_t)(w.y >> 16);
-        }
-    }
-}
-
 // ------------------------------------------------------------------ host ----
 struct Operand {
     const void* p;
@@ -612,29 +585,9 @@ int launch_pair(const CUtensorMap (&m)[9], const PairArgs& args, cudaStream_t st
     return SFFN_OK;
 }
 
-constexpr int P_PAIRS = 74;  // CTA pairs of a B200
-
-// How many parts K is split into: a product of few tiles leaves pairs idle, so
-// its k-blocks are dealt to more of them.  Costs are counted in k-blocks of one
-// pair (about 0.27 us at 256 x 256 x 64): the rounds of tasks times a part's
-// blocks, 4 to fill the pipeline, and for parts their float32 traffic (8 bytes
-// an element and part through HBM: 0.011 us a tile and part over 74 pairs) and
-// the second kernel (3 us).
-int split_of(long long tiles, long long nkb) {
-    long long best = 0;
-    int best_s = 1;
-    for (int s = 1; s <= 32 && s <= nkb; ++s) {
-        const long long per = (nkb + s - 1) / s;
-        if ((nkb + per - 1) / per != s) continue;
-        const long long rounds = (tiles * s + P_PAIRS - 1) / P_PAIRS;
-        const long long cost = 100 * rounds * (per + 4) + (s > 1 ? 1100 + 30 * tiles * s : 0);
-        if (s == 1 || cost < best) best = cost, best_s = s;
-    }
-    return best_s;
-}
-long long tiles_of(long long M, long long N) { return (M + 255) / 256 * ((N + 255) / 256); }
+// How many parts K is split into; a k-block of a pair takes about 0.27 us.
+int split16(long long M, long long N, long long nkb) { return split_of(M, N, nkb, 1, 0.27); }
 long long kblocks(long long K) { return (K + P_BK - 1) / P_BK; }
-long long part_ld(long long N) { return (N + 3) / 4 * 4; }
 
 bool sizes_ok(long long M, long long N, long long K) {
     const long long most = 0x7FFFFF00;
@@ -652,7 +605,7 @@ int gemm16(const Operand& A, bool a_mn, const Operand& B, bool b_mn, const Opera
     a.tiles_n = (int)((N + 255) / 256);
     a.nkb1 = (int)kblocks(K);
     a.nkb = a.nkb1 + (K2 ? (int)kblocks(K2) : 0);
-    a.splits = split_of(tiles_of(M, N), a.nkb);
+    a.splits = split16(M, N, a.nkb);
     a.ldp = part_ld(N);
     if (a.splits > 1 && (!ws || ws_bytes < (size_t)a.splits * (size_t)M * (size_t)a.ldp * 4)) return SFFN_ERR_WORKSPACE;
     a.per_split = (a.nkb + a.splits - 1) / a.splits;
@@ -676,12 +629,7 @@ int gemm16(const Operand& A, bool a_mn, const Operand& B, bool b_mn, const Opera
              : b_mn         ? launch_pair<DT, true, true, P_STORE, 0>(m, a, st)
                             : launch_pair<DT, true, false, P_STORE, 0>(m, a, st);
     if (rc || a.splits == 1) return rc;
-    const long long quads = M * (a.ldp / 4);
-    const int grid = (int)std::min<long long>((quads + 255) / 256, 148 * 8);
-    join_parts_kernel<DT><<<grid, 256, 0, st>>>(a.part, a.splits, M, (int)N, a.ldp, a.out, ldc,
-                                                 reinterpret_cast<uintptr_t>(C) % 8 == 0 && ldc % 4 == 0);
-    SFFN_CHECK_LAUNCH();
-    return SFFN_OK;
+    return join_parts<DT>(a.part, a.splits, M, (int)N, C, ldc, st);
 }
 
 template <int DT, int EPI, bool B_MN>
@@ -730,7 +678,7 @@ using namespace sffn;
 
 extern "C" size_t sffn_gemm16_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t K2) {
     if (M <= 0 || N <= 0 || K <= 0 || K2 < 0 || !sizes_ok(M, N, K) || !sizes_ok(M, N, K2)) return 0;
-    const int s = split_of(tiles_of(M, N), kblocks(K) + (K2 ? kblocks(K2) : 0));
+    const int s = split16(M, N, kblocks(K) + (K2 ? kblocks(K2) : 0));
     return s > 1 ? (size_t)s * (size_t)M * (size_t)part_ld(N) * 4 : 0;
 }
 

@@ -24,7 +24,7 @@ __all__ = ["BLOCK", "Fp8Tensor", "fp8_pack", "fp8_unpack", "fp8_matmul", "ckpt_l
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
-FEW_ROWS = 32  # products of at most so many rows read the weights by the few-row kernels
+FEW_ROWS = 16  # products of at most so many rows go by the few-row kernels
 OUT_TYPES = (torch.bfloat16, torch.float16)
 
 
@@ -192,19 +192,47 @@ def fp8_unpack(q, dtype=torch.bfloat16):
 # ---------------------------------------------------------------------------
 # The product
 # ---------------------------------------------------------------------------
+@functools.lru_cache(maxsize=4096)
+def _product_workspace(packed, M, N, K):
+    return getattr(_lib.load(), "sffn_fp8_mm_workspace_bytes" if packed else "sffn_fp8_linear_workspace_bytes")(M, N, K)
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 def _matmul(av, at, bv, bt, out_dtype):
     M, K = av.shape
     N = bv.shape[0]
     dev = av.device
     out = torch.empty((M, N), dtype=out_dtype, device=dev)
-    if not out.numel():
+    if not (M and N):
         return out
+    code, status, stream = _lib._DTYPES[out_dtype], _lib.status_word(dev).data_ptr(), stream_handle(dev)
     if M <= FEW_ROWS:
         call("sffn_few_rows_fp8", av.data_ptr(), _stride(av), at.data_ptr(), bv.data_ptr(), _stride(bv), bt.data_ptr(), M, N,
-             K, out.data_ptr(), _lib._DTYPES[out_dtype], N, _lib.status_word(dev).data_ptr(), stream_handle(dev))
+             K, out.data_ptr(), code, N, status, stream)
     else:
+        n = _product_workspace(True, M, N, K)
+        ws = _workspace(n, dev)
         call("sffn_fp8_mm", av.data_ptr(), _stride(av), at.data_ptr(), bv.data_ptr(), _stride(bv), bt.data_ptr(), M, N, K,
-             out.data_ptr(), _lib._DTYPES[out_dtype], N, _lib.status_word(dev).data_ptr(), stream_handle(dev))
+             out.data_ptr(), code, N, ptr(ws), n, status, stream)
+    return out
+
+
+def _pack_matmul(x, bv, bt, out_dtype):
+    """x [..., K] packed on the way, in one call."""
+    x2 = _rows(x)
+    M, K = x2.shape
+    N = bv.shape[0]
+    dev = x.device
+    out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    if M and N:
+        n = _product_workspace(False, M, N, K)
+        ws = _workspace(n, dev)
+        call("sffn_fp8_linear", x2.data_ptr(), _lib._DTYPES[x.dtype], _ld(x2), bv.data_ptr(), _stride(bv), bt.data_ptr(), M, N,
+             K, out.data_ptr(), _lib._DTYPES[out_dtype], N, ws.data_ptr(), n, _lib.status_word(dev).data_ptr(),
+             stream_handle(dev))
     return out
 
 
@@ -216,7 +244,7 @@ def _check_product(av, bv, out_dtype):
         raise ValueError(f"a has rows of {av.shape[-1]}, b of {bv.shape[-1]}")
     if av.device != bv.device:
         raise ValueError(f"a is on {av.device}, b on {bv.device}")
-    if av.data_ptr() % 16 or bv.data_ptr() % 16:
+    if bv.data_ptr() % 16 or (av.dtype == E4M3 and av.data_ptr() % 16):
         raise ValueError("values must start on 16 bytes")
 
 
@@ -230,20 +258,22 @@ def fp8_matmul(a, b, out_dtype=None):
     Not differentiable."""
     if not isinstance(b, Fp8Tensor) or len(b.shape) != 2:
         raise TypeError("b must be an Fp8Tensor [N, K]")
-    if not isinstance(a, Fp8Tensor):
+    packed = isinstance(a, Fp8Tensor)
+    if not packed:
         _check_pack(a)
         _refuse_grad("fp8_matmul", a)
         if out_dtype is None and a.dtype in OUT_TYPES:
             out_dtype = a.dtype
-        if a.shape[-1] != b.shape[-1]:
-            raise ValueError(f"a has rows of {a.shape[-1]}, b of {b.shape[-1]}")
-        a = fp8_pack(a)
     out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
     if torch.compiler.is_compiling():
-        out = torch.ops.sparseffn.fp8_matmul(a.values, a.scale_tiles, b.values, b.scale_tiles, out_dtype)
-    else:
+        av, at = (a.values, a.scale_tiles) if packed else torch.ops.sparseffn.fp8_pack(a)
+        out = torch.ops.sparseffn.fp8_matmul(av, at, b.values, b.scale_tiles, out_dtype)
+    elif packed:
         _check_product(a.values, b.values, out_dtype)
         out = _matmul(a.values, a.scale_tiles, b.values, b.scale_tiles, out_dtype)
+    else:
+        _check_product(a, b.values, out_dtype)
+        out = _pack_matmul(a, b.values, b.scale_tiles, out_dtype)
     return out if len(a.shape) == 2 else out.view(*a.shape[:-1], b.shape[0])
 
 
@@ -281,10 +311,6 @@ def _check_linear(x, W):
 @functools.lru_cache(maxsize=4096)
 def _linear_workspace(backward, odd, want, T, N, K):
     return _lib.load().sffn_ckpt_linear_workspace_bytes(backward, odd, want, T, N, K)
-
-
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _linear_forward(x, W, keep):

@@ -647,10 +647,20 @@ int sffn_fp8_unpack(const void* values, int64_t ldv, const void* scales, int64_t
                     void* out, int64_t ldo, void* stream);
 
 /* C [M, N] (SFFN_BF16 or SFFN_F16) = A [M, K] B [N, K]^T, both in 8-bit blocks,
- * on the block-scaled tensor cores. */
+ * on the block-scaled tensor cores.  Products of few tiles and a long K are split
+ * over K: their float32 parts go to the workspace (NULL where
+ * sffn_fp8_mm_workspace_bytes is 0). */
+size_t sffn_fp8_mm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int sffn_fp8_mm(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb, const void* b_scales,
-                int64_t M, int64_t N, int64_t K, void* C, int c_dtype, int64_t ldc, uint32_t* status_dev,
-                void* stream);
+                int64_t M, int64_t N, int64_t K, void* C, int c_dtype, int64_t ldc, void* workspace,
+                size_t workspace_bytes, uint32_t* status_dev, void* stream);
+
+/* The same with A = x [M, K] of dtype (any alignment), packed first: into the
+ * workspace, with the parts.  Up to 16 rows go by sffn_few_rows_fp8. */
+size_t sffn_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int sffn_fp8_linear(const void* x, int dtype, int64_t ldx, const void* b, int64_t ldb, const void* b_scales, int64_t M,
+                    int64_t N, int64_t K, void* C, int c_dtype, int64_t ldc, void* workspace, size_t workspace_bytes,
+                    uint32_t* status_dev, void* stream);
 
 /* Copies up to four 16-bit matrices to rows on 16 bytes.  desc: six numbers a
  * matrix -- source address, rows, columns, row stride, destination address (on
@@ -696,7 +706,7 @@ int sffn_gemm16(int dtype, const void* A, int64_t lda, int a_mn, const void* B, 
                 int64_t lda2, const void* B2, int64_t ldb2, int64_t K2, int64_t M, int64_t N, int64_t K, void* C,
                 int64_t ldc, void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream);
 
-/* Products of at most 32 rows with long weights (any alignment): out [T, N] =
+/* Products of at most 16 rows with long weights (any alignment): out [T, N] =
  * x w^T; h [T, F] = act(x wg^T) * (x wu^T); and x w^T in 8-bit blocks. */
 int sffn_few_rows_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t T, int64_t N, int64_t K,
                      void* out, int64_t ldo, uint32_t* status_dev, void* stream);

@@ -249,19 +249,26 @@ def test_pack_entry(lib):
 
 
 def test_product_entries(lib):
-    ok = [P, 48, P, P, 48, P, 100, 8, 40, P, 1, 8, P, None]
     for f, few in ((lib.sffn_fp8_mm, False), (lib.sffn_few_rows_fp8, True)):
+        ok = [P, 48, P, P, 48, P, 100, 8, 40, P, 1, 8, None, 0, P, None]
         if few:
-            ok[6] = 10
-            assert rc(f, ok, _6=33) == 1
+            ok[6:] = [10, 8, 40, P, 1, 8, P, None]
+            assert rc(f, ok, _6=17) == 1
         assert rc(f, ok, _10=0) == 2 and rc(f, ok, _6=-1) == 1 and rc(f, ok, _8=0) == 1 and rc(f, ok, _6=0) == 0 and rc(f, ok, _7=0) == 0
-        for i in (0, 2, 3, 5, 9, 12):
+        for i in (0, 2, 3, 5, 9, len(ok) - 2):
             assert rc(f, ok, **{f"_{i}": None}) == 1
         assert rc(f, ok, _1=32) == 1 and rc(f, ok, _4=32) == 1 and rc(f, ok, _11=7) == 1
         assert rc(f, ok, _1=56) == 3 and rc(f, ok, _0=ODD) == 3 and rc(f, ok, _3=ODD) == 3 and rc(f, ok, _9=vp((1 << 20) + 1)) == 3
         assert rc(f, ok, _2=ODD) == 3 and rc(f, ok, _5=ODD) == 3
         assert rc(f, ok, _7=BIG, _11=BIG) == 8
-    assert rc(lib.sffn_fp8_mm, [P, 48, P, P, 48, P, BIG, 8, 40, P, 1, 8, P, None]) == 8
+    f, ok = lib.sffn_fp8_mm, [P, 16384, P, P, 16384, P, 100, 512, 16384, P, 1, 512, P, 1 << 30, P, None]
+    assert rc(f, ok, _6=BIG) == 8 and rc(f, ok, _12=None) == 4 and rc(f, ok, _13=100) == 4 and rc(f, ok, _12=ODD) == 3
+    w = lib.sffn_fp8_mm_workspace_bytes
+    assert w(16384, 8192, 4096) == 0 and w(0, 8, 8) == 0 and w(100, 512, 16384) % (100 * 512 * 4) == 0 and w(100, 512, 16384)
+    f, ok = lib.sffn_fp8_linear, [P, 1, 40, P, 48, P, 100, 8, 40, P, 1, 8, P, 1 << 20, P, None]
+    assert lib.sffn_fp8_linear_workspace_bytes(100, 8, 40) == 100 * 48 + (-100 * 48) % 256 + 512
+    assert rc(f, ok, _1=3) == 2 and rc(f, ok, _6=0) == 1 and rc(f, ok, _0=None) == 1 and rc(f, ok, _12=None) == 4 and rc(f, ok, _13=100) == 4
+    assert rc(f, ok, _12=ODD) == 3
 
 
 def test_gemm_entry(lib):
@@ -296,16 +303,16 @@ def test_gated_entries(lib):
 def test_few_row_entries(lib):
     mm = [1, P, 40, P, 40, 10, 64, 40, P, 64, P, None]
     f = lib.sffn_few_rows_mm
-    assert rc(f, mm, _0=0) == 2 and rc(f, mm, _5=33) == 1 and rc(f, mm, _7=0) == 1 and rc(f, mm, _5=0) == 0 and rc(f, mm, _6=0) == 0
+    assert rc(f, mm, _0=0) == 2 and rc(f, mm, _5=17) == 1 and rc(f, mm, _7=0) == 1 and rc(f, mm, _5=0) == 0 and rc(f, mm, _6=0) == 0
     for i in (1, 3, 8, 10):
         assert rc(f, mm, **{f"_{i}": None}) == 1
     assert rc(f, mm, _2=39) == 1 and rc(f, mm, _4=39) == 1 and rc(f, mm, _9=63) == 1 and rc(f, mm, _1=vp((1 << 20) + 1)) == 3
     g = [1, 2, P, 40, P, 40, P, 40, 10, 40, 64, P, 64, P, None]
     f = lib.sffn_few_rows_glu
-    assert rc(f, g, _0=0) == 2 and rc(f, g, _1=-1) == 1 and rc(f, g, _8=33) == 1 and rc(f, g, _8=0) == 0 and rc(f, g, _5=39) == 1
+    assert rc(f, g, _0=0) == 2 and rc(f, g, _1=-1) == 1 and rc(f, g, _8=17) == 1 and rc(f, g, _8=0) == 0 and rc(f, g, _5=39) == 1
     f = lib.sffn_few_rows_ffn
     b = [1, 2, P, 40, P, 40, P, 40, P, 64, 10, 40, 64, P, 64, P, 40, P, None]
-    assert rc(f, b, _0=0) == 2 and rc(f, b, _13=None) == 1 and rc(f, b, _10=33) == 1
+    assert rc(f, b, _0=0) == 2 and rc(f, b, _13=None) == 1 and rc(f, b, _10=17) == 1
 
 
 def test_pad_entry(lib):
@@ -327,6 +334,10 @@ def test_workspace_and_launches(lib):
     a = [None] * 21
     assert _lib._launches("sffn_gemm16", a) == 1
     a[18] = n
+    b = [None] * 6 + [100, 512, 16384] + [None] * 7
+    assert _lib._launches("sffn_fp8_mm", b) == 1 and _lib._launches("sffn_fp8_linear", b) == 3
+    b[6], b[12] = 16, 1
+    assert _lib._launches("sffn_fp8_mm", b) == 2 and _lib._launches("sffn_fp8_linear", b) == 2
     assert _lib._launches("sffn_gemm16", a) == 2 and _lib._launches("sffn_few_rows_ffn", []) == 2
 
 

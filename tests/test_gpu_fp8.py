@@ -143,7 +143,8 @@ def test_pack_of_no_rows():
 SIZES = [(1, 64, 64), (1, 1000, 4096), (8, 48, 16), (9, 130, 1001), (16, 256, 640), (17, 33, 129), (32, 300, 2048),
          (33, 64, 64), (64, 100, 130), (128, 128, 128), (129, 257, 513), (200, 1000, 1333), (256, 256, 512), (300, 515, 4096),
          (777, 1001, 96), (1, 1, 1), (40, 1, 7), (513, 768, 16384), (1, 5003, 3000), (16, 4800, 1100),
-         (30, 9001, 700)]  # the last three: several groups of rows a multiprocessor
+         (10, 9001, 700),  # these three: several groups of rows a multiprocessor
+         (40, 300, 14336), (300, 257, 9000), (17, 1001, 2049)]  # in parts of K
 
 
 @pytest.mark.parametrize("out", [BF16, F16])
@@ -223,6 +224,8 @@ def test_product_beside_others_rows():
         big = torch.full((M + 2, N + 3), 7.0, device=DEV, dtype=BF16)
         args = [qa.values.data_ptr(), 208, qa.scale_tiles.data_ptr(), qb.values.data_ptr(), 208, qb.scale_tiles.data_ptr(), M,
                 N, K, big[1:, 1:].data_ptr(), 1, N + 3]
+        if M > fp8.FEW_ROWS:
+            args += [None, 0]
         _lib.call("sffn_few_rows_fp8" if M <= fp8.FEW_ROWS else "sffn_fp8_mm", *args,
                   _lib.status_word(big.device).data_ptr(), _lib.stream_handle(big.device))
         inner = torch.zeros_like(big, dtype=torch.bool)
