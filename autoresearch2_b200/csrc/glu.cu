@@ -1,14 +1,20 @@
 // The gated feed-forward block h = act(x Wg^T) * (x Wu^T), y = h W2^T, and the
 // products of its backward, in bfloat16 or float16 on the tcgen05 tensor cores.
 //
+// Bound by the tensor cores under the power limit where K is long (UP of 8192 x
+// 4096 x 14336: 1.54 ms, 1250 TF), by the operands' way from L2 where it is short:
+// at 32768 x 768 x 2048 UP reads 1.57 GB of tiles from L2 in 165 us, 9.5 TB/s, the
+// rate that plain products of this K have too (32768 x 768 x 2304: 96 us).  DGRAD,
+// 167 us there, adds 0.13 GB of g and u and 0.4 GB of results to 0.8 GB of tiles.
+//
 // One kernel: CTA pairs (tcgen05.mma.cta_group::2, 256 x 256 tiles, float32
 // accumulation in tensor memory, two accumulators), persistent over tiles;
 // operands by TMA in a ring of 64-wide k-blocks, either major order, so no
 // operand is transposed.
-//   warps 0,2 / 3,12  issuers of A / B (even / odd k-blocks)
-//   warp 1            MMA issuer (leader CTA)
-//   warp 2            also tensor memory
-//   warps 4-11        epilogue, two warpgroups; thread = accumulator row
+//   warps 0,2 / 3 and the last  issuers of A / B (even / odd k-blocks)
+//   warp 1                      MMA issuer (leader CTA)
+//   warp 2                      also tensor memory
+//   warps 4-11 or 4-19          epilogue, two or four warpgroups; thread = accumulator row
 // Epilogues:
 //   STORE  C in 16 bits; or, split over K, float32 parts that a second kernel
 //          adds in order (few tiles and a long K: weight gradients).  K may run
@@ -39,21 +45,26 @@ enum { P_STORE = 0, P_UP = 1, P_DGRAD = 2 };
 enum { KEEP_NONE = 0, KEEP_16 = 1, KEEP_8 = 2 };
 
 constexpr int P_BK = 64;
-constexpr int P_THREADS = 416;
+// Warps of the epilogue: eight store, sixteen where they compute as well: chains of
+// conversions, exponentials and reciprocals, and copies to wait for (with eight, UP
+// and DGRAD of 32768 x 768 x 2048 took 173 and 178 us instead of 165 and 167).
+template <int EPI>
+constexpr int p_epi() { return EPI == P_STORE ? 8 : 16; }
+template <int EPI>
+constexpr int p_threads() { return (5 + p_epi<EPI>()) * 32; }
 constexpr int P_OPERAND = 128 * P_BK * 2;  // bytes of one operand a stage and CTA
 constexpr int P_STAGE = 2 * P_OPERAND;
-// The fused epilogues store three matrices instead of one and have more staging
-// buffers a warp; their operand rings have four stages to make room.  Even
-// counts: the issuers take alternate k-blocks.
+// Even counts: the issuers take alternate k-blocks.
 template <int EPI>
 constexpr int p_stages() { return EPI == P_STORE ? 6 : 4; }
+// Bytes an epilogue warp has for staging: STORE two blocks of 32 x 32, UP three
+// (h, g, u; in 8 bits g and u share one, the third is for the amax), DGRAD two
+// and its g and u as kept.
 template <int EPI>
-constexpr int p_bufs() { return EPI == P_STORE ? 2 : EPI == P_UP ? 5 : 4; }
-constexpr int P_KEPT = 4096;  // DGRAD: a warp's 32 x 32 of g and of u as kept
+constexpr int p_own() { return EPI == P_STORE ? 4096 : 6144; }
 template <int EPI>
-constexpr int p_smem() { return p_stages<EPI>() * P_STAGE + 8 * (p_bufs<EPI>() * 2048 + (EPI == P_DGRAD ? P_KEPT : 0)) + 1024; }
-static_assert(p_smem<P_STORE>() <= 227 * 1024 - 1024 && p_smem<P_UP>() <= 227 * 1024 - 6144 &&
-              p_smem<P_DGRAD>() <= 227 * 1024 - 1024, "shared memory");
+constexpr int p_smem() { return p_stages<EPI>() * P_STAGE + p_epi<EPI>() * p_own<EPI>() + 1024; }
+static_assert(p_smem<P_STORE>() <= 227 * 1024 - 1024 && p_smem<P_UP>() <= 227 * 1024 - 1024, "shared memory");
 
 struct PairArgs {
     int M, N;
@@ -86,7 +97,7 @@ __device__ __forceinline__ uint32_t fp8_four(Float2 lo, Float2 hi) {
 }
 
 template <int DT, bool A_MN, bool B_MN, int EPI, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(p_threads<EPI>(), 1)
     pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2,
                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmC2,
@@ -96,15 +107,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     constexpr uint32_t IDESC = idesc16<DT>(A_MN, B_MN);
     constexpr uint32_t MN_LBO = P_BK * 128;  // MN-major: 64-element blocks of 64 K rows x 128 bytes
     constexpr int TILE_N = EPI == P_UP ? 128 : 256;
+    constexpr int EW = p_epi<EPI>(), WG_N = TILE_N / (EW / 4);  // epilogue warps; columns of a warpgroup
     extern __shared__ __align__(1024) unsigned char p_smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p_smem_raw) + 1023) &
                                                            ~static_cast<uintptr_t>(1023));
     __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST];
     __shared__ __align__(8) uint64_t tfull_bar[2], tempty_bar[2];
-    __shared__ __align__(8) uint64_t kept_bar[8][2];  // DGRAD: each epilogue warp's g and u have come
+    __shared__ __align__(8) uint64_t kept_bar[EW];  // DGRAD: each epilogue warp's g and u have come
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_dead;
-    __shared__ uint2 s_amax[EPI == P_UP ? 2 : 1][2][128];  // UP: [tile parity][warpgroup][row], of g and u
+    __shared__ int s_abort;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tiles_mp = (args.tiles_m + 1) / 2;
@@ -136,10 +147,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&tfull_bar[a], 1);
-            mbar_init(&tempty_bar[a], 16);  // the epilogue warps of both CTAs
+            mbar_init(&tempty_bar[a], 2 * EW);  // the epilogue warps of both CTAs
         }
-        for (int w = 0; w < 16; ++w) mbar_init(&kept_bar[w >> 1][w & 1], 1);
-        s_abort = s_dead = 0;
+        for (int w = 0; w < EW; ++w) mbar_init(&kept_bar[w], 1);
+        s_abort = 0;
         fence_mbar_init();
         prefetch_tmap(&tmA);
         prefetch_tmap(&tmB);
@@ -153,7 +164,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     tc_fence_after();
     const uint32_t tmem_base = s_tmem;
 
-    if (warp == 0 || warp == 2 || warp == 3 || warp == 12) {
+    if (warp == 0 || warp == 2 || warp == 3 || warp == 4 + EW) {
         // ----------------------------------------------------- producers --
         // Four issuing threads, one per (operand, k-block parity): one thread's
         // copies complete one after another.  B's bytes may land before the A
@@ -263,44 +274,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             }
         }
         __syncwarp();
-    } else if (warp >= 4 && warp < 12) {
+    } else if (warp >= 4) {
         // ------------------------------------------------------ epilogue --
         const int wg = (warp - 4) >> 2, ew = warp & 3;
-        unsigned char* sbuf = smem + NST * P_STAGE + (warp - 4) * (p_bufs<EPI>() * 2048);
-        StageRing<p_bufs<EPI>()> ring(sbuf);
+        unsigned char* sbuf = smem + NST * P_STAGE + (warp - 4) * p_own<EPI>();
+        StageRing<2> ring(sbuf);
         const uint32_t tempty_leader[2] = {leader_smem_addr(&tempty_bar[0]), leader_smem_addr(&tempty_bar[1])};
-        // DGRAD: 32 columns of g and u as kept come by TMA, one such chunk ahead in 16
-        // bits and two in 8, across tiles (each lane's own loads, of 32 rows an
+        // DGRAD: g and u as kept come by TMA, 32 bytes of the warp's 32 rows of each,
+        // one such piece ahead, across tiles (each lane's own loads, of 32 rows an
         // instruction, took half of the kernel's time)
-        unsigned char* kept = smem + NST * P_STAGE + 8 * (p_bufs<EPI>() * 2048) + (warp - 4) * P_KEPT;
-        uint64_t* kbar = kept_bar[warp - 4];
-        const int slots = args.keep == KEEP_8 ? 2 : 1;
-        const uint32_t kept_bytes = args.keep == KEEP_8 ? 1024u : 2048u;  // of one matrix
-        int f_task = first_task, f_chunk = 0, k_slot = 0;  // the next chunk to fetch; the slot of the next one to read
-        uint32_t k_phase = 0, k_due = 0;                   // a bit a slot: its phase; a fetch is under way
-        auto fetch_kept = [&](int slot) {                  // what the slot held is in registers
+        unsigned char* kept = sbuf + 4096;
+        uint64_t* kbar = &kept_bar[warp - 4];
+        const int piece = args.keep == KEEP_8 ? 32 : 16;  // columns
+        int f_task = first_task, f_col = 0;               // the next piece to fetch
+        uint32_t k_phase = 0;
+        bool k_due = false;           // a fetch is under way
+        auto fetch_kept = [&] {       // what the place held is in registers
             __syncwarp();
+            k_due = false;
             while (f_task < ntasks) {
                 int pm, tn, kb0, kb1;
                 locate(f_task, pm, tn, kb0, kb1);
-                const int row0 = (pm * 2 + (int)rank) * 128 + ew * 32, col = tn * TILE_N + wg * (TILE_N / 2) + f_chunk * 32;
-                if (f_chunk < 4 && row0 < args.M && col < args.N) {
+                const int row0 = (pm * 2 + (int)rank) * 128 + ew * 32, col = tn * TILE_N + wg * WG_N + f_col;
+                if (f_col < WG_N && row0 < args.M && col < args.N) {
                     if (lane == 0) {
-                        unsigned char* to = kept + slot * 2048;
-                        mbar_arrive_expect_tx(&kbar[slot], 2 * kept_bytes);
-                        tma_load_2d(to, &tmG, col, row0, &kbar[slot]);
-                        tma_load_2d(to + kept_bytes, &tmU, col, row0, &kbar[slot]);
+                        mbar_arrive_expect_tx(kbar, 2048);
+                        tma_load_2d(kept, &tmG, col, row0, kbar);
+                        tma_load_2d(kept + 1024, &tmU, col, row0, kbar);
                     }
-                    k_due |= 1u << slot;
-                    ++f_chunk;
+                    k_due = true;
+                    f_col += piece;
                     return;
                 }
                 f_task += task_stride;
-                f_chunk = 0;
+                f_col = 0;
             }
         };
-        if constexpr (EPI == P_DGRAD)
-            for (int i = 0; i < slots; ++i) fetch_kept(i);
+        auto wait_kept = [&] {
+            if (!__all_sync(FULL, mbar_wait_bounded(kbar, k_phase))) {
+                if (lane == 0) atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
+                return false;
+            }
+            k_phase ^= 1u;
+            k_due = false;
+            return true;
+        };
+        if constexpr (EPI == P_DGRAD) fetch_kept();
         int acc = 0, it = 0;
         uint32_t acc_phase = 0;
         for (int task = first_task; task < ntasks; task += task_stride, ++it) {
@@ -309,7 +328,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             const int row0 = (pm * 2 + (int)rank) * 128 + ew * 32;  // first row of this warp
             const int row = row0 + lane;
             const bool row_ok = row < args.M;
-            const int gcol0 = tn * TILE_N + wg * (TILE_N / 2);  // first column of this warpgroup
+            const int gcol0 = tn * TILE_N + wg * WG_N;  // first column of this warpgroup
             float2 scales_ahead = make_float2(1.f, 1.f);
             if constexpr (EPI == P_DGRAD) {  // while the products still run
                 if (args.keep == KEEP_8 && row_ok && gcol0 < args.N) {
@@ -320,20 +339,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             const bool ok = __all_sync(FULL, mbar_wait_bounded(&tfull_bar[acc], acc_phase));
             if (!ok && lane == 0) atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
             bool dead = !ok || __any_sync(FULL, s_abort != 0);
-            // The epilogue warps meet below (UP keeping 8 bits): all of them go on or
-            // none.  s_dead is theirs alone, written before the first barrier and
-            // read between the two.
-            if constexpr (EPI == P_UP) {
-                if (args.keep == KEEP_8) {
-                    if (dead && lane == 0) s_dead = 1;
-                    named_bar_sync(1, 256);
-                    dead = *reinterpret_cast<volatile int*>(&s_dead) != 0;
-                    named_bar_sync(1, 256);
-                }
-            }
-            if (dead) break;
+            if (dead && !(EPI == P_UP && args.keep == KEEP_8)) break;
             tc_fence_after();
-            const uint32_t tbase = tmem_base + ((uint32_t)(ew * 32) << 16) + (uint32_t)(acc * 256 + wg * (TILE_N / 2));
+            const uint32_t tbase = tmem_base + ((uint32_t)(ew * 32) << 16) + (uint32_t)(acc * 256 + wg * WG_N);
 
             if constexpr (EPI == P_STORE) {
 #pragma unroll 1
@@ -362,38 +370,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     else stage_store_plain(args.out, args.ldc, args.M, args.N, sbuf, lane, w, col, row0);
                 }
             } else if constexpr (EPI == P_UP) {
+                // 32 columns of h a warp, 16 at a time
+                const bool live = !dead && row0 < args.M && gcol0 < args.N;
                 float gtop = 0.f, utop = 0.f;
-                const bool warp_live = row0 < args.M;
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    const int col = gcol0 + c * 32;
-                    if (!warp_live || col >= args.N) break;
-                    uint32_t g[32], u[32], w[16];
-                    tmem_ld32(tbase + c * 32, g);
-                    tmem_ld32(tbase + 128 + c * 32, u);
-                    tmem_wait_ld();
+                if (live) {
+                    if (lane == 0) bulk_wait_group_read0();
+                    __syncwarp();
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) {
-                        Float2 unused;
-                        const Float2 gp = join2(__uint_as_float(g[2 * q]), __uint_as_float(g[2 * q + 1]));
-                        const Float2 up = join2(__uint_as_float(u[2 * q]), __uint_as_float(u[2 * q + 1]));
-                        const float2 h = split2(pair_mul(glu_act2<ACT, false>(gp, unused), up));
-                        w[q] = pack16x2<DT>(h.x, h.y);
-                    }
-                    ring.store(&tmC, lane, w, col, row0);
-                    if (args.keep == KEEP_16) {
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t g[16], u[16], w[8];
+                        tmem_ld16(tbase + half * 16, g);
+                        tmem_ld16(tbase + 128 + half * 16, u);
+                        tmem_wait_ld();
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) w[q] = pack16x2<DT>(__uint_as_float(g[2 * q]), __uint_as_float(g[2 * q + 1]));
-                        ring.store(&tmG, lane, w, col, row0);
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) w[q] = pack16x2<DT>(__uint_as_float(u[2 * q]), __uint_as_float(u[2 * q + 1]));
-                        ring.store(&tmU, lane, w, col, row0);
-                    } else if (args.keep == KEEP_8) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            gtop = fmaxf(gtop, fabsf(__uint_as_float(g[j])));  // NaN does not count
-                            utop = fmaxf(utop, fabsf(__uint_as_float(u[j])));
+                        for (int q = 0; q < 8; ++q) {
+                            Float2 unused;
+                            const Float2 gp = join2(__uint_as_float(g[2 * q]), __uint_as_float(g[2 * q + 1]));
+                            const Float2 up = join2(__uint_as_float(u[2 * q]), __uint_as_float(u[2 * q + 1]));
+                            const float2 h = split2(pair_mul(glu_act2<ACT, false>(gp, unused), up));
+                            w[q] = pack16x2<DT>(h.x, h.y);
                         }
+                        stage16(sbuf, lane, half, w);
+                        if (args.keep == KEEP_16) {
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) w[q] = pack16x2<DT>(__uint_as_float(g[2 * q]), __uint_as_float(g[2 * q + 1]));
+                            stage16(sbuf + 2048, lane, half, w);
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) w[q] = pack16x2<DT>(__uint_as_float(u[2 * q]), __uint_as_float(u[2 * q + 1]));
+                            stage16(sbuf + 4096, lane, half, w);
+                        } else if (args.keep == KEEP_8) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                gtop = fmaxf(gtop, fabsf(__uint_as_float(g[j])));  // NaN does not count
+                                utop = fmaxf(utop, fabsf(__uint_as_float(u[j])));
+                            }
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmC, sbuf, gcol0, row0);
+                        if (args.keep == KEEP_16) {
+                            tma_store_2d(&tmG, sbuf + 2048, gcol0, row0);
+                            tma_store_2d(&tmU, sbuf + 4096, gcol0, row0);
+                        }
+                        bulk_commit_group();
                     }
                 }
                 if (args.keep == KEEP_8) {
@@ -403,120 +424,140 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     if (!finite) {
                         gmax = umax = 0;
 #pragma unroll 1
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t g[32], u[32];
-                            tmem_ld32(tbase + c * 32, g);
-                            tmem_ld32(tbase + 128 + c * 32, u);
+                        for (int half = 0; half < 2; ++half) {
+                            uint32_t g[16], u[16];
+                            tmem_ld16(tbase + half * 16, g);
+                            tmem_ld16(tbase + 128 + half * 16, u);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
+                            for (int j = 0; j < 16; ++j) {
                                 gmax = max(gmax, finite_mag(__uint_as_float(g[j])));
                                 umax = max(umax, finite_mag(__uint_as_float(u[j])));
                             }
                         }
                     }
-                    // the block of 128 columns spans both warpgroups (columns past N are zero)
-                    s_amax[it & 1][wg][ew * 32 + lane] = make_uint2(gmax, umax);
-                    named_bar_sync(1, 256);
-                    const uint2 other = s_amax[it & 1][wg ^ 1][ew * 32 + lane];
-                    const int ge = fp8_exponent(max(gmax, other.x)), ue = fp8_exponent(max(umax, other.y));
-                    if (row_ok) {
-                        const long long at = fp8_scale_at(row, tn, args.bt);
-                        if (wg == 0) args.gs[at] = (uint8_t)(ge + 127);
-                        else args.us[at] = (uint8_t)(ue + 127);
+                    // The block of 128 columns spans the four warps of these rows (columns past
+                    // N are zero).  A warp that gives up says so here, and all four leave: they
+                    // meet once a tile or not at all.
+                    const int slot = 4096 + (it & 1) * 256 + lane * 8;
+                    *reinterpret_cast<uint2*>(sbuf + slot) = dead ? make_uint2(0xFFFFFFFFu, 0u) : make_uint2(gmax, umax);
+                    named_bar_sync(1 + ew, 128);
+#pragma unroll
+                    for (int o = 1; o < 4; ++o) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(smem + NST * P_STAGE + ((wg ^ o) * 4 + ((warp - 4) & 3)) * p_own<EPI>() + slot);
+                        gmax = max(gmax, v.x), umax = max(umax, v.y);
                     }
-                    // 64 columns of g, then of u, a lane's 64 bytes as 32 16-bit values are
-#pragma unroll 1
-                    for (int m = 0; m < 2; ++m) {
-                        if (!warp_live || gcol0 >= args.N) break;
-                        const float inv = two_to(m ? -ue : -ge);
-                        uint32_t w[16];
+                    if (dead || gmax == 0xFFFFFFFFu) break;
+                    const int ge = fp8_exponent(gmax), ue = fp8_exponent(umax);
+                    if (row_ok && wg < 2) (wg ? args.us : args.gs)[fp8_scale_at(row, tn, args.bt)] = (uint8_t)((wg ? ue : ge) + 127);
+                    if (live) {  // 32 bytes of g, then of u a row
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t r[32];
-                            tmem_ld32(tbase + m * 128 + c * 32, r);
-                            tmem_wait_ld();
+                        for (int m = 0; m < 2; ++m) {
+                            const float inv = two_to(m ? -ue : -ge);
+                            const Float2 inv2 = join2(inv, inv);
 #pragma unroll
-                            for (int q = 0; q < 8; ++q) {
-                                const float v0 = __uint_as_float(r[4 * q]), v1 = __uint_as_float(r[4 * q + 1]);
-                                const float v2 = __uint_as_float(r[4 * q + 2]), v3 = __uint_as_float(r[4 * q + 3]);
-                                if (finite) {
-                                    const Float2 s2 = join2(inv, inv);
-                                    w[c * 8 + q] = fp8_four(pair_mul(join2(v0, v1), s2), pair_mul(join2(v2, v3), s2));
-                                } else {
-                                    w[c * 8 + q] = fp8_pack4<false>(v0, v1, v2, v3, inv);
+                            for (int half = 0; half < 2; ++half) {
+                                uint32_t r[16], w[4];
+                                tmem_ld16(tbase + m * 128 + half * 16, r);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    const float v0 = __uint_as_float(r[4 * q]), v1 = __uint_as_float(r[4 * q + 1]);
+                                    const float v2 = __uint_as_float(r[4 * q + 2]), v3 = __uint_as_float(r[4 * q + 3]);
+                                    w[q] = finite ? fp8_four(pair_mul(join2(v0, v1), inv2), pair_mul(join2(v2, v3), inv2))
+                                                  : fp8_pack4<false>(v0, v1, v2, v3, inv);
                                 }
+                                *reinterpret_cast<uint4*>(sbuf + 2048 + m * 1024 + lane * 32 + half * 16) = make_uint4(w[0], w[1], w[2], w[3]);
                             }
                         }
-                        ring.store(m ? &tmU : &tmG, lane, w, gcol0, row0);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&tmG, sbuf + 2048, gcol0, row0);
+                            tma_store_2d(&tmU, sbuf + 3072, gcol0, row0);
+                            bulk_commit_group();
+                        }
                     }
                 }
             } else {  // P_DGRAD
-                const float gscale = scales_ahead.x, uscale = scales_ahead.y;
+                const Float2 gs2 = join2(scales_ahead.x, scales_ahead.x), us2 = join2(scales_ahead.y, scales_ahead.y);
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < WG_N / 32; ++c) {
                     const int col = gcol0 + c * 32;
                     if (row0 >= args.M || col >= args.N) break;
-                    if (!__all_sync(FULL, mbar_wait_bounded(&kbar[k_slot], (k_phase >> k_slot) & 1u))) {
-                        if (lane == 0) atomicOr(args.status, SFFN_STATUS_WAIT_TIMEOUT);
-                        dead = true;
-                        break;
+                    // dg and du go to the two buffers as they are formed, h to the first one
+                    // once dg has left it
+                    if (lane == 0) bulk_wait_group_read0();
+                    __syncwarp();
+                    uint32_t wh_[16];
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t r[16], wg_[8], wu_[8], gw[8], uw[8];  // gw, uw: this row's 16-bit pairs, or four words of bytes
+                        const bool some = args.keep == KEEP_8 ? half == 0 : col + half * 16 < args.N;  // a piece begins
+                        if (some && !dead) dead = !wait_kept();
+                        const unsigned char* at = kept + lane * 32;
+                        if (args.keep == KEEP_8) {
+                            const uint4 a = *reinterpret_cast<const uint4*>(at + 16 * half);
+                            const uint4 b = *reinterpret_cast<const uint4*>(at + 1024 + 16 * half);
+                            gw[0] = a.x, gw[1] = a.y, gw[2] = a.z, gw[3] = a.w;
+                            uw[0] = b.x, uw[1] = b.y, uw[2] = b.z, uw[3] = b.w;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint4 a = *reinterpret_cast<const uint4*>(at + 16 * i);
+                                const uint4 b = *reinterpret_cast<const uint4*>(at + 1024 + 16 * i);
+                                gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
+                                uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
+                            }
+                        }
+                        if (!dead && (args.keep == KEEP_8 ? half == 1 : some)) fetch_kept();
+                        tmem_ld16(tbase + c * 32 + half * 16, r);
+                        tmem_wait_ld();
+                        auto two = [&](int q, Float2 g, Float2 u) {  // elements 2q, 2q + 1
+                            Float2 d;
+                            const Float2 dh = join2(__uint_as_float(r[2 * q]), __uint_as_float(r[2 * q + 1]));
+                            const Float2 a = glu_act2<ACT, true>(g, d);
+                            const float2 dg = split2(pair_mul(pair_mul(dh, u), d)), du = split2(pair_mul(dh, a));
+                            const float2 h = split2(pair_mul(a, u));
+                            wg_[q] = pack16x2<DT>(dg.x, dg.y);
+                            wu_[q] = pack16x2<DT>(du.x, du.y);
+                            wh_[half * 8 + q] = pack16x2<DT>(h.x, h.y);
+                        };
+                        if (args.keep == KEEP_8) {
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) {
+                                const uint32_t sh = 16 * (q & 1);
+                                const float2 g = __half22float2(fp8_half2(gw[q >> 1] >> sh)), u = __half22float2(fp8_half2(uw[q >> 1] >> sh));
+                                two(q, pair_mul(join2(g.x, g.y), gs2), pair_mul(join2(u.x, u.y), us2));
+                            }
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) {
+                                const float2 g = unpack16x2<DT>(gw[q]), u = unpack16x2<DT>(uw[q]);
+                                two(q, join2(g.x, g.y), join2(u.x, u.y));
+                            }
+                        }
+                        stage16(sbuf, lane, half, wg_);
+                        stage16(sbuf + 2048, lane, half, wu_);
                     }
-                    k_phase ^= 1u << k_slot;
-                    k_due &= ~(1u << k_slot);
-                    uint32_t gw[16], uw[16];  // this row's: 16-bit pairs, or 8 words of four bytes
-                    if (args.keep == KEEP_8) {
-                        const unsigned char* at = kept + k_slot * 2048 + lane * 32;
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint4 a = *reinterpret_cast<const uint4*>(at + 16 * i);
-                            const uint4 b = *reinterpret_cast<const uint4*>(at + 1024 + 16 * i);
-                            gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
-                            uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const unsigned char* at = kept + lane * 64 + 16 * (i ^ ((lane >> 1) & 3));
-                            const uint4 a = *reinterpret_cast<const uint4*>(at);
-                            const uint4 b = *reinterpret_cast<const uint4*>(at + 2048);
-                            gw[4 * i] = a.x, gw[4 * i + 1] = a.y, gw[4 * i + 2] = a.z, gw[4 * i + 3] = a.w;
-                            uw[4 * i] = b.x, uw[4 * i + 1] = b.y, uw[4 * i + 2] = b.z, uw[4 * i + 3] = b.w;
-                        }
+                    if (dead) break;
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmC, sbuf, col, row0);
+                        bulk_commit_group();
+                        tma_store_2d(&tmC2, sbuf + 2048, col, row0);
+                        bulk_commit_group();
+                        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
                     }
-                    fetch_kept(k_slot);
-                    k_slot = slots == 2 ? k_slot ^ 1 : 0;
-                    uint32_t r[32], wg_[16], wu_[16], wh_[16];
-                    tmem_ld32(tbase + c * 32, r);
-                    tmem_wait_ld();
-                    auto two = [&](int q, Float2 g, Float2 u) {  // elements 2q, 2q + 1
-                        Float2 d;
-                        const Float2 dh = join2(__uint_as_float(r[2 * q]), __uint_as_float(r[2 * q + 1]));
-                        const Float2 a = glu_act2<ACT, true>(g, d);
-                        const float2 dg = split2(pair_mul(pair_mul(dh, u), d)), du = split2(pair_mul(dh, a));
-                        const float2 h = split2(pair_mul(a, u));
-                        wg_[q] = pack16x2<DT>(dg.x, dg.y);
-                        wu_[q] = pack16x2<DT>(du.x, du.y);
-                        wh_[q] = pack16x2<DT>(h.x, h.y);
-                    };
-                    if (args.keep == KEEP_8) {
-                        const Float2 gs2 = join2(gscale, gscale), us2 = join2(uscale, uscale);
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) {
-                            const uint32_t sh = 16 * (q & 1);
-                            const float2 g = __half22float2(fp8_half2(gw[q >> 1] >> sh)), u = __half22float2(fp8_half2(uw[q >> 1] >> sh));
-                            two(q, pair_mul(join2(g.x, g.y), gs2), pair_mul(join2(u.x, u.y), us2));
-                        }
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) {
-                            const float2 g = unpack16x2<DT>(gw[q]), u = unpack16x2<DT>(uw[q]);
-                            two(q, join2(g.x, g.y), join2(u.x, u.y));
-                        }
+                    __syncwarp();
+                    stage32(sbuf, lane, wh_);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmC3, sbuf, col, row0);
+                        bulk_commit_group();
                     }
-                    ring.store(&tmC, lane, wg_, col, row0);
-                    ring.store(&tmC2, lane, wu_, col, row0);
-                    ring.store(&tmC3, lane, wh_, col, row0);
                 }
             }
             if (EPI == P_DGRAD && dead) break;
@@ -530,8 +571,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             }
         }
         if constexpr (EPI == P_DGRAD)  // left early: what is under way lands first
-            for (int i = 0; i < 2; ++i)
-                if ((k_due >> i) & 1u) (void)mbar_wait_bounded(&kbar[i], (k_phase >> i) & 1u);
+            if (k_due) (void)mbar_wait_bounded(kbar, k_phase);
         if (lane == 0) bulk_wait_group0();
         __syncwarp();
     }
@@ -561,12 +601,11 @@ int store_map(CUtensorMap* m, const void* p, long long rows, long long cols, lon
     return tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p, cols, rows, ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// Maps of g or u as kept, to write (UP) and to read (DGRAD): 64 bytes of 32 rows,
-// or 32 bytes in 8 bits where DGRAD reads 32 columns.
+// Maps of g or u as kept: UP writes 32 columns of 32 rows, DGRAD reads 32 bytes of them.
 int kept_map(CUtensorMap* m, int keep, const void* p, long long T, long long F, long long ldk, bool read) {
-    if (keep == KEEP_16) return store_map(m, p, T, F, ldk);
-    return tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p, F, T, ldk, read ? 32 : 64, 32,
-                   read ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B);
+    if (keep == KEEP_8) return tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p, F, T, ldk, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE);
+    return read ? tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p, F, T, ldk, 16, 32, CU_TENSOR_MAP_SWIZZLE_NONE)
+                : store_map(m, p, T, F, ldk);
 }
 
 bool operand_ok(const void* p, long long ld) { return aligned16(p) && ld % 8 == 0; }
@@ -577,10 +616,10 @@ int launch_pair(const CUtensorMap (&m)[9], const PairArgs& args, cudaStream_t st
     constexpr int smem = p_smem<EPI>();
     static SmemOnce once;
     SFFN_CUDA_TRY(once.set(k, smem));
-    static const int pairs = resident_pairs(k, P_THREADS, smem);
+    static const int pairs = resident_pairs(k, p_threads<EPI>(), smem);
     const long long tasks = (long long)((args.tiles_m + 1) / 2) * args.tiles_n * args.splits;
     const int clusters = (int)std::min<long long>(tasks, pairs);
-    k<<<clusters * 2, P_THREADS, smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7], m[8], args);
+    k<<<clusters * 2, p_threads<EPI>(), smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7], m[8], args);
     SFFN_CHECK_LAUNCH();
     return SFFN_OK;
 }

@@ -8,14 +8,19 @@ namespace sffn {
 
 // Into a 2 KB buffer, in the layout of a tensor map with 64-byte swizzle
 // (16-byte chunk ch of row r at r * 64 + 16 * (ch ^ ((r >> 1) & 3))).
-__device__ __forceinline__ void stage32(unsigned char* sbuf, int lane, const uint32_t (&w)[16]) {
+// 16 of the 32 columns:
+__device__ __forceinline__ void stage16(unsigned char* sbuf, int lane, int half, const uint32_t* w) {
     const uint32_t rb = smem_u32(sbuf) + (uint32_t)lane * 64u;
     const int sw = (lane >> 1) & 3;
 #pragma unroll
-    for (int ch = 0; ch < 4; ++ch)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rb + 16u * (uint32_t)(ch ^ sw)), "r"(w[4 * ch]),
+    for (int ch = 0; ch < 2; ++ch)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rb + 16u * (uint32_t)((2 * half + ch) ^ sw)), "r"(w[4 * ch]),
                      "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3])
                      : "memory");
+}
+__device__ __forceinline__ void stage32(unsigned char* sbuf, int lane, const uint32_t (&w)[16]) {
+    stage16(sbuf, lane, 0, w);
+    stage16(sbuf, lane, 1, w + 8);
 }
 
 // A warp's R staging buffers, used in turn: each store is a bulk group of its own,
