@@ -125,7 +125,6 @@ SIGNATURES = {
     "sffn_gemm16": (_int, [_int, _vp, _i64, _int, _vp, _i64, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64,
                            _vp, _sz, _vp, _vp]),
     "sffn_few_rows_mm": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
-    "sffn_few_rows_glu": (_int, [_int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "sffn_few_rows_ffn": (_int, [_int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp,
                                  _i64, _vp, _vp]),
     "sffn_pad_rows16": (_int, [_int, _vp, _vp]),
@@ -177,7 +176,7 @@ LAUNCHING = {"sffn_sp24_compress": 1, "sffn_gemm_sp24": 1, "sffn_sp24_overflow_a
              "sffn_round_tf32": 1, "sffn_token_logprobs": 1, "sffn_token_logprobs_bwd": 1, "sffn_distill_topk": 1,
              "sffn_distill_topk_bwd": 1, "sffn_residual_norm": 1, "sffn_residual_norm_bwd": 1,
              "sffn_fp8_pack": 1, "sffn_fp8_unpack": 1, "sffn_fp8_mm": 1, "sffn_fp8_linear": 2, "sffn_glu_up": 1, "sffn_glu_dgrad": 1,
-             "sffn_gemm16": 1, "sffn_few_rows_mm": 1, "sffn_few_rows_glu": 1, "sffn_few_rows_fp8": 1,
+             "sffn_gemm16": 1, "sffn_few_rows_mm": 1, "sffn_few_rows_fp8": 1,
              "sffn_few_rows_ffn": 2, "sffn_pad_rows16": 1, "sffn_ckpt_linear": 1, "sffn_ckpt_linear_bwd": 1,
              "sffn_gated_ffn": 2, "sffn_gated_ffn_bwd": 1}
 launch_count = 0

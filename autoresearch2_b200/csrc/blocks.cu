@@ -275,7 +275,7 @@ extern "C" int sffn_fp8_linear(const void* x, int dtype, int64_t ldx, const void
     void* scales = ws.take((size_t)((M + 127) / 128 * fp8_block_tiles(K) * 512));
     TRY(sffn_fp8_pack(x, dtype, M, K, ldx, values, up16(K), scales, stream));
     if (M <= FEW)
-        return sffn_few_rows_fp8(values, up16(K), scales, b, ldb, b_scales, M, N, K, C, c_dtype, ldc, status_dev, stream);
+        return few_rows_fp8(values, up16(K), scales, b, ldb, b_scales, M, N, K, C, c_dtype, ldc, true, status_dev, stream);
     const size_t bytes = sffn_fp8_mm_workspace_bytes(M, N, K);
     void* parts = bytes ? ws.take(bytes) : nullptr;
     return sffn_fp8_mm(values, up16(K), scales, b, ldb, b_scales, M, N, K, C, c_dtype, ldc, parts, bytes, status_dev, stream);

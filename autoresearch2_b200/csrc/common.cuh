@@ -384,4 +384,11 @@ __device__ __forceinline__ void copy_run16(const uint16_t* __restrict__ src, uin
     }
 }
 
+// A kernel launched with programmatic stream serialization may start once all blocks
+// of the one before have called the first; it touches nothing that this one
+// writes before the second returns, which is when this one has ended.  Neither
+// does anything between other kernels.
+__device__ __forceinline__ void grid_dependents_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 }  // namespace sffn

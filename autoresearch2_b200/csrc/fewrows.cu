@@ -47,6 +47,7 @@ struct FewArgs {
     uint16_t* out;
     long long ldo;
     uint32_t* status;
+    bool after;  // the kernel before on the stream wrote x and lets this one start early
 };
 
 template <int DT>
@@ -62,13 +63,10 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 bytes of a row from byte k on (zeros past its `bytes`), aligned for VEC.
-template <bool VEC, int ESIZE, bool STREAM>
+// 16 bytes of a row from byte k on, element by element (zeros past its `bytes`): rows
+// that are not on 16 bytes, and a row's last bytes.
+template <int ESIZE>
 __device__ __forceinline__ uint4 load_piece(const uint8_t* row, long long k, long long bytes) {
-    if (VEC && k + 16 <= bytes) {
-        const uint4* p = reinterpret_cast<const uint4*>(row + k);
-        return STREAM ? __ldcs(p) : __ldg(p);
-    }
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 16 / ESIZE; ++i) {
@@ -139,50 +137,62 @@ __global__ void __launch_bounds__(S_THREADS, 1)
         fence_mbar_init();
     }
     __syncthreads();
+    grid_dependents_start();
 
     if (warp == S_WARPS) {
         // -------------------------------------------------------- copies --
         if constexpr (VEC) {
             const uint32_t count = (uint32_t)(a.per * MATS + a.T) * S_ROW;  // whole boxes: zeros past the edges
             // the scales of a stage's eight blocks: lane = half of them of a row of W or of x
-            auto copy_scales = [&](int group, int c, uint32_t to, uint64_t* bar) {
+            auto copy_scales = [&](const uint8_t* tiles, long long row, int c, int stage, int place) {
                 const int block = c * 8 + (lane & 1) * 4;
-                if (block < (int)fp8_blocks(a.K)) {
-                    auto copy = [&](const uint8_t* tiles, long long row, int place) {
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + place * 8 + (lane & 1) * 4),
-                                     "l"(tiles + fp8_scale_at(row, block, a.bt))
-                                     : "memory");
-                    };
-                    copy(a.ws, min(group * a.per + (lane >> 1), a.N - 1), lane >> 1);
+                if (block < (int)fp8_blocks(a.K))
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(few_smem + stage * STAGE + St::SCALES) + place * 8 + (lane & 1) * 4),
+                                 "l"(tiles + fp8_scale_at(row, block, a.bt))
+                                 : "memory");
+            };
+            auto copy_w = [&](int group, int c, int stage) {
+                if (lane == 0) {
+                    unsigned char* to = few_smem + stage * STAGE;
+                    mbar_arrive_expect_tx(&full_bar[stage], count);
+                    tma_load_2d(to, &tmW, c * (S_ROW / 4), group * a.per, &full_bar[stage]);
+                    if constexpr (MATS == 2) tma_load_2d(to + 16 * S_ROW, &tmW2, c * (S_ROW / 4), group * a.per, &full_bar[stage]);
+                }
+                if constexpr (FP8) copy_scales(a.ws, min(group * a.per + (lane >> 1), a.N - 1), c, stage, lane >> 1);
+            };
+            auto copy_x = [&](int c, int stage) {
+                if (lane == 0) tma_load_2d(few_smem + stage * STAGE + ROWS * S_ROW, &tmX, c * (S_ROW / 4), 0, &full_bar[stage]);
+                if constexpr (FP8) {
 #pragma unroll
                     for (int i = 0; i < (NT + 1) / 2; ++i) {
                         const int t = i * 16 + (lane >> 1);
-                        if (t < NT * 8) copy(a.xs, min(t, a.T - 1), 16 + t);
+                        if (t < NT * 8) copy_scales(a.xs, min(t, a.T - 1), c, stage, 16 + t);
                     }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full_bar[stage])) : "memory");
                 }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
             };
+            // W into all stages while the kernel before may still be writing x
+            int ahead = 0;
+            for (int group = blockIdx.x; a.after && group < groups && ahead < DEPTH; group += gridDim.x)
+                for (int c = 0; c < chunks && ahead < DEPTH; ++c) copy_w(group, c, ahead++);
+            grid_dependency_wait();
             int stage = 0;
             uint32_t phase = 1;
             for (int group = blockIdx.x; group < groups; group += gridDim.x)
                 for (int c = 0; c < chunks; ++c) {
-                    if (!__all_sync(FULL, mbar_wait_bounded(&empty_bar[stage], phase))) {
-                        if (lane == 0) atomicOr(a.status, SFFN_STATUS_WAIT_TIMEOUT);
-                        // no copy lands after the block has left
-                        for (int s = 0; s < DEPTH; ++s) (void)mbar_wait_bounded(&full_bar[s], (s < stage ? phase : phase ^ 1u) ^ 1u);
-                        return;
+                    if (ahead > 0) {
+                        --ahead;
+                    } else {
+                        if (!__all_sync(FULL, mbar_wait_bounded(&empty_bar[stage], phase))) {
+                            if (lane == 0) atomicOr(a.status, SFFN_STATUS_WAIT_TIMEOUT);
+                            // no copy lands after the block has left
+                            for (int s = 0; s < DEPTH; ++s) (void)mbar_wait_bounded(&full_bar[s], (s < stage ? phase : phase ^ 1u) ^ 1u);
+                            return;
+                        }
+                        copy_w(group, c, stage);
                     }
-                    unsigned char* to = few_smem + stage * STAGE;
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&full_bar[stage], count);
-                        tma_load_2d(to, &tmW, c * (S_ROW / 4), group * a.per, &full_bar[stage]);
-                        if constexpr (MATS == 2) tma_load_2d(to + 16 * S_ROW, &tmW2, c * (S_ROW / 4), group * a.per, &full_bar[stage]);
-                        tma_load_2d(to + ROWS * S_ROW, &tmX, c * (S_ROW / 4), 0, &full_bar[stage]);
-                    }
-                    if constexpr (FP8) {
-                        __syncwarp();
-                        copy_scales(group, c, smem_u32(to + St::SCALES), &full_bar[stage]);
-                    }
+                    copy_x(c, stage);
+                    if constexpr (FP8) __syncwarp();
                     if (++stage == DEPTH) stage = 0, phase ^= 1u;
                 }
             asm volatile("cp.async.wait_all;" ::: "memory");
@@ -191,6 +201,7 @@ __global__ void __launch_bounds__(S_THREADS, 1)
     }
     if (warp > S_WARPS) {
         // -------------------------------------------------------- adders --
+        grid_dependency_wait();
         uint32_t phase = 0;
         for (int group = blockIdx.x; group < groups; group += gridDim.x, phase ^= 1u) {
             if (!__all_sync(FULL, mbar_wait_bounded(&sums_bar, phase))) {
@@ -225,6 +236,7 @@ __global__ void __launch_bounds__(S_THREADS, 1)
     }
 
     // ------------------------------------------------------------ products --
+    grid_dependency_wait();
     const uint8_t* xrow[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) xrow[t] = static_cast<const uint8_t*>(a.x) + (long long)min(t * 8 + gid, a.T - 1) * a.ldx * ESIZE;
@@ -264,8 +276,8 @@ __global__ void __launch_bounds__(S_THREADS, 1)
                 }
                 uint4 w[MATS][2][2], x[NT][2];  // [][half of the rows][half of the piece]
                 auto direct = [&](const uint8_t* row, uint4(&v)[2]) {
-                    v[0] = load_piece<false, ESIZE, true>(row, k, bytes);
-                    v[1] = load_piece<false, ESIZE, true>(row, k + 64, bytes);
+                    v[0] = load_piece<ESIZE>(row, k, bytes);
+                    v[1] = load_piece<ESIZE>(row, k + 64, bytes);
                 };
                 const bool ring = VEC && k + 80 <= whole;
 #pragma unroll
@@ -400,8 +412,17 @@ int launch_few_nt(FewArgs a, cudaStream_t st) {
         }
     }
     const int groups = (a.N + a.per - 1) / a.per;
-    k<<<groups < sms ? groups : sms, S_THREADS, smem, st>>>(m[0], m[1], m[2], a);
-    SFFN_CHECK_LAUNCH();
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(groups < sms ? groups : sms);
+    config.blockDim = dim3(S_THREADS);
+    config.dynamicSmemBytes = smem;
+    config.stream = st;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = a.after ? 1 : 0;
+    SFFN_CUDA_TRY(cudaLaunchKernelEx(&config, k, m[0], m[1], m[2], a));
     return SFFN_OK;
 }
 
@@ -435,7 +456,7 @@ using namespace sffn;
 namespace sffn {
 namespace {
 int few_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t T, int64_t N, int64_t K, void* out,
-           int64_t ldo, uint32_t* status_dev, cudaStream_t st, DeviceScope& scope) {
+           int64_t ldo, bool after, uint32_t* status_dev, cudaStream_t st, DeviceScope& scope) {
     if (dtype != SFFN_BF16 && dtype != SFFN_F16) return SFFN_ERR_DTYPE;
     if (int rc = check_few(T, N, K)) return rc;
     if (T == 0 || N == 0) return SFFN_OK;
@@ -449,6 +470,7 @@ int few_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, in
     a.x = x, a.ldx = ldx;
     a.w[0] = w, a.ldw[0] = ldw;
     a.out = static_cast<uint16_t*>(out), a.ldo = ldo;
+    a.after = after;
     const bool vec = rows16(x, ldx, 2) && rows16(w, ldw, 2);
     if (dtype == SFFN_BF16)
         return vec ? launch_few<SFFN_BF16, SFFN_BF16, false, S_PLAIN, 0, true>(a, st)
@@ -486,15 +508,7 @@ int few_glu(int dtype, int act, const void* x, int64_t ldx, const void* wg, int6
 extern "C" int sffn_few_rows_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t T, int64_t N,
                                 int64_t K, void* out, int64_t ldo, uint32_t* status_dev, void* stream) {
     DeviceScope scope;
-    return few_mm(dtype, x, ldx, w, ldw, T, N, K, out, ldo, status_dev, reinterpret_cast<cudaStream_t>(stream), scope);
-}
-
-extern "C" int sffn_few_rows_glu(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
-                                 int64_t ldwu, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, uint32_t* status_dev,
-                                 void* stream) {
-    DeviceScope scope;
-    return few_glu(dtype, act, x, ldx, wg, ldwg, wu, ldwu, T, D, F, h, ldh, status_dev, reinterpret_cast<cudaStream_t>(stream),
-                   scope);
+    return few_mm(dtype, x, ldx, w, ldw, T, N, K, out, ldo, false, status_dev, reinterpret_cast<cudaStream_t>(stream), scope);
 }
 
 extern "C" int sffn_few_rows_ffn(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
@@ -503,12 +517,18 @@ extern "C" int sffn_few_rows_ffn(int dtype, int act, const void* x, int64_t ldx,
     DeviceScope scope;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (int rc = few_glu(dtype, act, x, ldx, wg, ldwg, wu, ldwu, T, D, F, h, ldh, status_dev, st, scope)) return rc;
-    return few_mm(dtype, h, ldh, w2, ldw2, T, D, F, y, ldy, status_dev, st, scope);
+    return few_mm(dtype, h, ldh, w2, ldw2, T, D, F, y, ldy, T > 0 && F > 0, status_dev, st, scope);
 }
 
 extern "C" int sffn_few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw,
                                  const void* w_scales, int64_t T, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
                                  uint32_t* status_dev, void* stream) {
+    return few_rows_fp8(x, ldx, x_scales, w, ldw, w_scales, T, N, K, out, out_dtype, ldo, false, status_dev, stream);
+}
+
+int sffn::few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw, const void* w_scales,
+                       int64_t T, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo, bool after,
+                       uint32_t* status_dev, void* stream) {
     if (out_dtype != SFFN_BF16 && out_dtype != SFFN_F16) return SFFN_ERR_DTYPE;
     if (int rc = check_few(T, N, K)) return rc;
     if (T == 0 || N == 0) return SFFN_OK;
@@ -525,6 +545,7 @@ extern "C" int sffn_few_rows_fp8(const void* x, int64_t ldx, const void* x_scale
     a.w[0] = w, a.ldw[0] = ldw;
     a.xs = static_cast<const uint8_t*>(x_scales), a.ws = static_cast<const uint8_t*>(w_scales);
     a.bt = (int)fp8_block_tiles(K);
+    a.after = after;
     a.out = static_cast<uint16_t*>(out), a.ldo = ldo;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return out_dtype == SFFN_BF16 ? launch_few<SFFN_F16, SFFN_BF16, true, S_PLAIN, 0, true>(a, st)

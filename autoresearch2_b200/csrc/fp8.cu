@@ -72,6 +72,7 @@ template <int DT, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS)
     fp8_pack_kernel(const void* __restrict__ x, long long rows, long long width, long long ld, uint8_t* __restrict__ values,
                     long long ldv, uint8_t* __restrict__ scales, uint32_t blocks4, uint32_t groups) {
+    grid_dependents_start();
     const int sub = threadIdx.x & 7;
     const unsigned lanes = 0xFFu << (threadIdx.x & 24);
     uint32_t row[Q_PER];

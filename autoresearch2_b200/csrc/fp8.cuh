@@ -20,6 +20,10 @@
 
 namespace sffn {
 
+// sffn_few_rows_fp8; `after`: right behind the pack of x on the stream.
+int few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw, const void* w_scales, int64_t T,
+                 int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo, bool after, uint32_t* status_dev, void* stream);
+
 constexpr int FP8_BLOCK = 128;
 constexpr int FP8_LOWEST = -118;
 

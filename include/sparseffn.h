@@ -707,13 +707,10 @@ int sffn_gemm16(int dtype, const void* A, int64_t lda, int a_mn, const void* B, 
                 int64_t ldc, void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream);
 
 /* Products of at most 16 rows with long weights (any alignment): out [T, N] =
- * x w^T; h [T, F] = act(x wg^T) * (x wu^T); and x w^T in 8-bit blocks. */
+ * x w^T; h [T, F] = act(x wg^T) * (x wu^T) and y [T, D] = h w2^T; and x w^T in
+ * 8-bit blocks. */
 int sffn_few_rows_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t T, int64_t N, int64_t K,
                      void* out, int64_t ldo, uint32_t* status_dev, void* stream);
-int sffn_few_rows_glu(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
-                      int64_t ldwu, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh, uint32_t* status_dev,
-                      void* stream);
-/* sffn_few_rows_glu and then y [T, D] = h w2^T, in one call. */
 int sffn_few_rows_ffn(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
                       int64_t ldwu, const void* w2, int64_t ldw2, int64_t T, int64_t D, int64_t F, void* h, int64_t ldh,
                       void* y, int64_t ldy, uint32_t* status_dev, void* stream);

@@ -307,12 +307,9 @@ def test_few_row_entries(lib):
     for i in (1, 3, 8, 10):
         assert rc(f, mm, **{f"_{i}": None}) == 1
     assert rc(f, mm, _2=39) == 1 and rc(f, mm, _4=39) == 1 and rc(f, mm, _9=63) == 1 and rc(f, mm, _1=vp((1 << 20) + 1)) == 3
-    g = [1, 2, P, 40, P, 40, P, 40, 10, 40, 64, P, 64, P, None]
-    f = lib.sffn_few_rows_glu
-    assert rc(f, g, _0=0) == 2 and rc(f, g, _1=-1) == 1 and rc(f, g, _8=17) == 1 and rc(f, g, _8=0) == 0 and rc(f, g, _5=39) == 1
     f = lib.sffn_few_rows_ffn
     b = [1, 2, P, 40, P, 40, P, 40, P, 64, 10, 40, 64, P, 64, P, 40, P, None]
-    assert rc(f, b, _0=0) == 2 and rc(f, b, _13=None) == 1 and rc(f, b, _10=17) == 1
+    assert rc(f, b, _0=0) == 2 and rc(f, b, _1=-1) == 1 and rc(f, b, _13=None) == 1 and rc(f, b, _10=17) == 1 and rc(f, b, _10=0) == 0 and rc(f, b, _5=39) == 1
 
 
 def test_pad_entry(lib):
