@@ -212,7 +212,8 @@ class KernelTimer:
         return out
 
 
-_FEW_ROWS = 16  # as in csrc/blocks.cu
+def _few(T, odd):  # as in csrc/blocks.cu
+    return T <= 16 or (T <= 48 and not odd)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -221,7 +222,7 @@ def _gemm16(M, N, K, K2=0):
 
 
 def _linear_launches(_dtype, _x, _ldx, _W, _ldw, odd, T, N, K, _y, values, *_):
-    return ((odd == 1) + 1 if T <= _FEW_ROWS else bool(odd) + _gemm16(T, N, K)) + bool(values)
+    return ((odd == 1) + 1 if _few(T, odd & 2) else bool(odd) + _gemm16(T, N, K)) + bool(values)
 
 
 def _linear_bwd_launches(_dtype, _dy, _ldy, _W, _ldw, odd, _v, _ldv, _s, T, N, K, dx, dW, *_):
@@ -229,9 +230,10 @@ def _linear_bwd_launches(_dtype, _dy, _ldy, _W, _ldw, odd, _v, _ldv, _s, T, N, K
 
 
 def _gated_launches(_dtype, _act, keep, _x, _ldx, _wg, _ldg, _wu, _ldu, _w2, _ld2, odd, T, D, F, *_):
-    if keep == 0 and T <= _FEW_ROWS:
+    if keep == 0 and _few(T, odd & 14):
         return 2 + (odd & 7 == 1)
-    return bool(odd & (7 if T <= _FEW_ROWS else 15)) + 1 + (1 if T <= _FEW_ROWS else _gemm16(T, D, F)) + (keep == 2)
+    few = _few(T, odd & 8)
+    return bool(odd & (7 if few else 15)) + 1 + (1 if few else _gemm16(T, D, F)) + (keep == 2)
 
 
 def _gated_bwd_launches(_dtype, _act, keep, steps, *a):
@@ -270,7 +272,7 @@ def _launches(name, args):
     if name == "sffn_fp8_mm":
         return 2 if args[12] else 1
     if name == "sffn_fp8_linear":
-        return 2 + (args[6] > _FEW_ROWS and load().sffn_fp8_mm_workspace_bytes(*args[6:9]) > 0)
+        return 2 + (not _few(args[6], 0) and load().sffn_fp8_mm_workspace_bytes(*args[6:9]) > 0)
     if name in _BLOCKS:
         return _BLOCKS[name](*args)
     if name == "sffn_residual_norm_bwd":

@@ -53,10 +53,12 @@ struct Pads {
         if (int _rc = (call)) return _rc; \
     } while (0)
 
-// Rows up to which the few-row kernels are taken: 16 rows through 4096 x 14336 and
-// back (bfloat16, gated) take them 67 us, 24 rows 153 where the 256-row tiles take
-// 95 for up to 64.
-constexpr int FEW = 16;
+// Rows that the few-row kernels take: up to 16 of any alignment, up to 48 where the
+// weights' rows are on 16 bytes.  The 256-row tiles against them, us in bfloat16:
+// gated 4096 x 14336, 16 rows 87 and 64, 17 rows 87 and 69, 48 rows 89 and 71; gated
+// 1024 x 2816, 17 rows 21 and 15, 48 rows 22 and 21; y = x W^T with 14336 x 4096, 17
+// rows 28 and 27, 2048 x 8192 14 and 15.  At 64 rows either may be the slower one.
+bool few_rows(long long T, int odd) { return T <= 16 || (T <= 48 && !odd); }
 
 struct Product {
     int dtype;
@@ -84,11 +86,11 @@ int linear_fwd(int dtype, const void* x, long long ldx, const void* W, long long
                long long K, void* y, void* values, void* scales, Scratch& ws, uint32_t* status, void* stream, bool count) {
     Mat X = mat(x, ldx, T, K, odd & 1), V = mat(W, ldw, N, K, odd & 2);
     Pads pads;
-    if (T <= FEW) {
+    if (few_rows(T, odd & 2)) {
         if (!(odd & 2)) pads.place(X, ws);  // few rows are copied for the fast way through many
         if (count) return SFFN_OK;
         TRY(pads.run(stream));
-        TRY(sffn_few_rows_mm(dtype, X.p, X.ld, W, ldw, T, N, K, y, N, status, stream));
+        TRY(sffn_few_rows_mm(dtype, X.p, X.ld, V.p, V.ld, T, N, K, y, N, status, stream));
     } else {
         pads.place(X, ws);
         pads.place(V, ws);
@@ -129,23 +131,24 @@ int gated_fwd(int dtype, int act, int keep, const void* x, long long ldx, const 
     void* h = ws.take((size_t)T * up8(F) * 2);
     const Mat H = mat(h, up8(F), T, F, false);
     Pads pads;
-    if (keep == SFFN_KEEP_NONE && T <= FEW) {
+    if (keep == SFFN_KEEP_NONE && few_rows(T, odd & 14)) {
         if (!(odd & 6)) pads.place(X, ws);  // few rows are copied for the fast way through many
         if (count) return SFFN_OK;
         TRY(pads.run(stream));
-        return sffn_few_rows_ffn(dtype, act, X.p, X.ld, wg, ldg, wu, ldu, w2, ld2, T, D, F, h, H.ld, y, D, status, stream);
+        return sffn_few_rows_ffn(dtype, act, X.p, X.ld, G.p, G.ld, U.p, U.ld, W2.p, W2.ld, T, D, F, h, H.ld, y, D, status, stream);
     }
     pads.place(X, ws);
     pads.place(G, ws);
     pads.place(U, ws);
-    if (T > FEW) pads.place(W2, ws);
+    const bool few_down = few_rows(T, odd & 8);
+    if (!few_down) pads.place(W2, ws);
     if (!count) {
         TRY(pads.run(stream));
         TRY(sffn_glu_up(dtype, act, X.p, X.ld, G.p, G.ld, U.p, U.ld, T, D, F, h, H.ld, keep, g, u,
                         keep == SFFN_KEEP_8 ? up16(F) : up8(F), gs, us, status, stream));
     }
-    if (T > FEW) TRY((Product{dtype, &ws, status, stream, count}(y, D, T, D, F, H, 0, W2, 0)));
-    else if (!count) TRY(sffn_few_rows_mm(dtype, h, H.ld, w2, ld2, T, D, F, y, D, status, stream));
+    if (!few_down) TRY((Product{dtype, &ws, status, stream, count}(y, D, T, D, F, H, 0, W2, 0)));
+    else if (!count) TRY(sffn_few_rows_mm(dtype, h, H.ld, W2.p, W2.ld, T, D, F, y, D, status, stream));
     if (keep == SFFN_KEEP_8 && !count) TRY(sffn_fp8_pack(X.p, dtype, T, D, X.ld, xv, up16(D), xs, stream));
     return SFFN_OK;
 }
@@ -256,7 +259,7 @@ extern "C" size_t sffn_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t 
     Scratch ws{nullptr};
     ws.take((size_t)M * up16(K));
     ws.take((size_t)((M + 127) / 128 * fp8_block_tiles(K) * 512));
-    if (M > FEW) ws.take(sffn_fp8_mm_workspace_bytes(M, N, K));
+    if (!few_rows(M, 0)) ws.take(sffn_fp8_mm_workspace_bytes(M, N, K));
     return ws.used;
 }
 
@@ -274,7 +277,7 @@ extern "C" int sffn_fp8_linear(const void* x, int dtype, int64_t ldx, const void
     void* values = ws.take((size_t)M * up16(K));
     void* scales = ws.take((size_t)((M + 127) / 128 * fp8_block_tiles(K) * 512));
     TRY(sffn_fp8_pack(x, dtype, M, K, ldx, values, up16(K), scales, stream));
-    if (M <= FEW)
+    if (few_rows(M, 0))
         return few_rows_fp8(values, up16(K), scales, b, ldb, b_scales, M, N, K, C, c_dtype, ldc, true, status_dev, stream);
     const size_t bytes = sffn_fp8_mm_workspace_bytes(M, N, K);
     void* parts = bytes ? ws.take(bytes) : nullptr;

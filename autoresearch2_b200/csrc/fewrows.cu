@@ -1,10 +1,15 @@
 // Products of few rows (single tokens, small batches) with long weights:
 // out[T, N] = x[T, K] W[N, K]^T for T <= 16, in 16 bits or in the 8-bit block
-// format, and the gated pair act(x Wg^T) * (x Wu^T).
+// format, and the gated pair act(x Wg^T) * (x Wu^T); and the entry points, which go
+// on to narrow.cu for up to 48 rows.
 //
 // Bound by reading the weights once.  A tensor-core tile of 128 or 256 rows of
 // x would leave most multiprocessors without a tile; here the weights are the
 // rows of mma.sync (m16n8k16, float32 accumulation) and the tokens its columns.
+// Measured: 1 row through 4096 x 14336 and back in bfloat16 57 us, 6.2 TB/s, 16 rows
+// 64; 1 x 14336 x 4096 in 8 bits 18.7 us, 3.1 TB/s (8-bit operands are converted
+// for mma.sync: two conversions for four elements of W and of x, and x's
+// again for every 16 rows of W; the instruction for e4m3 itself takes as long).
 // A block a multiprocessor, up to 16 rows of W (of Wg and Wu) at a time:
 //   warp 16       copies 1 KB of each of these rows and of x a stage, by one TMA box
 //                 a matrix
@@ -444,7 +449,7 @@ int launch_gated(int act, const FewArgs& a, cudaStream_t st) {
 bool rows16(const void* p, long long ld, int esize) { return aligned16(p) && ld * esize % 16 == 0; }
 
 int check_few(long long T, long long N, long long K) {
-    if (T < 0 || N < 0 || K <= 0 || T > S_MAX_ROWS) return SFFN_ERR_ARG;
+    if (T < 0 || N < 0 || K <= 0 || T > NARROW_MAX_ROWS) return SFFN_ERR_ARG;
     return N > 0x7FFFFF00 || K > 0x7FFFFF00 ? SFFN_ERR_TOO_LARGE : SFFN_OK;
 }
 
@@ -462,8 +467,11 @@ int few_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, in
     if (T == 0 || N == 0) return SFFN_OK;
     if (!x || !w || !out || !status_dev || ldx < K || ldw < K || ldo < N) return SFFN_ERR_ARG;
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) & 1) return SFFN_ERR_ALIGN;
+    const bool vec = rows16(x, ldx, 2) && rows16(w, ldw, 2);
+    if (T > S_MAX_ROWS && !vec) return SFFN_ERR_ALIGN;
     if (scope.device() < 0)
         if (int rc = scope.bind(x)) return rc;
+    if (T > S_MAX_ROWS) return narrow_mm(dtype, x, ldx, w, ldw, T, N, K, out, ldo, after, status_dev, st);
     FewArgs a{};
     a.status = status_dev;
     a.T = (int)T, a.N = (int)N, a.K = (int)K;
@@ -471,7 +479,6 @@ int few_mm(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, in
     a.w[0] = w, a.ldw[0] = ldw;
     a.out = static_cast<uint16_t*>(out), a.ldo = ldo;
     a.after = after;
-    const bool vec = rows16(x, ldx, 2) && rows16(w, ldw, 2);
     if (dtype == SFFN_BF16)
         return vec ? launch_few<SFFN_BF16, SFFN_BF16, false, S_PLAIN, 0, true>(a, st)
                    : launch_few<SFFN_BF16, SFFN_BF16, false, S_PLAIN, 0, false>(a, st);
@@ -489,8 +496,11 @@ int few_glu(int dtype, int act, const void* x, int64_t ldx, const void* wg, int6
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(wg) | reinterpret_cast<uintptr_t>(wu) |
          reinterpret_cast<uintptr_t>(h)) & 1)
         return SFFN_ERR_ALIGN;
+    const bool vec = rows16(x, ldx, 2) && rows16(wg, ldwg, 2) && rows16(wu, ldwu, 2);
+    if (T > S_MAX_ROWS && !vec) return SFFN_ERR_ALIGN;
     if (scope.device() < 0)
         if (int rc = scope.bind(x)) return rc;
+    if (T > S_MAX_ROWS) return narrow_glu(dtype, act, x, ldx, wg, ldwg, wu, ldwu, T, D, F, h, ldh, status_dev, st);
     FewArgs a{};
     a.status = status_dev;
     a.T = (int)T, a.N = (int)F, a.K = (int)D;
@@ -498,7 +508,6 @@ int few_glu(int dtype, int act, const void* x, int64_t ldx, const void* wg, int6
     a.w[0] = wg, a.ldw[0] = ldwg;
     a.w[1] = wu, a.ldw[1] = ldwu;
     a.out = static_cast<uint16_t*>(h), a.ldo = ldh;
-    const bool vec = rows16(x, ldx, 2) && rows16(wg, ldwg, 2) && rows16(wu, ldwu, 2);
     if (dtype == SFFN_BF16) return vec ? launch_gated<SFFN_BF16, true>(act, a, st) : launch_gated<SFFN_BF16, false>(act, a, st);
     return vec ? launch_gated<SFFN_F16, true>(act, a, st) : launch_gated<SFFN_F16, false>(act, a, st);
 }
@@ -514,6 +523,7 @@ extern "C" int sffn_few_rows_mm(int dtype, const void* x, int64_t ldx, const voi
 extern "C" int sffn_few_rows_ffn(int dtype, int act, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
                                  int64_t ldwu, const void* w2, int64_t ldw2, int64_t T, int64_t D, int64_t F, void* h,
                                  int64_t ldh, void* y, int64_t ldy, uint32_t* status_dev, void* stream) {
+    if (T > S_MAX_ROWS && !(rows16(h, ldh, 2) && rows16(w2, ldw2, 2))) return SFFN_ERR_ALIGN;
     DeviceScope scope;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (int rc = few_glu(dtype, act, x, ldx, wg, ldwg, wu, ldwu, T, D, F, h, ldh, status_dev, st, scope)) return rc;
@@ -548,6 +558,7 @@ int sffn::few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const v
     a.after = after;
     a.out = static_cast<uint16_t*>(out), a.ldo = ldo;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (T > S_MAX_ROWS) return narrow_fp8(x, ldx, x_scales, w, ldw, w_scales, T, N, K, out, out_dtype, ldo, after, status_dev, st);
     return out_dtype == SFFN_BF16 ? launch_few<SFFN_F16, SFFN_BF16, true, S_PLAIN, 0, true>(a, st)
                                   : launch_few<SFFN_F16, SFFN_F16, true, S_PLAIN, 0, true>(a, st);
 }

@@ -321,22 +321,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(X_THREADS, 1)
     }
 }
 
-// Scale tiles [tiles][32 * bt] rows of 16 bytes; boxes of one block tile's 32 rows
-// in `count` row tiles (zeros past the last one, whose values are zero too).
-int scale_map(CUtensorMap* m, const void* p, long long tiles, long long bt, int count) {
-    const auto fn = tmap_encoder();
-    const cuuint64_t dims[3] = {4, (cuuint64_t)(bt * 32), (cuuint64_t)tiles};
-    const cuuint64_t strides[2] = {16, (cuuint64_t)(bt * 512)};
-    const cuuint32_t box[3] = {4, 32, (cuuint32_t)count}, estr[3] = {1, 1, 1};
-    if (!fn || fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(p), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
-        set_error_text("cuTensorMapEncodeTiled failed for the scale tiles");
-        return SFFN_ERR_CUDA;
-    }
-    return SFFN_OK;
-}
-
 template <int DT>
 int launch_mm(const void* a, long long lda, const void* as, const void* b, long long ldb, const void* bs, MmArgs args,
               cudaStream_t st) {

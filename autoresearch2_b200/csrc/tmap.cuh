@@ -62,6 +62,22 @@ inline int tmap_2d(CUtensorMap* m, CUtensorMapDataType type, int esize, const vo
     return SFFN_OK;
 }
 
+// Scale tiles [tiles][32 * bt] rows of 16 bytes; boxes of one block tile's 32 rows
+// in `count` row tiles (zeros past the last one, whose values are zero too).
+inline int scale_map(CUtensorMap* m, const void* p, long long tiles, long long bt, int count) {
+    const auto fn = tmap_encoder();
+    const cuuint64_t dims[3] = {4, (cuuint64_t)(bt * 32), (cuuint64_t)tiles};
+    const cuuint64_t strides[2] = {16, (cuuint64_t)(bt * 512)};
+    const cuuint32_t box[3] = {4, 32, (cuuint32_t)count}, estr[3] = {1, 1, 1};
+    if (!fn || fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(p), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+        set_error_text("cuTensorMapEncodeTiled failed for the scale tiles");
+        return SFFN_ERR_CUDA;
+    }
+    return SFFN_OK;
+}
+
 // The current device's multiprocessors; 0 unless it is sm_100.  Asked of the
 // driver once a device.
 inline int sm100_sms() {
@@ -93,16 +109,16 @@ struct SmemOnce {
     }
 };
 
-// CTA pairs of this kernel that are resident at once (one CTA fills an SM).
+// Clusters of `size` CTAs of this kernel that are resident at once (one CTA fills an SM).
 template <typename K>
-int resident_pairs(K kernel, int threads, int smem) {
+int resident_clusters(K kernel, int threads, int smem, int size) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * 64);
+    cfg.gridDim = dim3((unsigned)size * 128);
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.x = (unsigned)size;
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
@@ -110,9 +126,13 @@ int resident_pairs(K kernel, int threads, int smem) {
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, (void*)kernel, &cfg) != cudaSuccess || n <= 0) {
         cudaGetLastError();
-        n = sm100_sms() / 2;
+        n = sm100_sms() / size;
     }
     return n > 0 ? n : 1;
+}
+template <typename K>
+int resident_pairs(K kernel, int threads, int smem) {
+    return resident_clusters(kernel, threads, smem, 2);
 }
 
 }  // namespace sffn

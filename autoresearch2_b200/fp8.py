@@ -24,7 +24,7 @@ __all__ = ["BLOCK", "Fp8Tensor", "fp8_pack", "fp8_unpack", "fp8_matmul", "ckpt_l
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
-FEW_ROWS = 16  # products of at most so many rows go by the few-row kernels
+FEW_ROWS = 48  # products of at most so many rows go by the few-row kernels
 OUT_TYPES = (torch.bfloat16, torch.float16)
 
 

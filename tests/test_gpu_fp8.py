@@ -144,7 +144,8 @@ SIZES = [(1, 64, 64), (1, 1000, 4096), (8, 48, 16), (9, 130, 1001), (16, 256, 64
          (33, 64, 64), (64, 100, 130), (128, 128, 128), (129, 257, 513), (200, 1000, 1333), (256, 256, 512), (300, 515, 4096),
          (777, 1001, 96), (1, 1, 1), (40, 1, 7), (513, 768, 16384), (1, 5003, 3000), (16, 4800, 1100),
          (10, 9001, 700),  # these three: several groups of rows a multiprocessor
-         (40, 300, 14336), (300, 257, 9000), (17, 1001, 2049)]  # in parts of K
+         (40, 300, 14336), (300, 257, 9000), (17, 1001, 2049),  # in parts of K
+         (20, 20000, 300), (24, 2048, 8192), (37, 4096, 5120), (48, 640, 8200), (49, 640, 8200)]  # up to 48 rows
 
 
 @pytest.mark.parametrize("out", [BF16, F16])
@@ -162,7 +163,7 @@ def test_product(M, N, K, out):
     sf.check_status()
 
 
-@pytest.mark.parametrize("M", [4, 300])
+@pytest.mark.parametrize("M", [4, 20, 300])
 def test_product_picks_each_blocks_scale(M):
     """One element a block: every (row, block) scale of both operands is told apart."""
     K, N = 1280, 270
@@ -174,7 +175,7 @@ def test_product_picks_each_blocks_scale(M):
     close_sum(got, a.to(F64), b.to(F64))
 
 
-@pytest.mark.parametrize("M", [2, 140])
+@pytest.mark.parametrize("M", [2, 20, 140])
 def test_product_of_far_scales(M):
     """Exponents whose sum leaves the scales' own range, NaN rows."""
     a, b = randn(M, 256, seed=8), randn(130, 256, seed=9)
@@ -218,7 +219,7 @@ def test_misaligned_blocks_are_refused(M):
 def test_product_beside_others_rows():
     """Nothing is written past the result, with rows that are not 16 bytes apart."""
     from autoresearch2_b200 import _lib
-    for M in (5, 70):
+    for M in (5, 20, 70):
         N, K = 77, 200
         qa, qb = sf.fp8_pack(randn(M, K, seed=4)), sf.fp8_pack(randn(N, K, seed=5))
         big = torch.full((M + 2, N + 3), 7.0, device=DEV, dtype=BF16)
@@ -239,7 +240,7 @@ def test_product_beside_others_rows():
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("T,N,K", [(1, 64, 64), (7, 33, 65), (32, 128, 256), (33, 48, 1001), (300, 515, 130), (1024, 200, 96),
-                                   (2000, 1, 3), (257, 256, 2048)])
+                                   (2000, 1, 3), (257, 256, 2048), (20, 2048, 8192), (48, 19001, 72), (47, 1024, 1000), (17, 1, 3)])
 def test_linear(T, N, K, dtype):
     x = randn(T, K, seed=1, dtype=dtype).requires_grad_()
     W = randn(N, K, seed=2, scale=K ** -0.5, dtype=dtype).requires_grad_()
