@@ -558,7 +558,10 @@ int sffn::few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const v
     a.after = after;
     a.out = static_cast<uint16_t*>(out), a.ldo = ldo;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (T > S_MAX_ROWS) return narrow_fp8(x, ldx, x_scales, w, ldw, w_scales, T, N, K, out, out_dtype, ldo, after, status_dev, st);
+    // Nine rows and more of long weights, too: the second tile of 8 tokens costs conversions
+    // (16 rows, us: 58 MB of weights 24.3 here and 18.2 there, 34 MB 15.4 and 14.3, but 17
+    // MB 8.9 and 9.5; 8 rows of 58 MB 18.8).
+    if (T > S_MAX_ROWS || (T > 8 && N >= (1LL << 25) / K)) return narrow_fp8(x, ldx, x_scales, w, ldw, w_scales, T, N, K, out, out_dtype, ldo, after, status_dev, st);
     return out_dtype == SFFN_BF16 ? launch_few<SFFN_F16, SFFN_BF16, true, S_PLAIN, 0, true>(a, st)
                                   : launch_few<SFFN_F16, SFFN_F16, true, S_PLAIN, 0, true>(a, st);
 }

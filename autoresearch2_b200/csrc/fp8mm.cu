@@ -22,7 +22,10 @@
 //                the epilogue frees it fast, as 16-bit pairs in 128 spare
 //                columns, and stores from there while the next tile runs.
 // The 256 x 256 tile is as large as tensor memory allows: at 8 bits a stage's
-// 32 KB a CTA feed 512 cycles of MMA, about what L2 can deliver.
+// 32 KB a CTA feed 512 cycles of MMA, 64 bytes a cycle, and L2 delivers 40 to 45: its
+// bound.  16384 x 8192 x 4096: 456 us, 2.4 PFLOP/s, 1.47 times the measured 16-bit
+// rate (one issuer an operand, scales with every k-block: 490).  Few tiles
+// and a long K are split over K: 256 x 4096 x 14336 32 us, 54 unsplit.
 #include <cuda.h>
 #include <string.h>
 

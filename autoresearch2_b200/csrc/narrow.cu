@@ -9,9 +9,10 @@
 // one, each a part of K, and every CTA adds the parts of its share of the tokens, in
 // order, from its shared memory.  17 rows through 4096 x 14336 and back, bfloat16:
 // 69 us, 5.1 TB/s (256-row tiles: 87); 17 x 14336 x 4096 in 8 bits 18.1 us (20.2).
-// What is left: four products of M = 128 take 620 cycles however few tokens there
-// are, which bounds a CTA to 50 GB/s -- more stages, more issuers, independent sums
-// and tiles of fewer rows made no difference -- and the tiles rarely deal out evenly.
+// What is left: 16 KB of W take a CTA 0.33 us, 50 GB/s, whatever K's place or the
+// number of tokens (more stages, more issuers, separate sums for the products, and
+// tiles of fewer rows on more CTAs made no difference; the tensor pipe is active 10
+// to 16%), and tiles rarely deal out evenly over the multiprocessors.
 //   warps 0-2 or 0-3  TMA issuers of W: a third of the k-blocks each, or half of Wg's or of Wu's
 //   next 3 or 2       TMA issuers of x
 //   next warp         tensor memory, scales (tcgen05.cp) and MMA issuer
@@ -350,9 +351,8 @@ __global__ void __launch_bounds__(R_THREADS, 1)
 // ------------------------------------------------------------------ host ----
 // How many CTAs share a tile, 1 to 8, and how many clusters of them are
 // launched (8192 x 512 of 17 rows by clusters of 1, 2, 4, 8: 45, 27, 17, 11 us).  In
-// us: a k-block takes a CTA 0.33 a matrix (four tcgen05.mma of 155 cycles, however
-// few the tokens), all weights come at 6 TB/s, and a tile's results take a few, more
-// where parts are added.  `resident`: such clusters that run at once, asked of the
+// us: a k-block takes a CTA 0.33 a matrix, all weights come at 6 TB/s, and a tile's
+// results take a few, more where parts are added.  `resident`: such clusters that run at once, asked of the
 // driver once a kernel.
 struct Share {
     int size, clusters, per;
