@@ -313,3 +313,42 @@ def test_train_gpt_command(capsys):
     assert train_gpt.main([*argv, "--gated=silu", "--ckpt8"]) == 0
     out = capsys.readouterr().out
     assert '"mlp": "gated_silu"' in out and '"ckpt8": true' in out
+
+
+def test_offsets_beyond_32_bits():
+    """Matrices of 2.2e9 elements: their last rows are those of a small call's definition."""
+    from test_gpu_fp8 import close_sum
+    from test_gpu_glu import act, check_forward, half, s as sums
+    T, D, F, n = 66000, 64, 33000, 8
+    x, Wg, Wu, W2 = (randn(*s, seed=i, scale=s[-1] ** -0.5 if i else 1.0) for i, s in enumerate([(T, D), (F, D), (F, D), (D, F)]))
+    xd, Wgd, Wud, W2d = (t.to(F64) for t in (x[-n:], Wg, Wu, W2))
+    a, d = act(xd @ Wgd.T, "silu")
+    dh = xd @ W2d
+    mag = (dh * (xd @ Wud.T) * d).abs() @ Wgd.abs() + (dh * a).abs() @ Wud.abs()
+    big = torch.zeros(T, F, device=DEV, dtype=BF16)
+    big[-n:] = randn(n, F, seed=7)
+    q, part = sf.fp8_pack(big), sf.fp8_pack(big[-n:].clone())
+    assert torch.equal(q.values[-n:].view(torch.uint8), part.values.view(torch.uint8)) and torch.equal(q.exponents[-n:], part.exponents)
+    big.fill_(1.0)
+    assert torch.equal(sf.fp8_unpack(q)[-n:], part.to_dense())
+    del big
+    y = sf.fp8_matmul(q, sf.fp8_pack(W2), out_dtype=BF16)  # a long a
+    close_sum(y[-n:], part.to_dense(F32).to(F64), sf.fp8_pack(W2).to_dense(F32).to(F64))
+    assert (y[:-n] == 0).all()
+    del q, y
+    wide = sf.fp8_matmul(sf.fp8_pack(x), sf.fp8_pack(Wg))  # a long result
+    close_sum(wide[-n:], sf.fp8_pack(x[-n:].clone()).to_dense(F32).to(F64), sf.fp8_pack(Wg).to_dense(F32).to(F64))
+    del wide
+    leaf = x.clone().requires_grad_()
+    for checkpoint in (None, "fp8"):
+        y = sf.gated_ffn(leaf, Wg, Wu, W2, checkpoint=checkpoint)
+        check_forward(y.detach()[-n:], x[-n:], Wg, Wu, W2, "silu")
+        dx = torch.autograd.grad(y, leaf, x)[0]
+        few = x[-n:].clone().requires_grad_()
+        y = sf.gated_ffn(few, Wg, Wu, W2, checkpoint=checkpoint)
+        want = torch.autograd.grad(y, few, x[-n:].clone())[0]
+        # dg and du are equal bit for bit, dx's sums in another order, each rounded once; the
+        # magnitudes within 1 + 2^-4 of the kept factors
+        tol = 2 * (half(BF16) * want.to(F64).abs() + sums(2 * F) * 1.25 * mag)
+        assert ((dx[-n:].to(F64) - want.to(F64)).abs() <= tol).all()
+    sf.check_status()
