@@ -89,12 +89,13 @@ def test_captured_and_replayed():
     leaves = [a.detach().requires_grad_() for a in args]
     dy = randn(*args[0].shape, seed=9)
     w8 = sf.fp8_pack(args[2])
-    few = [randn(3, 96, seed=11), *args[2:]]
+    few, narrow = [randn(3, 96, seed=11), *args[2:]], [randn(40, 96, seed=12), *args[2:]]
 
     def step():
         y = chain(*leaves)
         with torch.no_grad():
-            out = sf.gated_ffn(*few), sf.fp8_matmul(leaves[0], w8), sf.fp8_matmul(few[0], w8)
+            out = (sf.gated_ffn(*few), sf.fp8_matmul(leaves[0], w8), sf.fp8_matmul(few[0], w8), sf.gated_ffn(*narrow),
+                   sf.fp8_matmul(narrow[0], w8))
         return [y.detach(), *torch.autograd.grad(y, leaves, dy), *out]
 
     side = torch.cuda.Stream()
@@ -114,11 +115,37 @@ def test_captured_and_replayed():
             leaves[0].copy_(randn(*args[0].shape, seed=seed))
             dy.copy_(randn(*args[0].shape, seed=seed + 50))
             few[0].copy_(randn(3, 96, seed=seed + 90))
+            narrow[0].copy_(randn(40, 96, seed=seed + 91))
         want = [t.clone() for t in step()]
         for graph, out in zip(graphs, outs):
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, want)), seed
+    sf.check_status()
+
+
+@pytest.mark.parametrize("T", [1, 12, 40, 90])
+def test_operands_rewritten_between_calls(T):
+    """Calls under way one behind the other, every operand written anew before each:
+    kernels that start while the one before ends read none of it too early."""
+    D, F, n = 520, 3000, 12
+    sets = [[randn(*s, seed=10 * i + j, scale=0.05 if j else 1.0) for j, s in enumerate([(T, D), (F, D), (F, D), (D, F)])] for i in range(n)]
+    live = [t.clone() for t in sets[0]]
+
+    def calls():
+        q = sf.fp8_pack(live[1])
+        return sf.gated_ffn(*live), sf.fp8_matmul(live[0], q), sf.ckpt_linear(live[0], live[1])
+
+    wanted, got = [], []
+    for wait in (True, False):
+        for s in sets:
+            for a, b in zip(live, s):
+                a.copy_(b)
+            (wanted if wait else got).append(calls())
+            if wait:
+                torch.cuda.synchronize()
+    for w, g in zip(wanted, got):
+        assert all(torch.equal(a, b) for a, b in zip(w, g))
     sf.check_status()
 
 
@@ -145,7 +172,8 @@ def test_threads_with_different_sizes_at_once():
         def call():
             y = sf.gated_ffn(x, Wg, Wu, W2, checkpoint=checkpoint)
             with torch.no_grad():
-                return (y.detach(), *torch.autograd.grad(y, x, x.detach()), sf.fp8_matmul(x, w8), sf.gated_ffn(x[0, :9], Wg, Wu, W2))
+                return (y.detach(), *torch.autograd.grad(y, x, x.detach()), sf.fp8_matmul(x, w8), sf.gated_ffn(x[0, :9], Wg, Wu, W2),
+                        sf.gated_ffn(x[0, :30], Wg, Wu, W2), sf.fp8_matmul(x[0, :30], w8))
         return call
 
     calls = [of(200, 64, 96, None, 0), of(900, 264, 520, "fp8", 1), of(64, 1000, 130, "fp8", 2)]
