@@ -213,7 +213,7 @@ class KernelTimer:
 
 
 def _few(T, odd):  # as in csrc/blocks.cu
-    return T <= 16 or (T <= 48 and not odd)
+    return T <= 16 or (T <= 64 and not odd)
 
 
 @functools.lru_cache(maxsize=4096)

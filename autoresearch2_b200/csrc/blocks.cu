@@ -53,12 +53,12 @@ struct Pads {
         if (int _rc = (call)) return _rc; \
     } while (0)
 
-// Rows that the few-row kernels take: up to 16 of any alignment, up to 48 where the
+// Rows that the few-row kernels take: up to 16 of any alignment, up to 64 where the
 // weights' rows are on 16 bytes.  The 256-row tiles against them, us in bfloat16:
-// gated 4096 x 14336, 16 rows 87 and 64, 17 rows 87 and 69, 48 rows 89 and 71; gated
-// 1024 x 2816, 17 rows 21 and 15, 48 rows 22 and 21; y = x W^T with 14336 x 4096, 17
-// rows 28 and 27, 2048 x 8192 14 and 15.  At 64 rows either may be the slower one.
-bool few_rows(long long T, int odd) { return T <= 16 || (T <= 48 && !odd); }
+// gated 4096 x 14336, 16 rows 87 and 64, 17 rows 87 and 70, 64 rows 91 and 73; gated
+// 1024 x 2816, 17 rows 21 and 15, 64 rows 22 and 22; y = x W^T with 14336 x 4096, 17
+// rows 28 and 27, with 2048 x 8192 (few tiles, a long K) 13 and 14, the worst case.
+bool few_rows(long long T, int odd) { return T <= 16 || (T <= 64 && !odd); }
 
 struct Product {
     int dtype;

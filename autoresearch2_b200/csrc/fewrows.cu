@@ -1,7 +1,7 @@
 // Products of few rows (single tokens, small batches) with long weights:
 // out[T, N] = x[T, K] W[N, K]^T for T <= 16, in 16 bits or in the 8-bit block
 // format, and the gated pair act(x Wg^T) * (x Wu^T); and the entry points, which go
-// on to narrow.cu for up to 48 rows.
+// on to narrow.cu for up to 64 rows.
 //
 // Bound by reading the weights once.  A tensor-core tile of 128 or 256 rows of
 // x would leave most multiprocessors without a tile; here the weights are the

@@ -24,8 +24,8 @@ namespace sffn {
 int few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw, const void* w_scales, int64_t T,
                  int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo, bool after, uint32_t* status_dev, void* stream);
 
-// The same products of up to 48 rows, of operands whose rows are on 16 bytes.
-constexpr int NARROW_MAX_ROWS = 48;
+// The same products of up to 64 rows, of operands whose rows are on 16 bytes.
+constexpr int NARROW_MAX_ROWS = 64;
 int narrow_mm(int dtype, const void* x, long long ldx, const void* w, long long ldw, long long T, long long N, long long K, void* out,
               long long ldo, bool after, uint32_t* status, cudaStream_t st);
 int narrow_glu(int dtype, int act, const void* x, long long ldx, const void* wg, long long ldwg, const void* wu, long long ldwu, long long T,

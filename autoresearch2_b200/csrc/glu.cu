@@ -474,7 +474,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(p_threads<EPI>(), 1)
                         __syncwarp();
                         if (lane == 0) {
                             tma_store_2d(&tmG, sbuf + 2048, gcol0, row0);
-                            tma_store_2d(&tmU, sbuf + 3072, gcol0, row0);
+                            tma_store_2d(&tmU, sbuf + 2048 + 1024, gcol0, row0);
                             bulk_commit_group();
                         }
                     }

@@ -1,14 +1,14 @@
-// Products of up to 48 rows with long weights on the tcgen05 tensor cores:
+// Products of up to 64 rows with long weights on the tcgen05 tensor cores:
 // out[T, N] = x[T, K] W[N, K]^T in 16 bits or in the 8-bit block format, and the
 // gated pair act(x Wg^T) * (x Wu^T).
 //
 // Bound by reading the weights once.  W's rows are the M of tcgen05.mma (128) and
-// the tokens its N (48, those past the last hold anything), so that 8-bit operands
+// the tokens its N (48 or 64, those past the last hold anything), so that 8-bit operands
 // need no conversion and tokens cost next to nothing.  A CTA takes a tile of 128
 // rows of W (of Wg and of Wu); where tiles are few a cluster of up to 8 CTAs shares
 // one, each a part of K, and every CTA adds the parts of its share of the tokens, in
 // order, from its shared memory.  17 rows through 4096 x 14336 and back, bfloat16:
-// 69 us, 5.1 TB/s (256-row tiles: 87); 17 x 14336 x 4096 in 8 bits 18.1 us (20.2).
+// 70 us, 5.1 TB/s, 64 rows 73 (256-row tiles: 87 and 91); 17 x 14336 x 4096 in 8 bits 18.1 us (20.2).
 // What is left: 16 KB of W take a CTA 0.33 us, 50 GB/s, whatever K's place or the
 // number of tokens (more stages, more issuers, separate sums for the products, and
 // tiles of fewer rows on more CTAs made no difference; the tensor pipe is active 10
@@ -33,20 +33,20 @@ namespace {
 constexpr int R_THREADS = 512, R_EPI = 8;  // first epilogue warp
 constexpr int R_W = 128 * 128;  // bytes of a stage's tile of one W
 
-constexpr int R_N = NARROW_MAX_ROWS;  // tokens of a product: tcgen05.mma's N
-constexpr int R_PLACES = R_N + 8;     // token rows for the parts of K, however they are dealt
-
-template <bool FP8, int MATS>
+// NT: the tokens of a product, tcgen05.mma's N, 48 or 64.
+template <bool FP8, int MATS, int NT>
 struct Narrow {
     static constexpr int STAGES = MATS == 2 ? 4 : 6;
     static constexpr int ISSUERS = STAGES / 2;     // of each matrix: a stage belongs to one
-    static constexpr int STAGE = MATS * R_W + R_N * 128;
+    static constexpr int STAGE = MATS * R_W + NT * 128;
     static constexpr int SCALES = FP8 ? 1024 : 0;  // W's tile, x's
-    static constexpr int PARTS = R_PLACES * MATS * 512;
+    // token rows for the parts of K: those of 8 more, where they fit, take any deal
+    static constexpr int PLACES = MATS == 2 && NT == 64 ? 64 : NT + 8;
+    static constexpr int PARTS = PLACES * MATS * 512;
     static constexpr int SMEM = STAGES * (STAGE + SCALES) + PARTS + 1024;
-    static constexpr int ACC = MATS * R_N;         // tensor memory columns, twice
+    static constexpr int ACC = MATS * NT;          // tensor memory columns, twice
     static constexpr int SCALE_COL = 2 * ACC;      // 8 columns a group of four k-blocks
-    static_assert(SMEM <= 232448 - 1024 && SCALE_COL + (FP8 ? 8 * STAGES : 0) <= 512 && R_N % 16 == 0, "");
+    static_assert(SMEM <= 232448 - 1024 && SCALE_COL + (FP8 ? 8 * STAGES : 0) <= 512 && NT % 16 == 0, "");
 };
 
 struct NarrowArgs {
@@ -86,13 +86,13 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int c0,
         : "memory");
 }
 
-template <bool FP8, int DT, int MATS, int ACT>
+template <bool FP8, int DT, int MATS, int ACT, int NT>
 __global__ void __launch_bounds__(R_THREADS, 1)
     narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW2,
                   const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmSW,
                   const __grid_constant__ CUtensorMap tmSX, const NarrowArgs args) {
-    using C = Narrow<FP8, MATS>;
-    constexpr uint32_t IDESC = idesc_narrow<DT>(FP8, R_N);
+    using C = Narrow<FP8, MATS, NT>;
+    constexpr uint32_t IDESC = idesc_narrow<DT>(FP8, NT);
     constexpr int BK = FP8 ? 128 : 64;
     extern __shared__ __align__(1024) unsigned char narrow_smem[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(narrow_smem) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(R_THREADS, 1)
                         for (int m = 0; m < MATS; ++m)
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                tc_mma_f16(d + m * R_N, umma_desc_sw128(sw + m * R_W + 32 * j, 16, 1024),
+                                tc_mma_f16(d + m * NT, umma_desc_sw128(sw + m * R_W + 32 * j, 16, 1024),
                                            umma_desc_sw128(sx + 32 * j, 16, 1024), IDESC, !start || j ? 1u : 0u);
                     }
                     tc_commit(&empty_bar[stage]);
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(R_THREADS, 1)
             for (int t = half * 16; t < args.T; t += 32) {
                 uint32_t r[MATS][16];
 #pragma unroll
-                for (int m = 0; m < MATS; ++m) tmem_ld16(t0 + m * R_N + t, r[m]);
+                for (int m = 0; m < MATS; ++m) tmem_ld16(t0 + m * NT + t, r[m]);
                 tmem_wait_ld();
                 if (size == 1) {
                     uint16_t* o = out + t * args.ldo;
@@ -358,13 +358,14 @@ struct Share {
     int size, clusters, per;
 };
 template <typename K>
-Share share_tiles(K kernel, int smem, std::atomic<int> (&resident)[8], long long tiles, long long nkb, int grain, int mats, int T) {
+Share share_tiles(K kernel, int smem, std::atomic<int> (&resident)[8], long long tiles, long long nkb, int grain, int mats, int T, int places) {
     const long long units = (nkb + grain - 1) / grain;
     Share best{};
     double least = 0;
     for (int i = 0; i < 8; ++i) {
         const long long size = i + 1, per = (units + size - 1) / size;
-        if ((units + per - 1) / per != size) continue;  // a CTA without a part
+        if ((units + per - 1) / per != size) continue;          // a CTA without a part
+        if (size * ((T + size - 1) / size) > places) continue;  // no room for the parts
         int n = resident[i].load(std::memory_order_relaxed);
         if (!n) resident[i].store(n = resident_clusters(kernel, R_THREADS, smem, (int)size), std::memory_order_relaxed);
         const long long at_once = std::min<long long>(tiles, n), rounds = (tiles + n - 1) / n;
@@ -391,10 +392,10 @@ struct NarrowCall {
     cudaStream_t st;
 };
 
-template <bool FP8, int DT, int MATS, int ACT>
-int launch_narrow(const NarrowCall& c) {
-    using S = Narrow<FP8, MATS>;
-    auto k = narrow_kernel<FP8, DT, MATS, ACT>;
+template <bool FP8, int DT, int MATS, int ACT, int NT>
+int launch_narrow_nt(const NarrowCall& c) {
+    using S = Narrow<FP8, MATS, NT>;
+    auto k = narrow_kernel<FP8, DT, MATS, ACT, NT>;
     static SmemOnce once;
     SFFN_CUDA_TRY(once.set(k, S::SMEM));
     constexpr int ES = FP8 ? 1 : 2, BK = 128 / ES;
@@ -404,7 +405,7 @@ int launch_narrow(const NarrowCall& c) {
     a.out = c.out, a.ldo = c.ldo, a.status = c.status;
     a.tiles = (int)((c.N + 127) / 128);
     static std::atomic<int> resident[8];
-    const Share share = share_tiles(k, S::SMEM, resident, a.tiles, a.nkb, FP8 ? 4 : 1, MATS, c.T);
+    const Share share = share_tiles(k, S::SMEM, resident, a.tiles, a.nkb, FP8 ? 4 : 1, MATS, c.T, S::PLACES);
     a.per = share.per;
     const auto type = FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
     const auto sw = CU_TENSOR_MAP_SWIZZLE_128B;
@@ -432,6 +433,11 @@ int launch_narrow(const NarrowCall& c) {
     config.numAttrs = c.after ? 2 : 1;
     SFFN_CUDA_TRY(cudaLaunchKernelEx(&config, k, m[0], m[1], m[2], m[3], m[4], a));
     return SFFN_OK;
+}
+
+template <bool FP8, int DT, int MATS, int ACT>
+int launch_narrow(const NarrowCall& c) {
+    return c.T <= 48 ? launch_narrow_nt<FP8, DT, MATS, ACT, 48>(c) : launch_narrow_nt<FP8, DT, MATS, ACT, 64>(c);
 }
 
 template <int DT>

@@ -24,7 +24,7 @@ __all__ = ["BLOCK", "Fp8Tensor", "fp8_pack", "fp8_unpack", "fp8_matmul", "ckpt_l
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
-FEW_ROWS = 48  # products of at most so many rows go by the few-row kernels
+FEW_ROWS = 64  # products of at most so many rows go by the few-row kernels
 OUT_TYPES = (torch.bfloat16, torch.float16)
 
 
@@ -121,13 +121,13 @@ def _empty_rows(t, rows, cols, multiple):
     """[rows, cols] of t's type, its rows padded to a multiple of so many elements."""
     ld = -(-cols // multiple) * multiple
     out = t.new_empty((rows, ld))
-    return out if ld == cols else out[:, :cols]
+    return out if ld == cols else out.narrow(1, 0, cols)
 
 
 def _empty_values(rows, width, device, multiple=16):
     ld = -(-width // multiple) * multiple
     out = torch.empty((rows, ld), dtype=E4M3, device=device)
-    return out if ld == width else out[:, :width]
+    return out if ld == width else out.narrow(1, 0, width)
 
 
 def _empty_tiles(rows, width, device):

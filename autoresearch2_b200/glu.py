@@ -161,7 +161,8 @@ def gated_ffn(x, Wg, Wu, W2, activation="silu", checkpoint=None):
     activation: "silu", "gelu" (exact), "relu" or "relu2".  checkpoint=None keeps
     x, x Wg^T and x Wu^T for the backward in their type, "fp8" in 8 bits; the
     output is the same.  Nothing is kept where no gradient is wanted; calls of up
-    to 16 rows then take the few-row kernels.  Weight gradients are handed to an
+    to 16 rows (64 where the weights' rows are on 16 bytes) then take the few-row
+    kernels.  Weight gradients are handed to an
     attached parallel.GradAllReduce as they are produced.  Differentiable once,
     in reverse mode."""
     if activation not in ACTIVATIONS:

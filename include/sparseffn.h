@@ -706,7 +706,7 @@ int sffn_gemm16(int dtype, const void* A, int64_t lda, int a_mn, const void* B, 
                 int64_t lda2, const void* B2, int64_t ldb2, int64_t K2, int64_t M, int64_t N, int64_t K, void* C,
                 int64_t ldc, void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream);
 
-/* Products of few rows with long weights, at most 16 at any alignment, at most 48
+/* Products of few rows with long weights, at most 16 at any alignment, at most 64
  * where the rows of x, h and the weights are on 16 bytes: out [T, N] = x w^T;
  * h [T, F] = act(x wg^T) * (x wu^T) and y [T, D] = h w2^T; and x w^T in 8-bit
  * blocks. */

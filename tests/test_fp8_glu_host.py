@@ -253,7 +253,7 @@ def test_product_entries(lib):
         ok = [P, 48, P, P, 48, P, 100, 8, 40, P, 1, 8, None, 0, P, None]
         if few:
             ok[6:] = [10, 8, 40, P, 1, 8, P, None]
-            assert rc(f, ok, _6=49) == 1
+            assert rc(f, ok, _6=65) == 1
         assert rc(f, ok, _10=0) == 2 and rc(f, ok, _6=-1) == 1 and rc(f, ok, _8=0) == 1 and rc(f, ok, _6=0) == 0 and rc(f, ok, _7=0) == 0
         for i in (0, 2, 3, 5, 9, len(ok) - 2):
             assert rc(f, ok, **{f"_{i}": None}) == 1
@@ -303,15 +303,15 @@ def test_gated_entries(lib):
 def test_few_row_entries(lib):
     mm = [1, P, 40, P, 40, 10, 64, 40, P, 64, P, None]
     f = lib.sffn_few_rows_mm
-    assert rc(f, mm, _0=0) == 2 and rc(f, mm, _5=49) == 1 and rc(f, mm, _7=0) == 1 and rc(f, mm, _5=0) == 0 and rc(f, mm, _6=0) == 0
+    assert rc(f, mm, _0=0) == 2 and rc(f, mm, _5=65) == 1 and rc(f, mm, _7=0) == 1 and rc(f, mm, _5=0) == 0 and rc(f, mm, _6=0) == 0
     for i in (1, 3, 8, 10):
         assert rc(f, mm, **{f"_{i}": None}) == 1
     assert rc(f, mm, _2=39) == 1 and rc(f, mm, _4=39) == 1 and rc(f, mm, _9=63) == 1 and rc(f, mm, _1=vp((1 << 20) + 1)) == 3
     # more than 16 rows: only on 16 bytes
-    assert rc(f, mm, _5=17, _2=41) == 3 and rc(f, mm, _5=17, _4=44) == 3 and rc(f, mm, _5=48, _3=vp((1 << 20) + 8)) == 3
+    assert rc(f, mm, _5=17, _2=41) == 3 and rc(f, mm, _5=17, _4=44) == 3 and rc(f, mm, _5=64, _3=vp((1 << 20) + 8)) == 3
     f = lib.sffn_few_rows_ffn
     b = [1, 2, P, 40, P, 40, P, 40, P, 64, 10, 40, 64, P, 64, P, 40, P, None]
-    assert rc(f, b, _0=0) == 2 and rc(f, b, _1=-1) == 1 and rc(f, b, _13=None) == 1 and rc(f, b, _10=49) == 1 and rc(f, b, _10=0) == 0 and rc(f, b, _5=39) == 1
+    assert rc(f, b, _0=0) == 2 and rc(f, b, _1=-1) == 1 and rc(f, b, _13=None) == 1 and rc(f, b, _10=65) == 1 and rc(f, b, _10=0) == 0 and rc(f, b, _5=39) == 1
     for i in (3, 5, 7, 9, 14):
         assert rc(f, b, _10=17, **{f"_{i}": 68}) == 3, i
 

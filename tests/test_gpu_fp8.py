@@ -145,7 +145,7 @@ SIZES = [(1, 64, 64), (1, 1000, 4096), (8, 48, 16), (9, 130, 1001), (16, 256, 64
          (777, 1001, 96), (1, 1, 1), (40, 1, 7), (513, 768, 16384), (1, 5003, 3000), (16, 4800, 1100),
          (10, 9001, 700),  # these three: several groups of rows a multiprocessor
          (40, 300, 14336), (300, 257, 9000), (17, 1001, 2049),  # in parts of K
-         (20, 20000, 300), (24, 2048, 8192), (37, 4096, 5120), (48, 640, 8200), (49, 640, 8200), (9, 8200, 4100)]  # up to 48 rows
+         (20, 20000, 300), (24, 2048, 8192), (37, 4096, 5120), (48, 640, 8200), (49, 640, 8200), (64, 2048, 8192), (57, 20000, 300), (65, 640, 8200), (9, 8200, 4100)]  # up to 64 rows
 
 
 @pytest.mark.parametrize("out", [BF16, F16])

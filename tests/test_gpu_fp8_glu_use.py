@@ -124,7 +124,7 @@ def test_captured_and_replayed():
     sf.check_status()
 
 
-@pytest.mark.parametrize("T", [1, 12, 40, 90])
+@pytest.mark.parametrize("T", [1, 12, 40, 64, 90])
 def test_operands_rewritten_between_calls(T):
     """Calls under way one behind the other, every operand written anew before each:
     kernels that start while the one before ends read none of it too early."""

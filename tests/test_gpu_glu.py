@@ -128,7 +128,7 @@ SIZES = [(1, 64, 64), (3, 8, 40), (5, 129, 65), (16, 768, 256), (32, 96, 1001), 
 @pytest.mark.parametrize("T,D,F", SIZES)
 def test_forward(T, D, F, dtype):
     x, Wg, Wu, W2, _ = inputs(T, D, F, dtype)
-    for name in ACTS if T in (5, 33, 129) else ("silu",):
+    for name in ACTS if T in (5, 33, 64, 129) else ("silu",):
         y = sf.gated_ffn(x, Wg, Wu, W2, name)
         check_forward(y, x, Wg, Wu, W2, name)
         assert torch.equal(y, sf.gated_ffn(x, Wg, Wu, W2, name))
@@ -136,7 +136,8 @@ def test_forward(T, D, F, dtype):
 
 
 @pytest.mark.parametrize("T,D,F", [(1, 3000, 5003), (8, 600, 2500), (16, 2600, 4096), (27, 2500, 7001), (32, 515, 9000),
-                                   (20, 256, 20480), (48, 2048, 8192), (24, 8192, 1000), (47, 5120, 640), (49, 640, 1024)])
+                                   (20, 256, 20480), (48, 2048, 8192), (24, 8192, 1000), (47, 5120, 640), (49, 640, 1024), (64, 2048, 8192), (61, 8192, 1000),
+                                   (63, 264, 20480), (65, 640, 1024)])
 def test_forward_of_few_rows_and_long_weights(T, D, F):
     """Several groups of weight rows a multiprocessor, in both projections; many
     calls under way at once."""
