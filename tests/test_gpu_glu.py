@@ -275,3 +275,16 @@ def test_infinities_and_nan_stay_in_their_rows():
     for checkpoint in (None, "fp8"):
         dx = torch.autograd.grad(sf.gated_ffn(x, Wg, Wu, W2, checkpoint=checkpoint), x, dy)[0]
         assert torch.isnan(dx[2]).any() and torch.isfinite(dx[rest]).all()
+
+
+@pytest.mark.parametrize("T", [12, 40, 1537])
+def test_gelu_keeps_small_tails(T):
+    """x gelu(x) alone, one weight of 1 each: Phi is within 2^-16 of itself for |x| <= 12
+    (2.7e-6 for |x| < 5, its exponent's rounding beyond), the products' float32 roundings
+    below 2^-21, h is rounded once and y is h."""
+    x = torch.linspace(-12, 12, T, device=DEV).to(BF16)[:, None]
+    one = torch.ones(1, 1, device=DEV, dtype=BF16)
+    y = sf.gated_ffn(x, one, one, one, "gelu").to(F64)
+    x = x.to(F64)
+    want = x * x * 0.5 * torch.erfc(-x / 2 ** 0.5)
+    assert ((y - want).abs() <= (half(BF16) + 2 ** -15) * want.abs()).all()
