@@ -134,6 +134,24 @@ def _empty_tiles(rows, width, device):
     return torch.empty(_tile_shape(rows, width), dtype=torch.uint8, device=device)
 
 
+def _kept_rows(t, rows, width, dtype, device, multiple):
+    """A matrix that a forward kept, its rows padded to a multiple of so many elements.
+    Saved-tensor hooks (save_on_cpu and the like) may give back a dense copy,
+    which is laid out again; what is not that matrix is refused."""
+    if t.shape != (rows, width) or t.dtype is not dtype or t.device != device:
+        raise ValueError(f"a kept tensor must be {dtype} {(rows, width)} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    ld = -(-width // multiple) * multiple
+    if (rows <= 1 or t.stride(0) == ld) and (width <= 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0:
+        return t
+    return t.new_empty((rows, ld)).narrow(1, 0, width).copy_(t)
+
+
+def _kept_tiles(t, rows, width, device):
+    if t.shape != _tile_shape(rows, width) or t.dtype is not torch.uint8 or t.device != device:
+        raise ValueError(f"kept scale_tiles must be uint8 {_tile_shape(rows, width)} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.contiguous()
+
+
 def _pack(x):
     """(values, scale tiles) of x [..., width]."""
     x2 = _rows(x)

@@ -115,6 +115,21 @@ def _backward(dy, x, Wg, Wu, W2, g, u, gt, ut, xv, xt, act, want, apart=False):
     return dx, dWg, dWu, dW2
 
 
+def _as_kept(dy, x, F, g, u, gt, ut, xv, xt):
+    """(x, g, u, g_tiles, u_tiles, x_values, x_tiles) on the strides that the kernels read,
+    which a forward gives them and a copy by saved-tensor hooks does not; refused
+    where they are not what was kept.  x is None with 8-bit checkpoints, the
+    last four without."""
+    rows, D, dev = dy.numel() // dy.shape[-1], dy.shape[-1], dy.device
+    if x is None:
+        kept = fp8._kept_rows
+        return (None, kept(g, rows, F, fp8.E4M3, dev, 16), kept(u, rows, F, fp8.E4M3, dev, 16), fp8._kept_tiles(gt, rows, F, dev),
+                fp8._kept_tiles(ut, rows, F, dev), kept(xv, rows, D, fp8.E4M3, dev, 16), fp8._kept_tiles(xt, rows, D, dev))
+    if x.shape != dy.shape or x.dtype is not dy.dtype or x.device != dev:
+        raise ValueError(f"the kept x must be {dy.dtype} {tuple(dy.shape)} on {dev}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    return x, *(fp8._kept_rows(t, rows, F, dy.dtype, dev, 8) for t in (g, u)), None, None, None, None
+
+
 def _check_kept(dy, x, F, g, u, gt, ut, xv, xt):
     """The backward op's: what it is given is what a forward keeps."""
     rows, D = dy.numel() // dy.shape[-1], dy.shape[-1]
@@ -142,7 +157,10 @@ class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         _lib.once_differentiable("gated_ffn")
-        return *_backward(dy, *ctx.saved_tensors, ctx.act, ctx.needs_input_grad[:4]), None, None
+        x, Wg, Wu, W2, *kept = ctx.saved_tensors
+        _check(dy, Wg, Wu, W2)
+        x, *kept = _as_kept(dy, x, Wg.shape[0], *kept)
+        return *_backward(dy, x, Wg, Wu, W2, *kept, ctx.act, ctx.needs_input_grad[:4]), None, None
 
 
 def _check(x, Wg, Wu, W2):

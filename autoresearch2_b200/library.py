@@ -491,8 +491,8 @@ def gated_ffn_bwd(dy: Tensor, x: Optional[Tensor], Wg: Tensor, Wu: Tensor, W2: T
                   ut: Tensor, xv: Tensor, xt: Tensor, act: int,
                   want: list[bool]) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     glu._check(dy, Wg, Wu, W2)
-    glu._check_kept(dy, x, Wg.shape[0], g, u, gt, ut, xv, xt)
-    kept = (g, u, gt, ut, xv, xt) if x is None else (g, u, None, None, None, None)
+    x, *kept = glu._as_kept(dy, x, Wg.shape[0], g, u, gt, ut, xv, xt)
+    glu._check_kept(dy, x, Wg.shape[0], *kept)
     return _or_empty(dy, glu._backward(dy, x, Wg, Wu, W2, *kept, act, want, apart=True))
 
 
