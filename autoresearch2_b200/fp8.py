@@ -378,6 +378,17 @@ def _linear_backward(dy, W, values, tiles, x_shape, want_x, want_W):
     return dx, dW
 
 
+def _check_backward(dy, W, x_shape):
+    if not _fits(dy, W, dy.shape[-1], x_shape[-1]):
+        _check_weights(dy, W=(W, (dy.shape[-1], x_shape[-1])))
+
+
+def _kept_input(dy, values, tiles, x_shape):
+    """x as kept, on the strides that the kernels read."""
+    rows, width = dy.numel() // dy.shape[-1], x_shape[-1]
+    return _kept_rows(values, rows, width, E4M3, dy.device, 16), _kept_tiles(tiles, rows, width, dy.device)
+
+
 class _CkptLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W):
@@ -390,6 +401,9 @@ class _CkptLinear(torch.autograd.Function):
     def backward(ctx, dy):
         _lib.once_differentiable("ckpt_linear")
         W, values, tiles = ctx.saved_tensors
+        _check_backward(dy, W, ctx.x_shape)
+        if values is not None:
+            values, tiles = _kept_input(dy, values, tiles, ctx.x_shape)
         return _linear_backward(dy, W, values, tiles, ctx.x_shape, *ctx.needs_input_grad)
 
 

@@ -435,9 +435,7 @@ def ckpt_linear_bwd(dy: Tensor, W: Tensor, values: Tensor, tiles: Tensor, x_shap
         raise ValueError(f"dy must be {(*x_shape[:-1], W.shape[0])}, got {tuple(dy.shape)}")
     fp8._check_weights(dy, W=(W, (dy.shape[-1], x_shape[-1])))
     if want_W:
-        _check_blocks(values, tiles)
-        if values.shape != (dy.numel() // dy.shape[-1], x_shape[-1]) or values.device != dy.device:
-            raise ValueError("values are not the forward's")
+        values, tiles = fp8._kept_input(dy, values, tiles, x_shape)
     return _or_empty(dy, fp8._linear_backward(dy, W, values, tiles, torch.Size(x_shape), want_x, want_W))
 
 

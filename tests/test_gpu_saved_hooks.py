@@ -72,3 +72,28 @@ def test_what_a_hook_must_not_return(checkpoint):
             y = sf.gated_ffn(*leaves, checkpoint=checkpoint)
         with pytest.raises((TypeError, ValueError)):
             torch.autograd.grad(y, leaves, dy)
+
+
+@pytest.mark.parametrize("hook", HOOKS)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,K,N", [(1499, 1001, 515), (130, 96, 200), (1, 21, 37), (65, 1, 1)])
+def test_ckpt_linear(T, K, N, dtype, hook):
+    x, W = randn(T, K, seed=1, dtype=dtype).requires_grad_(), randn(N, K, seed=2, scale=K ** -0.5, dtype=dtype).requires_grad_()
+    dy = randn(T, N, seed=3, dtype=dtype)
+    want = torch.autograd.grad(sf.ckpt_linear(x, W), [x, W], dy)
+    ys = []
+    with HOOKS[hook]():
+        ys += [sf.ckpt_linear(x, W), torch.ops.sparseffn.ckpt_linear(x, W, True)[0], sf.ckpt_linear(x, W.detach())]
+    for y in ys[:2]:
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, [x, W], dy), want))
+    assert torch.equal(torch.autograd.grad(ys[2], x, dy)[0], want[0])
+    sf.check_status()
+
+
+def test_what_a_hook_must_not_return_to_ckpt_linear():
+    x, W, dy = randn(77, 101).requires_grad_(), randn(37, 101, seed=1).requires_grad_(), randn(77, 37, seed=2)
+    for bad in (lambda t: t[:-1], lambda t: t.float(), lambda t: t.cpu()):
+        with saved_tensors_hooks(lambda t: t, bad):
+            y = sf.ckpt_linear(x, W)
+        with pytest.raises((TypeError, ValueError)):
+            torch.autograd.grad(y, [x, W], dy)

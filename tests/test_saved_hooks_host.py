@@ -131,3 +131,44 @@ def test_gated_ffn_refuses_what_was_not_kept(monkeypatch, calls, keep):
         with pytest.raises((TypeError, ValueError)):
             gated_step(monkeypatch, calls, 7, 21, 37, BF16, keep, one)
     assert not calls
+
+
+def linear_step(monkeypatch, seen, T, K, N, dtype, hook):
+    kept = [values(T, K, 1), tiles(T, K, 2)]
+    monkeypatch.setattr(fp8, "_linear_forward", lambda x, W, keep: (torch.zeros(T, N, dtype=dtype), *kept))
+
+    def call(name, *a):
+        assert name == "sffn_ckpt_linear_bwd"
+        W, ldw, v, ldv, t = a[3], a[4], a[6], a[7], a[8]
+        assert v % 16 == 0 and ldv % 16 == 0
+        seen.append([read(v, T, K, ldv, kept[0]), torch.frombuffer(bytearray(ctypes.string_at(t, kept[1].numel())), dtype=torch.uint8).view(kept[1].shape),
+                     read(W, N, K, ldw, fill(1, 1, seed=0, dtype=dtype))])
+
+    monkeypatch.setattr(fp8, "call", call)
+    x, W = (fill(*s, seed=i, dtype=dtype).requires_grad_() for i, s in enumerate([(T, K), (N, K)]))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, hook):
+        y = fp8._CkptLinear.apply(x, W)
+    y.backward(fill(T, N, seed=14, dtype=dtype))
+    return as_bytes(kept[0]), kept[1], as_bytes(W.detach())
+
+
+@pytest.mark.parametrize("hook", [moved, lambda t: t], ids=["moved", "kept"])
+@pytest.mark.parametrize("T,K,N", [(7, 21, 37), (1, 21, 37), (5, 32, 48), (9, 1, 1), (130, 1001, 5)])
+def test_ckpt_linear_reads_what_was_kept(monkeypatch, calls, T, K, N, hook):
+    want = linear_step(monkeypatch, calls, T, K, N, F16, hook)
+    (got,) = calls
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_ckpt_linear_refuses_what_was_not_kept(monkeypatch, calls):
+    for bad in (lambda t: t.float(), lambda t: t[:-1], lambda t: t.to("meta")):
+        for i in range(3):
+            count = [0]
+
+            def one(t):
+                count[0] += 1
+                return bad(t) if count[0] == i + 1 else t
+
+            with pytest.raises((TypeError, ValueError)):
+                linear_step(monkeypatch, calls, 7, 21, 37, BF16, one)
+    assert not calls
