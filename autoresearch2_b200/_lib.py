@@ -245,7 +245,7 @@ def _gated_bwd_launches(_dtype, _act, keep, steps, *a):
         n += _gemm16(D, F, T)
     if steps & 4 and (dwg or dwu):
         ld = (F + 7) // 8 * 8
-        joint = dwg and dwu == dwg + ld * D * 2
+        joint = dwg and dwu and (steps & 16 if steps & 48 else F % 8 == 0 and dwu == dwg + ld * D * 2)
         n += (1 if keep == 2 else bool(odd & 16)) + (_gemm16(2 * ld, D, T) if joint else (bool(dwg) + bool(dwu)) * _gemm16(F, D, T))
     if steps & 8 and dx:
         n += _gemm16(T, D, F, F)

@@ -153,6 +153,17 @@ int gated_fwd(int dtype, int act, int keep, const void* x, long long ldx, const 
     return SFFN_OK;
 }
 
+bool adjacent(const void* dwg, const void* dwu, long long D, long long F) {
+    return dwu == static_cast<const char*>(dwg) + up8(F) * D * 2;
+}
+// Whether dWg and dWu are one product, which writes the rows between and behind them
+// too: on request, and where there are none.  (By the two places alone it overwrote what
+// lay there when separate buffers happened to be so far apart.)
+bool joint_weights(int steps, const void* dwg, const void* dwu, long long D, long long F) {
+    if (steps & (SFFN_GATED_JOINT | SFFN_GATED_APART)) return steps & SFFN_GATED_JOINT;
+    return F % 8 == 0 && adjacent(dwg, dwu, D, F);
+}
+
 // odd: bit 0 dy, 1 Wg, 2 Wu, 3 W2, 4 x.  steps: SFFN_GATED_*, each on the same workspace.
 int gated_bwd(int dtype, int act, int keep, int steps, const void* dy, long long lddy, const void* x, long long ldx,
               const void* wg, long long ldg, const void* wu, long long ldu, const void* w2, long long ld2, int odd,
@@ -190,11 +201,12 @@ int gated_bwd(int dtype, int act, int keep, int steps, const void* dy, long long
             if (keep == SFFN_KEEP_8) TRY(sffn_fp8_unpack(xv, up16(D), xs, T, D, dtype, const_cast<void*>(X.p), X.ld, stream));
             else TRY(pad_x.run(stream));
         }
-        if (want_g && want_u && (count || dwu == static_cast<char*>(dwg) + ldf * D * 2)) {
+        const bool joint = want_g && want_u && joint_weights(steps, dwg, dwu, D, F);
+        if (joint || (count && want_g && want_u)) {
             const Mat both{d, 2 * ldf, T, 2 * ldf, false};
             TRY(product(dwg, D, 2 * ldf, D, T, both, 1, X, 1));
         }
-        if (count || dwu != static_cast<char*>(dwg) + ldf * D * 2 || !(want_g && want_u)) {
+        if (!joint || count) {
             if (want_g) TRY(product(dwg, D, F, D, T, DG, 1, X, 1));
             if (want_u) TRY(product(dwu, D, F, D, T, DU, 1, X, 1));
         }
@@ -326,6 +338,7 @@ extern "C" int sffn_gated_ffn_bwd(int dtype, int act, int keep, int steps, const
     if (keep != SFFN_KEEP_16 && keep != SFFN_KEEP_8) return SFFN_ERR_ARG;
     const int want = (dx ? 1 : 0) | (dwg ? 2 : 0) | (dwu ? 4 : 0) | (dw2 ? 8 : 0);
     TRY(enter(scope, dtype, dy, T, D, F, workspace, workspace_bytes, sffn_gated_ffn_workspace_bytes(1, keep, odd, want, T, D, F), status_dev));
+    if ((steps & SFFN_GATED_JOINT) && ((steps & SFFN_GATED_APART) || !dwg || !dwu || !adjacent(dwg, dwu, D, F))) return SFFN_ERR_ARG;
     if (!wg || !wu || !w2 || ((dwg || dwu) && (keep == SFFN_KEEP_8 ? !x_values || !x_scales : !x))) return SFFN_ERR_ARG;
     OuterScope outer(scope);
     Scratch ws{static_cast<char*>(workspace)};

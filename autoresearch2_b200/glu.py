@@ -30,6 +30,7 @@ __all__ = ["ACTIVATIONS", "gated_ffn"]
 ACTIVATIONS = {"relu": 0, "relu2": 1, "silu": 2, "gelu": 3}
 KEEP = {None: 1, "fp8": 2}
 DGRAD, DW2, DWGU, DX = 1, 2, 4, 8  # steps of the backward
+JOINT, APART = 16, 32  # dWg and dWu as one product, or as two
 
 
 def _kept_ld(F, keep):
@@ -79,10 +80,12 @@ def _backward(dy, x, Wg, Wu, W2, g, u, gt, ut, xv, xt, act, want, apart=False):
         dx = dy2.new_empty(dy.shape)
     if not T:
         return (dx, *(submit_grad(w.new_zeros(w.shape)) if n else None for w, n in zip((Wg, Wu, W2), want[1:])))
+    how = APART
     if want[1] and want[2] and not apart:  # one product, rows of dWu after F rounded up to 8 of dWg
         ld = (F + 7) // 8 * 8
         both = dy2.new_empty((2 * ld, D))
         dWg, dWu = both[:F], both[ld:ld + F]
+        how = JOINT
     else:
         dWg, dWu = (dy2.new_empty((F, D)) if w else None for w in want[1:3])
     if want[3]:
@@ -99,7 +102,7 @@ def _backward(dy, x, Wg, Wu, W2, g, u, gt, ut, xv, xt, act, want, apart=False):
     code, status, stream = _lib._DTYPES[dy.dtype], _lib.status_word(dev).data_ptr(), stream_handle(dev)
 
     def run(steps):
-        call("sffn_gated_ffn_bwd", code, act, keep, steps, dy2.data_ptr(), ldy, ptr(x2), ldx, Wg.data_ptr(), ldg, Wu.data_ptr(),
+        call("sffn_gated_ffn_bwd", code, act, keep, steps | how, dy2.data_ptr(), ldy, ptr(x2), ldx, Wg.data_ptr(), ldg, Wu.data_ptr(),
              ldu, W2.data_ptr(), ld2, odd, g.data_ptr(), u.data_ptr(), ptr(gt), ptr(ut), ptr(xv), ptr(xt), T, D, F, ptr(dx),
              ptr(dWg), ptr(dWu), ptr(dW2), ptr(ws), n, status, stream)
 

@@ -736,14 +736,18 @@ enum { /* steps of the gated block's backward, on one workspace, in this order *
     SFFN_GATED_DGRAD = 1,
     SFFN_GATED_DW2 = 2,
     SFFN_GATED_DWGU = 4,
-    SFFN_GATED_DX = 8
+    SFFN_GATED_DX = 8,
+    /* with each of the steps: dwu is right behind dwg's F rounded up to 8 rows, in one
+     * buffer of twice as many rows, all of which may be written: one product */
+    SFFN_GATED_JOINT = 16,
+    SFFN_GATED_APART = 32 /* two products, wherever dwg and dwu are */
 };
 
 /* The gated block, all of a direction: y [T, D] = (act(x wg^T) * (x wu^T)) w2^T,
  * keeping as sffn_glu_up does (rows of g and u as wide as F rounded up to 16 bytes)
- * and, for SFFN_KEEP_8, x too; and the gradients (each NULL: not wanted; dwu
- * right behind dwg's F rounded up to 8 rows makes the two one product, whose
- * rows beyond F are written).  odd: bits of the operands whose rows are not on 16
+ * and, for SFFN_KEEP_8, x too; and the gradients (each NULL: not wanted).  Without
+ * SFFN_GATED_JOINT or _APART, dwu right behind dwg makes the two one product where F is a
+ * multiple of 8, so that it writes nothing else.  odd: bits of the operands whose rows are not on 16
  * bytes (1 x, or dy in the backward, 2 wg, 4 wu, 8 w2, 16 x in the backward).
  * want: 1 dx, 2 dwg, 4 dwu, 8 dw2. */
 size_t sffn_gated_ffn_workspace_bytes(int backward, int keep, int odd, int want, int64_t T, int64_t D, int64_t F);
