@@ -50,3 +50,52 @@ def test_buffers_that_lie_as_for_one_product(monkeypatch, T, D, F, checkpoint):
         monkeypatch.setattr(glu, "call", call)
         glu._backward(dy, kept_x, Wg, Wu, W2, *kept, 2, [True] * 4, apart=True)
     sf.check_status()
+
+
+class Comm(sf.parallel.GradAllReduce):
+    """Keeps a copy of each gradient as it is when it is submitted."""
+
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def submit(self, t):
+        self.seen.append((t, t.clone()))
+        return t
+
+
+def with_and_without_a_communicator(f, leaves, dy):
+    want = torch.autograd.grad(f(*leaves), leaves, dy)
+    comm = Comm()
+    with comm.attached():
+        got = torch.autograd.grad(f(*leaves), leaves, dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    return got, comm.seen
+
+
+SIZES = [(160, 96, 200), (777, 1001, 1357), (40, 64, 37), (1, 21, 8), (33, 101, 96)]
+
+
+@pytest.mark.parametrize("checkpoint", [None, "fp8"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,D,F", SIZES)
+def test_gated_ffn_with_a_communicator(T, D, F, dtype, checkpoint):
+    """Step by step instead of in one call, all gradients wanted: the same ones, each final
+    when it is handed on (dW2 first, then dWg and dWu)."""
+    leaves, dy = inputs(T, D, F, dtype)
+    leaves = [t.requires_grad_() for t in leaves]
+    got, seen = with_and_without_a_communicator(lambda *a: sf.gated_ffn(*a, checkpoint=checkpoint), leaves, dy)
+    assert [t.data_ptr() for t, _ in seen] == [got[i].data_ptr() for i in (3, 1, 2)]
+    for (t, then), i in zip(seen, (3, 1, 2)):
+        assert torch.equal(then, got[i])
+    sf.check_status()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,K,N", SIZES)
+def test_ckpt_linear_with_a_communicator(T, K, N, dtype):
+    leaves = [randn(T, K, seed=1, dtype=dtype).requires_grad_(), randn(N, K, seed=2, scale=K ** -0.5, dtype=dtype).requires_grad_()]
+    got, seen = with_and_without_a_communicator(sf.ckpt_linear, leaves, randn(T, N, seed=3, dtype=dtype))
+    ((t, then),) = seen
+    assert t.data_ptr() == got[1].data_ptr() and torch.equal(then, got[1])
+    sf.check_status()
