@@ -175,13 +175,14 @@ class GPT(nn.Module):
 
     def forward(self, idx, targets=None, weights=None):
         B, T = idx.shape
-        if weights is None:
+        packed = weights is not None
+        if not packed:
             weights = [None] * len(self.blocks)
         elif torch.is_grad_enabled() or len(weights) != len(self.blocks):
             raise ValueError("packed weights are for calls without gradients, one dict a block")
         x = self.wte[idx] + self.wpe[:T]
         arena = None
-        if self.sparse and not self.cfg.gated and weights[0] is None:
+        if self.sparse and not self.cfg.gated and not packed:
             arena = self.arena_for(B * T).as_sparse_data()
         if self.cfg.sandwich:
             pres = [blk.attn_pre for blk in self.blocks] + [self.norm_out]
