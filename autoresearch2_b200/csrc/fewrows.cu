@@ -69,14 +69,16 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 }
 
 // 16 bytes of a row from byte k on, element by element (zeros past its `bytes`): rows
-// that are not on 16 bytes, and a row's last bytes.
+// that are not on 16 bytes, and a row's last bytes.  Not by __ldg: x may be written by
+// the kernel before while this one is already resident, which the read-only path
+// does not allow (for the weights alone it gains nothing).
 template <int ESIZE>
 __device__ __forceinline__ uint4 load_piece(const uint8_t* row, long long k, long long bytes) {
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 16 / ESIZE; ++i) {
         if (k + i * ESIZE < bytes) {
-            const uint32_t v = ESIZE == 2 ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(row + k) + i) : (uint32_t)__ldg(row + k + i);
+            const uint32_t v = ESIZE == 2 ? (uint32_t)reinterpret_cast<const uint16_t*>(row + k)[i] : (uint32_t)row[k + i];
             w[i * ESIZE / 4] |= v << (8 * (i * ESIZE % 4));
         }
     }
@@ -342,7 +344,7 @@ __global__ void __launch_bounds__(S_THREADS, 1)
                             for (int h = 0; h < 2; ++h) xe[t][h] = at[(16 + t * 8 + tig * 2 + h) * 8];
                     } else {
                         const int block = c * (S_WARPS / 2) + (warp & 7);
-                        auto byte = [&](const uint8_t* p, long long row) { return (int)__ldg(p + fp8_scale_at(row, block, a.bt)); };
+                        auto byte = [&](const uint8_t* p, long long row) { return (int)p[fp8_scale_at(row, block, a.bt)]; };
 #pragma unroll
                         for (int h = 0; h < 2; ++h) we[h] = byte(a.ws, row_of(group, h));
 #pragma unroll
