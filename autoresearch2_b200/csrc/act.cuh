@@ -47,8 +47,12 @@ __device__ __forceinline__ float rcp_approx(float x) {  // 1 / x within 1 ulp
 }
 
 // act(g) and act'(g) of two elements.  SiLU: s = 1 / (1 + 2^(-g log2 e)) by the
-// hardware's exp2 and reciprocal, within 2^-21 max(|g|, 1) of the value: below a
-// twentieth of a 16-bit rounding.  GELU is the exact one: Phi(-|g|) = e^(-g^2 / 2)
+// hardware's exp2 and reciprocal, within 2^-21 max(|g|, 2) of the value for g >= -92:
+// below a tenth of a 16-bit rounding down to the smallest normal results.  (Exponential,
+// sum and reciprocal are held 2^8 apart from their values: the reciprocal of a sum
+// above 2^126 is flushed to 0, and at g = -88 it is s that is so small, not g s.  Below
+// -92 the result may be 0.  Forward of 32768 x 768 x 2048: 287 us without, 288 with.)
+// GELU is the exact one: Phi(-|g|) = e^(-g^2 / 2)
 // t Q(t) with t = 1 / (1 + 0.2333 |g|), Q of degree 7 fitted here for the least relative
 // error over all t (9.4e-8), so that small tails keep their digits: within 2.7e-6 of
 // Phi for |g| < 5 in float32, 1.3e-5 at 12, where the exponent's rounding grows.
@@ -56,9 +60,10 @@ __device__ __forceinline__ float rcp_approx(float x) {  // 1 / x within 1 ulp
 template <int ACT, bool GRAD>
 __device__ __forceinline__ Float2 glu_act2(Float2 g, Float2& d) {
     if constexpr (ACT == GLU_SILU) {
-        const float2 t = split2(pair_mul(g, join2(-1.4426950408889634f, -1.4426950408889634f)));
-        const float2 e = split2(pair_add(join2(exp2_approx(t.x), exp2_approx(t.y)), join2(1.f, 1.f)));
-        const Float2 s = join2(rcp_approx(e.x), rcp_approx(e.y));
+        constexpr float low = 1.f / 256;
+        const float2 t = split2(pair_fma(g, join2(-1.4426950408889634f, -1.4426950408889634f), join2(-8.f, -8.f)));
+        const float2 e = split2(pair_add(join2(exp2_approx(t.x), exp2_approx(t.y)), join2(low, low)));
+        const Float2 s = pair_mul(join2(rcp_approx(e.x), rcp_approx(e.y)), join2(low, low));
         const Float2 a = pair_mul(g, s);
         if constexpr (GRAD) d = pair_fma(a, pair_fma(s, join2(-1.f, -1.f), join2(1.f, 1.f)), s);
         return a;
