@@ -656,7 +656,7 @@ int sffn_fp8_mm(const void* a, int64_t lda, const void* a_scales, const void* b,
                 size_t workspace_bytes, uint32_t* status_dev, void* stream);
 
 /* The same with A = x [M, K] of dtype (any alignment), packed first: into the
- * workspace, with the parts.  Up to 16 rows go by sffn_few_rows_fp8. */
+ * workspace, with the parts.  Up to 64 rows go by sffn_few_rows_fp8. */
 size_t sffn_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int sffn_fp8_linear(const void* x, int dtype, int64_t ldx, const void* b, int64_t ldb, const void* b_scales, int64_t M,
                     int64_t N, int64_t K, void* C, int c_dtype, int64_t ldc, void* workspace, size_t workspace_bytes,
