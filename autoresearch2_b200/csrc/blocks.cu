@@ -55,9 +55,11 @@ struct Pads {
 
 // Rows that the few-row kernels take: up to 16 of any alignment, up to 64 where the
 // weights' rows are on 16 bytes.  The 256-row tiles against them, us in bfloat16:
-// gated 4096 x 14336, 16 rows 87 and 64, 17 rows 87 and 70, 64 rows 91 and 73; gated
-// 1024 x 2816, 17 rows 21 and 15, 64 rows 22 and 22; y = x W^T with 14336 x 4096, 17
-// rows 28 and 27, with 2048 x 8192 (few tiles, a long K) 13 and 14, the worst case.
+// gated 4096 x 14336, 16 rows 87 and 63, 17 rows 87 and 69, 64 rows 91 and 73; gated
+// 2048 x 8192, 17 rows 34 and 29, 64 rows 35 and 35; gated 768 x 2048, 17 rows 20 and 15,
+// 64 rows 23 and 24; y = x W^T with 14336 x 4096, 17 rows 28 and 27, 64 rows 28 and 27.
+// They lose where tiles are few and K is long: 2048 x 8192, 17 rows 12.7 and 13.4; 1024 x
+// 16384, 17 rows 14.0 and 16.5, 64 rows 15.6 and 18.1, the worst of the 13 shapes timed.
 bool few_rows(long long T, int odd) { return T <= 16 || (T <= 64 && !odd); }
 
 struct Product {

@@ -561,8 +561,10 @@ int sffn::few_rows_fp8(const void* x, int64_t ldx, const void* x_scales, const v
     a.out = static_cast<uint16_t*>(out), a.ldo = ldo;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     // Nine rows and more of long weights, too: the second tile of 8 tokens costs conversions
-    // (16 rows, us: 58 MB of weights 24.3 here and 18.2 there, 34 MB 15.4 and 14.3, but 17
-    // MB 8.9 and 9.5; 8 rows of 58 MB 18.8).
+    // (16 rows, us, here and there: 14336 x 4096 23.3 and 16.7, 8192 x 4096 14.6 and 12.7,
+    // 65536 x 512 34.0 and 11.6, 1024 x 32768 24.6 and 18.6, but 4096 x 4096 8.8 and 9.1, 8192 x
+    // 2048 9.5 and 10.1; of the 13 shapes timed the rule is wrong for 2048 x 16384, 13.8 and 15.7;
+    // 8 rows of 14336 x 4096 18.8).
     if (T > S_MAX_ROWS || (T > 8 && N >= (1LL << 25) / K)) return narrow_fp8(x, ldx, x_scales, w, ldw, w_scales, T, N, K, out, out_dtype, ldo, after, status_dev, st);
     return out_dtype == SFFN_BF16 ? launch_few<SFFN_F16, SFFN_BF16, true, S_PLAIN, 0, true>(a, st)
                                   : launch_few<SFFN_F16, SFFN_F16, true, S_PLAIN, 0, true>(a, st);

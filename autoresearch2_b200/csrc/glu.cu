@@ -4,8 +4,11 @@
 // Bound by the tensor cores under the power limit where K is long (UP of 8192 x
 // 4096 x 14336: 1.54 ms, 1250 TF), by the operands' way from L2 where it is short:
 // at 32768 x 768 x 2048 UP reads 1.57 GB of tiles from L2 in 165 us, 9.5 TB/s, the
-// rate that plain products of this K have too (32768 x 768 x 2304: 96 us).  DGRAD,
-// 167 us there, adds 0.13 GB of g and u and 0.4 GB of results to 0.8 GB of tiles.
+// rate that plain products of this K have too (32768 x 768 x 2304: 96 us).  DGRAD takes
+// 167 us there with nothing saturated: 0.13 GB of g and u and 0.4 GB of results beside
+// 0.8 GB of tiles, in all 6.5 TB/s read from L2, DRAM at half its rate, tensor pipe 30%,
+// issue slots 38%.  What holds it is not known; its epilogue waits twice every 32
+// columns for its own stores to be read.
 //
 // One kernel: CTA pairs (tcgen05.mma.cta_group::2, 256 x 256 tiles, float32
 // accumulation in tensor memory, two accumulators), persistent over tiles;

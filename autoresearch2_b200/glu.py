@@ -184,8 +184,11 @@ def gated_ffn(x, Wg, Wu, W2, activation="silu", checkpoint=None):
     output is the same.  Nothing is kept where no gradient is wanted; calls of up
     to 16 rows (64 where the weights' rows are on 16 bytes) then take the few-row
     kernels.  Weight gradients are handed to an
-    attached parallel.GradAllReduce as they are produced.  Differentiable once,
-    in reverse mode."""
+    attached parallel.GradAllReduce as they are produced; those of Wg and Wu share
+    one storage where both are wanted (clone one to keep or save it alone).
+    h, dg and du are rounded to the inputs' type: in float16 they overflow beyond
+    65504 ("relu2" soon does) and lose digits below 6e-5, so scale the loss there
+    as for any float16 layer.  Differentiable once, in reverse mode."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
     if checkpoint not in KEEP:
