@@ -52,6 +52,26 @@ def test_gated_ffn_op(checkpoint):
     sf.check_status()
 
 
+@pytest.mark.parametrize("checkpoint", [None, "fp8"])
+@pytest.mark.parametrize("hook", ["save_on_cpu", "clone"])
+def test_compiled(checkpoint, hook):
+    leaves, _ = gated_inputs(77, 101, 137, BF16)
+    leaves.append(randn(37, 101, seed=5).requires_grad_())
+    dy = randn(77, 37, seed=9)
+
+    def f(x, Wg, Wu, W2, W):
+        return sf.ckpt_linear(sf.gated_ffn(x, Wg, Wu, W2, checkpoint=checkpoint), W)
+
+    want = torch.autograd.grad(f(*leaves), leaves, dy)
+    torch._dynamo.reset()
+    compiled = torch.compile(f, backend="aot_eager", fullgraph=True)
+    with HOOKS[hook]():
+        y = compiled(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dy), want))
+    torch._dynamo.reset()
+    sf.check_status()
+
+
 def test_activation_checkpointing():
     """torch.utils.checkpoint recomputes the forward; twice through the same graph."""
     from torch.utils.checkpoint import checkpoint
